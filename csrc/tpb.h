@@ -273,6 +273,11 @@ int tpb_latent_join(const void* dlat, const void* drot, void* dckv, const float*
 int tpb_router_bwd(const void* logits, int logits_is_bf16, const int* idx, const float* dw, const float* dscores,
                    void* dlogits, int tokens, int E, int K, int mode, int norm_topk, float scale, void* stream);
 
+// ---- paged cache (paged_kv.cu): rows of keys and values written to (`write`) or read from the pools
+int tpb_paged_rows(int write, void* k, void* v, void* k_pool, void* v_pool, void* k_scale, void* v_scale,
+                   const long long* slots, long long T, int H, int Dk, int Dv, int pages, int page,
+                   const long long* x_strides, const long long* strides, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,99 @@
+"""Paged cache on the CPU: the definitions, what is refused, and pages and slots that do not exist."""
+
+import pytest
+import torch
+
+from torchprime_b200.ops import paged_kv, reference as ref
+from torchprime_b200.ops.paged_kv import E4M3, E8M0, PagedKV
+
+
+def test_quantised_rows_take_the_smallest_power_of_two_that_fits():
+  x = torch.tensor([[448.0, 1.0], [449.0, -1.0], [0.0, 0.0], [224.0, 0.5], [2.0 ** -120, 0.0], [1.984375 * 2.0 ** 127, 1.0]])
+  q, e = ref.quantise_e4m3(x)
+  assert e.dtype == E8M0 and e.view(torch.uint8).tolist() == [127, 128, 127, 126, 27, 247]
+  # half a step of four significant bits, and half a step of 2^-9 below 2^-6
+  held = q.float() * ref.power_of_two(e.view(torch.uint8).int() - 127)[:, None]
+  scale = ref.power_of_two(e.view(torch.uint8).int() - 127)[:, None]
+  assert bool(((held - x).abs() <= torch.maximum(x.abs() * 2.0 ** -4, scale * 2.0 ** -10))[:5].all())
+
+
+def test_quantising_twice_changes_nothing():
+  torch.manual_seed(0)
+  x = torch.randn(200, 64) * torch.exp2(torch.randn(200, 1) * 8)
+  q, e = ref.quantise_e4m3(x)
+  held = q.float() * ref.power_of_two(e.view(torch.uint8).int() - 127)[:, None]
+  q2, e2 = ref.quantise_e4m3(held)
+  again = q2.float() * ref.power_of_two(e2.view(torch.uint8).int() - 127)[:, None]
+  assert torch.equal(held, again)
+
+
+def test_infinities_saturate_and_nan_stays():
+  q, e = ref.quantise_e4m3(torch.tensor([[float("inf"), float("-inf"), float("nan"), 3.0]]))
+  assert q.float()[0, :2].tolist() == [448.0, -448.0] and q.float()[0, 2].isnan() and q.float()[0, 3] * 2.0 ** (int(e.view(torch.uint8)) - 127) == 3.0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+def test_rows_come_back_and_others_stay(dtype):
+  torch.manual_seed(1)
+  c = PagedKV.allocate(5, 16, 3, 24, 16, dtype=dtype)
+  slots = torch.tensor([79, 0, -1, 17, 40])
+  k, v = torch.randn(5, 3, 24).bfloat16(), torch.randn(5, 3, 16).bfloat16()
+  before = [t.clone() for t in c if t is not None]
+  paged_kv.append(c, k, v, slots)
+  gk, gv = paged_kv.read(c, slots)
+  for got, x in ((gk, k), (gv, v)):
+    want = x.float() if dtype == torch.bfloat16 else None
+    if want is None:
+      q, e = ref.quantise_e4m3(x)
+      want = q.float() * ref.power_of_two(e.view(torch.uint8).int() - 127)[..., None]
+    assert torch.equal(got[[0, 1, 3, 4]].float(), want[[0, 1, 3, 4]]) and not got[2].any()
+  rest = torch.ones(80, dtype=torch.bool)
+  rest[slots[slots >= 0]] = False
+  for t, b in zip([t for t in c if t is not None], before):
+    t8, b8 = t.contiguous().view(torch.uint8).reshape(80, -1), b.contiguous().view(torch.uint8).reshape(80, -1)
+    assert torch.equal(t8[rest], b8[rest])
+
+
+def test_slots_outside_the_pool_are_left_out():
+  c = PagedKV.allocate(2, 16, 1, 8)
+  x = torch.ones(3, 1, 8).bfloat16()
+  paged_kv.append(c, x, x, torch.tensor([32, -7, 31]))
+  assert c.k.float().sum() == 8
+  k, _ = paged_kv.read(c, torch.tensor([1 << 40, 31]))
+  assert not k[0].any() and bool((k[1] == 1).all())
+
+
+def test_debug_mode_names_bad_and_repeated_slots(monkeypatch):
+  monkeypatch.setenv("TPB_DEBUG_BOUNDS", "1")
+  c = PagedKV.allocate(2, 16, 1, 8)
+  x = torch.ones(2, 1, 8).bfloat16()
+  with pytest.raises(IndexError, match="slots"):
+    paged_kv.append(c, x, x, torch.tensor([32, 0]))
+  with pytest.raises(IndexError, match="twice"):
+    paged_kv.append(c, x, x, torch.tensor([3, 3]))
+  with pytest.raises(IndexError, match="slots"):
+    paged_kv.read(c, torch.tensor([-2]))
+
+
+def test_refusals():
+  c = PagedKV.allocate(2, 16, 1, 8)
+  x = torch.ones(2, 1, 8).bfloat16()
+  s = torch.tensor([0, 1])
+  with pytest.raises(ValueError):
+    paged_kv.append(c, x[:1], x, s)
+  with pytest.raises(ValueError):
+    paged_kv.append(c, x, x, s.int())
+  with pytest.raises(ValueError):
+    paged_kv.read(c, s[None])
+  with pytest.raises(ValueError):
+    paged_kv.append(PagedKV(c.k, c.v.to(E4M3)), x, x, s)
+  with pytest.raises(ValueError):
+    paged_kv.read(PagedKV(c.k.to(E4M3), c.v.to(E4M3)), s)
+  q = PagedKV.allocate(2, 16, 1, 16, dtype=E4M3)
+  with pytest.raises(ValueError):
+    paged_kv.read(PagedKV(q.k, q.v, q.k_scale, q.v_scale.view(torch.uint8)), s)
+
+
+def test_cache_bytes():
+  c, q = PagedKV.allocate(4, 16, 2, 64), PagedKV.allocate(4, 16, 2, 64, dtype=E4M3)
+  assert c.nbytes() == 4 * 16 * 2 * 128 * 2 and q.nbytes() == 4 * 16 * 2 * (128 + 2)

@@ -238,3 +238,49 @@ def adamw_step(p32, g, m, v, lr, beta1, beta2, eps, wd, step, grad_scale=1.0):
   denom = (v.sqrt() / math.sqrt(bc2)).add_(eps)
   p32.addcdiv_(m, denom, value=-lr / bc1)
   return p32
+
+
+# ----------------------------------------------------------------------------- paged cache
+def power_of_two(e: torch.Tensor) -> torch.Tensor:
+  """2^e in fp32 for whole numbers e in [-126, 127], exactly."""
+  return ((e.to(torch.int32) + 127) << 23).view(torch.float32)
+
+
+def quantise_e4m3(x: torch.Tensor):
+  """Rows [..., D] as e4m3 values and one e8m0 power of two each: the smallest, from 2^-100 on, under which the finite values
+  fit into +-448.  Infinities become +-448 times it, NaN stays."""
+  x = x.float()
+  amax = torch.where(x.isfinite(), x.abs(), torch.zeros_like(x)).amax(-1)
+  m, e = torch.frexp(amax)                          # 448 = 0.875 * 2^9
+  e = torch.where(m <= 0.875, e - 9, e - 8).clamp(-100, 120)
+  e = torch.where(amax > 0, e, torch.zeros_like(e))
+  q = (x * power_of_two(-e)[..., None]).clamp(-448.0, 448.0).to(torch.float8_e4m3fn)
+  return q, (e + 127).to(torch.uint8).view(torch.float8_e8m0fnu)
+
+
+def paged_append(pool, scale, x, slots):
+  """In place: rows ``slots`` of a pool [P, page, H, D] become those of x [T, H, D]; -1 and slots outside the pool are skipped."""
+  page = pool.shape[1]
+  keep = (slots >= 0) & (slots < pool.shape[0] * page)
+  at = slots[keep]
+  at = (torch.div(at, page, rounding_mode="floor"), at % page)
+  if scale is None:
+    pool[at] = x[keep].to(pool.dtype)
+    return
+  q, e = quantise_e4m3(x[keep])
+  pool.view(torch.uint8)[at] = q.view(torch.uint8)
+  scale.view(torch.uint8)[at] = e.view(torch.uint8)
+
+
+def paged_read(pool, scale, slots):
+  """Rows ``slots`` (any shape) of a pool, [..., H, D]: bf16 or fp32 as they are, e4m3 in fp32; zeros for slots outside the pool."""
+  page = pool.shape[1]
+  inside = (slots >= 0) & (slots < pool.shape[0] * page)
+  s = torch.where(inside, slots, torch.zeros_like(slots))
+  at = (torch.div(s, page, rounding_mode="floor"), s % page)
+  if scale is None:
+    rows = pool[at]
+  else:
+    e = scale.view(torch.uint8)[at].to(torch.int32) - 127
+    rows = pool.view(torch.uint8)[at].view(torch.float8_e4m3fn).float() * power_of_two(e)[..., None]
+  return torch.where(inside[..., None, None], rows, torch.zeros_like(rows))
