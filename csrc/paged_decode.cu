@@ -1,0 +1,672 @@
+// Attention of one new token per sequence over a paged cache of keys and values, grouped heads.
+//
+//   o[b, h] = sum_i softmax_i(scale * q[b, h] . K[i, h / G]) V[i, h / G],   i over the visible tokens of sequence b:
+//   all `lengths[b]` of them, or the last `window`; scores may be capped (cap * tanh(s / cap)).
+//
+// Every cached row is read once per 16 query heads that share it: 2 * 16 operations a byte at most, so memory bounds it, and
+// what the kernel is built for is to keep loads under way on every SM from the first to the last token.
+//
+// * The work is cut into units: the rows of one sequence, one key head and up to 16 of its query heads, NW * 32 tokens.  In the
+//   order sequence, head, token they form one list, of which every CTA (one per SM) takes an equal, contiguous part; how long the
+//   sequences are only the device knows, so each CTA adds up the lengths itself.  A (sequence, head) whose units fall to
+//   several CTAs is joined by paged_join_kernel from their running maxima, sums and unnormalised results; a CTA has at most
+//   two of those, so the scratch is bounded by the grid and not by the batch.  Nothing is added by atomics: the order of every
+//   sum follows from the lengths.
+// * A warp takes 32 tokens of each unit by itself: a ring of stages of its own, filled by TMA boxes of 16 tokens (a page is a
+//   multiple of 16) that its elected lane asks for as soon as it has used a stage up, across the borders of sequences.  The warps
+//   of a CTA meet only where a (sequence, head) ends.
+// * Scores and weighted sums are mma.sync m16n8k16: the query heads of a key head are its 16 rows.  (A tcgen05 tile would be
+//   seven eighths empty, and its operands would still come through shared memory once.)  Statistics and sums are fp32; the
+//   weights of the sum are rounded to the operand type of the product, half a step of 2^-9 (bf16) or 2^-12 (f16) each, to
+//   either side, against a result that is rounded to bf16 itself; the sum of the weights is not rounded.
+// * An e4m3 cache is turned into f16 in registers, exactly; queries become f16 with a power of two for each head that puts the
+//   largest at 2^14 (f16 has more bits than bf16; what falls below 2^-38 of the largest is lost).  The keys' powers of two
+//   multiply the scores, the values' are added to the exponent of the weights, so that no weight overflows: o = sum_i 2^(s_i + e_i
+//   - m) v_i / sum_i 2^(s_i - m) with m the maximum of s_i + e_i.  K's columns go to the product in another order than Q's would
+//   (four neighbouring bytes to a lane instead of two and two); the queries are loaded in the same one.
+
+#include "common.cuh"
+#include "tpb.h"
+
+namespace tpb {
+
+int sm_count();
+int make_tmap_pages(CUtensorMap* map, const void* ptr, int elem_bytes, uint64_t d, uint64_t page, uint64_t heads, uint64_t pages,
+                    uint64_t row_stride, uint64_t head_stride, uint64_t page_stride);
+
+struct PagedDecode {
+  const __nv_bfloat16* q;
+  long long q_b, q_h;                      // strides
+  __nv_bfloat16* out;                      // [B, Hkv * G, DV]
+  const int* table;
+  long long table_b;
+  const int* lengths;
+  const uint8_t *k_scale, *v_scale;        // a row's scales are contiguous within a page
+  long long ks_page, ks_head, vs_page, vs_head;
+  float* part_o;                           // [2 * grid][16][DV]
+  float* part_ml;                          // [2 * grid][16][2]: running maximum in log2 units, sum
+  int* start;                              // [B + 1]: units of the sequences before, per head block
+  int* status;
+  int B, Hkv, G, blocks;                   // blocks of up to 16 query heads to a key head
+  int pages, page, capacity;               // tokens that a row of the table can name
+  int window, stages;
+  float scale_log2, cap_log2;              // cap_log2: the cap in log2 units, 0 for none
+};
+
+constexpr int PD_KEYS = 32;                // tokens of a warp's step, two boxes
+constexpr int PD_PAD = 8;                  // floats between rows where the warps meet: no two rows of a quad in one bank
+
+template <int DK, int DV, bool F8>
+struct PagedTile {
+  static constexpr int ELT = F8 ? 1 : 2;
+  static constexpr int ROW = 64 * ELT;                       // bytes of a 64-column block's row: the swizzle's width
+  static constexpr int BLOCK = 16 * ROW;
+  static constexpr int K_BOX = 16 * DK * ELT, V_BOX = 16 * DV * ELT;
+  static constexpr int STAGE = 2 * (K_BOX + V_BOX);
+  static constexpr int SCALES = F8 ? 64 : 0;                 // 32 of the keys, 32 of the values
+};
+
+__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int row, int head, int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %3, %5, %6}], [%2];"
+      :
+      : "r"(dst), "l"(map), "r"(smem_u32(bar)), "r"(0), "r"(row), "r"(head), "r"(page)
+      : "memory");
+}
+__device__ __forceinline__ void bulk_load_16(uint32_t dst, const void* src, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 16, [%2];"
+               :
+               : "r"(dst), "l"(src), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void pd_ldsm(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void pd_ldsm_t(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// d += A (16 x 16) B (16 x 8), operands bf16 or f16
+template <bool F16>
+__device__ __forceinline__ void pd_mma(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if (F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t e4m3_to_f16(uint32_t v) {      // the low two bytes
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)v));
+  return h;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// What is visible of a sequence, in tokens and in units of `per` tokens.
+struct Visible {
+  int len, lo, first, units;
+};
+__device__ __forceinline__ Visible pd_visible(const PagedDecode& p, int b, int per) {
+  Visible s;
+  s.len = min(max(p.lengths[b], 0), p.capacity);
+  s.lo = p.window > 0 ? max(0, s.len - p.window) : 0;
+  s.first = s.lo / per;
+  s.units = s.len > 0 ? (s.len - 1) / per - s.first + 1 : 0;
+  return s;
+}
+
+// A place in the list of units.
+struct PagedCursor {
+  int b, hb, at;           // sequence, head block, unit of the sequence
+  Visible s;
+  __device__ __forceinline__ void next_head(const PagedDecode& p, int per) {
+    at = 0;
+    if (++hb < p.Hkv * p.blocks) return;
+    hb = 0;
+    do {
+      ++b;
+      if (b >= p.B) return;
+      s = pd_visible(p, b, per);
+    } while (s.units == 0);
+  }
+};
+
+template <int DK, int DV, bool F8, int NW, bool WIDE>
+__global__ void __launch_bounds__(NW * 32, 1)
+paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const PagedDecode p) {
+  using T = PagedTile<DK, DV, F8>;
+  constexpr int PER = NW * PD_KEYS, THREADS = NW * 32;
+  extern __shared__ uint8_t pd_smem_raw[];
+  uint8_t* pd_smem = pd_smem_raw + ((1024u - (smem_u32(pd_smem_raw) & 1023u)) & 1023u);
+  __shared__ int s_scan[NW], s_at[4];
+  __shared__ float2 s_ml[NW][16];
+  const int warp = warp_index(), lane = threadIdx.x & 31, ST = p.stages;
+  const int HB = p.Hkv * p.blocks, R = min(16, p.G);
+  uint8_t* ring = pd_smem + (size_t)warp * ST * T::STAGE;
+  uint8_t* scales = pd_smem + (size_t)NW * ST * T::STAGE + (size_t)warp * ST * T::SCALES;
+  float* meet = reinterpret_cast<float*>(pd_smem + (size_t)NW * ST * (T::STAGE + T::SCALES));     // [NW][R][DV + PD_PAD]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(meet + NW * R * (DV + PD_PAD)) + warp * ST;
+  const uint32_t ring_at = smem_u32(ring), scales_at = smem_u32(scales);
+  if (lane == 0)
+    for (int i = 0; i < ST; ++i) mbar_init(&bars[i], 1);
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&k_map);
+    tma_prefetch_desc(&v_map);
+  }
+  fence_barrier_init();
+  chain_launch();
+  if (!chain_wait()) return;
+
+  // The list's length, and where this CTA's part begins.
+  int total = 0, share = 1, first = 0, last = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    int running = 0;
+    for (int base = 0; base < p.B; base += THREADS) {
+      const int b = base + threadIdx.x, n = b < p.B ? pd_visible(p, b, PER).units : 0;
+      int sum = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      __syncthreads();
+      if (lane == 31) s_scan[warp] = sum;
+      __syncthreads();
+      int before = running, all = 0;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        if (w < warp) before += s_scan[w];
+        all += s_scan[w];
+      }
+      before += sum - n;
+      if (pass == 0) {
+        if (blockIdx.x == 0 && b < p.B) {
+          p.start[b] = before;
+          if (p.lengths[b] < 0 || p.lengths[b] > p.capacity) report(p.status, kBadArgument, 71);
+        }
+      } else if (before * HB <= first && first < (before + n) * HB) {
+        s_at[0] = b;
+        s_at[1] = (first - before * HB) / n;
+        s_at[2] = (first - before * HB) % n;
+      }
+      running += all;
+    }
+    if (pass == 0) {
+      total = running;
+      if (blockIdx.x == 0 && threadIdx.x == 0) p.start[p.B] = total;
+      share = max(1, (total * HB + (int)gridDim.x - 1) / (int)gridDim.x);
+      first = blockIdx.x * share;
+      last = min(total * HB, first + share);
+      if (first >= last) return;
+    }
+  }
+  __syncthreads();
+  PagedCursor c = {s_at[0], s_at[1], s_at[2], {}};
+  c.s = pd_visible(p, c.b, PER);
+  PagedCursor ahead = c;
+  const int units = last - first;
+  int asked = 0, ask_stage = 0, stage = 0, parity = 0;
+  bool alive = true;
+
+  auto ask = [&]() {
+    const int key0 = (ahead.s.first + ahead.at) * PER + warp * PD_KEYS;
+    uint64_t* bar = &bars[ask_stage];
+    if (key0 < ahead.s.len && key0 + PD_KEYS > ahead.s.lo) {
+      const int boxes = key0 + 16 < ahead.s.len ? 2 : 1, head = ahead.hb / p.blocks;
+      int pg[2], row[2];
+      uint32_t bytes = 0;
+      for (int i = 0; i < boxes; ++i) {
+        const unsigned key = key0 + 16 * i, at = key / (unsigned)p.page;
+        row[i] = key - at * p.page;
+        pg[i] = p.table[ahead.b * p.table_b + at];
+        const bool inside = pg[i] >= 0 && pg[i] < p.pages;
+        if (!inside) {                     // a box outside the pool reads as zeros
+          if (lane == 0) report(p.status, kBadArgument, 72);
+          pg[i] = -1;
+        }
+        bytes += T::K_BOX + T::V_BOX + (F8 && inside ? 32 : 0);
+      }
+      one_lane([&]() {
+        mbar_expect_tx(bar, bytes);
+        const uint32_t at = ring_at + ask_stage * T::STAGE;
+        for (int i = 0; i < boxes; ++i) {
+          tma_load_page(at + i * T::K_BOX, &k_map, bar, row[i], head, pg[i]);
+          tma_load_page(at + 2 * T::K_BOX + i * T::V_BOX, &v_map, bar, row[i], head, pg[i]);
+          if (F8 && pg[i] >= 0) {
+            const uint32_t sc = scales_at + ask_stage * T::SCALES + i * 16;
+            bulk_load_16(sc, p.k_scale + pg[i] * p.ks_page + head * p.ks_head + row[i], bar);
+            bulk_load_16(sc + 32, p.v_scale + pg[i] * p.vs_page + head * p.vs_head + row[i], bar);
+          }
+        }
+      });
+    } else {
+      one_lane([&]() { mbar_arrive(bar); });
+    }
+    ++asked;
+    if (++ask_stage == ST) ask_stage = 0;
+    if (++ahead.at == ahead.s.units) ahead.next_head(p, PER);
+  };
+  while (asked < units && asked < ST) ask();
+
+  const int g = lane >> 2, t = lane & 3;
+  int done = 0;
+  while (done < units) {
+    const int seg = min(units - done, c.s.units - c.at);
+    const bool whole = seg == c.s.units;
+    const int kv_head = c.hb / p.blocks, row0 = (c.hb - kv_head * p.blocks) * 16, rows = min(16, p.G - row0);
+    const int h0 = kv_head * p.G + row0;
+    // ---- the queries as A operands
+    uint32_t qa[DK / 16][4];
+    float qs0 = p.scale_log2, qs1 = p.scale_log2;
+    {
+      const __nv_bfloat16* q0 = p.q + c.b * p.q_b + (h0 + g) * p.q_h;
+      const __nv_bfloat16* q1 = q0 + 8 * p.q_h;
+      const bool has0 = g < rows, has1 = WIDE && g + 8 < rows;
+      if constexpr (!F8) {
+#pragma unroll
+        for (int k = 0; k < DK / 16; ++k) {
+          qa[k][0] = has0 ? *reinterpret_cast<const uint32_t*>(q0 + k * 16 + 2 * t) : 0;
+          qa[k][2] = has0 ? *reinterpret_cast<const uint32_t*>(q0 + k * 16 + 8 + 2 * t) : 0;
+          qa[k][1] = has1 ? *reinterpret_cast<const uint32_t*>(q1 + k * 16 + 2 * t) : 0;
+          qa[k][3] = has1 ? *reinterpret_cast<const uint32_t*>(q1 + k * 16 + 8 + 2 * t) : 0;
+        }
+      } else {
+        uint32_t m0 = 0, m1 = 0;
+#pragma unroll
+        for (int k = 0; k < DK / 16; ++k) {
+          const uint2 a = has0 ? *reinterpret_cast<const uint2*>(q0 + k * 16 + 4 * t) : make_uint2(0, 0);
+          const uint2 b = has1 ? *reinterpret_cast<const uint2*>(q1 + k * 16 + 4 * t) : make_uint2(0, 0);
+          qa[k][0] = a.x; qa[k][2] = a.y; qa[k][1] = b.x; qa[k][3] = b.y;
+          m0 = __vmaxu2(m0, __vmaxu2(a.x & 0x7fff7fffu, a.y & 0x7fff7fffu));
+          m1 = __vmaxu2(m1, __vmaxu2(b.x & 0x7fff7fffu, b.y & 0x7fff7fffu));
+        }
+        auto factor = [&](uint32_t m, float& back) {       // 2^(14 - exponent of the largest), and 1 / of it into `back`
+          m = max(m & 0xffffu, m >> 16);
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          const int e = min(max((int)(m >> 7) - 127 - 14, -100), 113);
+          back *= __int_as_float((127 + e) << 23);
+          return __int_as_float((127 - e) << 23);
+        };
+        const float f0 = factor(m0, qs0), f1 = WIDE ? factor(m1, qs1) : 0.f;
+#pragma unroll
+        for (int k = 0; k < DK / 16; ++k)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            if (!WIDE && (x & 1)) { qa[k][x] = 0; continue; }
+            const float2 v = unpack_bf16(qa[k][x]);
+            const float f = x & 1 ? f1 : f0;
+            qa[k][x] = pack_f16(v.x * f, v.y * f);
+          }
+      }
+    }
+    float o[DV / 8][4] = {};
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+
+    for (int i = 0; i < seg; ++i) {
+      const int key0 = (c.s.first + c.at + i) * PER + warp * PD_KEYS;
+      if (done + i < asked && !mbar_wait_warp(&bars[stage], parity, p.status, kTimeoutTmaFull, 73)) alive = false;
+      if (alive && key0 < c.s.len && key0 + PD_KEYS > c.s.lo) {
+        const uint32_t k_at = ring_at + stage * T::STAGE, v_at = k_at + 2 * T::K_BOX;
+        const bool edge = key0 < c.s.lo || key0 + PD_KEYS > c.s.len;
+        if (edge) {
+          // Rows behind the end (or in front of the window) hold anything, NaN too: zeros in the values, -inf in the scores.
+          uint4* v = reinterpret_cast<uint4*>(ring + stage * T::STAGE + 2 * T::K_BOX);
+          for (int x = lane; x < 2 * T::V_BOX / 16; x += 32) {
+            const int key = key0 + x / (T::V_BOX / 16) * 16 + x % (T::BLOCK / 16) / (T::ROW / 16);
+            if (key < c.s.lo || key >= c.s.len) v[x] = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async();
+          __syncwarp();
+        }
+        // ---- scores: 16 heads x 32 tokens
+        float s[4][4] = {};
+        if constexpr (!F8) {
+          const uint32_t at = k_at + (lane & 7) * 128;
+#pragma unroll
+          for (int kk = 0; kk < DK / 32; ++kk)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              uint32_t b[4];
+              pd_ldsm(at + (n >> 1) * T::K_BOX + (kk >> 1) * T::BLOCK + (n & 1) * 1024 + ((((kk & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4), b);
+              pd_mma<false>(s[n], qa[2 * kk], b[0], b[1]);
+              pd_mma<false>(s[n], qa[2 * kk + 1], b[2], b[3]);
+            }
+        } else {
+          const uint32_t at = k_at + (lane & 7) * 64 + (((lane >> 3) ^ ((lane & 7) >> 1)) << 4);
+#pragma unroll
+          for (int hf = 0; hf < DK / 64; ++hf)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              uint32_t b[4];
+              pd_ldsm(at + (n >> 1) * T::K_BOX + hf * T::BLOCK + (n & 1) * 512, b);
+#pragma unroll
+              for (int x = 0; x < 4; ++x) pd_mma<true>(s[n], qa[4 * hf + x], e4m3_to_f16(b[x]), e4m3_to_f16(b[x] >> 16));
+            }
+        }
+        // ---- running softmax
+        float add[4][2];                   // exponents of the values' rows
+        const uint8_t* sc = scales + stage * T::SCALES;
+        float n0 = m0, n1 = m1;
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int key = key0 + n * 8 + 2 * t + x;
+            float f = 1.f;
+            add[n][x] = 0.f;
+            if (F8) {
+              f = __int_as_float((int)sc[n * 8 + 2 * t + x] << 23);
+              add[n][x] = (float)((int)sc[32 + n * 8 + 2 * t + x] - 127);
+            }
+            const bool dead = edge && (key < c.s.lo || key >= c.s.len);
+            auto score = [&](float v, float qs) {
+              v *= F8 ? qs * f : qs;
+              if (p.cap_log2 > 0.f) v = p.cap_log2 * (1.f - __fdividef(2.f, ex2_approx(v / p.cap_log2 * 2.8853900817779268f) + 1.f));
+              return dead ? -INFINITY : v;
+            };
+            s[n][x] = score(s[n][x], qs0);
+            n0 = fmaxf(n0, s[n][x] + add[n][x]);
+            if (WIDE) {
+              s[n][2 + x] = score(s[n][2 + x], qs1);
+              n1 = fmaxf(n1, s[n][2 + x] + add[n][x]);
+            }
+          }
+        n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 1));
+        n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 2));
+        if (WIDE) {
+          n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 1));
+          n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 2));
+        }
+        if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
+          const float a0 = n0 > m0 ? ex2_approx(m0 - n0) : 1.f, a1 = n1 > m1 ? ex2_approx(m1 - n1) : 1.f;
+          l0 *= a0;
+          l1 *= a1;
+#pragma unroll
+          for (int n = 0; n < DV / 8; ++n) {
+            o[n][0] *= a0; o[n][1] *= a0;
+            if (WIDE) { o[n][2] *= a1; o[n][3] *= a1; }
+          }
+          m0 = n0;
+          m1 = n1;
+        }
+        const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;      // (all scores so far are NaN or -inf)
+        uint32_t pa[2][4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          float w[4] = {};
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            w[x] = ex2_approx(s[n][x] + add[n][x] - r0);
+            l0 += F8 ? ex2_approx(s[n][x] - r0) : w[x];
+            if (WIDE) {
+              w[2 + x] = ex2_approx(s[n][2 + x] + add[n][x] - r1);
+              l1 += F8 ? ex2_approx(s[n][2 + x] - r1) : w[2 + x];
+            }
+          }
+          pa[n >> 1][(n & 1) * 2] = F8 ? pack_f16(w[0], w[1]) : pack_bf16(w[0], w[1]);
+          pa[n >> 1][(n & 1) * 2 + 1] = !WIDE ? 0 : F8 ? pack_f16(w[2], w[3]) : pack_bf16(w[2], w[3]);
+        }
+        // ---- weighted sum
+        const int vr = (lane & 7) + ((lane >> 3) & 1) * 8;
+        if constexpr (!F8) {
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int np = 0; np < DV / 16; ++np) {
+              uint32_t b[4];
+              pd_ldsm_t(v_at + ks * T::V_BOX + (np >> 2) * T::BLOCK + vr * 128 + ((((np & 3) * 2 + (lane >> 4)) ^ (lane & 7)) << 4), b);
+              pd_mma<false>(o[2 * np], pa[ks], b[0], b[1]);
+              pd_mma<false>(o[2 * np + 1], pa[ks], b[2], b[3]);
+            }
+        } else {
+#pragma unroll
+          for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int cp = 0; cp < DV / 32; ++cp) {
+              uint32_t b[4];
+              pd_ldsm_t(v_at + ks * T::V_BOX + (cp >> 1) * T::BLOCK + vr * 64 + ((((cp & 1) * 2 + (lane >> 4)) ^ ((vr >> 1) & 3)) << 4), b);
+#pragma unroll
+              for (int x = 0; x < 4; ++x) b[x] = __byte_perm(b[x], 0, 0x3120);      // even columns of two tokens, odd ones
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                pd_mma<true>(o[4 * cp + 2 * x], pa[ks], e4m3_to_f16(b[2 * x]), e4m3_to_f16(b[2 * x + 1]));
+                pd_mma<true>(o[4 * cp + 2 * x + 1], pa[ks], e4m3_to_f16(b[2 * x] >> 16), e4m3_to_f16(b[2 * x + 1] >> 16));
+              }
+            }
+        }
+      }
+      __syncwarp();                        // the stage is used up
+      if (alive && asked < units) ask();
+      if (++stage == ST) {
+        stage = 0;
+        parity ^= 1;
+      }
+    }
+
+    // ---- the warps' parts of this (sequence, head block) come together
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+    if (WIDE) {
+      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+    }
+    if (t == 0) {
+      s_ml[warp][g] = make_float2(m0, l0);
+      if (WIDE) s_ml[warp][g + 8] = make_float2(m1, l1);
+    }
+#pragma unroll
+    for (int hh = 0; hh < (WIDE ? 2 : 1); ++hh) {
+      const int r = g + 8 * hh;
+      if (r >= rows) continue;
+      float* dst = meet + (warp * R + r) * (DV + PD_PAD);
+      if constexpr (!F8) {
+#pragma unroll
+        for (int n = 0; n < DV / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8 + 2 * t) = make_float2(o[n][2 * hh], o[n][2 * hh + 1]);
+      } else {
+#pragma unroll
+        for (int n = 0; n < DV / 8; n += 2)
+          *reinterpret_cast<float4*>(dst + n * 8 + 4 * t) = make_float4(o[n][2 * hh], o[n + 1][2 * hh], o[n][2 * hh + 1], o[n + 1][2 * hh + 1]);
+      }
+    }
+    __syncthreads();
+    const int slot = 2 * blockIdx.x + (done > 0 ? 1 : 0);
+    for (int x = threadIdx.x; x < rows * (DV / 4); x += THREADS) {
+      const int r = x / (DV / 4), col = x % (DV / 4) * 4;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) top = fmaxf(top, s_ml[w][r].x);
+      float l = 0.f;
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float2 ml = s_ml[w][r];
+        const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
+        const float4 v = *reinterpret_cast<const float4*>(meet + (w * R + r) * (DV + PD_PAD) + col);
+        l += f * ml.y;
+        a.x += f * v.x; a.y += f * v.y; a.z += f * v.z; a.w += f * v.w;
+      }
+      if (whole) {
+        const float inv = 1.f / l;
+        uint2 u;
+        u.x = pack_bf16(a.x * inv, a.y * inv);
+        u.y = pack_bf16(a.z * inv, a.w * inv);
+        *reinterpret_cast<uint2*>(p.out + ((long long)c.b * p.Hkv * p.G + h0 + r) * DV + col) = u;
+      } else {
+        *reinterpret_cast<float4*>(p.part_o + ((long long)slot * 16 + r) * DV + col) = a;
+        if (col == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * 16 + r) * 2) = make_float2(top, l);
+      }
+    }
+    __syncthreads();
+    done += seg;
+    c.at += seg;
+    if (c.at == c.s.units) c.next_head(p, PER);
+  }
+}
+
+// One CTA per sequence and query head: joins the parts of a head whose units fell to several CTAs (the part that begins at a CTA's
+// first unit is in its slot 0, one that begins later in slot 1), writes zeros for a sequence of no visible token.
+template <int DV>
+__global__ void __launch_bounds__(128)
+paged_join_kernel(const PagedDecode p, int grid) {
+  if (!chain_begin()) return;
+  constexpr int COLS = DV / 4, SETS = 128 / COLS;
+  __shared__ float4 sums[SETS][COLS];
+  const int b = blockIdx.x, h = blockIdx.y, Hq = p.Hkv * p.G, HB = p.Hkv * p.blocks;
+  const int kv_head = h / p.G, in = h - kv_head * p.G, hb = kv_head * p.blocks + in / 16, r = in % 16;
+  const int n = p.start[b + 1] - p.start[b];
+  const int col = threadIdx.x % COLS, set = threadIdx.x / COLS, lane = threadIdx.x & 31;
+  uint2* dst = reinterpret_cast<uint2*>(p.out + ((long long)b * Hq + h) * DV) + col;
+  if (n == 0) {
+    if (set == 0) *dst = make_uint2(0, 0);
+    return;
+  }
+  const int share = max(1, (p.start[p.B] * HB + grid - 1) / grid);
+  const int a = p.start[b] * HB + hb * n, f = a / share, l = (a + n - 1) / share;
+  if (f == l) return;
+  auto slot = [&](int c) { return (2 * c + (c == f && a > f * share ? 1 : 0)) * 16 + r; };
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
+  float top = -INFINITY;
+  for (int c = f + lane; c <= l; c += 32) top = fmaxf(top, ml[slot(c)].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float sum = 0.f;
+  for (int c = f + lane; c <= l; c += 32) {
+    const float2 x = ml[slot(c)];
+    sum += x.x == -INFINITY ? 0.f * x.y : ex2_approx(x.x - top) * x.y;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int c = f + set; c <= l; c += SETS) {
+    const float m = ml[slot(c)].x, w = m == -INFINITY ? 0.f : ex2_approx(m - top);
+    const float4 v = *reinterpret_cast<const float4*>(p.part_o + (long long)slot(c) * DV + 4 * col);
+    acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
+  }
+  sums[set][col] = acc;
+  __syncthreads();
+  if (set == 0) {
+    for (int k = 1; k < SETS; ++k) {
+      const float4 v = sums[k][col];
+      acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+    }
+    const float inv = 1.f / sum;
+    *dst = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+  }
+}
+
+constexpr int PD_WARPS = 4;
+
+static int pd_grid(long long most_units) {
+  const long long sms = sm_count();
+  return (int)(most_units < 1 ? 1 : most_units < sms ? most_units : sms);
+}
+
+template <int DK, int DV, bool F8, bool WIDE>
+static int launch_paged_decode(PagedDecode p, int grid, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t stream) {
+  using T = PagedTile<DK, DV, F8>;
+  constexpr int NW = PD_WARPS, MOST = 227 * 1024 - 2048 - 1024;      // (static arrays; alignment)
+  const int meet = NW * (p.G < 16 ? p.G : 16) * (DV + PD_PAD) * 4;
+  p.stages = (MOST - meet) / (NW * (T::STAGE + T::SCALES + 8));
+  if (p.stages > 8) p.stages = 8;
+  const int smem = 1024 + NW * p.stages * (T::STAGE + T::SCALES + 8) + meet;
+  auto* f = paged_decode_kernel<DK, DV, F8, NW, WIDE>;
+  cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return 1000 + (int)e;
+  chain(f, grid, NW * 32, smem, stream, km, vm, p);
+  chain(paged_join_kernel<DV>, dim3(p.B, p.Hkv * p.G), 128, 0, stream, p, grid);
+  e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : 1000 + (int)e;
+}
+
+}  // namespace tpb
+
+using namespace tpb;
+
+// Bytes of scratch for tpb_paged_decode (B up to 2^24).
+extern "C" int tpb_paged_decode_scratch(int B, int Hkv, int G, int DV, int capacity) {
+  const long long units = (long long)B * Hkv * ((G + 15) / 16) * ((capacity + 127) / 128);
+  return pd_grid(units) * 2 * 16 * (DV + 2) * 4 + (B + 1) * 4;
+}
+
+// q [B, Hkv * G, DK] bf16 (strides q_b, q_h), pools as in tpb_paged_rows (strides of pages, tokens, heads; scales contiguous over
+// a page's tokens), table [B, table_width] with rows table_b apart, lengths [B]; out [B, Hkv * G, DV] bf16, contiguous.
+// window 0: none; softcap 0: none.  scratch: 16-byte aligned.
+extern "C" int tpb_paged_decode(const void* q, long long q_b, long long q_h, const void* k_pool, const void* v_pool,
+                                const void* k_scale, const void* v_scale, const long long* strides, const int* table, long long table_b,
+                                int table_width, const int* lengths, void* out, void* scratch, int B, int Hkv, int G, int DK, int DV,
+                                int pages, int page, int window, float scale, float softcap, void* stream_) {
+  const bool held8 = k_scale != nullptr;
+  const int elt = held8 ? 1 : 2;
+  if (B < 0 || B > (1 << 24) || Hkv < 1 || G < 1 || pages < 1 || page < 16 || page % 16 || window < 0 || table_width < 0 || softcap < 0.f) return -2;
+  if ((long long)pages * page > 0x7fffffffLL || (long long)Hkv * G > 65535) return -2;
+  if (held8 != (v_scale != nullptr)) return -2;
+  for (const void* a : {q, k_pool, v_pool, (const void*)out, (const void*)scratch, k_scale, v_scale})
+    if (reinterpret_cast<uintptr_t>(a) % 16) return -2;
+  if (q_b % 8 || q_h % 8) return -2;
+  for (int i = 0; i < 2; ++i) {
+    for (int j = 0; j < 3; ++j)
+      if (strides[6 * i + j] * elt % 16 || strides[6 * i + j] < 0) return -2;
+    if (held8 && (strides[6 * i + 3] % 16 || strides[6 * i + 4] != 1 || strides[6 * i + 5] % 16)) return -2;
+  }
+  if (B == 0) return 0;
+  long long capacity = (long long)table_width * page;
+  if (capacity > (long long)0x7fffff00) return -2;
+  const int blocks = (G + 15) / 16;
+  const long long units = (long long)B * Hkv * blocks * ((capacity + 127) / 128);
+  if (units > 0x3fffffffLL) return -2;
+  PagedDecode p = {};
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_b = q_b;
+  p.q_h = q_h;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.table = table;
+  p.table_b = table_b;
+  p.lengths = lengths;
+  p.k_scale = static_cast<const uint8_t*>(k_scale);
+  p.v_scale = static_cast<const uint8_t*>(v_scale);
+  p.ks_page = strides[3];
+  p.ks_head = strides[5];
+  p.vs_page = strides[9];
+  p.vs_head = strides[11];
+  const int grid = pd_grid(units);
+  p.part_o = static_cast<float*>(scratch);
+  p.part_ml = p.part_o + (long long)grid * 2 * 16 * DV;
+  p.start = reinterpret_cast<int*>(p.part_ml + (long long)grid * 2 * 16 * 2);
+  p.status = status_block();
+  p.B = B;
+  p.Hkv = Hkv;
+  p.G = G;
+  p.blocks = blocks;
+  p.pages = pages;
+  p.page = page;
+  p.capacity = (int)capacity;
+  p.window = window;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.cap_log2 = softcap * 1.4426950408889634f;
+  CUtensorMap km, vm;
+  if (make_tmap_pages(&km, k_pool, elt, DK, page, Hkv, pages, strides[1] * elt, strides[2] * elt, strides[0] * elt)) return -3;
+  if (make_tmap_pages(&vm, v_pool, elt, DV, page, Hkv, pages, strides[7] * elt, strides[8] * elt, strides[6] * elt)) return -4;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  const bool wide = G > 8;
+#define PD_CASE(dk, dv)                                                                                        \
+  if (DK == dk && DV == dv)                                                                                    \
+    return held8 ? (wide ? launch_paged_decode<dk, dv, true, true>(p, grid, km, vm, stream)                    \
+                         : launch_paged_decode<dk, dv, true, false>(p, grid, km, vm, stream))                  \
+                 : (wide ? launch_paged_decode<dk, dv, false, true>(p, grid, km, vm, stream)                   \
+                         : launch_paged_decode<dk, dv, false, false>(p, grid, km, vm, stream));
+  PD_CASE(128, 128)
+  PD_CASE(192, 128)
+  PD_CASE(64, 64)
+#undef PD_CASE
+  return -2;
+}

@@ -84,4 +84,21 @@ int make_tmap_out(CUtensorMap* map, const void* ptr, uint64_t cols, uint64_t row
   return r == CUDA_SUCCESS ? 0 : (int)r;
 }
 
+// Pools of a paged cache: 16 tokens of one page and head, all `d` columns, in blocks of 64 columns [d / 64][16 tokens][64].
+// Swizzle over a block's row: 128 bytes of bf16, 64 of 8-bit values.  Strides in bytes.
+int make_tmap_pages(CUtensorMap* map, const void* ptr, int elem_bytes, uint64_t d, uint64_t page, uint64_t heads, uint64_t pages,
+                    uint64_t row_stride, uint64_t head_stride, uint64_t page_stride) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return -1;
+  bind_context_once();
+  cuuint64_t dims[5] = {64, page, d / 64, heads, pages};
+  cuuint64_t strides[4] = {row_stride, (cuuint64_t)(64 * elem_bytes), head_stride, page_stride};
+  cuuint32_t box[5] = {64, 16, (cuuint32_t)(d / 64), 1, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  CUresult r = fn(map, elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(ptr), dims,
+                  strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, elem_bytes == 2 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : (int)r;
+}
+
 }  // namespace tpb

@@ -97,3 +97,52 @@ def test_refusals():
 def test_cache_bytes():
   c, q = PagedKV.allocate(4, 16, 2, 64), PagedKV.allocate(4, 16, 2, 64, dtype=E4M3)
   assert c.nbytes() == 4 * 16 * 2 * 128 * 2 and q.nbytes() == 4 * 16 * 2 * (128 + 2)
+
+
+# ----------------------------------------------------------------------------- attention over the pages
+def _dense(q, k, v, n, scale, window=0, softcap=0.0):
+  """One sequence against the plain attention definition: keys [S, H, D], the query after all of them."""
+  lo = max(0, n - window) if window else 0
+  return ref.attention(q[None, None], k[None, lo:n], v[None, lo:n], causal=False, scale=scale, softcap=softcap or None)[0, 0]
+
+
+@pytest.mark.parametrize("window,softcap", [(0, 0.0), (5, 0.0), (0, 3.0)])
+def test_decode_attention_is_attention_over_the_pages(window, softcap):
+  torch.manual_seed(2)
+  c = PagedKV.allocate(8, 16, 2, 24, 16, dtype=torch.float32)
+  c.k.fill_(float("nan"))
+  c.v.fill_(float("nan"))
+  lens = [40, 1, 0, 16]
+  table = torch.full((4, 3), 10 ** 6, dtype=torch.int32)
+  table[0], table[1, 0], table[3, 0] = torch.tensor([7, 2, 4]), 1, 6
+  q = torch.randn(4, 6, 24)
+  rows = {}
+  for b, n in enumerate(lens):
+    k, v = torch.randn(n, 2, 24), torch.randn(n, 2, 16)
+    pos = torch.arange(n)
+    paged_kv.append(c, k, v, table[b].long()[pos // 16] * 16 + pos % 16)
+    rows[b] = k, v
+  got = paged_kv.decode_attention(q, c, table, torch.tensor(lens, dtype=torch.int32), window=window, softcap=softcap)
+  for b, n in enumerate(lens):
+    want = _dense(q[b], *rows[b], n, 24 ** -0.5, window, softcap) if n else torch.zeros(6, 16)
+    assert torch.allclose(got[b], want, atol=1e-5)
+
+
+def test_decode_attention_refusals():
+  c = PagedKV.allocate(4, 16, 2, 8)
+  q, table, lens = torch.randn(3, 4, 8).bfloat16(), torch.zeros(3, 2, dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+  assert paged_kv.decode_attention(q, c, table, lens).shape == (3, 4, 8)
+  for bad in ((q[:, :3], c, table, lens), (q[..., :4], c, table, lens), (q, c, table[:2], lens), (q, c, table, lens[:2]),
+              (q, c, table.long(), lens), (q, c, table, lens.long()), (q[0], c, table, lens), (q[:, :0], c, table, lens)):
+    with pytest.raises(ValueError):
+      paged_kv.decode_attention(*bad)
+  for kw in ({"window": -1}, {"softcap": -2.0}, {"softcap": float("nan")}):
+    with pytest.raises(ValueError):
+      paged_kv.decode_attention(q, c, table, lens, **kw)
+
+
+def test_debug_mode_names_lengths_beyond_the_table(monkeypatch):
+  monkeypatch.setenv("TPB_DEBUG_BOUNDS", "1")
+  c = PagedKV.allocate(4, 16, 2, 8)
+  with pytest.raises(IndexError, match="lengths"):
+    paged_kv.decode_attention(torch.randn(1, 4, 8).bfloat16(), c, torch.zeros(1, 2, dtype=torch.int32), torch.tensor([33], dtype=torch.int32))

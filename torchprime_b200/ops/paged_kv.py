@@ -11,7 +11,7 @@ On CUDA/bf16 these run as sm_100a kernels; elsewhere the same math runs in plain
 
 from __future__ import annotations
 
-from ctypes import c_int, c_longlong, c_void_p
+from ctypes import c_float, c_int, c_longlong, c_void_p
 from typing import NamedTuple
 
 import torch
@@ -19,8 +19,10 @@ import torch
 from . import _debug, _lib, reference as ref
 from ._lib import check, lib, ptr, stream_ptr
 
-P, I, LL = c_void_p, c_int, c_longlong
+P, I, LL, F = c_void_p, c_int, c_longlong, c_float
 _lib.register_signature("tpb_paged_rows", [I, P, P, P, P, P, P, P, LL, I, I, I, I, I, P, P, P])
+_lib.register_signature("tpb_paged_decode_scratch", [I, I, I, I, I])
+_lib.register_signature("tpb_paged_decode", [P, LL, LL, P, P, P, P, P, P, LL, I, P, P, P, I, I, I, I, I, I, I, I, F, F, P])
 
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
@@ -137,3 +139,58 @@ def read(cache: PagedKV, slots, dtype=torch.bfloat16):
     _move(False, k, v, cache, slots.contiguous())
     return k, v
   return ref.paged_read(cache.k, cache.k_scale, slots).to(dtype), ref.paged_read(cache.v, cache.v_scale, slots).to(dtype)
+
+
+# ----------------------------------------------------------------------------- attention over the pages
+_DECODE_DIMS = ((128, 128), (192, 128), (64, 64))
+
+
+def _decode_ok(q, c: PagedKV) -> bool:
+  """What the attention kernel takes: see :func:`decode_attention`."""
+  return (c.page % 16 == 0 and c.k.shape[0] > 0 and (c.k.shape[3], c.v.shape[3]) in _DECODE_DIMS and q.shape[1] <= 65535 and q.shape[0] <= 1 << 24
+          and _rows_ok(c, c.k.shape[2], c.k.shape[3], c.v.shape[3])
+          and all(0 < s for t in c[:2] for s in t.stride()[:3])
+          and (c.k.dtype != E4M3 or all(s.stride(1) == 1 and s.stride(0) % 16 == 0 and s.stride(2) % 16 == 0 and s.data_ptr() % 16 == 0
+                                        for s in c[2:])))
+
+
+def decode_attention(q, cache: PagedKV, block_table, lengths, scale=None, window=None, softcap=None):
+  """softmax(q K^T * scale + mask) V for one token per sequence: q [B, Hq, Dk], Hq a multiple of the cache's heads, over the
+  ``lengths[b]`` tokens (int32) that ``block_table[b]`` (int32 [B, pages]) names, of which ``window`` leaves the last ones;
+  ``softcap`` makes scores ``softcap * tanh(score / softcap)``.  Returns [B, Hq, Dv] in q's type; a sequence of no token gives zeros.
+
+  The kernel takes bf16 queries, pools of bf16 or e4m3 whose pages are multiples of 16 tokens, and heads of 128, 192 / 128 or
+  64 columns.  It reads nothing of the table and of the pages behind a sequence's last token (what a page holds there may be
+  anything); a page outside the pool counts as zeros, a length beyond the table as the whole table, a negative one as none, and all three are
+  reported (``_lib.raise_on_device_timeout``)."""
+  from .functional import inference_only, use_kernels
+  _check_cache(cache)
+  if q.dim() != 3 or q.shape[2] != cache.k.shape[3] or q.shape[1] % cache.k.shape[2] or q.shape[1] == 0:
+    raise ValueError(f"decode_attention: queries {tuple(q.shape)} over keys {tuple(cache.k.shape)}")
+  b, hq, dk = q.shape
+  if block_table.dim() != 2 or block_table.shape[0] != b or lengths.shape != (b,):
+    raise ValueError(f"decode_attention: block_table {tuple(block_table.shape)} and lengths {tuple(lengths.shape)} for {b} sequences")
+  if block_table.dtype != torch.int32 or lengths.dtype != torch.int32:
+    raise ValueError("decode_attention: block_table and lengths must be int32")
+  if any(t.device != cache.k.device for t in (q, block_table, lengths)):
+    raise ValueError("decode_attention: queries, block_table and lengths must be on the cache's device")
+  window, softcap = int(window or 0), float(softcap or 0.0)
+  if window < 0 or not softcap >= 0.0:
+    raise ValueError(f"decode_attention: window {window}, softcap {softcap}")
+  scale = float(scale) if scale is not None else dk ** -0.5
+  _debug.check_index("decode_attention", "lengths", lengths, 0, block_table.shape[1] * cache.page + 1)
+  if (use_kernels(q) and q.is_cuda and _decode_ok(q, cache) and (inference_only() or not q.requires_grad)):
+    q = _vectors(q)
+    block_table = block_table if block_table.stride(1) == 1 else block_table.contiguous()
+    pages, page, hkv, _ = cache.k.shape
+    dv, width = cache.v.shape[3], block_table.shape[1]
+    out = torch.empty(b, hq, dv, dtype=q.dtype, device=q.device)
+    with torch.cuda.device(q.device):
+      n = lib().tpb_paged_decode_scratch(b, hkv, hq // hkv, dv, width * page)
+      scratch = torch.empty(n, dtype=torch.uint8, device=q.device)
+      rc = lib().tpb_paged_decode(ptr(q), q.stride(0), q.stride(1), ptr(cache.k), ptr(cache.v), ptr(cache.k_scale), ptr(cache.v_scale),
+                                  _c_strides(cache), ptr(block_table), block_table.stride(0), width, ptr(lengths.contiguous()), ptr(out),
+                                  ptr(scratch), b, hkv, hq // hkv, dk, dv, pages, page, window, scale, softcap, stream_ptr())
+    check(rc, f"paged_decode q{tuple(q.shape)} pool{tuple(cache.k.shape)}")
+    return out
+  return ref.paged_attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, lengths, scale, window, softcap)

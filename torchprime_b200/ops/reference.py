@@ -284,3 +284,24 @@ def paged_read(pool, scale, slots):
     e = scale.view(torch.uint8)[at].to(torch.int32) - 127
     rows = pool.view(torch.uint8)[at].view(torch.float8_e4m3fn).float() * power_of_two(e)[..., None]
   return torch.where(inside[..., None, None], rows, torch.zeros_like(rows))
+
+
+def paged_attention(q, k_pool, v_pool, k_scale, v_scale, block_table, lengths, scale, window=0, softcap=0.0):
+  """One token per sequence: q [B, Hq, D] over the first ``lengths`` [B] tokens of the pages ``block_table`` [B, pages], the last
+  ``window`` of them if it is not 0.  Rows that cannot be seen may hold anything.  fp32; zeros for sequences of no token."""
+  b, hq, d = q.shape
+  page, hkv = k_pool.shape[1], k_pool.shape[2]
+  pos = torch.arange(block_table.shape[1] * page, device=q.device)
+  n = lengths.long().clamp(0, pos.numel())[:, None]
+  seen = pos[None] < n
+  if window:
+    seen = seen & (pos[None] >= n - window)
+  slots = torch.where(seen, block_table.long()[:, torch.div(pos, page, rounding_mode="floor")] * page + pos % page, -1)
+  rows = lambda pool, sc: torch.where(seen[..., None, None], paged_read(pool, sc, slots), 0).float()  # noqa: E731
+  s = torch.einsum("bhgd,bshd->bhgs", q.float().view(b, hkv, hq // hkv, d), rows(k_pool, k_scale)) * scale
+  if softcap:
+    s = softcap * torch.tanh(s / softcap)
+  s = s.masked_fill(~seen[:, None, None], float("-inf"))
+  p = torch.softmax(s, dim=-1)
+  p = torch.where((n > 0)[:, None, None], p, torch.zeros_like(p))
+  return torch.einsum("bhgs,bshd->bhgd", p, rows(v_pool, v_scale)).reshape(b, hq, -1).to(q.dtype)
