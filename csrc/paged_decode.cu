@@ -6,15 +6,15 @@
 // Every cached row is read once per 16 query heads that share it: 2 * 16 operations a byte at most, so memory bounds it, and
 // what the kernel is built for is to keep loads under way on every SM from the first to the last token.
 //
-// * The work is cut into units: the rows of one sequence, one key head and up to 16 of its query heads, NW * 32 tokens.  In the
-//   order sequence, head, token they form one list, of which every CTA (one per SM) takes an equal, contiguous part; how long the
-//   sequences are only the device knows, so each CTA adds up the lengths itself.  A (sequence, head) whose units fall to
-//   several CTAs is joined by paged_join_kernel from their running maxima, sums and unnormalised results; a CTA has at most
+// * The work is cut into steps: 32 tokens of one sequence, for one key head and up to 16 of its query heads.  In the order
+//   sequence, head, token they form one list, of which every WARP of the grid (one CTA per SM) takes an equal, contiguous part;
+//   how long the sequences are only the device knows, so each CTA adds up the lengths itself.  A (sequence, head) whose steps fall to
+//   several warps is joined by paged_join_kernel from their running maxima, sums and unnormalised results; a warp has at most
 //   two of those, so the scratch is bounded by the grid and not by the batch.  Nothing is added by atomics: the order of every
-//   sum follows from the lengths.
-// * A warp takes 32 tokens of each unit by itself: a ring of stages of its own, filled by TMA boxes of 16 tokens (a page is a
-//   multiple of 16) that its elected lane asks for as soon as it has used a stage up, across the borders of sequences.  The warps
-//   of a CTA meet only where a (sequence, head) ends.
+//   sum follows from the lengths.  (Eight warps sharing units of 256 tokens met in a block barrier wherever a sequence ended: 24
+//   sequences of up to 3001 tokens, 16 heads of 192 / 128 in e4m3, 69 us, the SMs idle for half of it.)
+// * A warp has a ring of stages of its own, filled by TMA boxes of 16 tokens (a page is a multiple of 16) that its elected lane asks
+//   for as soon as it has used a stage up, across the borders of sequences.  Warps never wait for one another.
 // * Scores and weighted sums are mma.sync m16n8k16: the query heads of a key head are its 16 rows.  (A tcgen05 tile would be
 //   seven eighths empty, and its operands would still come through shared memory once.)  Statistics and sums are fp32; the
 //   weights of the sum are rounded to the operand type of the product, half a step of 2^-9 (bf16) or 2^-12 (f16) each, to
@@ -43,18 +43,17 @@ struct PagedDecode {
   const int* lengths;
   const uint8_t *k_scale, *v_scale;        // a row's scales are contiguous within a page
   long long ks_page, ks_head, vs_page, vs_head;
-  float* part_o;                           // [2 * grid][16][DV]
-  float* part_ml;                          // [2 * grid][16][2]: running maximum in log2 units, sum
-  int* start;                              // [B + 1]: units of the sequences before, per head block
+  float* part_o;                           // [2 * warps of the grid][rows][DV]
+  float* part_ml;                          // [2 * warps of the grid][rows][2]: running maximum in log2 units, sum
+  int* start;                              // [B + 1]: steps of the sequences before, per head block
   int* status;
-  int B, Hkv, G, blocks;                   // blocks of up to 16 query heads to a key head
+  int B, Hkv, G, blocks, rows;             // blocks of up to 16 query heads to a key head; rows of the largest block
   int pages, page, capacity;               // tokens that a row of the table can name
   int window, stages;
   float scale_log2, cap_log2;              // cap_log2: the cap in log2 units, 0 for none
 };
 
 constexpr int PD_KEYS = 32;                // tokens of a warp's step, two boxes
-constexpr int PD_PAD = 8;                  // floats between rows where the warps meet: no two rows of a quad in one bank
 
 template <int DK, int DV, bool F8>
 struct PagedTile {
@@ -64,6 +63,9 @@ struct PagedTile {
   static constexpr int K_BOX = 16 * DK * ELT, V_BOX = 16 * DV * ELT;
   static constexpr int STAGE = 2 * (K_BOX + V_BOX);
   static constexpr int SCALES = F8 ? 64 : 0;                 // 32 of the keys, 32 of the values
+  // Warps to a CTA: as many as have two stages or more each, up to eight.  An 8-bit cache brings a step's bytes in half the time,
+  // and the step takes longer (conversions): four warps 159 us for 64 sequences of up to 8192 tokens, 64 / 8 heads of 128; eight 118.
+  static constexpr int WARPS = STAGE <= 10240 ? 8 : 4;
 };
 
 __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int row, int head, int page) {
@@ -110,50 +112,52 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return r;
 }
 
-// What is visible of a sequence, in tokens and in units of `per` tokens.
+// What is visible of a sequence, in tokens and in steps.
 struct Visible {
-  int len, lo, first, units;
+  int len, lo, first, steps;
 };
-__device__ __forceinline__ Visible pd_visible(const PagedDecode& p, int b, int per) {
+__device__ __forceinline__ Visible pd_visible(const PagedDecode& p, int b) {
   Visible s;
   s.len = min(max(p.lengths[b], 0), p.capacity);
   s.lo = p.window > 0 ? max(0, s.len - p.window) : 0;
-  s.first = s.lo / per;
-  s.units = s.len > 0 ? (s.len - 1) / per - s.first + 1 : 0;
+  s.first = s.lo / PD_KEYS;
+  s.steps = s.len > 0 ? (s.len - 1) / PD_KEYS - s.first + 1 : 0;
   return s;
 }
 
-// A place in the list of units.
+// Steps of each of `warps` warps.
+__device__ __forceinline__ int pd_share(int steps, int warps) { return max(1, (steps + warps - 1) / warps); }
+
+// A place in the list of steps.
 struct PagedCursor {
-  int b, hb, at;           // sequence, head block, unit of the sequence
+  int b, hb, at;           // sequence, head block, step of the sequence
   Visible s;
-  __device__ __forceinline__ void next_head(const PagedDecode& p, int per) {
+  __device__ __forceinline__ int key0() const { return (s.first + at) * PD_KEYS; }
+  __device__ __forceinline__ void next_head(const PagedDecode& p) {
     at = 0;
     if (++hb < p.Hkv * p.blocks) return;
     hb = 0;
     do {
       ++b;
       if (b >= p.B) return;
-      s = pd_visible(p, b, per);
-    } while (s.units == 0);
+      s = pd_visible(p, b);
+    } while (s.steps == 0);
   }
 };
 
-template <int DK, int DV, bool F8, int NW, bool WIDE>
-__global__ void __launch_bounds__(NW * 32, 1)
+template <int DK, int DV, bool F8, bool WIDE>
+__global__ void __launch_bounds__(PagedTile<DK, DV, F8>::WARPS * 32, 1)
 paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const PagedDecode p) {
   using T = PagedTile<DK, DV, F8>;
-  constexpr int PER = NW * PD_KEYS, THREADS = NW * 32;
+  constexpr int NW = T::WARPS, THREADS = NW * 32;
   extern __shared__ uint8_t pd_smem_raw[];
   uint8_t* pd_smem = pd_smem_raw + ((1024u - (smem_u32(pd_smem_raw) & 1023u)) & 1023u);
-  __shared__ int s_scan[NW], s_at[4];
-  __shared__ float2 s_ml[NW][16];
+  __shared__ int s_scan[NW], s_at[NW][3];
   const int warp = warp_index(), lane = threadIdx.x & 31, ST = p.stages;
-  const int HB = p.Hkv * p.blocks, R = min(16, p.G);
+  const int HB = p.Hkv * p.blocks;
   uint8_t* ring = pd_smem + (size_t)warp * ST * T::STAGE;
   uint8_t* scales = pd_smem + (size_t)NW * ST * T::STAGE + (size_t)warp * ST * T::SCALES;
-  float* meet = reinterpret_cast<float*>(pd_smem + (size_t)NW * ST * (T::STAGE + T::SCALES));     // [NW][R][DV + PD_PAD]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(meet + NW * R * (DV + PD_PAD)) + warp * ST;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(pd_smem + (size_t)NW * ST * (T::STAGE + T::SCALES)) + warp * ST;
   const uint32_t ring_at = smem_u32(ring), scales_at = smem_u32(scales);
   if (lane == 0)
     for (int i = 0; i < ST; ++i) mbar_init(&bars[i], 1);
@@ -165,12 +169,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   chain_launch();
   if (!chain_wait()) return;
 
-  // The list's length, and where this CTA's part begins.
-  int total = 0, share = 1, first = 0, last = 0;
+  // The list's length, and where the warps' parts begin.  Neighbours in the list are on different SMs: few steps use all of them.
+  int total = 0, share = 1;
   for (int pass = 0; pass < 2; ++pass) {
     int running = 0;
     for (int base = 0; base < p.B; base += THREADS) {
-      const int b = base + threadIdx.x, n = b < p.B ? pd_visible(p, b, PER).units : 0;
+      const int b = base + threadIdx.x, n = b < p.B ? pd_visible(p, b).steps : 0;
       int sum = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -192,75 +196,85 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
           p.start[b] = before;
           if (p.lengths[b] < 0 || p.lengths[b] > p.capacity) report(p.status, kBadArgument, 71);
         }
-      } else if (before * HB <= first && first < (before + n) * HB) {
-        s_at[0] = b;
-        s_at[1] = (first - before * HB) / n;
-        s_at[2] = (first - before * HB) % n;
+      } else if (n > 0) {
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const int in = (w * (int)gridDim.x + (int)blockIdx.x) * share - before * HB;
+          if (in >= 0 && in < n * HB) {
+            s_at[w][0] = b;
+            s_at[w][1] = in / n;
+            s_at[w][2] = in % n;
+          }
+        }
       }
       running += all;
     }
     if (pass == 0) {
-      total = running;
-      if (blockIdx.x == 0 && threadIdx.x == 0) p.start[p.B] = total;
-      share = max(1, (total * HB + (int)gridDim.x - 1) / (int)gridDim.x);
-      first = blockIdx.x * share;
-      last = min(total * HB, first + share);
-      if (first >= last) return;
+      total = running * HB;
+      if (blockIdx.x == 0 && threadIdx.x == 0) p.start[p.B] = running;
+      share = pd_share(total, gridDim.x * NW);
     }
   }
   __syncthreads();
-  PagedCursor c = {s_at[0], s_at[1], s_at[2], {}};
-  c.s = pd_visible(p, c.b, PER);
+  const int part = warp * gridDim.x + blockIdx.x;
+  const int steps = min(share, total - part * share);
+  if (steps <= 0) return;
+  PagedCursor c = {s_at[warp][0], s_at[warp][1], s_at[warp][2], {}};
+  c.s = pd_visible(p, c.b);
   PagedCursor ahead = c;
-  const int units = last - first;
   int asked = 0, ask_stage = 0, stage = 0, parity = 0;
   bool alive = true;
+  // The pages of the step that is asked for next, on their way from the table since the one before was.
+  int pg0 = -1, pg1 = -1, row0_next = 0, row1_next = 0;
+  auto look_up = [&]() {
+    const int key0 = ahead.key0();
+    const int* row = p.table + ahead.b * p.table_b;
+    const unsigned at0 = (unsigned)key0 / (unsigned)p.page, at1 = (unsigned)(key0 + 16) / (unsigned)p.page;
+    row0_next = key0 - at0 * p.page;
+    row1_next = key0 + 16 - at1 * p.page;
+    pg0 = row[at0];
+    if (key0 + 16 < ahead.s.len) pg1 = row[at1];
+  };
+  look_up();
 
   auto ask = [&]() {
-    const int key0 = (ahead.s.first + ahead.at) * PER + warp * PD_KEYS;
     uint64_t* bar = &bars[ask_stage];
-    if (key0 < ahead.s.len && key0 + PD_KEYS > ahead.s.lo) {
-      const int boxes = key0 + 16 < ahead.s.len ? 2 : 1, head = ahead.hb / p.blocks;
-      int pg[2], row[2];
-      uint32_t bytes = 0;
-      for (int i = 0; i < boxes; ++i) {
-        const unsigned key = key0 + 16 * i, at = key / (unsigned)p.page;
-        row[i] = key - at * p.page;
-        pg[i] = p.table[ahead.b * p.table_b + at];
-        const bool inside = pg[i] >= 0 && pg[i] < p.pages;
-        if (!inside) {                     // a box outside the pool reads as zeros
-          if (lane == 0) report(p.status, kBadArgument, 72);
-          pg[i] = -1;
-        }
-        bytes += T::K_BOX + T::V_BOX + (F8 && inside ? 32 : 0);
+    const int boxes = ahead.key0() + 16 < ahead.s.len ? 2 : 1, head = ahead.hb / p.blocks;
+    int pg[2] = {pg0, pg1}, row[2] = {row0_next, row1_next};
+    uint32_t bytes = 0;
+    for (int i = 0; i < boxes; ++i) {
+      const bool inside = pg[i] >= 0 && pg[i] < p.pages;
+      if (!inside) {                       // a box outside the pool reads as zeros
+        if (lane == 0) report(p.status, kBadArgument, 72);
+        pg[i] = -1;
       }
-      one_lane([&]() {
-        mbar_expect_tx(bar, bytes);
-        const uint32_t at = ring_at + ask_stage * T::STAGE;
-        for (int i = 0; i < boxes; ++i) {
-          tma_load_page(at + i * T::K_BOX, &k_map, bar, row[i], head, pg[i]);
-          tma_load_page(at + 2 * T::K_BOX + i * T::V_BOX, &v_map, bar, row[i], head, pg[i]);
-          if (F8 && pg[i] >= 0) {
-            const uint32_t sc = scales_at + ask_stage * T::SCALES + i * 16;
-            bulk_load_16(sc, p.k_scale + pg[i] * p.ks_page + head * p.ks_head + row[i], bar);
-            bulk_load_16(sc + 32, p.v_scale + pg[i] * p.vs_page + head * p.vs_head + row[i], bar);
-          }
-        }
-      });
-    } else {
-      one_lane([&]() { mbar_arrive(bar); });
+      bytes += T::K_BOX + T::V_BOX + (F8 && inside ? 32 : 0);
     }
+    one_lane([&]() {
+      mbar_expect_tx(bar, bytes);
+      const uint32_t at = ring_at + ask_stage * T::STAGE;
+      for (int i = 0; i < boxes; ++i) {
+        tma_load_page(at + i * T::K_BOX, &k_map, bar, row[i], head, pg[i]);
+        tma_load_page(at + 2 * T::K_BOX + i * T::V_BOX, &v_map, bar, row[i], head, pg[i]);
+        if (F8 && pg[i] >= 0) {
+          const uint32_t sc = scales_at + ask_stage * T::SCALES + i * 16;
+          bulk_load_16(sc, p.k_scale + pg[i] * p.ks_page + head * p.ks_head + row[i], bar);
+          bulk_load_16(sc + 32, p.v_scale + pg[i] * p.vs_page + head * p.vs_head + row[i], bar);
+        }
+      }
+    });
     ++asked;
     if (++ask_stage == ST) ask_stage = 0;
-    if (++ahead.at == ahead.s.units) ahead.next_head(p, PER);
+    if (++ahead.at == ahead.s.steps) ahead.next_head(p);
+    if (asked < steps) look_up();
   };
-  while (asked < units && asked < ST) ask();
+  while (asked < steps && asked < ST) ask();
 
   const int g = lane >> 2, t = lane & 3;
   int done = 0;
-  while (done < units) {
-    const int seg = min(units - done, c.s.units - c.at);
-    const bool whole = seg == c.s.units;
+  while (done < steps) {
+    const int seg = min(steps - done, c.s.steps - c.at);
+    const bool whole = seg == c.s.steps;
     const int kv_head = c.hb / p.blocks, row0 = (c.hb - kv_head * p.blocks) * 16, rows = min(16, p.G - row0);
     const int h0 = kv_head * p.G + row0;
     // ---- the queries as A operands
@@ -312,9 +326,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 
     for (int i = 0; i < seg; ++i) {
-      const int key0 = (c.s.first + c.at + i) * PER + warp * PD_KEYS;
+      const int key0 = c.key0() + i * PD_KEYS;
       if (done + i < asked && !mbar_wait_warp(&bars[stage], parity, p.status, kTimeoutTmaFull, 73)) alive = false;
-      if (alive && key0 < c.s.len && key0 + PD_KEYS > c.s.lo) {
+      if (alive) {
         const uint32_t k_at = ring_at + stage * T::STAGE, v_at = k_at + 2 * T::K_BOX;
         const bool edge = key0 < c.s.lo || key0 + PD_KEYS > c.s.len;
         if (edge) {
@@ -445,78 +459,62 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         }
       }
       __syncwarp();                        // the stage is used up
-      if (alive && asked < units) ask();
+      if (alive && asked < steps) ask();
       if (++stage == ST) {
         stage = 0;
         parity ^= 1;
       }
     }
 
-    // ---- the warps' parts of this (sequence, head block) come together
+    // ---- the result, or this warp's part of it
     l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
     l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
     if (WIDE) {
       l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
       l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
     }
-    if (t == 0) {
-      s_ml[warp][g] = make_float2(m0, l0);
-      if (WIDE) s_ml[warp][g + 8] = make_float2(m1, l1);
-    }
+    const int slot = (2 * part + (done > 0 ? 1 : 0)) * p.rows;
 #pragma unroll
     for (int hh = 0; hh < (WIDE ? 2 : 1); ++hh) {
       const int r = g + 8 * hh;
       if (r >= rows) continue;
-      float* dst = meet + (warp * R + r) * (DV + PD_PAD);
-      if constexpr (!F8) {
-#pragma unroll
-        for (int n = 0; n < DV / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8 + 2 * t) = make_float2(o[n][2 * hh], o[n][2 * hh + 1]);
-      } else {
-#pragma unroll
-        for (int n = 0; n < DV / 8; n += 2)
-          *reinterpret_cast<float4*>(dst + n * 8 + 4 * t) = make_float4(o[n][2 * hh], o[n + 1][2 * hh], o[n][2 * hh + 1], o[n + 1][2 * hh + 1]);
-      }
-    }
-    __syncthreads();
-    const int slot = 2 * blockIdx.x + (done > 0 ? 1 : 0);
-    for (int x = threadIdx.x; x < rows * (DV / 4); x += THREADS) {
-      const int r = x / (DV / 4), col = x % (DV / 4) * 4;
-      float top = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < NW; ++w) top = fmaxf(top, s_ml[w][r].x);
-      float l = 0.f;
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const float2 ml = s_ml[w][r];
-        const float f = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
-        const float4 v = *reinterpret_cast<const float4*>(meet + (w * R + r) * (DV + PD_PAD) + col);
-        l += f * ml.y;
-        a.x += f * v.x; a.y += f * v.y; a.z += f * v.z; a.w += f * v.w;
-      }
       if (whole) {
-        const float inv = 1.f / l;
-        uint2 u;
-        u.x = pack_bf16(a.x * inv, a.y * inv);
-        u.y = pack_bf16(a.z * inv, a.w * inv);
-        *reinterpret_cast<uint2*>(p.out + ((long long)c.b * p.Hkv * p.G + h0 + r) * DV + col) = u;
+        const float inv = 1.f / (hh ? l1 : l0);
+        __nv_bfloat16* dst = p.out + ((long long)c.b * p.Hkv * p.G + h0 + r) * DV;
+        if constexpr (!F8) {
+#pragma unroll
+          for (int n = 0; n < DV / 8; ++n)
+            *reinterpret_cast<uint32_t*>(dst + n * 8 + 2 * t) = pack_bf16(o[n][2 * hh] * inv, o[n][2 * hh + 1] * inv);
+        } else {
+#pragma unroll
+          for (int n = 0; n < DV / 8; n += 2)
+            *reinterpret_cast<uint2*>(dst + n * 8 + 4 * t) = make_uint2(pack_bf16(o[n][2 * hh] * inv, o[n + 1][2 * hh] * inv),
+                                                                        pack_bf16(o[n][2 * hh + 1] * inv, o[n + 1][2 * hh + 1] * inv));
+        }
       } else {
-        *reinterpret_cast<float4*>(p.part_o + ((long long)slot * 16 + r) * DV + col) = a;
-        if (col == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * 16 + r) * 2) = make_float2(top, l);
+        float* dst = p.part_o + (long long)(slot + r) * DV;
+        if constexpr (!F8) {
+#pragma unroll
+          for (int n = 0; n < DV / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8 + 2 * t) = make_float2(o[n][2 * hh], o[n][2 * hh + 1]);
+        } else {
+#pragma unroll
+          for (int n = 0; n < DV / 8; n += 2)
+            *reinterpret_cast<float4*>(dst + n * 8 + 4 * t) = make_float4(o[n][2 * hh], o[n + 1][2 * hh], o[n][2 * hh + 1], o[n + 1][2 * hh + 1]);
+        }
+        if (t == 0) *reinterpret_cast<float2*>(p.part_ml + (slot + r) * 2) = make_float2(hh ? m1 : m0, hh ? l1 : l0);
       }
     }
-    __syncthreads();
     done += seg;
     c.at += seg;
-    if (c.at == c.s.units) c.next_head(p, PER);
+    if (c.at == c.s.steps) c.next_head(p);
   }
 }
 
-// One CTA per sequence and query head: joins the parts of a head whose units fell to several CTAs (the part that begins at a CTA's
-// first unit is in its slot 0, one that begins later in slot 1), writes zeros for a sequence of no visible token.
+// One CTA per sequence and query head: joins the parts of a head whose steps fell to several warps (the part that begins at a
+// warp's first step is in its slot 0, one that begins later in slot 1), writes zeros for a sequence of no visible token.
 template <int DV>
 __global__ void __launch_bounds__(128)
-paged_join_kernel(const PagedDecode p, int grid) {
+paged_join_kernel(const PagedDecode p, int warps) {
   if (!chain_begin()) return;
   constexpr int COLS = DV / 4, SETS = 128 / COLS;
   __shared__ float4 sums[SETS][COLS];
@@ -529,10 +527,10 @@ paged_join_kernel(const PagedDecode p, int grid) {
     if (set == 0) *dst = make_uint2(0, 0);
     return;
   }
-  const int share = max(1, (p.start[p.B] * HB + grid - 1) / grid);
+  const int share = pd_share(p.start[p.B] * HB, warps);
   const int a = p.start[b] * HB + hb * n, f = a / share, l = (a + n - 1) / share;
   if (f == l) return;
-  auto slot = [&](int c) { return (2 * c + (c == f && a > f * share ? 1 : 0)) * 16 + r; };
+  auto slot = [&](int c) { return (2 * c + (c == f && a > f * share ? 1 : 0)) * p.rows + r; };
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
   float top = -INFINITY;
   for (int c = f + lane; c <= l; c += 32) top = fmaxf(top, ml[slot(c)].x);
@@ -564,26 +562,24 @@ paged_join_kernel(const PagedDecode p, int grid) {
   }
 }
 
-constexpr int PD_WARPS = 4;
-
-static int pd_grid(long long most_units) {
+static int pd_warps(int DK, int DV, bool held8) { return 64 * (DK + DV) / (held8 ? 2 : 1) <= 10240 ? 8 : 4; }
+static int pd_grid(long long most_steps) {
   const long long sms = sm_count();
-  return (int)(most_units < 1 ? 1 : most_units < sms ? most_units : sms);
+  return (int)(most_steps < 1 ? 1 : most_steps < sms ? most_steps : sms);
 }
 
 template <int DK, int DV, bool F8, bool WIDE>
 static int launch_paged_decode(PagedDecode p, int grid, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t stream) {
   using T = PagedTile<DK, DV, F8>;
-  constexpr int NW = PD_WARPS, MOST = 227 * 1024 - 2048 - 1024;      // (static arrays; alignment)
-  const int meet = NW * (p.G < 16 ? p.G : 16) * (DV + PD_PAD) * 4;
-  p.stages = (MOST - meet) / (NW * (T::STAGE + T::SCALES + 8));
+  constexpr int MOST = 227 * 1024 - 1024 - 1024;      // (static arrays; alignment)
+  p.stages = MOST / (T::WARPS * (T::STAGE + T::SCALES + 8));
   if (p.stages > 8) p.stages = 8;
-  const int smem = 1024 + NW * p.stages * (T::STAGE + T::SCALES + 8) + meet;
-  auto* f = paged_decode_kernel<DK, DV, F8, NW, WIDE>;
+  const int smem = 1024 + T::WARPS * p.stages * (T::STAGE + T::SCALES + 8);
+  auto* f = paged_decode_kernel<DK, DV, F8, WIDE>;
   cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return 1000 + (int)e;
-  chain(f, grid, NW * 32, smem, stream, km, vm, p);
-  chain(paged_join_kernel<DV>, dim3(p.B, p.Hkv * p.G), 128, 0, stream, p, grid);
+  chain(f, grid, T::WARPS * 32, smem, stream, km, vm, p);
+  chain(paged_join_kernel<DV>, dim3(p.B, p.Hkv * p.G), 128, 0, stream, p, grid * T::WARPS);
   e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 1000 + (int)e;
 }
@@ -593,9 +589,9 @@ static int launch_paged_decode(PagedDecode p, int grid, const CUtensorMap& km, c
 using namespace tpb;
 
 // Bytes of scratch for tpb_paged_decode (B up to 2^24).
-extern "C" int tpb_paged_decode_scratch(int B, int Hkv, int G, int DV, int capacity) {
-  const long long units = (long long)B * Hkv * ((G + 15) / 16) * ((capacity + 127) / 128);
-  return pd_grid(units) * 2 * 16 * (DV + 2) * 4 + (B + 1) * 4;
+extern "C" int tpb_paged_decode_scratch(int B, int Hkv, int G, int DK, int DV, int held8, int capacity) {
+  const long long steps = (long long)B * Hkv * ((G + 15) / 16) * (((long long)capacity + PD_KEYS - 1) / PD_KEYS);
+  return pd_grid(steps) * pd_warps(DK, DV, held8 != 0) * 2 * (G < 16 ? G : 16) * (DV + 2) * 4 + (B + 1) * 4;
 }
 
 // q [B, Hkv * G, DK] bf16 (strides q_b, q_h), pools as in tpb_paged_rows (strides of pages, tokens, heads; scales contiguous over
@@ -622,8 +618,8 @@ extern "C" int tpb_paged_decode(const void* q, long long q_b, long long q_h, con
   long long capacity = (long long)table_width * page;
   if (capacity > (long long)0x7fffff00) return -2;
   const int blocks = (G + 15) / 16;
-  const long long units = (long long)B * Hkv * blocks * ((capacity + 127) / 128);
-  if (units > 0x3fffffffLL) return -2;
+  const long long steps = (long long)B * Hkv * blocks * ((capacity + PD_KEYS - 1) / PD_KEYS);
+  if (steps > 0x3fffffffLL) return -2;
   PagedDecode p = {};
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.q_b = q_b;
@@ -638,10 +634,12 @@ extern "C" int tpb_paged_decode(const void* q, long long q_b, long long q_h, con
   p.ks_head = strides[5];
   p.vs_page = strides[9];
   p.vs_head = strides[11];
-  const int grid = pd_grid(units);
+  const int grid = pd_grid(steps);
+  p.rows = G < 16 ? G : 16;
+  const long long part_rows = (long long)grid * pd_warps(DK, DV, held8) * 2 * p.rows;
   p.part_o = static_cast<float*>(scratch);
-  p.part_ml = p.part_o + (long long)grid * 2 * 16 * DV;
-  p.start = reinterpret_cast<int*>(p.part_ml + (long long)grid * 2 * 16 * 2);
+  p.part_ml = p.part_o + part_rows * DV;
+  p.start = reinterpret_cast<int*>(p.part_ml + part_rows * 2);
   p.status = status_block();
   p.B = B;
   p.Hkv = Hkv;

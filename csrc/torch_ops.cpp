@@ -1052,6 +1052,121 @@ py::object grouped_mlp_few_rows(py::handle x_, py::handle rw_, py::handle idx_, 
   return py::cast(y);
 }
 
+// The pools of a paged cache and, where they are e4m3, their scales: layouts that the kernels take, on the current device; see
+// paged_kv.PagedKV.
+struct Pools {
+  Tensor k, v, ks, vs;
+  int64_t pages = 0, page = 0, heads = 0, dk = 0, dv = 0;
+  long long strides[12] = {};
+  bool held8 = false;
+
+  bool take(py::handle k_, py::handle v_, py::handle ks_, py::handle vs_) {
+    if (!unpack(k_, k) || !unpack(v_, v) || !unpack(ks_, ks) || !unpack(vs_, vs) || !k.defined() || !v.defined()) return false;
+    held8 = k.scalar_type() == at::kFloat8_e4m3fn;
+    const auto type = held8 ? at::kFloat8_e4m3fn : at::kBFloat16;
+    if (!plain(k, type) || !plain(v, type) || k.dim() != 4 || v.dim() != 4 || k.get_device() != c10::cuda::current_device() ||
+        v.get_device() != k.get_device() || held8 != ks.defined() || held8 != vs.defined())
+      return false;
+    pages = k.size(0), page = k.size(1), heads = k.size(2), dk = k.size(3), dv = v.size(3);
+    if (v.size(0) != pages || v.size(1) != page || v.size(2) != heads || page < 1 || heads < 1 || pages * page > 0x7fffffff) return false;
+    const int64_t unit = held8 ? 16 : 8;
+    for (int i = 0; i < 2; ++i) {
+      const Tensor &t = i ? v : k, &s = i ? vs : ks;
+      const int64_t d = t.size(3);
+      if (d < 8 || d > 512 || d % unit || t.stride(3) != 1 || !aligned(t)) return false;
+      for (int j = 0; j < 3; ++j) {
+        if (t.stride(j) % unit) return false;
+        strides[6 * i + j] = t.stride(j);
+      }
+      if (!held8) continue;
+      if (!plain(s, at::kFloat8_e8m0fnu) || s.dim() != 3 || s.get_device() != k.get_device() || s.size(0) != pages || s.size(1) != page ||
+          s.size(2) != heads)
+        return false;
+      for (int j = 0; j < 3; ++j) strides[6 * i + 3 + j] = s.stride(j);
+    }
+    return true;
+  }
+  bool rows(const Tensor& x, int64_t t, int64_t d) const {     // [t, heads, d] as the kernel reads it
+    return plain(x) && x.dim() == 3 && x.size(0) == t && x.size(1) == heads && x.size(2) == d && x.get_device() == k.get_device() &&
+           x.stride(2) == 1 && x.stride(0) % 8 == 0 && x.stride(1) % 8 == 0 && aligned(x);
+  }
+  void move(bool write, const Tensor& xk, const Tensor& xv, const Tensor& slots) {
+    const long long x[4] = {xk.stride(0), xk.stride(1), xv.stride(0), xv.stride(1)};
+    check(tpb_paged_rows(write, mptr(xk), mptr(xv), mptr(k), mptr(v), mptr(ks), mptr(vs), static_cast<const long long*>(cptr(slots)),
+                         slots.size(0), (int)heads, (int)dk, (int)dv, (int)pages, (int)page, x, strides, stream()),
+          "paged_rows");
+  }
+};
+
+bool slots_of(const Pools& c, py::handle h, Tensor& slots) {
+  return unpack(h, slots) && plain(slots, at::kLong) && slots.dim() == 1 && slots.is_contiguous() && slots.get_device() == c.k.get_device() &&
+         slots.numel() > 0 && slots.numel() <= 0x7fffffff / c.heads;
+}
+
+// Rows of keys and values to a cache, and back; see paged_kv.append and paged_kv.read.
+py::object paged_append(py::handle k_, py::handle v_, py::handle ks_, py::handle vs_, py::handle xk_, py::handle xv_, py::handle slots_) {
+  Pools c;
+  Tensor xk, xv, slots;
+  if (!unobserved() || !c.take(k_, v_, ks_, vs_) || !unpack(xk_, xk) || !unpack(xv_, xv) || !slots_of(c, slots_, slots) ||
+      !c.rows(xk, slots.size(0), c.dk) || !c.rows(xv, slots.size(0), c.dv))
+    return py::none();
+  {
+    py::gil_scoped_release nogil;
+    c.move(true, xk, xv, slots);
+  }
+  return py::bool_(true);
+}
+py::object paged_read(py::handle k_, py::handle v_, py::handle ks_, py::handle vs_, py::handle slots_) {
+  Pools c;
+  Tensor xk, xv, slots;
+  if (!unobserved() || !c.take(k_, v_, ks_, vs_) || !slots_of(c, slots_, slots)) return py::none();
+  {
+    py::gil_scoped_release nogil;
+    xk = empty_like_type(c.k, {slots.size(0), c.heads, c.dk}, at::kBFloat16);
+    xv = empty_like_type(c.k, {slots.size(0), c.heads, c.dv}, at::kBFloat16);
+    c.move(false, xk, xv, slots);
+  }
+  return py::make_tuple(xk, xv);
+}
+
+// Attention of one token per sequence over a cache; see paged_kv.decode_attention.
+py::object paged_decode(py::handle q_, py::handle k_, py::handle v_, py::handle ks_, py::handle vs_, py::handle table_, py::handle lens_,
+                        double scale, int64_t window, double softcap) {
+  Pools c;
+  Tensor q, table, lens, out;
+  if (!unobserved() || !unpack(q_, q) || !plain(q) || q.dim() != 3 || !c.take(k_, v_, ks_, vs_) || !unpack(table_, table) ||
+      !unpack(lens_, lens) || (at::GradMode::is_enabled() && recording(q)))
+    return py::none();
+  const int64_t b = q.size(0), hq = q.size(1);
+  if (b < 1 || b > (1 << 24) || hq < 1 || hq > 65535 || hq % c.heads || q.size(2) != c.dk || c.pages < 1 || c.page % 16 ||
+      q.get_device() != c.k.get_device() || q.stride(2) != 1 || q.stride(0) % 8 || q.stride(1) % 8 || !aligned(q) ||
+      !plain(table, at::kInt) || !plain(lens, at::kInt) || table.dim() != 2 || lens.dim() != 1 || table.size(0) != b || lens.size(0) != b ||
+      table.get_device() != q.get_device() || lens.get_device() != q.get_device() || (table.size(1) > 1 && table.stride(1) != 1) ||
+      !lens.is_contiguous() || window < 0 || window > 0x7fffffff || !(softcap >= 0))
+    return py::none();
+  if (!((c.dk == 128 && c.dv == 128) || (c.dk == 192 && c.dv == 128) || (c.dk == 64 && c.dv == 64))) return py::none();
+  for (int i = 0; i < 2; ++i) {
+    for (int j = 0; j < 3; ++j)
+      if (c.strides[6 * i + j] <= 0) return py::none();
+    if (c.held8 && (c.strides[6 * i + 4] != 1 || c.strides[6 * i + 3] % 16 || c.strides[6 * i + 5] % 16 || !aligned(i ? c.vs : c.ks)))
+      return py::none();
+  }
+  const int64_t width = table.size(1);
+  if (width * c.page > 0x7fffff00) return py::none();
+  {
+    py::gil_scoped_release nogil;
+    out = empty_as(q, {b, hq, c.dv});
+    const int g = (int)(hq / c.heads);
+    Tensor scratch = empty_like_type(
+        q, {tpb_paged_decode_scratch((int)b, (int)c.heads, g, (int)c.dk, (int)c.dv, c.held8, (int)(width * c.page))}, at::kByte);
+    check(tpb_paged_decode(cptr(q), q.stride(0), q.stride(1), cptr(c.k), cptr(c.v), cptr(c.ks), cptr(c.vs), c.strides, iptr(table),
+                           table.stride(0), (int)width, iptr(lens), mptr(out), mptr(scratch), (int)b, (int)c.heads, g, (int)c.dk,
+                           (int)c.dv, (int)c.pages, (int)c.page, (int)window, (float)scale, (float)softcap, stream()),
+          "paged_decode");
+  }
+  return py::cast(out);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_tpb_torch, m) {
@@ -1081,4 +1196,7 @@ PYBIND11_MODULE(_tpb_torch, m) {
   m.def("linear_f32", &linear_f32);
   m.def("router_topk", &router_topk);
   m.def("grouped_mlp_few_rows", &grouped_mlp_few_rows);
+  m.def("paged_append", &paged_append);
+  m.def("paged_read", &paged_read);
+  m.def("paged_decode", &paged_decode);
 }

@@ -265,3 +265,17 @@ def test_a_decode_step_writes_and_attends(cuda_lib):
     lens = torch.full((2,), n, dtype=torch.int32, device="cuda")
     q = torch.randn(2, 8, 128, generator=g, device="cuda").bfloat16()
     _check(paged_kv.decode_attention(q, c, table, lens), q, c, table, lens)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+def test_native_and_python_calls_are_the_same(cuda_lib, monkeypatch, dtype):
+  q, c, table, lens = _problem([200, 130, 0], 8, 2, 128, 128, 16, dtype)
+  a = paged_kv.decode_attention(q, c, table, lens, window=150, softcap=20.0)
+  slots = torch.arange(0, 90, 7, device="cuda")
+  rows = paged_kv.read(c, slots)
+  monkeypatch.setattr(ops, "_native", lambda: None)
+  assert torch.equal(a, paged_kv.decode_attention(q, c, table, lens, window=150, softcap=20.0))
+  for x, y in zip(rows, paged_kv.read(c, slots)):
+    assert torch.equal(x.view(torch.int16), y.view(torch.int16))
+  with pytest.raises(ValueError):
+    paged_kv.decode_attention(q, c, table, lens.long())

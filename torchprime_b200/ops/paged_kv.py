@@ -21,7 +21,7 @@ from ._lib import check, lib, ptr, stream_ptr
 
 P, I, LL, F = c_void_p, c_int, c_longlong, c_float
 _lib.register_signature("tpb_paged_rows", [I, P, P, P, P, P, P, P, LL, I, I, I, I, I, P, P, P])
-_lib.register_signature("tpb_paged_decode_scratch", [I, I, I, I, I])
+_lib.register_signature("tpb_paged_decode_scratch", [I, I, I, I, I, I, I])
 _lib.register_signature("tpb_paged_decode", [P, LL, LL, P, P, P, P, P, P, LL, I, P, P, P, I, I, I, I, I, I, I, I, F, F, P])
 
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
@@ -105,7 +105,9 @@ def append(cache: PagedKV, k, v, slots):
   """Writes keys [T, H, Dk] and values [T, H, Dv] to the rows ``slots`` [T] (int64) of the cache, quantised where it is
   e4m3; a token of slot -1 (padding) is not written, and neither is one whose slot lies outside the pool, which the kernel
   reports (``_lib.raise_on_device_timeout``).  No slot may come twice: which of its tokens a row of it holds is not defined."""
-  from .functional import use_kernels
+  from .functional import _native, use_kernels
+  if not _debug.bounds_enabled() and (nat := _native()) is not None and nat.paged_append(*cache, k, v, slots):
+    return
   _check_cache(cache)
   _check_slots("paged_append", cache, slots)
   t, h = slots.shape[0], cache.k.shape[2]
@@ -129,7 +131,11 @@ def append(cache: PagedKV, k, v, slots):
 def read(cache: PagedKV, slots, dtype=torch.bfloat16):
   """The rows ``slots`` [T] of the cache as (keys [T, H, Dk], values [T, H, Dv]) of ``dtype``; zeros for slot -1 and, reported as in
   :func:`append`, for slots outside the pool."""
-  from .functional import use_kernels
+  from .functional import _native, use_kernels
+  if dtype == torch.bfloat16 and not _debug.bounds_enabled() and (nat := _native()) is not None:
+    rows = nat.paged_read(*cache, slots)
+    if rows is not None:
+      return rows
   _check_cache(cache)
   _check_slots("paged_read", cache, slots)
   h, dk, dv = cache.k.shape[2], cache.k.shape[3], cache.v.shape[3]
@@ -163,7 +169,13 @@ def decode_attention(q, cache: PagedKV, block_table, lengths, scale=None, window
   64 columns.  It reads nothing of the table and of the pages behind a sequence's last token (what a page holds there may be
   anything); a page outside the pool counts as zeros, a length beyond the table as the whole table, a negative one as none, and all three are
   reported (``_lib.raise_on_device_timeout``)."""
-  from .functional import inference_only, use_kernels
+  from .functional import _native, inference_only, use_kernels
+  window, softcap = int(window or 0), float(softcap or 0.0)
+  scale = float(scale) if scale is not None else q.shape[-1] ** -0.5
+  if not _debug.bounds_enabled() and (nat := _native()) is not None:
+    o = nat.paged_decode(q, *cache, block_table, lengths, scale, window, softcap)
+    if o is not None:
+      return o
   _check_cache(cache)
   if q.dim() != 3 or q.shape[2] != cache.k.shape[3] or q.shape[1] % cache.k.shape[2] or q.shape[1] == 0:
     raise ValueError(f"decode_attention: queries {tuple(q.shape)} over keys {tuple(cache.k.shape)}")
@@ -174,10 +186,8 @@ def decode_attention(q, cache: PagedKV, block_table, lengths, scale=None, window
     raise ValueError("decode_attention: block_table and lengths must be int32")
   if any(t.device != cache.k.device for t in (q, block_table, lengths)):
     raise ValueError("decode_attention: queries, block_table and lengths must be on the cache's device")
-  window, softcap = int(window or 0), float(softcap or 0.0)
   if window < 0 or not softcap >= 0.0:
     raise ValueError(f"decode_attention: window {window}, softcap {softcap}")
-  scale = float(scale) if scale is not None else dk ** -0.5
   _debug.check_index("decode_attention", "lengths", lengths, 0, block_table.shape[1] * cache.page + 1)
   if (use_kernels(q) and q.is_cuda and _decode_ok(q, cache) and (inference_only() or not q.requires_grad)):
     q = _vectors(q)
@@ -186,7 +196,7 @@ def decode_attention(q, cache: PagedKV, block_table, lengths, scale=None, window
     dv, width = cache.v.shape[3], block_table.shape[1]
     out = torch.empty(b, hq, dv, dtype=q.dtype, device=q.device)
     with torch.cuda.device(q.device):
-      n = lib().tpb_paged_decode_scratch(b, hkv, hq // hkv, dv, width * page)
+      n = lib().tpb_paged_decode_scratch(b, hkv, hq // hkv, dk, dv, int(cache.k.dtype == E4M3), width * page)
       scratch = torch.empty(n, dtype=torch.uint8, device=q.device)
       rc = lib().tpb_paged_decode(ptr(q), q.stride(0), q.stride(1), ptr(cache.k), ptr(cache.v), ptr(cache.k_scale), ptr(cache.v_scale),
                                   _c_strides(cache), ptr(block_table), block_table.stride(0), width, ptr(lengths.contiguous()), ptr(out),
