@@ -7,14 +7,15 @@
 // what the kernel is built for is to keep loads under way on every SM from the first to the last token.
 //
 // * The work is cut into steps: 32 tokens of one sequence, for one key head and up to 16 of its query heads.  In the order
-//   sequence, head, token they form one list, of which every WARP of the grid (one CTA per SM) takes an equal, contiguous part;
-//   how long the sequences are only the device knows, so each CTA adds up the lengths itself.  A (sequence, head) whose steps fall to
-//   several warps is joined by paged_join_kernel from their running maxima, sums and unnormalised results; a warp has at most
-//   two of those, so the scratch is bounded by the grid and not by the batch.  Nothing is added by atomics: the order of every
-//   sum follows from the lengths.  (Eight warps sharing units of 256 tokens met in a block barrier wherever a sequence ended: 24
-//   sequences of up to 3001 tokens, 16 heads of 192 / 128 in e4m3, 69 us, the SMs idle for half of it.)
+//   sequence, head, token they form one list, of which every CTA (one per SM) takes an equal, contiguous part, and every warp of
+//   it an equal part of that; how long the sequences are only the device knows, so each CTA adds up the lengths itself.  Where a
+//   (sequence, head) goes on in the next warps, the warp that began it waits for them at the kernel's end and joins their
+//   running maxima, sums and unnormalised results with its own; where it goes on in the next CTAs, paged_join_kernel does.  A CTA
+//   has at most two of the latter, so the scratch is bounded by the grid and not by the batch.  Nothing is added by atomics: the
+//   order of every sum follows from the lengths.  (Eight warps sharing units of 256 tokens met in a block barrier wherever a
+//   sequence ended: 24 sequences of up to 3001 tokens, 16 heads of 192 / 128 in e4m3, 69 us, the SMs idle for half of it.)
 // * A warp has a ring of stages of its own, filled by TMA boxes of 16 tokens (a page is a multiple of 16) that its elected lane asks
-//   for as soon as it has used a stage up, across the borders of sequences.  Warps never wait for one another.
+//   for as soon as it has used a stage up, across the borders of sequences.
 // * Scores and weighted sums are mma.sync m16n8k16: the query heads of a key head are its 16 rows.  (A tcgen05 tile would be
 //   seven eighths empty, and its operands would still come through shared memory once.)  Statistics and sums are fp32; the
 //   weights of the sum are rounded to the operand type of the product, half a step of 2^-9 (bf16) or 2^-12 (f16) each, to
@@ -43,9 +44,9 @@ struct PagedDecode {
   const int* lengths;
   const uint8_t *k_scale, *v_scale;        // a row's scales are contiguous within a page
   long long ks_page, ks_head, vs_page, vs_head;
-  float* part_o;                           // [2 * warps of the grid][rows][DV]
-  float* part_ml;                          // [2 * warps of the grid][rows][2]: running maximum in log2 units, sum
-  int* start;                              // [B + 1]: steps of the sequences before, per head block
+  float* part_o;                           // [2 to a CTA, then one to a warp][rows][DV]
+  float* part_ml;                          // the same [rows][2]: running maximum in log2 units, sum
+  int4* split;                             // [CTAs] of the (sequence, head block) that begins in a CTA and goes on: last CTA, slot; or -1
   int* status;
   int B, Hkv, G, blocks, rows;             // blocks of up to 16 query heads to a key head; rows of the largest block
   int pages, page, capacity;               // tokens that a row of the table can name
@@ -125,8 +126,8 @@ __device__ __forceinline__ Visible pd_visible(const PagedDecode& p, int b) {
   return s;
 }
 
-// Steps of each of `warps` warps.
-__device__ __forceinline__ int pd_share(int steps, int warps) { return max(1, (steps + warps - 1) / warps); }
+// Steps of each of `n` CTAs or warps.
+__device__ __forceinline__ int pd_share(int steps, int n) { return max(1, (steps + n - 1) / n); }
 
 // A place in the list of steps.
 struct PagedCursor {
@@ -152,7 +153,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   constexpr int NW = T::WARPS, THREADS = NW * 32;
   extern __shared__ uint8_t pd_smem_raw[];
   uint8_t* pd_smem = pd_smem_raw + ((1024u - (smem_u32(pd_smem_raw) & 1023u)) & 1023u);
-  __shared__ int s_scan[NW], s_at[NW][3];
+  __shared__ int s_scan[NW], s_at[NW][3], s_ends[NW];
   const int warp = warp_index(), lane = threadIdx.x & 31, ST = p.stages;
   const int HB = p.Hkv * p.blocks;
   uint8_t* ring = pd_smem + (size_t)warp * ST * T::STAGE;
@@ -169,8 +170,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   chain_launch();
   if (!chain_wait()) return;
 
-  // The list's length, and where the warps' parts begin.  Neighbours in the list are on different SMs: few steps use all of them.
-  int total = 0, share = 1;
+  // The list's length, and where this CTA's part and its warps' begin.
+  int cta_first = 0, cta_share = 1, cta_steps = 0, share = 1;
   for (int pass = 0; pass < 2; ++pass) {
     int running = 0;
     for (int base = 0; base < p.B; base += THREADS) {
@@ -192,15 +193,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       }
       before += sum - n;
       if (pass == 0) {
-        if (blockIdx.x == 0 && b < p.B) {
-          p.start[b] = before;
-          if (p.lengths[b] < 0 || p.lengths[b] > p.capacity) report(p.status, kBadArgument, 71);
-        }
+        if (blockIdx.x == 0 && b < p.B && (p.lengths[b] < 0 || p.lengths[b] > p.capacity)) report(p.status, kBadArgument, 71);
       } else if (n > 0) {
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-          const int in = (w * (int)gridDim.x + (int)blockIdx.x) * share - before * HB;
-          if (in >= 0 && in < n * HB) {
+          const int in = cta_first + w * share - before * HB;
+          if (w * share < cta_steps && in >= 0 && in < n * HB) {
             s_at[w][0] = b;
             s_at[w][1] = in / n;
             s_at[w][2] = in % n;
@@ -210,17 +208,27 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       running += all;
     }
     if (pass == 0) {
-      total = running * HB;
-      if (blockIdx.x == 0 && threadIdx.x == 0) p.start[p.B] = running;
-      share = pd_share(total, gridDim.x * NW);
+      cta_share = pd_share(running * HB, gridDim.x);
+      cta_first = blockIdx.x * cta_share;
+      cta_steps = min(cta_share, running * HB - cta_first);
+      share = pd_share(cta_steps, NW);
     }
   }
+  if (threadIdx.x == 0) p.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  for (int b = blockIdx.x; b < p.B; b += gridDim.x)        // sequences of no visible token
+    if (pd_visible(p, b).steps == 0) {
+      uint4* dst = reinterpret_cast<uint4*>(p.out + (long long)b * p.Hkv * p.G * DV);
+      for (int i = threadIdx.x; i < p.Hkv * p.G * (DV / 8); i += THREADS) dst[i] = make_uint4(0, 0, 0, 0);
+    }
   __syncthreads();
-  const int part = warp * gridDim.x + blockIdx.x;
-  const int steps = min(share, total - part * share);
-  if (steps <= 0) return;
-  PagedCursor c = {s_at[warp][0], s_at[warp][1], s_at[warp][2], {}};
-  c.s = pd_visible(p, c.b);
+  const int steps = min(share, cta_steps - warp * share);      // (none: 0 or less)
+  PagedCursor c = {};
+  if (steps > 0) {
+    c.b = s_at[warp][0];
+    c.hb = s_at[warp][1];
+    c.at = s_at[warp][2];
+    c.s = pd_visible(p, c.b);
+  }
   PagedCursor ahead = c;
   int asked = 0, ask_stage = 0, stage = 0, parity = 0;
   bool alive = true;
@@ -235,7 +243,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     pg0 = row[at0];
     if (key0 + 16 < ahead.s.len) pg1 = row[at1];
   };
-  look_up();
+  if (steps > 0) look_up();
 
   auto ask = [&]() {
     uint64_t* bar = &bars[ask_stage];
@@ -271,12 +279,50 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   while (asked < steps && asked < ST) ask();
 
   const int g = lane >> 2, t = lane & 3;
-  int done = 0;
+  int done = 0, seg = 0, h0 = 0, rows = 0;
+  float o[DV / 8][4], m0, m1, l0, l1;
+  bool joins = false;          // this warp's last (sequence, head) goes on in the next one, and it is the one to join them
+  auto put_result = [&]() {
+#pragma unroll
+    for (int hh = 0; hh < (WIDE ? 2 : 1); ++hh) {
+      const int r = g + 8 * hh;
+      if (r >= rows) continue;
+      const float inv = 1.f / (hh ? l1 : l0);
+      __nv_bfloat16* dst = p.out + ((long long)c.b * p.Hkv * p.G + h0 + r) * DV;
+      if constexpr (!F8) {
+#pragma unroll
+        for (int n = 0; n < DV / 8; ++n)
+          *reinterpret_cast<uint32_t*>(dst + n * 8 + 2 * t) = pack_bf16(o[n][2 * hh] * inv, o[n][2 * hh + 1] * inv);
+      } else {
+#pragma unroll
+        for (int n = 0; n < DV / 8; n += 2)
+          *reinterpret_cast<uint2*>(dst + n * 8 + 4 * t) = make_uint2(pack_bf16(o[n][2 * hh] * inv, o[n + 1][2 * hh] * inv),
+                                                                      pack_bf16(o[n][2 * hh + 1] * inv, o[n + 1][2 * hh + 1] * inv));
+      }
+    }
+  };
+  auto put_part = [&](int slot) {
+#pragma unroll
+    for (int hh = 0; hh < (WIDE ? 2 : 1); ++hh) {
+      const int r = g + 8 * hh;
+      if (r >= rows) continue;
+      float* dst = p.part_o + (long long)(slot * p.rows + r) * DV;
+      if constexpr (!F8) {
+#pragma unroll
+        for (int n = 0; n < DV / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8 + 2 * t) = make_float2(o[n][2 * hh], o[n][2 * hh + 1]);
+      } else {
+#pragma unroll
+        for (int n = 0; n < DV / 8; n += 2)
+          *reinterpret_cast<float4*>(dst + n * 8 + 4 * t) = make_float4(o[n][2 * hh], o[n + 1][2 * hh], o[n][2 * hh + 1], o[n + 1][2 * hh + 1]);
+      }
+      if (t == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * p.rows + r) * 2) = make_float2(hh ? m1 : m0, hh ? l1 : l0);
+    }
+  };
   while (done < steps) {
-    const int seg = min(steps - done, c.s.steps - c.at);
-    const bool whole = seg == c.s.steps;
-    const int kv_head = c.hb / p.blocks, row0 = (c.hb - kv_head * p.blocks) * 16, rows = min(16, p.G - row0);
-    const int h0 = kv_head * p.G + row0;
+    seg = min(steps - done, c.s.steps - c.at);
+    const int kv_head = c.hb / p.blocks, row0 = (c.hb - kv_head * p.blocks) * 16;
+    rows = min(16, p.G - row0);
+    h0 = kv_head * p.G + row0;
     // ---- the queries as A operands
     uint32_t qa[DK / 16][4];
     float qs0 = p.scale_log2, qs1 = p.scale_log2;
@@ -322,8 +368,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
           }
       }
     }
-    float o[DV / 8][4] = {};
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+    for (int n = 0; n < DV / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    m0 = m1 = -INFINITY;
+    l0 = l1 = 0.f;
 
     for (int i = 0; i < seg; ++i) {
       const int key0 = c.key0() + i * PD_KEYS;
@@ -473,92 +521,121 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
       l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
     }
-    const int slot = (2 * part + (done > 0 ? 1 : 0)) * p.rows;
-#pragma unroll
-    for (int hh = 0; hh < (WIDE ? 2 : 1); ++hh) {
-      const int r = g + 8 * hh;
-      if (r >= rows) continue;
-      if (whole) {
-        const float inv = 1.f / (hh ? l1 : l0);
-        __nv_bfloat16* dst = p.out + ((long long)c.b * p.Hkv * p.G + h0 + r) * DV;
-        if constexpr (!F8) {
-#pragma unroll
-          for (int n = 0; n < DV / 8; ++n)
-            *reinterpret_cast<uint32_t*>(dst + n * 8 + 2 * t) = pack_bf16(o[n][2 * hh] * inv, o[n][2 * hh + 1] * inv);
-        } else {
-#pragma unroll
-          for (int n = 0; n < DV / 8; n += 2)
-            *reinterpret_cast<uint2*>(dst + n * 8 + 4 * t) = make_uint2(pack_bf16(o[n][2 * hh] * inv, o[n + 1][2 * hh] * inv),
-                                                                        pack_bf16(o[n][2 * hh + 1] * inv, o[n + 1][2 * hh + 1] * inv));
-        }
-      } else {
-        float* dst = p.part_o + (long long)(slot + r) * DV;
-        if constexpr (!F8) {
-#pragma unroll
-          for (int n = 0; n < DV / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8 + 2 * t) = make_float2(o[n][2 * hh], o[n][2 * hh + 1]);
-        } else {
-#pragma unroll
-          for (int n = 0; n < DV / 8; n += 2)
-            *reinterpret_cast<float4*>(dst + n * 8 + 4 * t) = make_float4(o[n][2 * hh], o[n + 1][2 * hh], o[n][2 * hh + 1], o[n + 1][2 * hh + 1]);
-        }
-        if (t == 0) *reinterpret_cast<float2*>(p.part_ml + (slot + r) * 2) = make_float2(hh ? m1 : m0, hh ? l1 : l0);
-      }
-    }
+    const bool starts = c.at == 0, ends = c.at + seg == c.s.steps;
     done += seg;
+    if (starts && ends) {
+      put_result();
+    } else if (!starts && warp > 0) {      // for the warp that began it, or began this CTA's part of it
+      put_part(2 * gridDim.x + blockIdx.x * NW + warp);
+      if (lane == 0) s_ends[warp] = ends;
+    } else if (ends) {
+      put_part(2 * blockIdx.x);
+    } else {
+      joins = true;                        // (the list's part of this warp ends here)
+      break;
+    }
     c.at += seg;
     if (c.at == c.s.steps) c.next_head(p);
   }
+  __syncthreads();
+  if (joins) {
+    bool ends = false;
+    for (int w = warp + 1; w < NW && w * share < cta_steps && !ends; ++w) {
+      const int at = 2 * gridDim.x + blockIdx.x * NW + w;
+      ends = s_ends[w];
+#pragma unroll
+      for (int hh = 0; hh < (WIDE ? 2 : 1); ++hh) {
+        const int r = g + 8 * hh;
+        if (r >= rows) continue;
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (at * p.rows + r) * 2);
+        const float* src = p.part_o + (long long)(at * p.rows + r) * DV;
+        float &m = hh ? m1 : m0, &l = hh ? l1 : l0;
+        const float top = fmaxf(m, ml.x);
+        const float fa = m == -INFINITY ? 0.f : ex2_approx(m - top), fb = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
+        m = top;
+        l = l * fa + ml.y * fb;
+        if constexpr (!F8) {
+#pragma unroll
+          for (int n = 0; n < DV / 8; ++n) {
+            const float2 v = *reinterpret_cast<const float2*>(src + n * 8 + 2 * t);
+            o[n][2 * hh] = o[n][2 * hh] * fa + v.x * fb;
+            o[n][2 * hh + 1] = o[n][2 * hh + 1] * fa + v.y * fb;
+          }
+        } else {
+#pragma unroll
+          for (int n = 0; n < DV / 8; n += 2) {
+            const float4 v = *reinterpret_cast<const float4*>(src + n * 8 + 4 * t);
+            o[n][2 * hh] = o[n][2 * hh] * fa + v.x * fb;
+            o[n + 1][2 * hh] = o[n + 1][2 * hh] * fa + v.y * fb;
+            o[n][2 * hh + 1] = o[n][2 * hh + 1] * fa + v.z * fb;
+            o[n + 1][2 * hh + 1] = o[n + 1][2 * hh + 1] * fa + v.w * fb;
+          }
+        }
+      }
+    }
+    if (c.at == 0 && ends) {
+      put_result();
+    } else {
+      const int slot = 2 * blockIdx.x + (warp == 0 && done == seg ? 0 : 1);
+      put_part(slot);
+      if (c.at == 0 && lane == 0)
+        p.split[blockIdx.x] = make_int4((cta_first + warp * share + done - seg + c.s.steps - 1) / cta_share, slot, c.b, c.hb);
+    }
+  }
 }
 
-// One CTA per sequence and query head: joins the parts of a head whose steps fell to several warps (the part that begins at a
-// warp's first step is in its slot 0, one that begins later in slot 1), writes zeros for a sequence of no visible token.
+// Grid (CTAs of the kernel before, rows): joins the parts of the (sequence, head block) that begins in a CTA and goes on, a row to a
+// block.  The first part is in the slot that the CTA has noted, the others, which begin with their CTA, in slot 0 of theirs.  What
+// a thread reads of the first parts is asked for before their weights are known.
 template <int DV>
-__global__ void __launch_bounds__(128)
-paged_join_kernel(const PagedDecode p, int warps) {
+__global__ void __launch_bounds__(256)
+paged_join_kernel(const PagedDecode p) {
   if (!chain_begin()) return;
-  constexpr int COLS = DV / 4, SETS = 128 / COLS;
+  constexpr int COLS = DV / 4, SETS = 256 / COLS, AHEAD = 4;
   __shared__ float4 sums[SETS][COLS];
-  const int b = blockIdx.x, h = blockIdx.y, Hq = p.Hkv * p.G, HB = p.Hkv * p.blocks;
-  const int kv_head = h / p.G, in = h - kv_head * p.G, hb = kv_head * p.blocks + in / 16, r = in % 16;
-  const int n = p.start[b + 1] - p.start[b];
-  const int col = threadIdx.x % COLS, set = threadIdx.x / COLS, lane = threadIdx.x & 31;
-  uint2* dst = reinterpret_cast<uint2*>(p.out + ((long long)b * Hq + h) * DV) + col;
-  if (n == 0) {
-    if (set == 0) *dst = make_uint2(0, 0);
-    return;
-  }
-  const int share = pd_share(p.start[p.B] * HB, warps);
-  const int a = p.start[b] * HB + hb * n, f = a / share, l = (a + n - 1) / share;
-  if (f == l) return;
-  auto slot = [&](int c) { return (2 * c + (c == f && a > f * share ? 1 : 0)) * p.rows + r; };
+  const int4 split = p.split[blockIdx.x];
+  const int f = blockIdx.x, l = split.x, r = blockIdx.y, lane = threadIdx.x & 31;
+  const int kv_head = split.w / p.blocks, row0 = (split.w - kv_head * p.blocks) * 16;
+  if (l < 0 || r >= p.G - row0) return;
+  const int col = threadIdx.x % COLS, set = threadIdx.x / COLS;
+  auto slot = [&](int c) { return (c == f ? split.y : 2 * c) * p.rows + r; };
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
+  auto part = [&](int c) { return *reinterpret_cast<const float4*>(p.part_o + (long long)slot(c) * DV + 4 * col); };
+  float4 v[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) v[i] = part(min(f + set + i * SETS, l));
   float top = -INFINITY;
   for (int c = f + lane; c <= l; c += 32) top = fmaxf(top, ml[slot(c)].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  auto weight = [&](float m) { return m == -INFINITY ? 0.f : ex2_approx(m - top); };
   float sum = 0.f;
   for (int c = f + lane; c <= l; c += 32) {
     const float2 x = ml[slot(c)];
-    sum += x.x == -INFINITY ? 0.f * x.y : ex2_approx(x.x - top) * x.y;
+    sum += weight(x.x) * x.y;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](const float4& x, int c) {
+    const float w = weight(ml[slot(c)].x);
+    acc.x += w * x.x; acc.y += w * x.y; acc.z += w * x.z; acc.w += w * x.w;
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (f + set + i * SETS <= l) add(v[i], f + set + i * SETS);
 #pragma unroll 4
-  for (int c = f + set; c <= l; c += SETS) {
-    const float m = ml[slot(c)].x, w = m == -INFINITY ? 0.f : ex2_approx(m - top);
-    const float4 v = *reinterpret_cast<const float4*>(p.part_o + (long long)slot(c) * DV + 4 * col);
-    acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
-  }
+  for (int c = f + set + AHEAD * SETS; c <= l; c += SETS) add(part(c), c);
   sums[set][col] = acc;
   __syncthreads();
   if (set == 0) {
     for (int k = 1; k < SETS; ++k) {
-      const float4 v = sums[k][col];
-      acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+      const float4 x = sums[k][col];
+      acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
     }
     const float inv = 1.f / sum;
-    *dst = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+    *(reinterpret_cast<uint2*>(p.out + ((long long)split.z * p.Hkv * p.G + kv_head * p.G + row0 + r) * DV) + col) =
+        make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
   }
 }
 
@@ -579,7 +656,7 @@ static int launch_paged_decode(PagedDecode p, int grid, const CUtensorMap& km, c
   cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return 1000 + (int)e;
   chain(f, grid, T::WARPS * 32, smem, stream, km, vm, p);
-  chain(paged_join_kernel<DV>, dim3(p.B, p.Hkv * p.G), 128, 0, stream, p, grid * T::WARPS);
+  if (grid > 1) chain(paged_join_kernel<DV>, dim3(grid, p.rows), 256, 0, stream, p);
   e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 1000 + (int)e;
 }
@@ -588,10 +665,10 @@ static int launch_paged_decode(PagedDecode p, int grid, const CUtensorMap& km, c
 
 using namespace tpb;
 
-// Bytes of scratch for tpb_paged_decode (B up to 2^24).
+// Bytes of scratch for tpb_paged_decode.
 extern "C" int tpb_paged_decode_scratch(int B, int Hkv, int G, int DK, int DV, int held8, int capacity) {
   const long long steps = (long long)B * Hkv * ((G + 15) / 16) * (((long long)capacity + PD_KEYS - 1) / PD_KEYS);
-  return pd_grid(steps) * pd_warps(DK, DV, held8 != 0) * 2 * (G < 16 ? G : 16) * (DV + 2) * 4 + (B + 1) * 4;
+  return pd_grid(steps) * ((2 + pd_warps(DK, DV, held8 != 0)) * (G < 16 ? G : 16) * (DV + 2) * 4 + 16);
 }
 
 // q [B, Hkv * G, DK] bf16 (strides q_b, q_h), pools as in tpb_paged_rows (strides of pages, tokens, heads; scales contiguous over
@@ -636,10 +713,10 @@ extern "C" int tpb_paged_decode(const void* q, long long q_b, long long q_h, con
   p.vs_head = strides[11];
   const int grid = pd_grid(steps);
   p.rows = G < 16 ? G : 16;
-  const long long part_rows = (long long)grid * pd_warps(DK, DV, held8) * 2 * p.rows;
-  p.part_o = static_cast<float*>(scratch);
+  const long long part_rows = (long long)grid * (2 + pd_warps(DK, DV, held8)) * p.rows;
+  p.split = static_cast<int4*>(scratch);
+  p.part_o = reinterpret_cast<float*>(p.split + grid);
   p.part_ml = p.part_o + part_rows * DV;
-  p.start = reinterpret_cast<int*>(p.part_ml + part_rows * 2);
   p.status = status_block();
   p.B = B;
   p.Hkv = Hkv;
