@@ -533,6 +533,20 @@ __device__ __forceinline__ float2 unpack_bf16(uint32_t u) {
   return __bfloat1622float2(v);
 }
 
+// Two floats to two e4m3 values, the first in the low byte; saturating, to nearest even.
+__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float2 from_e4m3x2(uint32_t v) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)v));
+  float2 f;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(f.x), "=f"(f.y) : "r"(h));
+  return f;
+}
+
 // ---- packed fp32 pairs (sm_100: one FMA-pipe instruction works on two floats held in an aligned
 // 64-bit register pair), the three-input maximum and the bare MUFU exponential.  The softmax loops
 // of the attention kernels are bound by instruction issue, not by any one pipe; these halve the

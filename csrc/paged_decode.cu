@@ -56,7 +56,12 @@ struct PagedDecode {
 
 constexpr int PD_KEYS = 32;                // tokens of a warp's step, two boxes
 
-template <int DK, int DV, bool F8>
+#ifndef PD_W8W
+#define PD_W8W 8
+#endif
+constexpr int pd_warps(bool held8, bool wide) { return held8 ? (wide ? PD_W8W : 16) : 8; }
+
+template <int DK, int DV, bool F8, bool WIDE>
 struct PagedTile {
   static constexpr int ELT = F8 ? 1 : 2;
   static constexpr int ROW = 64 * ELT;                       // bytes of a 64-column block's row: the swizzle's width
@@ -66,7 +71,7 @@ struct PagedTile {
   static constexpr int SCALES = F8 ? 64 : 0;                 // 32 of the keys, 32 of the values
   // Warps to a CTA: as many as have two stages or more each, up to eight.  An 8-bit cache brings a step's bytes in half the time,
   // and the step takes longer (conversions): four warps 159 us for 64 sequences of up to 8192 tokens, 64 / 8 heads of 128; eight 118.
-  static constexpr int WARPS = STAGE <= 10240 ? 8 : 4;
+  static constexpr int WARPS = pd_warps(F8, WIDE);
 };
 
 __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int row, int head, int page) {
@@ -113,6 +118,13 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return r;
 }
 
+// The 8 x 8 matrix of 16-bit values that a warp holds two to a lane, transposed.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
 // What is visible of a sequence, in tokens and in steps.
 struct Visible {
   int len, lo, first, steps;
@@ -147,9 +159,9 @@ struct PagedCursor {
 };
 
 template <int DK, int DV, bool F8, bool WIDE>
-__global__ void __launch_bounds__(PagedTile<DK, DV, F8>::WARPS * 32, 1)
+__global__ void __launch_bounds__(PagedTile<DK, DV, F8, WIDE>::WARPS * 32, 1)
 paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const PagedDecode p) {
-  using T = PagedTile<DK, DV, F8>;
+  using T = PagedTile<DK, DV, F8, WIDE>;
   constexpr int NW = T::WARPS, THREADS = NW * 32;
   extern __shared__ uint8_t pd_smem_raw[];
   uint8_t* pd_smem = pd_smem_raw + ((1024u - (smem_u32(pd_smem_raw) & 1023u)) & 1023u);
@@ -172,48 +184,49 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 
   // The list's length, and where this CTA's part and its warps' begin.
   int cta_first = 0, cta_share = 1, cta_steps = 0, share = 1;
-  for (int pass = 0; pass < 2; ++pass) {
-    int running = 0;
-    for (int base = 0; base < p.B; base += THREADS) {
-      const int b = base + threadIdx.x, n = b < p.B ? pd_visible(p, b).steps : 0;
-      int sum = n;
+  int before = 0, n = 0;                   // of this thread's sequence: steps in front of it (per head block), its own
+  auto add_up = [&](int base, int running) {
+    const int b = base + threadIdx.x;
+    n = b < p.B ? pd_visible(p, b).steps : 0;
+    int sum = n;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += v;
-      }
-      __syncthreads();
-      if (lane == 31) s_scan[warp] = sum;
-      __syncthreads();
-      int before = running, all = 0;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
+    }
+    __syncthreads();
+    if (lane == 31) s_scan[warp] = sum;
+    __syncthreads();
+    before = running + sum - n;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      if (w < warp) before += s_scan[w];
+      running += s_scan[w];
+    }
+    return running;
+  };
+  int all = 0;
+  for (int base = 0; base < p.B; base += THREADS) all = add_up(base, all);
+  cta_share = pd_share(all * HB, gridDim.x);
+  cta_first = blockIdx.x * cta_share;
+  cta_steps = min(cta_share, all * HB - cta_first);
+  share = pd_share(cta_steps, NW);
+  for (int base = 0, running = 0; base < p.B; base += THREADS) {
+    if (p.B > THREADS) running = add_up(base, running);      // (else as it was left)
+    if (n > 0)
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        if (w < warp) before += s_scan[w];
-        all += s_scan[w];
-      }
-      before += sum - n;
-      if (pass == 0) {
-        if (blockIdx.x == 0 && b < p.B && (p.lengths[b] < 0 || p.lengths[b] > p.capacity)) report(p.status, kBadArgument, 71);
-      } else if (n > 0) {
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-          const int in = cta_first + w * share - before * HB;
-          if (w * share < cta_steps && in >= 0 && in < n * HB) {
-            s_at[w][0] = b;
-            s_at[w][1] = in / n;
-            s_at[w][2] = in % n;
-          }
+        const int in = cta_first + w * share - before * HB;
+        if (w * share < cta_steps && in >= 0 && in < n * HB) {
+          s_at[w][0] = base + threadIdx.x;
+          s_at[w][1] = in / n;
+          s_at[w][2] = in % n;
         }
       }
-      running += all;
-    }
-    if (pass == 0) {
-      cta_share = pd_share(running * HB, gridDim.x);
-      cta_first = blockIdx.x * cta_share;
-      cta_steps = min(cta_share, running * HB - cta_first);
-      share = pd_share(cta_steps, NW);
-    }
   }
+  if (blockIdx.x == 0)
+    for (int b = threadIdx.x; b < p.B; b += THREADS)
+      if (p.lengths[b] < 0 || p.lengths[b] > p.capacity) report(p.status, kBadArgument, 71);
   if (threadIdx.x == 0) p.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
   for (int b = blockIdx.x; b < p.B; b += gridDim.x)        // sequences of no visible token
     if (pd_visible(p, b).steps == 0) {
@@ -233,152 +246,169 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   int asked = 0, ask_stage = 0, stage = 0, parity = 0;
   bool alive = true;
   // The pages of the step that is asked for next, on their way from the table since the one before was.
-  int pg0 = -1, pg1 = -1, row0_next = 0, row1_next = 0;
-  auto look_up = [&]() {
-    const int key0 = ahead.key0();
-    const int* row = p.table + ahead.b * p.table_b;
-    const unsigned at0 = (unsigned)key0 / (unsigned)p.page, at1 = (unsigned)(key0 + 16) / (unsigned)p.page;
-    row0_next = key0 - at0 * p.page;
-    row1_next = key0 + 16 - at1 * p.page;
-    pg0 = row[at0];
-    if (key0 + 16 < ahead.s.len) pg1 = row[at1];
+  int at_page = 0, at_row = 0;             // of its first token
+  int pg0 = -1, pg1 = -1, row1 = 0;
+  auto find_page = [&]() {
+    const unsigned key0 = ahead.key0();
+    at_page = key0 / (unsigned)p.page;
+    at_row = key0 - at_page * p.page;
   };
-  if (steps > 0) look_up();
+  auto look_up = [&]() {
+    const int* row = p.table + ahead.b * p.table_b + at_page;
+    const bool next = at_row + 16 >= p.page;
+    row1 = next ? 0 : at_row + 16;
+    pg0 = row[0];
+    if (ahead.key0() + 16 < ahead.s.len) pg1 = row[next];
+  };
+  if (steps > 0) {
+    find_page();
+    look_up();
+  }
 
+  // The fence orders the warp's reads of the stage, in front of the __syncwarp before, ahead of the copy that overwrites it.
   auto ask = [&]() {
-    uint64_t* bar = &bars[ask_stage];
     const int boxes = ahead.key0() + 16 < ahead.s.len ? 2 : 1, head = ahead.hb / p.blocks;
-    int pg[2] = {pg0, pg1}, row[2] = {row0_next, row1_next};
-    uint32_t bytes = 0;
-    for (int i = 0; i < boxes; ++i) {
-      const bool inside = pg[i] >= 0 && pg[i] < p.pages;
-      if (!inside) {                       // a box outside the pool reads as zeros
+    int pg[2] = {pg0, pg1};
+    const int row[2] = {at_row, row1};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (i < boxes && (pg[i] < 0 || pg[i] >= p.pages)) {      // a box outside the pool reads as zeros
         if (lane == 0) report(p.status, kBadArgument, 72);
         pg[i] = -1;
       }
-      bytes += T::K_BOX + T::V_BOX + (F8 && inside ? 32 : 0);
-    }
     one_lane([&]() {
-      mbar_expect_tx(bar, bytes);
-      const uint32_t at = ring_at + ask_stage * T::STAGE;
-      for (int i = 0; i < boxes; ++i) {
-        tma_load_page(at + i * T::K_BOX, &k_map, bar, row[i], head, pg[i]);
-        tma_load_page(at + 2 * T::K_BOX + i * T::V_BOX, &v_map, bar, row[i], head, pg[i]);
-        if (F8 && pg[i] >= 0) {
-          const uint32_t sc = scales_at + ask_stage * T::SCALES + i * 16;
-          bulk_load_16(sc, p.k_scale + pg[i] * p.ks_page + head * p.ks_head + row[i], bar);
-          bulk_load_16(sc + 32, p.v_scale + pg[i] * p.vs_page + head * p.vs_head + row[i], bar);
+      uint64_t* bar = &bars[ask_stage];
+      const uint32_t at = ring_at + ask_stage * T::STAGE, sc = scales_at + ask_stage * T::SCALES;
+      fence_proxy_async();
+      mbar_expect_tx(bar, boxes * (T::K_BOX + T::V_BOX) + (F8 ? 32 * ((pg[0] >= 0) + (boxes > 1 && pg[1] >= 0)) : 0));
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (i < boxes) {
+          tma_load_page(at + i * T::K_BOX, &k_map, bar, row[i], head, pg[i]);
+          tma_load_page(at + 2 * T::K_BOX + i * T::V_BOX, &v_map, bar, row[i], head, pg[i]);
+          if (F8 && pg[i] >= 0) {
+            bulk_load_16(sc + i * 16, p.k_scale + pg[i] * p.ks_page + head * p.ks_head + row[i], bar);
+            bulk_load_16(sc + 32 + i * 16, p.v_scale + pg[i] * p.vs_page + head * p.vs_head + row[i], bar);
+          }
         }
-      }
     });
     ++asked;
     if (++ask_stage == ST) ask_stage = 0;
-    if (++ahead.at == ahead.s.steps) ahead.next_head(p);
-    if (asked < steps) look_up();
+    if (asked >= steps) return;
+    if (++ahead.at == ahead.s.steps) {
+      ahead.next_head(p);
+      find_page();
+    } else {
+      for (at_row += PD_KEYS; at_row >= p.page; at_row -= p.page) ++at_page;
+    }
+    look_up();
   };
   while (asked < steps && asked < ST) ask();
 
   const int g = lane >> 2, t = lane & 3;
+  constexpr int NT = WIDE ? 2 : 1;         // blocks of eight query heads
   int done = 0, seg = 0, h0 = 0, rows = 0;
-  float o[DV / 8][4], m0, m1, l0, l1;
+  // Of heads 8 nt + 2t and the one after: columns 16 c + (0 .. 15), two of them to a lane (see column()), maxima and sums.
+  float o[NT][DV / 16][4], m[NT][2], l[NT][2];
   bool joins = false;          // this warp's last (sequence, head) goes on in the next one, and it is the one to join them
+  auto column = [&](int c, int hi) { return 16 * c + (F8 ? 2 * g + hi : g + 8 * hi); };
   auto put_result = [&]() {
 #pragma unroll
-    for (int hh = 0; hh < (WIDE ? 2 : 1); ++hh) {
-      const int r = g + 8 * hh;
-      if (r >= rows) continue;
-      const float inv = 1.f / (hh ? l1 : l0);
-      __nv_bfloat16* dst = p.out + ((long long)c.b * p.Hkv * p.G + h0 + r) * DV;
-      if constexpr (!F8) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int n = 0; n < DV / 8; ++n)
-          *reinterpret_cast<uint32_t*>(dst + n * 8 + 2 * t) = pack_bf16(o[n][2 * hh] * inv, o[n][2 * hh + 1] * inv);
-      } else {
+      for (int x = 0; x < 2; ++x) {
+        const int r = 8 * nt + 2 * t + x;
+        if (r >= rows) continue;
+        const float inv = 1.f / l[nt][x];
+        __nv_bfloat16* dst = p.out + ((long long)c.b * p.Hkv * p.G + h0 + r) * DV;
 #pragma unroll
-        for (int n = 0; n < DV / 8; n += 2)
-          *reinterpret_cast<uint2*>(dst + n * 8 + 4 * t) = make_uint2(pack_bf16(o[n][2 * hh] * inv, o[n + 1][2 * hh] * inv),
-                                                                      pack_bf16(o[n][2 * hh + 1] * inv, o[n + 1][2 * hh + 1] * inv));
+        for (int cb = 0; cb < DV / 16; ++cb) {
+          const uint32_t both = pack_bf16(o[nt][cb][x] * inv, o[nt][cb][2 + x] * inv);
+          if constexpr (F8) {
+            *reinterpret_cast<uint32_t*>(dst + column(cb, 0)) = both;
+          } else {
+            reinterpret_cast<uint16_t*>(dst)[column(cb, 0)] = (uint16_t)both;
+            reinterpret_cast<uint16_t*>(dst)[column(cb, 1)] = (uint16_t)(both >> 16);
+          }
+        }
       }
-    }
   };
   auto put_part = [&](int slot) {
 #pragma unroll
-    for (int hh = 0; hh < (WIDE ? 2 : 1); ++hh) {
-      const int r = g + 8 * hh;
-      if (r >= rows) continue;
-      float* dst = p.part_o + (long long)(slot * p.rows + r) * DV;
-      if constexpr (!F8) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int n = 0; n < DV / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8 + 2 * t) = make_float2(o[n][2 * hh], o[n][2 * hh + 1]);
-      } else {
+      for (int x = 0; x < 2; ++x) {
+        const int r = 8 * nt + 2 * t + x;
+        if (r >= rows) continue;
+        float* dst = p.part_o + (long long)(slot * p.rows + r) * DV;
 #pragma unroll
-        for (int n = 0; n < DV / 8; n += 2)
-          *reinterpret_cast<float4*>(dst + n * 8 + 4 * t) = make_float4(o[n][2 * hh], o[n + 1][2 * hh], o[n][2 * hh + 1], o[n + 1][2 * hh + 1]);
+        for (int cb = 0; cb < DV / 16; ++cb) {
+          if constexpr (F8) {
+            *reinterpret_cast<float2*>(dst + column(cb, 0)) = make_float2(o[nt][cb][x], o[nt][cb][2 + x]);
+          } else {
+            dst[column(cb, 0)] = o[nt][cb][x];
+            dst[column(cb, 1)] = o[nt][cb][2 + x];
+          }
+        }
+        if (g == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * p.rows + r) * 2) = make_float2(m[nt][x], l[nt][x]);
       }
-      if (t == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * p.rows + r) * 2) = make_float2(hh ? m1 : m0, hh ? l1 : l0);
-    }
   };
   while (done < steps) {
     seg = min(steps - done, c.s.steps - c.at);
     const int kv_head = c.hb / p.blocks, row0 = (c.hb - kv_head * p.blocks) * 16;
     rows = min(16, p.G - row0);
     h0 = kv_head * p.G + row0;
-    // ---- the queries as A operands
-    uint32_t qa[DK / 16][4];
-    float qs0 = p.scale_log2, qs1 = p.scale_log2;
-    {
-      const __nv_bfloat16* q0 = p.q + c.b * p.q_b + (h0 + g) * p.q_h;
-      const __nv_bfloat16* q1 = q0 + 8 * p.q_h;
-      const bool has0 = g < rows, has1 = WIDE && g + 8 < rows;
+    // ---- the queries as B operands: head g of each block of eight, two (e4m3: four) neighbouring columns to a register pair
+    uint32_t qb[DK / 16][NT][2];
+    float qs[NT][2];                       // factors of the scores of heads 2t and 2t + 1
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const __nv_bfloat16* q = p.q + c.b * p.q_b + (h0 + 8 * nt + g) * p.q_h;
+      const bool has = 8 * nt + g < rows;
       if constexpr (!F8) {
 #pragma unroll
         for (int k = 0; k < DK / 16; ++k) {
-          qa[k][0] = has0 ? *reinterpret_cast<const uint32_t*>(q0 + k * 16 + 2 * t) : 0;
-          qa[k][2] = has0 ? *reinterpret_cast<const uint32_t*>(q0 + k * 16 + 8 + 2 * t) : 0;
-          qa[k][1] = has1 ? *reinterpret_cast<const uint32_t*>(q1 + k * 16 + 2 * t) : 0;
-          qa[k][3] = has1 ? *reinterpret_cast<const uint32_t*>(q1 + k * 16 + 8 + 2 * t) : 0;
+          qb[k][nt][0] = has ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 2 * t) : 0;
+          qb[k][nt][1] = has ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 8 + 2 * t) : 0;
         }
+        qs[nt][0] = qs[nt][1] = p.scale_log2;
       } else {
-        uint32_t m0 = 0, m1 = 0;
+        uint32_t most = 0;
 #pragma unroll
         for (int k = 0; k < DK / 16; ++k) {
-          const uint2 a = has0 ? *reinterpret_cast<const uint2*>(q0 + k * 16 + 4 * t) : make_uint2(0, 0);
-          const uint2 b = has1 ? *reinterpret_cast<const uint2*>(q1 + k * 16 + 4 * t) : make_uint2(0, 0);
-          qa[k][0] = a.x; qa[k][2] = a.y; qa[k][1] = b.x; qa[k][3] = b.y;
-          m0 = __vmaxu2(m0, __vmaxu2(a.x & 0x7fff7fffu, a.y & 0x7fff7fffu));
-          m1 = __vmaxu2(m1, __vmaxu2(b.x & 0x7fff7fffu, b.y & 0x7fff7fffu));
+          const uint2 a = has ? *reinterpret_cast<const uint2*>(q + k * 16 + 4 * t) : make_uint2(0, 0);
+          qb[k][nt][0] = a.x;
+          qb[k][nt][1] = a.y;
+          most = __vmaxu2(most, __vmaxu2(a.x & 0x7fff7fffu, a.y & 0x7fff7fffu));
         }
-        auto factor = [&](uint32_t m, float& back) {       // 2^(14 - exponent of the largest), and 1 / of it into `back`
-          m = max(m & 0xffffu, m >> 16);
-          m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-          m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-          const int e = min(max((int)(m >> 7) - 127 - 14, -100), 113);
-          back *= __int_as_float((127 + e) << 23);
-          return __int_as_float((127 - e) << 23);
-        };
-        const float f0 = factor(m0, qs0), f1 = WIDE ? factor(m1, qs1) : 0.f;
+        most = max(most & 0xffffu, most >> 16);
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const int e = min(max((int)(most >> 7) - 127 - 14, -100), 113);       // the largest becomes 2^14 and more
+        const float f = __int_as_float((127 - e) << 23), back = p.scale_log2 * __int_as_float((127 + e) << 23);
+        qs[nt][0] = __shfl_sync(0xffffffffu, back, 8 * t);
+        qs[nt][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
 #pragma unroll
         for (int k = 0; k < DK / 16; ++k)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            if (!WIDE && (x & 1)) { qa[k][x] = 0; continue; }
-            const float2 v = unpack_bf16(qa[k][x]);
-            const float f = x & 1 ? f1 : f0;
-            qa[k][x] = pack_f16(v.x * f, v.y * f);
+          for (int x = 0; x < 2; ++x) {
+            const float2 v = unpack_bf16(qb[k][nt][x]);
+            qb[k][nt][x] = pack_f16(v.x * f, v.y * f);
           }
       }
-    }
 #pragma unroll
-    for (int n = 0; n < DV / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-    m0 = m1 = -INFINITY;
-    l0 = l1 = 0.f;
+      for (int cb = 0; cb < DV / 16; ++cb) o[nt][cb][0] = o[nt][cb][1] = o[nt][cb][2] = o[nt][cb][3] = 0.f;
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
 
     for (int i = 0; i < seg; ++i) {
       const int key0 = c.key0() + i * PD_KEYS;
+      // (a wait that gives up ends the asking; what was asked for is still waited for, each time with a limit)
       if (done + i < asked && !mbar_wait_warp(&bars[stage], parity, p.status, kTimeoutTmaFull, 73)) alive = false;
+      const uint32_t k_at = ring_at + stage * T::STAGE, v_at = k_at + 2 * T::K_BOX;
+      const bool edge = key0 < c.s.lo || key0 + PD_KEYS > c.s.len;
       if (alive) {
-        const uint32_t k_at = ring_at + stage * T::STAGE, v_at = k_at + 2 * T::K_BOX;
-        const bool edge = key0 < c.s.lo || key0 + PD_KEYS > c.s.len;
         if (edge) {
           // Rows behind the end (or in front of the window) hold anything, NaN too: zeros in the values, -inf in the scores.
           uint4* v = reinterpret_cast<uint4*>(ring + stage * T::STAGE + 2 * T::K_BOX);
@@ -386,127 +416,146 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             const int key = key0 + x / (T::V_BOX / 16) * 16 + x % (T::BLOCK / 16) / (T::ROW / 16);
             if (key < c.s.lo || key >= c.s.len) v[x] = make_uint4(0, 0, 0, 0);
           }
-          fence_proxy_async();
           __syncwarp();
         }
-        // ---- scores: 16 heads x 32 tokens
-        float s[4][4] = {};
+        float s[2][NT][4] = {};
+        float factor[2][2], add[2][2];     // e4m3: powers of two of the keys, exponents of the values
+        if constexpr (F8) {
+          const uint8_t* sc = scales + stage * T::SCALES;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            factor[x >> 1][x & 1] = __int_as_float((int)sc[x * 8 + g] << 23);
+            add[x >> 1][x & 1] = (float)((int)sc[32 + x * 8 + g] - 127);
+          }
+        }
+        // ---- scores, transposed: 2 x 16 tokens by 8 heads; s[mt][nt] = (token g: heads 2t, 2t + 1; token g + 8: the same)
         if constexpr (!F8) {
-          const uint32_t at = k_at + (lane & 7) * 128;
+          const uint32_t at = k_at + ((lane & 7) + ((lane >> 3) & 1) * 8) * 128;
 #pragma unroll
-          for (int kk = 0; kk < DK / 32; ++kk)
+          for (int k = 0; k < DK / 16; ++k)
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              uint32_t b[4];
-              pd_ldsm(at + (n >> 1) * T::K_BOX + (kk >> 1) * T::BLOCK + (n & 1) * 1024 + ((((kk & 1) * 4 + (lane >> 3)) ^ (lane & 7)) << 4), b);
-              pd_mma<false>(s[n], qa[2 * kk], b[0], b[1]);
-              pd_mma<false>(s[n], qa[2 * kk + 1], b[2], b[3]);
+            for (int mt = 0; mt < 2; ++mt) {
+              uint32_t a[4];
+              pd_ldsm(at + mt * T::K_BOX + (k >> 2) * T::BLOCK + ((((k & 3) * 2 + (lane >> 4)) ^ (lane & 7)) << 4), a);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) pd_mma<false>(s[mt][nt], a, qb[k][nt][0], qb[k][nt][1]);
             }
         } else {
           const uint32_t at = k_at + (lane & 7) * 64 + (((lane >> 3) ^ ((lane & 7) >> 1)) << 4);
 #pragma unroll
           for (int hf = 0; hf < DK / 64; ++hf)
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              uint32_t b[4];
-              pd_ldsm(at + (n >> 1) * T::K_BOX + hf * T::BLOCK + (n & 1) * 512, b);
+            for (int mt = 0; mt < 2; ++mt) {
+              uint32_t lo[4], hi[4];       // tokens 0 - 7 and 8 - 15, 16 columns each
+              pd_ldsm(at + mt * T::K_BOX + hf * T::BLOCK, lo);
+              pd_ldsm(at + mt * T::K_BOX + hf * T::BLOCK + 512, hi);
 #pragma unroll
-              for (int x = 0; x < 4; ++x) pd_mma<true>(s[n], qa[4 * hf + x], e4m3_to_f16(b[x]), e4m3_to_f16(b[x] >> 16));
+              for (int x = 0; x < 4; ++x) {
+                const uint32_t a[4] = {e4m3_to_f16(lo[x]), e4m3_to_f16(hi[x]), e4m3_to_f16(lo[x] >> 16), e4m3_to_f16(hi[x] >> 16)};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) pd_mma<true>(s[mt][nt], a, qb[4 * hf + x][nt][0], qb[4 * hf + x][nt][1]);
+              }
             }
         }
         // ---- running softmax
-        float add[4][2];                   // exponents of the values' rows
-        const uint8_t* sc = scales + stage * T::SCALES;
-        float n0 = m0, n1 = m1;
+        uint32_t pb[2][NT][2];             // the weights as B operands: token pairs by head
+        float top[NT][2];
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int nt = 0; nt < NT; ++nt) top[nt][0] = m[nt][0], top[nt][1] = m[nt][1];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const int key = key0 + n * 8 + 2 * t + x;
-            float f = 1.f;
-            add[n][x] = 0.f;
-            if (F8) {
-              f = __int_as_float((int)sc[n * 8 + 2 * t + x] << 23);
-              add[n][x] = (float)((int)sc[32 + n * 8 + 2 * t + x] - 127);
-            }
-            const bool dead = edge && (key < c.s.lo || key >= c.s.len);
-            auto score = [&](float v, float qs) {
-              v *= F8 ? qs * f : qs;
-              if (p.cap_log2 > 0.f) v = p.cap_log2 * (1.f - __fdividef(2.f, ex2_approx(v / p.cap_log2 * 2.8853900817779268f) + 1.f));
-              return dead ? -INFINITY : v;
-            };
-            s[n][x] = score(s[n][x], qs0);
-            n0 = fmaxf(n0, s[n][x] + add[n][x]);
-            if (WIDE) {
-              s[n][2 + x] = score(s[n][2 + x], qs1);
-              n1 = fmaxf(n1, s[n][2 + x] + add[n][x]);
-            }
-          }
-        n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 1));
-        n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, 2));
-        if (WIDE) {
-          n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 1));
-          n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, 2));
-        }
-        if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
-          const float a0 = n0 > m0 ? ex2_approx(m0 - n0) : 1.f, a1 = n1 > m1 ? ex2_approx(m1 - n1) : 1.f;
-          l0 *= a0;
-          l1 *= a1;
+        for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-          for (int n = 0; n < DV / 8; ++n) {
-            o[n][0] *= a0; o[n][1] *= a0;
-            if (WIDE) { o[n][2] *= a1; o[n][3] *= a1; }
-          }
-          m0 = n0;
-          m1 = n1;
-        }
-        const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;      // (all scores so far are NaN or -inf)
-        uint32_t pa[2][4];
+          for (int hi = 0; hi < 2; ++hi) {
+            const int in = mt * 16 + hi * 8 + g;
+            const bool dead = edge && (key0 + in < c.s.lo || key0 + in >= c.s.len);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          float w[4] = {};
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            w[x] = ex2_approx(s[n][x] + add[n][x] - r0);
-            l0 += F8 ? ex2_approx(s[n][x] - r0) : w[x];
-            if (WIDE) {
-              w[2 + x] = ex2_approx(s[n][2 + x] + add[n][x] - r1);
-              l1 += F8 ? ex2_approx(s[n][2 + x] - r1) : w[2 + x];
-            }
-          }
-          pa[n >> 1][(n & 1) * 2] = F8 ? pack_f16(w[0], w[1]) : pack_bf16(w[0], w[1]);
-          pa[n >> 1][(n & 1) * 2 + 1] = !WIDE ? 0 : F8 ? pack_f16(w[2], w[3]) : pack_bf16(w[2], w[3]);
-        }
-        // ---- weighted sum
-        const int vr = (lane & 7) + ((lane >> 3) & 1) * 8;
-        if constexpr (!F8) {
-#pragma unroll
-          for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-            for (int np = 0; np < DV / 16; ++np) {
-              uint32_t b[4];
-              pd_ldsm_t(v_at + ks * T::V_BOX + (np >> 2) * T::BLOCK + vr * 128 + ((((np & 3) * 2 + (lane >> 4)) ^ (lane & 7)) << 4), b);
-              pd_mma<false>(o[2 * np], pa[ks], b[0], b[1]);
-              pd_mma<false>(o[2 * np + 1], pa[ks], b[2], b[3]);
-            }
-        } else {
-#pragma unroll
-          for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-            for (int cp = 0; cp < DV / 32; ++cp) {
-              uint32_t b[4];
-              pd_ldsm_t(v_at + ks * T::V_BOX + (cp >> 1) * T::BLOCK + vr * 64 + ((((cp & 1) * 2 + (lane >> 4)) ^ ((vr >> 1) & 3)) << 4), b);
-#pragma unroll
-              for (int x = 0; x < 4; ++x) b[x] = __byte_perm(b[x], 0, 0x3120);      // even columns of two tokens, odd ones
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int x = 0; x < 2; ++x) {
-                pd_mma<true>(o[4 * cp + 2 * x], pa[ks], e4m3_to_f16(b[2 * x]), e4m3_to_f16(b[2 * x + 1]));
-                pd_mma<true>(o[4 * cp + 2 * x + 1], pa[ks], e4m3_to_f16(b[2 * x] >> 16), e4m3_to_f16(b[2 * x + 1] >> 16));
+                float v = s[mt][nt][2 * hi + x] * (F8 ? qs[nt][x] * factor[mt][hi] : qs[nt][x]);
+                if (p.cap_log2 > 0.f) v = p.cap_log2 * (1.f - __fdividef(2.f, ex2_approx(v / p.cap_log2 * 2.8853900817779268f) + 1.f));
+                v = dead ? -INFINITY : v;
+                s[mt][nt][2 * hi + x] = v;
+                top[nt][x] = fmaxf(top[nt][x], F8 ? v + add[mt][hi] : v);
+              }
+          }
+        bool grown = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) top[nt][x] = fmaxf(top[nt][x], __shfl_xor_sync(0xffffffffu, top[nt][x], off));
+            grown |= top[nt][x] > m[nt][x];
+          }
+        if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float a[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              a[x] = top[nt][x] > m[nt][x] ? ex2_approx(m[nt][x] - top[nt][x]) : 1.f;
+              l[nt][x] *= a[x];
+              m[nt][x] = top[nt][x];
+            }
+#pragma unroll
+            for (int cb = 0; cb < DV / 16; ++cb) {
+              o[nt][cb][0] *= a[0]; o[nt][cb][1] *= a[1];
+              o[nt][cb][2] *= a[0]; o[nt][cb][3] *= a[1];
+            }
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float from[2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x) from[x] = m[nt][x] == -INFINITY ? 0.f : m[nt][x];      // (all scores so far are NaN or -inf)
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int hi = 0; hi < 2; ++hi) {
+              float w[2];
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const float v = s[mt][nt][2 * hi + x] - from[x];
+                w[x] = ex2_approx(F8 ? v + add[mt][hi] : v);
+                l[nt][x] += F8 ? ex2_approx(v) : w[x];
+              }
+              pb[mt][nt][hi] = transpose_8x8(F8 ? pack_f16(w[0], w[1]) : pack_bf16(w[0], w[1]));
+            }
+        }
+        // ---- weighted sum, transposed: 16 columns by 8 heads
+        if constexpr (!F8) {
+          const uint32_t at = v_at + ((lane & 7) + (lane >> 4) * 8) * 128;
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int cb = 0; cb < DV / 16; ++cb) {
+              uint32_t a[4];
+              pd_ldsm_t(at + mt * T::V_BOX + (cb >> 2) * T::BLOCK + ((((cb & 3) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4), a);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) pd_mma<false>(o[nt][cb], a, pb[mt][nt][0], pb[mt][nt][1]);
+            }
+        } else {
+          const int vr = (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int cp = 0; cp < DV / 32; ++cp) {
+              uint32_t b[4];               // tokens 0 - 7 and 8 - 15 of 16 columns, then of the next 16
+              pd_ldsm_t(v_at + mt * T::V_BOX + (cp >> 1) * T::BLOCK + vr * 64 + ((((cp & 1) * 2 + (lane >> 4)) ^ ((vr >> 1) & 3)) << 4), b);
+#pragma unroll
+              for (int x = 0; x < 4; ++x) b[x] = __byte_perm(b[x], 0, 0x3120);      // two tokens of an even column, of the odd one behind it
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const uint32_t a[4] = {e4m3_to_f16(b[2 * x]), e4m3_to_f16(b[2 * x] >> 16), e4m3_to_f16(b[2 * x + 1]), e4m3_to_f16(b[2 * x + 1] >> 16)};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) pd_mma<true>(o[nt][2 * cp + x], a, pb[mt][nt][0], pb[mt][nt][1]);
               }
             }
         }
       }
-      __syncwarp();                        // the stage is used up
+      __syncwarp();                        // the stage has been read
       if (alive && asked < steps) ask();
       if (++stage == ST) {
         stage = 0;
@@ -515,12 +564,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     }
 
     // ---- the result, or this warp's part of it
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    if (WIDE) {
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], off);
     const bool starts = c.at == 0, ends = c.at + seg == c.s.steps;
     done += seg;
     if (starts && ends) {
@@ -544,34 +593,24 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       const int at = 2 * gridDim.x + blockIdx.x * NW + w;
       ends = s_ends[w];
 #pragma unroll
-      for (int hh = 0; hh < (WIDE ? 2 : 1); ++hh) {
-        const int r = g + 8 * hh;
-        if (r >= rows) continue;
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (at * p.rows + r) * 2);
-        const float* src = p.part_o + (long long)(at * p.rows + r) * DV;
-        float &m = hh ? m1 : m0, &l = hh ? l1 : l0;
-        const float top = fmaxf(m, ml.x);
-        const float fa = m == -INFINITY ? 0.f : ex2_approx(m - top), fb = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
-        m = top;
-        l = l * fa + ml.y * fb;
-        if constexpr (!F8) {
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int n = 0; n < DV / 8; ++n) {
-            const float2 v = *reinterpret_cast<const float2*>(src + n * 8 + 2 * t);
-            o[n][2 * hh] = o[n][2 * hh] * fa + v.x * fb;
-            o[n][2 * hh + 1] = o[n][2 * hh + 1] * fa + v.y * fb;
-          }
-        } else {
+        for (int x = 0; x < 2; ++x) {
+          const int r = 8 * nt + 2 * t + x;
+          if (r >= rows) continue;
+          const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (at * p.rows + r) * 2);
+          const float* src = p.part_o + (long long)(at * p.rows + r) * DV;
+          const float top = fmaxf(m[nt][x], ml.x);
+          const float fa = m[nt][x] == -INFINITY ? 0.f : ex2_approx(m[nt][x] - top), fb = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
+          m[nt][x] = top;
+          l[nt][x] = l[nt][x] * fa + ml.y * fb;
 #pragma unroll
-          for (int n = 0; n < DV / 8; n += 2) {
-            const float4 v = *reinterpret_cast<const float4*>(src + n * 8 + 4 * t);
-            o[n][2 * hh] = o[n][2 * hh] * fa + v.x * fb;
-            o[n + 1][2 * hh] = o[n + 1][2 * hh] * fa + v.y * fb;
-            o[n][2 * hh + 1] = o[n][2 * hh + 1] * fa + v.z * fb;
-            o[n + 1][2 * hh + 1] = o[n + 1][2 * hh + 1] * fa + v.w * fb;
+          for (int cb = 0; cb < DV / 16; ++cb) {
+            const float2 v = F8 ? *reinterpret_cast<const float2*>(src + column(cb, 0)) : make_float2(src[column(cb, 0)], src[column(cb, 1)]);
+            o[nt][cb][x] = o[nt][cb][x] * fa + v.x * fb;
+            o[nt][cb][2 + x] = o[nt][cb][2 + x] * fa + v.y * fb;
           }
         }
-      }
     }
     if (c.at == 0 && ends) {
       put_result();
@@ -639,7 +678,6 @@ paged_join_kernel(const PagedDecode p) {
   }
 }
 
-static int pd_warps(int DK, int DV, bool held8) { return 64 * (DK + DV) / (held8 ? 2 : 1) <= 10240 ? 8 : 4; }
 static int pd_grid(long long most_steps) {
   const long long sms = sm_count();
   return (int)(most_steps < 1 ? 1 : most_steps < sms ? most_steps : sms);
@@ -647,7 +685,7 @@ static int pd_grid(long long most_steps) {
 
 template <int DK, int DV, bool F8, bool WIDE>
 static int launch_paged_decode(PagedDecode p, int grid, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t stream) {
-  using T = PagedTile<DK, DV, F8>;
+  using T = PagedTile<DK, DV, F8, WIDE>;
   constexpr int MOST = 227 * 1024 - 1024 - 1024;      // (static arrays; alignment)
   p.stages = MOST / (T::WARPS * (T::STAGE + T::SCALES + 8));
   if (p.stages > 8) p.stages = 8;
@@ -666,9 +704,9 @@ static int launch_paged_decode(PagedDecode p, int grid, const CUtensorMap& km, c
 using namespace tpb;
 
 // Bytes of scratch for tpb_paged_decode.
-extern "C" int tpb_paged_decode_scratch(int B, int Hkv, int G, int DK, int DV, int held8, int capacity) {
+extern "C" int tpb_paged_decode_scratch(int B, int Hkv, int G, int DV, int held8, int capacity) {
   const long long steps = (long long)B * Hkv * ((G + 15) / 16) * (((long long)capacity + PD_KEYS - 1) / PD_KEYS);
-  return pd_grid(steps) * ((2 + pd_warps(DK, DV, held8 != 0)) * (G < 16 ? G : 16) * (DV + 2) * 4 + 16);
+  return pd_grid(steps) * ((2 + pd_warps(held8 != 0, G > 8)) * (G < 16 ? G : 16) * (DV + 2) * 4 + 16);
 }
 
 // q [B, Hkv * G, DK] bf16 (strides q_b, q_h), pools as in tpb_paged_rows (strides of pages, tokens, heads; scales contiguous over
@@ -713,7 +751,7 @@ extern "C" int tpb_paged_decode(const void* q, long long q_b, long long q_h, con
   p.vs_head = strides[11];
   const int grid = pd_grid(steps);
   p.rows = G < 16 ? G : 16;
-  const long long part_rows = (long long)grid * (2 + pd_warps(DK, DV, held8)) * p.rows;
+  const long long part_rows = (long long)grid * (2 + pd_warps(held8, G > 8)) * p.rows;
   p.split = static_cast<int4*>(scratch);
   p.part_o = reinterpret_cast<float*>(p.split + grid);
   p.part_ml = p.part_o + part_rows * DV;

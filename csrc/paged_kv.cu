@@ -31,19 +31,6 @@ struct PagedRows {
 constexpr int PAGED_THREADS = 256;
 constexpr int PAGED_ROWS = 4;        // sets of rows per warp under way together
 
-// Two floats to two e4m3 values, the first in the low byte; saturating, to nearest even.
-__device__ __forceinline__ uint32_t to_e4m3x2(float lo, float hi) {
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float2 from_e4m3x2(uint32_t v) {
-  uint32_t h;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)v));
-  float2 f;
-  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(f.x), "=f"(f.y) : "r"(h));
-  return f;
-}
 // The larger magnitude of each 16-bit half among finite bf16 values, as bits.
 __device__ __forceinline__ uint32_t finite_max(uint32_t m, uint32_t v) {
   v &= 0x7fff7fffu;
