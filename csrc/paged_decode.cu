@@ -49,17 +49,24 @@ struct PagedDecode {
   int4* split;                             // [CTAs] of the (sequence, head block) that begins in a CTA and goes on: last CTA, slot; or -1
   int* status;
   int B, Hkv, G, blocks, rows;             // blocks of up to 16 query heads to a key head; rows of the largest block
-  int pages, page, capacity;               // tokens that a row of the table can name
+  int pages, page, width, capacity;        // entries of a row of the table, tokens that it can name
   int window, stages;
   float scale_log2, cap_log2;              // cap_log2: the cap in log2 units, 0 for none
 };
 
-constexpr int PD_KEYS = 32;                // tokens of a warp's step, two boxes
 
-#ifndef PD_W8W
-#define PD_W8W 8
-#endif
-constexpr int pd_warps(bool held8, bool wide) { return held8 ? (wide ? PD_W8W : 16) : 8; }
+struct PagedShape {
+  int keys, warps;         // tokens of a warp's step, warps to a CTA
+};
+// One CTA takes the SM's shared memory, a warp at least one stage of it: many warps with one stage each keep as many bytes under way
+// as few with several, and hide the conversions of an 8-bit cache better.  us, 64 sequences of up to 8192 tokens, 64 / 8 heads of 128
+// in e4m3: 4 warps 159, 8 118, 16 (scores transposed) 90; 128 of 32 / 8 heads in bf16: 4 warps 277, 6 266, 8 261.  Narrow heads take 64
+// tokens to a step (8 / 8 heads of 64 columns, 64 sequences, bf16 50 -> 44 us, e4m3 60 -> 57), which costs wide ones their
+// registers or stages; with more than 8 query heads to a key head eight warps have registers (64 / 2 heads of 192 / 128 in e4m3:
+// 8 warps 35 us, 10 45, 12 40).
+constexpr PagedShape pd_shape(bool held8, bool wide, int width) {
+  return {width <= 128 || (held8 && wide && width <= 256) ? 64 : 32, held8 && !wide ? 16 : 8};
+}
 
 template <int DK, int DV, bool F8, bool WIDE>
 struct PagedTile {
@@ -67,11 +74,10 @@ struct PagedTile {
   static constexpr int ROW = 64 * ELT;                       // bytes of a 64-column block's row: the swizzle's width
   static constexpr int BLOCK = 16 * ROW;
   static constexpr int K_BOX = 16 * DK * ELT, V_BOX = 16 * DV * ELT;
-  static constexpr int STAGE = 2 * (K_BOX + V_BOX);
-  static constexpr int SCALES = F8 ? 64 : 0;                 // 32 of the keys, 32 of the values
-  // Warps to a CTA: as many as have two stages or more each, up to eight.  An 8-bit cache brings a step's bytes in half the time,
-  // and the step takes longer (conversions): four warps 159 us for 64 sequences of up to 8192 tokens, 64 / 8 heads of 128; eight 118.
-  static constexpr int WARPS = pd_warps(F8, WIDE);
+  static constexpr int KEYS = pd_shape(F8, WIDE, DK + DV).keys, BOXES = KEYS / 16;
+  static constexpr int STAGE = BOXES * (K_BOX + V_BOX);
+  static constexpr int SCALES = F8 ? 2 * KEYS : 0;           // of the keys, of the values
+  static constexpr int WARPS = pd_shape(F8, WIDE, DK + DV).warps;
 };
 
 __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int row, int head, int page) {
@@ -129,12 +135,13 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
 struct Visible {
   int len, lo, first, steps;
 };
+template <int KEYS>
 __device__ __forceinline__ Visible pd_visible(const PagedDecode& p, int b) {
   Visible s;
   s.len = min(max(p.lengths[b], 0), p.capacity);
   s.lo = p.window > 0 ? max(0, s.len - p.window) : 0;
-  s.first = s.lo / PD_KEYS;
-  s.steps = s.len > 0 ? (s.len - 1) / PD_KEYS - s.first + 1 : 0;
+  s.first = s.lo / KEYS;
+  s.steps = s.len > 0 ? (s.len - 1) / KEYS - s.first + 1 : 0;
   return s;
 }
 
@@ -142,10 +149,11 @@ __device__ __forceinline__ Visible pd_visible(const PagedDecode& p, int b) {
 __device__ __forceinline__ int pd_share(int steps, int n) { return max(1, (steps + n - 1) / n); }
 
 // A place in the list of steps.
+template <int KEYS>
 struct PagedCursor {
   int b, hb, at;           // sequence, head block, step of the sequence
   Visible s;
-  __device__ __forceinline__ int key0() const { return (s.first + at) * PD_KEYS; }
+  __device__ __forceinline__ int key0() const { return (s.first + at) * KEYS; }
   __device__ __forceinline__ void next_head(const PagedDecode& p) {
     at = 0;
     if (++hb < p.Hkv * p.blocks) return;
@@ -153,7 +161,7 @@ struct PagedCursor {
     do {
       ++b;
       if (b >= p.B) return;
-      s = pd_visible(p, b);
+      s = pd_visible<KEYS>(p, b);
     } while (s.steps == 0);
   }
 };
@@ -162,7 +170,7 @@ template <int DK, int DV, bool F8, bool WIDE>
 __global__ void __launch_bounds__(PagedTile<DK, DV, F8, WIDE>::WARPS * 32, 1)
 paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const PagedDecode p) {
   using T = PagedTile<DK, DV, F8, WIDE>;
-  constexpr int NW = T::WARPS, THREADS = NW * 32;
+  constexpr int NW = T::WARPS, THREADS = NW * 32, KEYS = T::KEYS, MT = T::BOXES;
   extern __shared__ uint8_t pd_smem_raw[];
   uint8_t* pd_smem = pd_smem_raw + ((1024u - (smem_u32(pd_smem_raw) & 1023u)) & 1023u);
   __shared__ int s_scan[NW], s_at[NW][3], s_ends[NW];
@@ -180,6 +188,24 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   }
   fence_barrier_init();
   chain_launch();
+  // Lengths, table and queries are read one after the other, each a trip to memory unless something has brought them to L2.
+  {
+    const int q_lines = DK * 2 / 128, t_lines = (p.width + 31) / 32, n_lines = (p.B + 31) / 32, stride = gridDim.x * THREADS;
+    const long long lines = n_lines + (long long)p.B * (t_lines + p.Hkv * p.G * q_lines);
+    if (lines <= 8 * stride)
+      for (int i = blockIdx.x * THREADS + threadIdx.x; i < lines; i += stride) {
+        int x = i - n_lines;
+        const void* at = p.lengths + 32 * i;
+        if (x >= p.B * t_lines) {
+          x -= p.B * t_lines;
+          const int row = x / q_lines;
+          at = p.q + row / (p.Hkv * p.G) * p.q_b + row % (p.Hkv * p.G) * p.q_h + x % q_lines * 64;
+        } else if (x >= 0) {
+          at = p.table + x / t_lines * p.table_b + x % t_lines * 32;
+        }
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+      }
+  }
   if (!chain_wait()) return;
 
   // The list's length, and where this CTA's part and its warps' begin.
@@ -187,7 +213,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   int before = 0, n = 0;                   // of this thread's sequence: steps in front of it (per head block), its own
   auto add_up = [&](int base, int running) {
     const int b = base + threadIdx.x;
-    n = b < p.B ? pd_visible(p, b).steps : 0;
+    n = b < p.B ? pd_visible<KEYS>(p, b).steps : 0;
     int sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -224,86 +250,68 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         }
       }
   }
+  __syncthreads();
+  const int steps = min(share, cta_steps - warp * share);      // (none: 0 or less)
+  PagedCursor<KEYS> c = {};
+  if (steps > 0) {
+    c.b = s_at[warp][0];
+    c.hb = s_at[warp][1];
+    c.at = s_at[warp][2];
+    c.s = pd_visible<KEYS>(p, c.b);
+  }
+  PagedCursor<KEYS> ahead = c;
+  int asked = 0, ask_stage = 0, stage = 0, parity = 0;
+  bool alive = true;
+  // A lane for each box.  The pages of the step that is asked for next are on their way from the table since the one before was.
+  int pg = -1, row = 0;
+  bool seen = false;
+  auto look_up = [&]() {
+    const int key = ahead.key0() + 16 * lane;
+    seen = lane < MT && key < ahead.s.len;
+    const unsigned at = (unsigned)key / (unsigned)p.page;
+    row = key - at * p.page;
+    if (seen) pg = p.table[ahead.b * p.table_b + at];
+  };
+  if (steps > 0) look_up();
+
+  // The fence orders the warp's reads of the stage, in front of the __syncwarp before, ahead of the copy that overwrites it.
+  auto ask = [&]() {
+    uint64_t* bar = &bars[ask_stage];
+    const bool inside = seen && pg >= 0 && pg < p.pages;
+    if (seen && !inside) report(p.status, kBadArgument, 72);      // a box outside the pool reads as zeros
+    const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, seen)) * (T::K_BOX + T::V_BOX) +
+                           (F8 ? __popc(__ballot_sync(0xffffffffu, inside)) * 32 : 0);
+    if (lane == 0) mbar_expect_tx(bar, bytes);
+    __syncwarp();
+    if (seen) {
+      const int head = ahead.hb / p.blocks;
+      const uint32_t at = ring_at + ask_stage * T::STAGE;
+      fence_proxy_async();
+      tma_load_page(at + lane * T::K_BOX, &k_map, bar, row, head, inside ? pg : -1);
+      tma_load_page(at + MT * T::K_BOX + lane * T::V_BOX, &v_map, bar, row, head, inside ? pg : -1);
+      if (F8 && inside) {
+        const uint32_t sc = scales_at + ask_stage * T::SCALES + lane * 16;
+        bulk_load_16(sc, p.k_scale + pg * p.ks_page + head * p.ks_head + row, bar);
+        bulk_load_16(sc + KEYS, p.v_scale + pg * p.vs_page + head * p.vs_head + row, bar);
+      }
+    }
+    __syncwarp();
+    ++asked;
+    if (++ask_stage == ST) ask_stage = 0;
+    if (asked >= steps) return;
+    if (++ahead.at == ahead.s.steps) ahead.next_head(p);
+    look_up();
+  };
+  while (asked < steps && asked < ST) ask();
   if (blockIdx.x == 0)
     for (int b = threadIdx.x; b < p.B; b += THREADS)
       if (p.lengths[b] < 0 || p.lengths[b] > p.capacity) report(p.status, kBadArgument, 71);
   if (threadIdx.x == 0) p.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
   for (int b = blockIdx.x; b < p.B; b += gridDim.x)        // sequences of no visible token
-    if (pd_visible(p, b).steps == 0) {
+    if (pd_visible<KEYS>(p, b).steps == 0) {
       uint4* dst = reinterpret_cast<uint4*>(p.out + (long long)b * p.Hkv * p.G * DV);
       for (int i = threadIdx.x; i < p.Hkv * p.G * (DV / 8); i += THREADS) dst[i] = make_uint4(0, 0, 0, 0);
     }
-  __syncthreads();
-  const int steps = min(share, cta_steps - warp * share);      // (none: 0 or less)
-  PagedCursor c = {};
-  if (steps > 0) {
-    c.b = s_at[warp][0];
-    c.hb = s_at[warp][1];
-    c.at = s_at[warp][2];
-    c.s = pd_visible(p, c.b);
-  }
-  PagedCursor ahead = c;
-  int asked = 0, ask_stage = 0, stage = 0, parity = 0;
-  bool alive = true;
-  // The pages of the step that is asked for next, on their way from the table since the one before was.
-  int at_page = 0, at_row = 0;             // of its first token
-  int pg0 = -1, pg1 = -1, row1 = 0;
-  auto find_page = [&]() {
-    const unsigned key0 = ahead.key0();
-    at_page = key0 / (unsigned)p.page;
-    at_row = key0 - at_page * p.page;
-  };
-  auto look_up = [&]() {
-    const int* row = p.table + ahead.b * p.table_b + at_page;
-    const bool next = at_row + 16 >= p.page;
-    row1 = next ? 0 : at_row + 16;
-    pg0 = row[0];
-    if (ahead.key0() + 16 < ahead.s.len) pg1 = row[next];
-  };
-  if (steps > 0) {
-    find_page();
-    look_up();
-  }
-
-  // The fence orders the warp's reads of the stage, in front of the __syncwarp before, ahead of the copy that overwrites it.
-  auto ask = [&]() {
-    const int boxes = ahead.key0() + 16 < ahead.s.len ? 2 : 1, head = ahead.hb / p.blocks;
-    int pg[2] = {pg0, pg1};
-    const int row[2] = {at_row, row1};
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (i < boxes && (pg[i] < 0 || pg[i] >= p.pages)) {      // a box outside the pool reads as zeros
-        if (lane == 0) report(p.status, kBadArgument, 72);
-        pg[i] = -1;
-      }
-    one_lane([&]() {
-      uint64_t* bar = &bars[ask_stage];
-      const uint32_t at = ring_at + ask_stage * T::STAGE, sc = scales_at + ask_stage * T::SCALES;
-      fence_proxy_async();
-      mbar_expect_tx(bar, boxes * (T::K_BOX + T::V_BOX) + (F8 ? 32 * ((pg[0] >= 0) + (boxes > 1 && pg[1] >= 0)) : 0));
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (i < boxes) {
-          tma_load_page(at + i * T::K_BOX, &k_map, bar, row[i], head, pg[i]);
-          tma_load_page(at + 2 * T::K_BOX + i * T::V_BOX, &v_map, bar, row[i], head, pg[i]);
-          if (F8 && pg[i] >= 0) {
-            bulk_load_16(sc + i * 16, p.k_scale + pg[i] * p.ks_page + head * p.ks_head + row[i], bar);
-            bulk_load_16(sc + 32 + i * 16, p.v_scale + pg[i] * p.vs_page + head * p.vs_head + row[i], bar);
-          }
-        }
-    });
-    ++asked;
-    if (++ask_stage == ST) ask_stage = 0;
-    if (asked >= steps) return;
-    if (++ahead.at == ahead.s.steps) {
-      ahead.next_head(p);
-      find_page();
-    } else {
-      for (at_row += PD_KEYS; at_row >= p.page; at_row -= p.page) ++at_page;
-    }
-    look_up();
-  };
-  while (asked < steps && asked < ST) ask();
 
   const int g = lane >> 2, t = lane & 3;
   constexpr int NT = WIDE ? 2 : 1;         // blocks of eight query heads
@@ -403,38 +411,38 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     }
 
     for (int i = 0; i < seg; ++i) {
-      const int key0 = c.key0() + i * PD_KEYS;
+      const int key0 = c.key0() + i * KEYS;
       // (a wait that gives up ends the asking; what was asked for is still waited for, each time with a limit)
       if (done + i < asked && !mbar_wait_warp(&bars[stage], parity, p.status, kTimeoutTmaFull, 73)) alive = false;
-      const uint32_t k_at = ring_at + stage * T::STAGE, v_at = k_at + 2 * T::K_BOX;
-      const bool edge = key0 < c.s.lo || key0 + PD_KEYS > c.s.len;
+      const uint32_t k_at = ring_at + stage * T::STAGE, v_at = k_at + MT * T::K_BOX;
+      const bool edge = key0 < c.s.lo || key0 + KEYS > c.s.len;
       if (alive) {
         if (edge) {
           // Rows behind the end (or in front of the window) hold anything, NaN too: zeros in the values, -inf in the scores.
-          uint4* v = reinterpret_cast<uint4*>(ring + stage * T::STAGE + 2 * T::K_BOX);
-          for (int x = lane; x < 2 * T::V_BOX / 16; x += 32) {
+          uint4* v = reinterpret_cast<uint4*>(ring + stage * T::STAGE + MT * T::K_BOX);
+          for (int x = lane; x < MT * T::V_BOX / 16; x += 32) {
             const int key = key0 + x / (T::V_BOX / 16) * 16 + x % (T::BLOCK / 16) / (T::ROW / 16);
             if (key < c.s.lo || key >= c.s.len) v[x] = make_uint4(0, 0, 0, 0);
           }
           __syncwarp();
         }
-        float s[2][NT][4] = {};
-        float factor[2][2], add[2][2];     // e4m3: powers of two of the keys, exponents of the values
+        float s[MT][NT][4] = {};
+        float factor[MT][2], add[MT][2];     // e4m3: powers of two of the keys, exponents of the values
         if constexpr (F8) {
           const uint8_t* sc = scales + stage * T::SCALES;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
+          for (int x = 0; x < 2 * MT; ++x) {
             factor[x >> 1][x & 1] = __int_as_float((int)sc[x * 8 + g] << 23);
-            add[x >> 1][x & 1] = (float)((int)sc[32 + x * 8 + g] - 127);
+            add[x >> 1][x & 1] = (float)((int)sc[KEYS + x * 8 + g] - 127);
           }
         }
-        // ---- scores, transposed: 2 x 16 tokens by 8 heads; s[mt][nt] = (token g: heads 2t, 2t + 1; token g + 8: the same)
+        // ---- scores, transposed: 16 tokens by 8 heads each; s[mt][nt] = (token g: heads 2t, 2t + 1; token g + 8: the same)
         if constexpr (!F8) {
           const uint32_t at = k_at + ((lane & 7) + ((lane >> 3) & 1) * 8) * 128;
 #pragma unroll
           for (int k = 0; k < DK / 16; ++k)
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
+            for (int mt = 0; mt < MT; ++mt) {
               uint32_t a[4];
               pd_ldsm(at + mt * T::K_BOX + (k >> 2) * T::BLOCK + ((((k & 3) * 2 + (lane >> 4)) ^ (lane & 7)) << 4), a);
 #pragma unroll
@@ -445,7 +453,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 #pragma unroll
           for (int hf = 0; hf < DK / 64; ++hf)
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
+            for (int mt = 0; mt < MT; ++mt) {
               uint32_t lo[4], hi[4];       // tokens 0 - 7 and 8 - 15, 16 columns each
               pd_ldsm(at + mt * T::K_BOX + hf * T::BLOCK, lo);
               pd_ldsm(at + mt * T::K_BOX + hf * T::BLOCK + 512, hi);
@@ -458,12 +466,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             }
         }
         // ---- running softmax
-        uint32_t pb[2][NT][2];             // the weights as B operands: token pairs by head
+        uint32_t pb[MT][NT][2];             // the weights as B operands: token pairs by head
         float top[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) top[nt][0] = m[nt][0], top[nt][1] = m[nt][1];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int hi = 0; hi < 2; ++hi) {
             const int in = mt * 16 + hi * 8 + g;
@@ -511,7 +519,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 #pragma unroll
           for (int x = 0; x < 2; ++x) from[x] = m[nt][x] == -INFINITY ? 0.f : m[nt][x];      // (all scores so far are NaN or -inf)
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
+          for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int hi = 0; hi < 2; ++hi) {
               float w[2];
@@ -528,7 +536,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         if constexpr (!F8) {
           const uint32_t at = v_at + ((lane & 7) + (lane >> 4) * 8) * 128;
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
+          for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int cb = 0; cb < DV / 16; ++cb) {
               uint32_t a[4];
@@ -539,7 +547,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         } else {
           const int vr = (lane & 7) + ((lane >> 3) & 1) * 8;
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
+          for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int cp = 0; cp < DV / 32; ++cp) {
               uint32_t b[4];               // tokens 0 - 7 and 8 - 15 of 16 columns, then of the next 16
@@ -687,6 +695,7 @@ template <int DK, int DV, bool F8, bool WIDE>
 static int launch_paged_decode(PagedDecode p, int grid, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t stream) {
   using T = PagedTile<DK, DV, F8, WIDE>;
   constexpr int MOST = 227 * 1024 - 1024 - 1024;      // (static arrays; alignment)
+  static_assert(T::WARPS * (T::STAGE + T::SCALES + 8) <= MOST, "every warp has a stage");
   p.stages = MOST / (T::WARPS * (T::STAGE + T::SCALES + 8));
   if (p.stages > 8) p.stages = 8;
   const int smem = 1024 + T::WARPS * p.stages * (T::STAGE + T::SCALES + 8);
@@ -704,9 +713,10 @@ static int launch_paged_decode(PagedDecode p, int grid, const CUtensorMap& km, c
 using namespace tpb;
 
 // Bytes of scratch for tpb_paged_decode.
-extern "C" int tpb_paged_decode_scratch(int B, int Hkv, int G, int DV, int held8, int capacity) {
-  const long long steps = (long long)B * Hkv * ((G + 15) / 16) * (((long long)capacity + PD_KEYS - 1) / PD_KEYS);
-  return pd_grid(steps) * ((2 + pd_warps(held8 != 0, G > 8)) * (G < 16 ? G : 16) * (DV + 2) * 4 + 16);
+extern "C" int tpb_paged_decode_scratch(int B, int Hkv, int G, int DK, int DV, int held8, int capacity) {
+  const PagedShape shape = pd_shape(held8 != 0, G > 8, DK + DV);
+  const long long steps = (long long)B * Hkv * ((G + 15) / 16) * (((long long)capacity + shape.keys - 1) / shape.keys);
+  return pd_grid(steps) * ((2 + shape.warps) * (G < 16 ? G : 16) * (DV + 2) * 4 + 16);
 }
 
 // q [B, Hkv * G, DK] bf16 (strides q_b, q_h), pools as in tpb_paged_rows (strides of pages, tokens, heads; scales contiguous over
@@ -733,7 +743,8 @@ extern "C" int tpb_paged_decode(const void* q, long long q_b, long long q_h, con
   long long capacity = (long long)table_width * page;
   if (capacity > (long long)0x7fffff00) return -2;
   const int blocks = (G + 15) / 16;
-  const long long steps = (long long)B * Hkv * blocks * ((capacity + PD_KEYS - 1) / PD_KEYS);
+  const PagedShape shape = pd_shape(held8, G > 8, DK + DV);
+  const long long steps = (long long)B * Hkv * blocks * ((capacity + shape.keys - 1) / shape.keys);
   if (steps > 0x3fffffffLL) return -2;
   PagedDecode p = {};
   p.q = static_cast<const __nv_bfloat16*>(q);
@@ -751,7 +762,7 @@ extern "C" int tpb_paged_decode(const void* q, long long q_b, long long q_h, con
   p.vs_head = strides[11];
   const int grid = pd_grid(steps);
   p.rows = G < 16 ? G : 16;
-  const long long part_rows = (long long)grid * (2 + pd_warps(held8, G > 8)) * p.rows;
+  const long long part_rows = (long long)grid * (2 + shape.warps) * p.rows;
   p.split = static_cast<int4*>(scratch);
   p.part_o = reinterpret_cast<float*>(p.split + grid);
   p.part_ml = p.part_o + part_rows * DV;
@@ -762,6 +773,7 @@ extern "C" int tpb_paged_decode(const void* q, long long q_b, long long q_h, con
   p.blocks = blocks;
   p.pages = pages;
   p.page = page;
+  p.width = table_width;
   p.capacity = (int)capacity;
   p.window = window;
   p.scale_log2 = scale * 1.4426950408889634f;

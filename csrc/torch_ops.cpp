@@ -1158,7 +1158,7 @@ py::object paged_decode(py::handle q_, py::handle k_, py::handle v_, py::handle 
     out = empty_as(q, {b, hq, c.dv});
     const int g = (int)(hq / c.heads);
     Tensor scratch = empty_like_type(
-        q, {tpb_paged_decode_scratch((int)b, (int)c.heads, g, (int)c.dv, c.held8, (int)(width * c.page))}, at::kByte);
+        q, {tpb_paged_decode_scratch((int)b, (int)c.heads, g, (int)c.dk, (int)c.dv, c.held8, (int)(width * c.page))}, at::kByte);
     check(tpb_paged_decode(cptr(q), q.stride(0), q.stride(1), cptr(c.k), cptr(c.v), cptr(c.ks), cptr(c.vs), c.strides, iptr(table),
                            table.stride(0), (int)width, iptr(lens), mptr(out), mptr(scratch), (int)b, (int)c.heads, g, (int)c.dk,
                            (int)c.dv, (int)c.pages, (int)c.page, (int)window, (float)scale, (float)softcap, stream()),

@@ -278,7 +278,7 @@ int tpb_paged_rows(int write, void* k, void* v, void* k_pool, void* v_pool, void
                    const long long* slots, long long T, int H, int Dk, int Dv, int pages, int page,
                    const long long* x_strides, const long long* strides, void* stream);
 // Attention of one new token per sequence over the pools (paged_decode.cu).
-int tpb_paged_decode_scratch(int B, int Hkv, int G, int DV, int held8, int capacity);
+int tpb_paged_decode_scratch(int B, int Hkv, int G, int DK, int DV, int held8, int capacity);
 int tpb_paged_decode(const void* q, long long q_b, long long q_h, const void* k_pool, const void* v_pool, const void* k_scale,
                      const void* v_scale, const long long* strides, const int* table, long long table_b, int table_width,
                      const int* lengths, void* out, void* scratch, int B, int Hkv, int G, int DK, int DV, int pages, int page,

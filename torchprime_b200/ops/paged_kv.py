@@ -21,7 +21,7 @@ from ._lib import check, lib, ptr, stream_ptr
 
 P, I, LL, F = c_void_p, c_int, c_longlong, c_float
 _lib.register_signature("tpb_paged_rows", [I, P, P, P, P, P, P, P, LL, I, I, I, I, I, P, P, P])
-_lib.register_signature("tpb_paged_decode_scratch", [I, I, I, I, I, I])
+_lib.register_signature("tpb_paged_decode_scratch", [I, I, I, I, I, I, I])
 _lib.register_signature("tpb_paged_decode", [P, LL, LL, P, P, P, P, P, P, LL, I, P, P, P, I, I, I, I, I, I, I, I, F, F, P])
 
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
@@ -196,7 +196,7 @@ def decode_attention(q, cache: PagedKV, block_table, lengths, scale=None, window
     dv, width = cache.v.shape[3], block_table.shape[1]
     out = torch.empty(b, hq, dv, dtype=q.dtype, device=q.device)
     with torch.cuda.device(q.device):
-      n = lib().tpb_paged_decode_scratch(b, hkv, hq // hkv, dv, int(cache.k.dtype == E4M3), width * page)
+      n = lib().tpb_paged_decode_scratch(b, hkv, hq // hkv, dk, dv, int(cache.k.dtype == E4M3), width * page)
       scratch = torch.empty(n, dtype=torch.uint8, device=q.device)
       rc = lib().tpb_paged_decode(ptr(q), q.stride(0), q.stride(1), ptr(cache.k), ptr(cache.v), ptr(cache.k_scale), ptr(cache.v_scale),
                                   _c_strides(cache), ptr(block_table), block_table.stride(0), width, ptr(lengths.contiguous()), ptr(out),
