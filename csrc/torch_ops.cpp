@@ -1167,6 +1167,44 @@ py::object paged_decode(py::handle q_, py::handle k_, py::handle v_, py::handle 
   return py::cast(out);
 }
 
+// One token per row of logits; see sampling.sample_tokens.
+py::object sample_tokens(py::handle x_, py::handle u_, py::handle t_, py::handle k_, py::handle p_, py::handle mp_) {
+  Tensor x, u, out, each[4];
+  if (!unobserved() || !unpack(x_, x) || !unpack(u_, u) || !(plain(x, at::kFloat) || plain(x)) || x.dim() != 2 ||
+      x.get_device() != c10::cuda::current_device())
+    return py::none();
+  const int64_t b = x.size(0), v = x.size(1);
+  if (b < 1 || v < 1 || v > (1 << 18) || b >= (1 << 26) || x.stride(1) != 1 || !plain_rows(u, at::kFloat) || u.dim() != 1 ||
+      u.size(0) != b || u.get_device() != x.get_device())
+    return py::none();
+  double number[4] = {1.0, 0.0, 1.0, 0.0};
+  const py::handle given[4] = {t_, k_, p_, mp_};
+  for (int i = 0; i < 4; ++i) {
+    if (THPVariable_Check(given[i].ptr())) {
+      each[i] = THPVariable_Unpack(given[i].ptr());
+      if (!plain_rows(each[i], i == 1 ? at::kInt : at::kFloat) || each[i].dim() != 1 || each[i].size(0) != b ||
+          each[i].get_device() != x.get_device())
+        return py::none();
+    } else if (i == 1) {
+      int64_t k;
+      if (!whole(given[i], 0, k)) return py::none();
+      number[i] = (double)std::min(std::max<int64_t>(k, 0), v);
+    } else if (!real(given[i], number[i], number[i])) {
+      return py::none();
+    }
+  }
+  {
+    py::gil_scoped_release nogil;
+    out = empty_like_type(x, {b}, at::kLong);
+    check(tpb_sample_tokens(cptr(x), x.scalar_type() == at::kBFloat16, x.stride(0), static_cast<const float*>(cptr(u)),
+                            static_cast<const float*>(cptr(each[0])), iptr(each[1]), static_cast<const float*>(cptr(each[2])),
+                            static_cast<const float*>(cptr(each[3])), number[0], (int)number[1], number[2], number[3],
+                            static_cast<long long*>(mptr(out)), (int)b, (int)v, stream()),
+          "sample_tokens");
+  }
+  return py::cast(out);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_tpb_torch, m) {
@@ -1199,4 +1237,5 @@ PYBIND11_MODULE(_tpb_torch, m) {
   m.def("paged_append", &paged_append);
   m.def("paged_read", &paged_read);
   m.def("paged_decode", &paged_decode);
+  m.def("sample_tokens", &sample_tokens);
 }

@@ -284,6 +284,11 @@ int tpb_paged_decode(const void* q, long long q_b, long long q_h, const void* k_
                      const int* lengths, void* out, void* scratch, int B, int Hkv, int G, int DK, int DV, int pages, int page,
                      int window, float scale, float softcap, void* stream);
 
+// ---- one token per row of logits by given random numbers (sampling.cu)
+int tpb_sample_tokens(const void* logits, int bf16, long long stride, const float* u, const float* temperature, const int* top_k,
+                      const float* top_p, const float* min_p, double temperature0, int top_k0, double top_p0, double min_p0,
+                      long long* out, int B, int V, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,160 @@
+"""The sampling kernel draws the token of the definition (64 bits), whatever the distribution and however many CTAs share a row."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from torchprime_b200.ops import _lib, functional as ops, reference as ref
+from torchprime_b200.ops.sampling import sample_tokens
+
+
+def _logits(g, b, v, kind):
+  x = torch.randn(b, v, generator=g, device="cuda") * 2
+  if kind == "peaks":
+    n = min(v, 20)
+    x.scatter_add_(1, torch.randint(0, v, (b, n), generator=g, device="cuda"), torch.rand(b, n, generator=g, device="cuda") * 9)
+  elif kind == "flat":
+    x *= 1e-3
+  elif kind == "equal":
+    x.fill_(1.25)
+  elif kind == "few values":
+    x = torch.randint(-3, 4, (b, v), generator=g, device="cuda").float()
+  elif kind == "masked":                      # a grammar that allows a few tokens, in one row none
+    x[torch.rand(b, v, generator=g, device="cuda") > 3 / v] = -math.inf
+    x[0] = -math.inf
+  elif kind == "huge":
+    x *= 1e30
+  elif kind == "tiny":
+    x *= 1e-42
+  return x
+
+
+def _same(x, u, **kw):
+  got = sample_tokens(x, u, **kw)
+  want = ref.sample_tokens(x, u, **{n: (kw.get(n) if kw.get(n) is not None else d) for n, d in
+                                    (("temperature", 1.0), ("top_k", 0), ("top_p", 1.0), ("min_p", 0.0))})
+  assert got.dtype == torch.int64 and got.shape == want.shape
+  bad = (got != want).nonzero()[:5, 0].tolist()
+  assert not bad, [(i, int(got[i]), int(want[i])) for i in bad]
+
+
+SETTINGS = [dict(), dict(temperature=0.0), dict(temperature=0.7, top_k=50), dict(top_p=0.9), dict(min_p=0.05),
+            dict(temperature=1.5, top_p=0.99), dict(temperature=0.8, top_k=40, top_p=0.95, min_p=0.02), dict(top_k=1), dict(top_p=0.0),
+            dict(top_k=3000), dict(top_k=3000, top_p=0.5), dict(temperature=2.0, top_k=2500, top_p=0.999, min_p=1e-4), dict(min_p=1.0),
+            dict(top_k=10 ** 9, top_p=1.0, min_p=-1.0), dict(temperature=math.inf, top_p=0.5, min_p=1.0), dict(temperature=1e-6)]
+
+
+@pytest.mark.parametrize("kw", SETTINGS, ids=str)
+@pytest.mark.parametrize("kind", ["normal", "peaks", "flat", "equal", "few values", "masked"])
+def test_every_setting_on_every_distribution(cuda_lib, kw, kind):
+  g = torch.Generator(device="cuda").manual_seed(len(kind))
+  for b, v in ((6, 32000), (3, 5003)):
+    x, u = _logits(g, b, v, kind), torch.rand(b, generator=g, device="cuda")
+    _same(x, u, **kw)
+    _same(x.bfloat16(), u, **kw)
+
+
+@pytest.mark.parametrize("v", [1, 2, 3, 31, 257, 1000, 2047, 2048, 2049, 4097, 65537, 128256, 202048, 262144])
+@pytest.mark.parametrize("b", [1, 5, 90])
+def test_sizes(cuda_lib, b, v):
+  g = torch.Generator(device="cuda").manual_seed(v + b)
+  x, u = _logits(g, b, v, "peaks"), torch.rand(b, generator=g, device="cuda")
+  for kw in (dict(), dict(top_p=0.95, temperature=0.8), dict(top_k=50, min_p=0.01), dict(top_p=0.98, temperature=3.0), dict(temperature=0)):
+    _same(x, u, **kw)
+
+
+def test_more_rows_than_the_machine_has_room_for(cuda_lib):
+  g = torch.Generator(device="cuda").manual_seed(4)
+  x, u = _logits(g, 1500, 8000, "peaks"), torch.rand(1500, generator=g, device="cuda")
+  _same(x, u, top_p=0.9)
+  _same(x, u, temperature=1.3, top_k=20)
+
+
+def test_settings_for_each_row(cuda_lib):
+  g = torch.Generator(device="cuda").manual_seed(6)
+  b, v = 64, 50000
+  x, u = _logits(g, b, v, "peaks"), torch.rand(b, generator=g, device="cuda")
+  i = torch.arange(b, device="cuda")
+  _same(x, u, temperature=(i % 5).float() * 0.4, top_k=((i % 7) * 700).int(), top_p=0.5 + (i % 6).float() * 0.1, min_p=(i % 3).float() * 0.03)
+
+
+@pytest.mark.parametrize("kind", ["huge", "tiny", "normal"])
+def test_extreme_logits(cuda_lib, kind):
+  g = torch.Generator(device="cuda").manual_seed(8)
+  x, u = _logits(g, 8, 3001, kind), torch.rand(8, generator=g, device="cuda")
+  x[1, 7], x[1, 2000] = math.inf, math.inf
+  x[2, ::3] = math.nan
+  x[3] = math.nan
+  x[4] = -math.inf
+  x[5, 1:] = -math.inf
+  x[6, :3000] = 0.0
+  x[6, ::2] = -0.0
+  for kw in SETTINGS:
+    _same(x, u, **kw)
+
+
+def test_first_and_last_numbers(cuda_lib):
+  g = torch.Generator(device="cuda").manual_seed(9)
+  x = _logits(g, 6, 40000, "peaks")
+  u = torch.tensor([0.0, 1 - 2.0 ** -24, 0.0, 1 - 2.0 ** -24, 0.5, 2.0 ** -24], device="cuda")
+  for kw in (dict(), dict(top_k=5), dict(top_p=0.7), dict(temperature=2.0, top_p=0.95)):
+    _same(x, u, **kw)
+  got = sample_tokens(x, torch.tensor([1.0, 7.0, -3.0, math.nan, math.inf, 0.0], device="cuda"), top_k=4)      # outside [0, 1): a kept token all the same
+  kept = x.topk(4)[1]
+  assert bool((kept == got[:, None]).any(1).all())
+
+
+def test_strided_rows(cuda_lib):
+  g = torch.Generator(device="cuda").manual_seed(10)
+  wide = _logits(g, 7, 9005, "peaks")
+  u = torch.rand(7, generator=g, device="cuda")
+  for x in (wide[:, 1:8002], wide[::2, 3:], wide.t().contiguous().t(), wide.bfloat16()[:, 1:7000]):
+    _same(x, u[: x.shape[0]], top_p=0.9)
+    _same(x, u[: x.shape[0]], temperature=2.5, top_k=30)
+
+
+def test_same_token_every_time_and_from_python(cuda_lib, monkeypatch):
+  g = torch.Generator(device="cuda").manual_seed(11)
+  x, u = _logits(g, 40, 30000, "normal"), torch.rand(40, generator=g, device="cuda")
+  kw = dict(temperature=torch.full((40,), 1.1, device="cuda"), top_k=5000, top_p=0.97)
+  first = sample_tokens(x, u, **kw)
+  assert all(torch.equal(first, sample_tokens(x, u, **kw)) for _ in range(3))
+  monkeypatch.setattr(ops, "_native", lambda: None)
+  n = _lib.launch_count()
+  assert torch.equal(first, sample_tokens(x, u, **kw)) and _lib.launch_count() == n + 1
+
+
+def test_captured_and_replayed(cuda_lib):
+  g = torch.Generator(device="cuda").manual_seed(12)
+  x, u = _logits(g, 3, 20000, "peaks"), torch.rand(3, generator=g, device="cuda")
+  t = torch.ones(3, device="cuda")
+  sample_tokens(x, u, t, top_p=0.9)
+  torch.cuda.synchronize()
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    out = sample_tokens(x, u, t, top_p=0.9)
+  for _ in range(4):
+    x.copy_(_logits(g, 3, 20000, "peaks"))
+    u.copy_(torch.rand(3, generator=g, device="cuda"))
+    t.copy_(torch.rand(3, generator=g, device="cuda") * 2)
+    graph.replay()
+    assert torch.equal(out, ref.sample_tokens(x, u, t, top_p=0.9))
+
+
+def test_frequencies_follow_the_distribution(cuda_lib):
+  g = torch.Generator(device="cuda").manual_seed(13)
+  n = 40000
+  x = torch.tensor([[0.0, 1.0, 2.0, -1.0, 1.5]], device="cuda").expand(n, 5)
+  f = torch.bincount(sample_tokens(x, torch.rand(n, generator=g, device="cuda"), 1.0, top_k=4), minlength=5) / n
+  want = torch.softmax(torch.tensor([0.0, 1.0, 2.0, -math.inf, 1.5], device="cuda"), 0)
+  assert torch.allclose(f, want, atol=5 * (0.25 / n) ** 0.5)
+
+
+def test_empty_batch_and_wide_rows(cuda_lib):
+  assert sample_tokens(torch.zeros(0, 9, device="cuda"), torch.zeros(0, device="cuda")).shape == (0,)
+  g = torch.Generator(device="cuda").manual_seed(14)
+  x, u = _logits(g, 2, (1 << 18) + 3, "peaks"), torch.rand(2, generator=g, device="cuda")
+  _same(x, u, top_p=0.9)                       # (more than the kernel takes: the definition)

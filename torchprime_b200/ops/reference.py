@@ -305,3 +305,32 @@ def paged_attention(q, k_pool, v_pool, k_scale, v_scale, block_table, lengths, s
   p = torch.softmax(s, dim=-1)
   p = torch.where((n > 0)[:, None, None], p, torch.zeros_like(p))
   return torch.einsum("bhgs,bshd->bhgd", p, rows(v_pool, v_scale)).reshape(b, hq, -1).to(q.dtype)
+
+
+# ----------------------------------------------------------------------------- sampling
+def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+  """One token per row of logits [B, V] by u [B], in 64 bits; see ``sampling.sample_tokens``."""
+  x = logits.double()
+  x = torch.where(x.isnan(), torch.full_like(x, float("-inf")), x)
+  b, v = x.shape
+  column = lambda t: (t.double() if torch.is_tensor(t) else torch.full((b,), float(t), dtype=torch.float64, device=x.device))[:, None]  # noqa: E731
+  t, k, p, mp, u = (column(a) for a in (temperature, top_k, top_p, min_p, u))
+  i = torch.arange(v, device=x.device)
+  most = x.amax(-1, keepdim=True)
+  none = most[:, 0] == float("-inf")
+  first = torch.where(x == most, i, v).amin(-1)
+  w = torch.exp((x - most) / torch.where(t > 0, t, torch.ones_like(t)))
+  w = torch.where(x == most, torch.ones_like(w), torch.where(x == float("-inf"), torch.zeros_like(w), w))
+  order = torch.sort(x, dim=-1, descending=True, stable=True)[1]
+  ws = w.gather(1, order)
+  ws = torch.where(((i < k) | ~(k > 0)) & ~(ws < mp.clamp(max=1.0)), ws, torch.zeros_like(ws))
+  c = ws.cumsum(-1)
+  ws = torch.where((c - ws < p * c[:, -1:]) | ~(p < 1) | (i == 0), ws, torch.zeros_like(ws))
+  w = torch.zeros_like(w).scatter_(1, order, ws)
+  c = w.cumsum(-1)
+  u = torch.where(u > 0, u, torch.zeros_like(u))
+  drawn = torch.where(c > u * c[:, -1:], i, v).amin(-1)
+  last = torch.where(w > 0, i, -1).amax(-1)                     # (u of 1 and more)
+  drawn = torch.where(drawn < v, drawn, last)
+  out = torch.where(t[:, 0] > 0, drawn, first)
+  return torch.where(none, torch.full_like(out, -1), out)
