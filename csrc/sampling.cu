@@ -6,15 +6,19 @@
 // kept weights exceeds u times their total.  T = 0 is the first index of the largest logit.  All three filters keep a leading part of
 // the order: a smallest logit and how many of that value.
 //
-// Which token comes out hangs on sums of up to 2^18 weights that are compared with a border, so weights are computed in 64 bits
-// (2^x by a table of 2^(j/16) and the series of the rest, 1e-15) and added as whole multiples of 2^-44: sums are exact, and
-// the same in any order.
+// Which token comes out hangs on sums of up to 2^18 weights that are compared with a border, so fp32 exponentials will not do: a
+// weight is a table's 2^(j / 1024) times the series of the rest, with the exponent as an unevaluated sum of two floats, good to 2^-34
+// (in fp64 throughout, the same 65 M weights took five times as long), and weights are added as whole multiples of 2^-44: sums are
+// exact, and the same in any order.
 //
 // Memory bounds it: a row has to be read once.  A cluster of 1 to 16 CTAs takes a row, each a contiguous slice; more CTAs the fewer
-// rows there are.  The first pass over the row finds m and counts the logits by the leading 11 bits of their order; the second, out of L2,
-// hands the few that can matter (the bins that hold the first k, those above min_p, the topmost bins) to one CTA, which sorts
-// them and finishes alone.  Where they are too many (a flat distribution, many equal logits) the border is found by counting or
-// adding up weights over the next bits, pass by pass, and the token in two more.
+// rows there are.  A slice comes through a ring of bulk copies, or stays in it where it fits.
+//   * The first pass finds m.
+//   * top-k: the k-th largest of the threads' own largest logits is a lower bound of the k-th largest of all; min-p has a bound of its
+//     own.  The logits from the bound on, usually little more than k, go to one CTA, which sorts them and finishes alone.
+//   * nucleus: a histogram of the weights over their exponents in steps of 1/32; the bin with the border goes to one CTA, which
+//     sorts it.  Then two more passes draw the token: sums of slices and of the parts of their warps, and along one of those.
+//   * Where a list is too long for one CTA (thousands of equal logits, large k) the border is found bit by bit of the order.
 
 #include "common.cuh"
 #include "tpb.h"
@@ -24,9 +28,11 @@ namespace tpb {
 int sm_count();
 
 constexpr int SMP_THREADS = 512, SMP_WARPS = SMP_THREADS / 32;
-constexpr int SMP_BINS = 2048;          // 11 bits of the order at a time: 31-21, 20-10, 9-0
+constexpr int SMP_BINS = 2048;          // 11 bits of the order at a time (31-21, 20-10, 9-0); 64 binary orders of weights in steps of 1/32
 constexpr int SMP_CAP = 2048;           // tokens that one CTA sorts
 constexpr int SMP_FIXED = 44;           // a weight of 1 is 2^44: 2^18 of them stay below 2^63
+constexpr int SMP_TABLE = 1024;         // 2^(j / 1024)
+constexpr int SMP_CHUNK = SMP_THREADS * 4, SMP_RING = 6;       // logits of a bulk copy, copies under way
 
 using u64 = unsigned long long;
 
@@ -37,9 +43,10 @@ struct SampleParams {
   const float *temperature, *top_p, *min_p;      // one a row, or null: the numbers below
   const int* top_k;
   double temperature0, top_p0, min_p0;
-  int top_k0, V, slice;                          // slice: logits of a CTA, a multiple of 4
+  int top_k0, V, slice;                          // slice: logits of a CTA, a multiple of 8
   long long* out;
-  int vec;                                       // rows can be read four logits at a time
+  int vec;                                       // rows can be read four logits at a time: 2, also by bulk copies (16-byte aligned)
+  int* status;
 };
 
 // The place of another CTA's copy of a shared variable.
@@ -60,39 +67,82 @@ __device__ __forceinline__ float smp_logit(unsigned key) { return __uint_as_floa
 
 struct SmpWeight {
   double per_unit;        // log2(e) / T
-  float top;
-  const double* table;    // 2^(j / 16), shared
-  __device__ __forceinline__ double real(float l) const {
-    if (l == top) return 1.0;
-    const double x = ((double)l - (double)top) * per_unit;
-    if (!(x > -64.0)) return 0.0;
-    const double shifted = fma(x, 16.0, 6755399441055744.0);      // 1.5 * 2^52: the nearest whole number ends up in the low bits
-    const int j = __double2loint(shifted);
-    const double y = fma(shifted - 6755399441055744.0, -0.0625, x) * 0.6931471805599453;      // |y| <= ln 2 / 32
-    double s = fma(y, 1.0 / 720, 1.0 / 120);
-    s = fma(s, y, 1.0 / 24);
-    s = fma(s, y, 1.0 / 6);
-    s = fma(s, y, 0.5);
-    s = fma(s, y, 1.0);
-    s = fma(s, y, 1.0);
-    s *= table[j & 15];
-    return __hiloint2double(__double2hiint(s) + ((j >> 4) << 20), __double2loint(s));
+  float top, hi, lo;      // 1024 log2(e) / T as a sum of two floats
+  bool slow;              // T, or the logits, near the ends of fp32's range
+  double min_p;
+  float sure, sure_not;   // 1024 log2 of weights that pass min_p, that do not
+  const u64* table;       // 2^62 2^(j / 1024), shared
+
+  __device__ __forceinline__ SmpWeight(double T, float top_, double min_p_, const u64* table_)
+      : per_unit(1.4426950408889634 / T), top(top_), min_p(min_p_), table(table_) {
+    const double c = per_unit * SMP_TABLE;
+    hi = (float)c;
+    lo = (float)(c - (double)hi);
+    slow = !(T > 1e-20 && T < 1e20 && fabsf(top) < 1e18f);
+    const double border = min_p > 0.0 ? log2(min_p) * SMP_TABLE : -1e30;
+    sure = (float)(border + 0.01 + 1e-6 * fabs(border));
+    sure_not = (float)(border - 0.01 - 1e-6 * fabs(border));
   }
-  static __device__ __forceinline__ u64 fixed(double w) {         // to the nearest multiple of 2^-44
-    return (u64)__double_as_longlong(fma(w, (double)(1LL << SMP_FIXED), 4503599627370496.0)) & 0xfffffffffffffULL;
+  // in 64 bits
+  __device__ __noinline__ double real(float l) const {
+    return l == top ? 1.0 : l == -INFINITY ? 0.0 : exp2(((double)l - (double)top) * per_unit);
   }
-  __device__ __forceinline__ u64 operator()(float l) const { return fixed(real(l)); }
+  // 1024 log2(w), the nearest float and what is missing
+  __device__ __forceinline__ float exponent(float l, float& rest) const {
+    const float d = l - top, back = d - l;
+    const float err = (l - (d - back)) - (top + back);          // l - top = d + err
+    const float x = d * hi;
+    rest = fmaf(err, hi, fmaf(d, lo, fmaf(d, hi, -x)));
+    return x;
+  }
+  // in multiples of 2^-44
+  __device__ __forceinline__ u64 operator()(float l) const {
+    if (slow) return __double2ull_rn(real(l) * (double)(1LL << SMP_FIXED));
+    float rest;
+    const float x = exponent(l, rest);
+    if (!(x > -45.0f * SMP_TABLE)) return 0;
+    const float shifted = x + 12582912.f;                       // 1.5 * 2^23: the nearest whole number ends up in the low bits
+    const int j = __float_as_int(shifted) - 0x4b400000;
+    const float y = ((x - (shifted - 12582912.f)) + rest) * (0.69314718056f / SMP_TABLE);
+    const float q = fmaf(0.5f * y, y, y);                       // 2^rest - 1, |q| < 2^-11; the next term is below 2^-37
+    const int qi = __float_as_int(q + 0.00146484375f) - 0x3ac00000;      // 1.5 * 2^-10: in multiples of 2^-33
+    const u64 t = table[j & (SMP_TABLE - 1)];
+    const u64 w = t + (u64)(((long long)(int)(t >> 32) * qi) >> 1);
+    const int down = 62 - SMP_FIXED - (j >> 10);
+    return (w + (1ULL << (down - 1))) >> down;
+  }
+  // w >= min_p
+  __device__ __forceinline__ bool passes(float l) const {
+    if (!(min_p > 0.0)) return true;
+    if (!slow) {
+      float rest;
+      const float x = exponent(l, rest);
+      if (x > sure) return true;
+      if (!(x > sure_not)) return false;
+    }
+    return real(l) >= min_p;
+  }
+  // Steps of 1/32 below the largest weight's exponent, the largest weights in the last bin.
+  __device__ __forceinline__ int bin(float l) const {
+    if (l == top) return SMP_BINS - 1;
+    float rest;
+    const float x = slow ? (float)(fmax((double)l - (double)top, -1e38) * per_unit * SMP_TABLE) : exponent(l, rest);
+    return x > -(float)(SMP_BINS - 1) * 32.f ? SMP_BINS - 1 - (int)(-x * 0.03125f) : 0;
+  }
 };
 
 struct SmpShared {
+  float ring[SMP_RING * SMP_CHUNK];     // bf16 logits take half of it
   u64 sums[SMP_BINS];                   // of weights, or counts
   u64 list[SMP_CAP], weight[SMP_CAP];
-  double table[16];
+  u64 table[SMP_TABLE];
   u64 warp[SMP_WARPS], warp2[SMP_WARPS];
   u64 tot[16], tot2[16];                // of the cluster's CTAs
-  u64 found[3];                         // bin, sum of the bins above, sum of the bin
+  uint64_t full[SMP_RING];              // barriers of the copies
+  u64 found[3];                         // bin, sum of the bins above, sum of all
   unsigned count;                       // of the list
-  int bad;
+  unsigned border, of_border;
+  int dead;                             // a copy has not come
 };
 
 __device__ __forceinline__ u64 smp_warp_sum(u64 v) {
@@ -137,8 +187,10 @@ __device__ __forceinline__ void smp_cluster_sync() {
   cluster_sync_all();
 }
 
-// Every CTA's s.sums, added up, from the last bin down: the bin in which the sum reaches `target` (which it does), in s.found.
-__device__ __forceinline__ void smp_find(SmpShared& s, u64 target, int rank, int ctas) {
+// Every CTA's s.sums, added up, from the last bin down: the bin in which the sum reaches target(sum of all), in s.found; the
+// sum of all alone where that is more.
+template <typename F>
+__device__ __forceinline__ void smp_find(SmpShared& s, int rank, int ctas, F&& target) {
   const int per = SMP_BINS / ctas, b0 = rank * per;
   smp_cluster_sync();
   // four neighbouring bins to a thread, the topmost to thread 0
@@ -150,22 +202,26 @@ __device__ __forceinline__ void smp_find(SmpShared& s, u64 target, int rank, int
       for (int c = 0; c < ctas; ++c) v[i] += smp_peer(s.sums, c)[high - i];
       mine += v[i];
     }
-  const u64 all = smp_block_sum(mine, s.warp), before = smp_block_before(mine, s.warp);
-  if ((int)threadIdx.x < ctas) smp_peer(s.tot, threadIdx.x)[rank] = all;
+  const u64 sum = smp_block_sum(mine, s.warp), before = smp_block_before(mine, s.warp);
+  if ((int)threadIdx.x < ctas) smp_peer(s.tot, threadIdx.x)[rank] = sum;
   smp_cluster_sync();
-  u64 above = before;
-  for (int c = rank + 1; c < ctas; ++c) above += s.tot[c];
+  u64 above = before, all = 0;
+  for (int c = 0; c < ctas; ++c) {
+    all += s.tot[c];
+    if (c > rank) above += s.tot[c];
+  }
+  const u64 t = target(all);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (high - i >= b0 && above < target && above + v[i] >= target)
+    if (high - i >= b0 && above < t && above + v[i] >= t)
       for (int c = 0; c < ctas; ++c) {
         u64* f = smp_peer(s.found, c);
         f[0] = high - i;
         f[1] = above;
-        f[2] = v[i];
       }
     above += v[i];
   }
+  if (threadIdx.x == 0) s.found[2] = all;
   smp_cluster_sync();
 }
 
@@ -233,35 +289,90 @@ __device__ __forceinline__ void smp_load(const L* row, int i, int end, int vec, 
 #pragma unroll
   for (int e = 0; e < 4; ++e) l[e] = l[e] != l[e] ? -INFINITY : l[e];
 }
-// f(index, logits, how many) for the CTA's slice, four at a time.
-template <typename L, typename F>
-__device__ __forceinline__ void smp_stream(const L* row, int begin, int end, int vec, F&& f) {
-  constexpr int AHEAD = 4, STEP = SMP_THREADS * 4;
-  for (int i0 = begin; i0 < end; i0 += AHEAD * STEP) {
-    float l[AHEAD][4];
-#pragma unroll
-    for (int x = 0; x < AHEAD; ++x) {
-      const int i = i0 + x * STEP + threadIdx.x * 4;
-      if (i < end) smp_load<L>(row, i, end, vec, l[x]);
-    }
-#pragma unroll
-    for (int x = 0; x < AHEAD; ++x) {
-      const int i = i0 + x * STEP + threadIdx.x * 4;
-      f(i, l[x], min(4, end - i));      // (none: 0 or less)
-    }
+
+// The CTA's slice, pass by pass.
+template <typename L>
+struct SmpSlice {
+  const L* row;
+  int begin, end, vec;
+  int copied;                           // what bulk copies can bring ends here: whole 16 bytes
+  bool kept = false;                    // all of it lies in the ring
+  unsigned parity = 0;                  // of the ring's barriers, a bit each
+
+  __device__ __forceinline__ void copy(SmpShared& s, int chunk) const {       // one thread
+    const int at = begin + chunk * SMP_CHUNK, n = min(SMP_CHUNK, copied - at) * (int)sizeof(L), slot = chunk % SMP_RING;
+    fence_proxy_async();                // (what the block has read of the slot, ahead of the copy that overwrites it)
+    mbar_expect_tx(&s.full[slot], max(n, 0));
+    if (n > 0)
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                   :
+                   : "r"(smem_u32(reinterpret_cast<L*>(s.ring) + slot * SMP_CHUNK)), "l"(row + at), "r"(n), "r"(smem_u32(&s.full[slot]))
+                   : "memory");
   }
-}
+  // f(index, four logits, how many there are) in every thread
+  template <typename F>
+  __device__ __forceinline__ void pass(SmpShared& s, int* status, F&& f) {
+    const int chunks = (end - begin + SMP_CHUNK - 1) / SMP_CHUNK, tid = threadIdx.x;
+    if (vec < 2) {
+      constexpr int AHEAD = 2;
+      for (int i0 = begin; i0 < end; i0 += AHEAD * SMP_CHUNK) {
+        float l[AHEAD][4];
+#pragma unroll
+        for (int x = 0; x < AHEAD; ++x) {
+          const int i = i0 + x * SMP_CHUNK + tid * 4;
+          if (i < end) smp_load<L>(row, i, end, vec, l[x]);
+        }
+#pragma unroll
+        for (int x = 0; x < AHEAD; ++x) {
+          const int i = i0 + x * SMP_CHUNK + tid * 4;
+          f(i, l[x], min(4, end - i));  // (none: 0 or less)
+        }
+      }
+      return;
+    }
+    if (!kept) {
+      __syncthreads();
+      if (tid == 0 && !s.dead)
+        for (int c = 0; c < min(chunks, SMP_RING); ++c) copy(s, c);
+    }
+    for (int c = 0; c < chunks; ++c) {
+      const int slot = c % SMP_RING, i = begin + c * SMP_CHUNK + tid * 4;
+      if (!kept) {
+        if (!s.dead && !mbar_wait(&s.full[slot], parity >> slot & 1, status, kTimeoutTmaFull, 76)) s.dead = 1;
+        parity ^= 1u << slot;
+      }
+      float l[4];
+      const L* ring = reinterpret_cast<const L*>(s.ring) + slot * SMP_CHUNK;
+      if (i + 4 <= copied) smp_load<L>(ring, tid * 4, SMP_CHUNK, 1, l);
+      else if (i < end) smp_load<L>(row, i, end, 0, l);
+      f(i, l, min(4, end - i));
+      if (!kept && chunks > SMP_RING) {
+        __syncthreads();
+        if (tid == 0 && !s.dead && c + SMP_RING < chunks) copy(s, c + SMP_RING);
+      }
+    }
+    kept = chunks <= SMP_RING;
+  }
+};
 
 template <typename L>
 __global__ void __launch_bounds__(SMP_THREADS, 2)
 sample_kernel(const SampleParams p, int ctas) {
-  if (!chain_begin()) return;
-  extern __shared__ __align__(16) uint8_t smp_smem[];
+  extern __shared__ __align__(128) uint8_t smp_smem[];
   SmpShared& s = *reinterpret_cast<SmpShared*>(smp_smem);
   const int rank = ctas > 1 ? (int)cluster_ctarank() : 0, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  for (int i = tid; i < SMP_BINS; i += SMP_THREADS) s.sums[i] = 0;
+  for (int i = tid; i < SMP_TABLE; i += SMP_THREADS) s.table[i] = __double2ull_rn(exp2(i / (double)SMP_TABLE) * 4611686018427387904.0);
+  if (tid < SMP_RING) mbar_init(&s.full[tid], 1);
+  if (tid == 0) s.count = 0, s.dead = 0;
+  fence_barrier_init();
+  __syncthreads();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // (nobody writes to a CTA that has not begun)
+  chain_launch();
+  if (!chain_wait()) return;
   const int b = blockIdx.x / ctas, V = p.V;
-  const L* row = static_cast<const L*>(p.logits) + b * p.stride;
-  const int begin = min(V, rank * p.slice), end = min(V, begin + p.slice);
+  SmpSlice<L> slice = {static_cast<const L*>(p.logits) + b * p.stride, min(V, rank * p.slice), min(V, (rank + 1) * p.slice), p.vec};
+  slice.copied = slice.end - (slice.end - slice.begin) % (16 / (int)sizeof(L));
   const double T = p.temperature ? (double)p.temperature[b] : p.temperature0;
   double top_p = p.top_p ? (double)p.top_p[b] : p.top_p0, min_p = p.min_p ? (double)p.min_p[b] : p.min_p0;
   int top_k = p.top_k ? p.top_k[b] : p.top_k0;
@@ -270,26 +381,20 @@ sample_kernel(const SampleParams p, int ctas) {
   const bool nucleus = top_p < 1.0;               // (NaN: off)
   top_p = fmax(top_p, 0.0);
   min_p = min_p > 0.0 ? fmin(min_p, 1.0) : 0.0;
-  const bool count = !greedy && (top_k || nucleus || min_p > 0.0);
-  for (int i = tid; i < SMP_BINS; i += SMP_THREADS) s.sums[i] = 0;
-  if (tid < 16) s.table[tid] = exp2(tid * 0.0625);
-  if (tid == 0) s.count = 0, s.bad = 0;
-  __syncthreads();
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // (nobody writes to a CTA that has not begun)
-  unsigned* const counts = reinterpret_cast<unsigned*>(s.sums);   // the low halves (little-endian) of the sums
+  const double u = fmin(fmax((double)p.u[b], 0.0), 1.0);
+  unsigned* const halves = reinterpret_cast<unsigned*>(s.sums);   // low and high words of the sums
 
-  // ---- the largest logit, its first index, and how many logits there are in each bin
+  // ---- the largest logit and its first index
   unsigned top_key = 0;
   int at = V;
-  smp_stream<L>(row, begin, end, p.vec, [&](int i, const float* l, int n) {
+  slice.pass(s, p.status, [&](int i, const float* l, int n) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < n) {
-        const unsigned key = smp_key(l[e]);
-        if (key > top_key) top_key = key, at = i + e;
-        if (count) atomicAdd(counts + 2 * (key >> 21), 1u);
-      }
+    for (int e = 0; e < 4; ++e) {
+      const unsigned key = smp_key(l[e]);
+      if (e < n && key > top_key) top_key = key, at = i + e;
+    }
   });
+  if (top_k && !greedy && top_key) atomicAdd(halves + 2 * (top_key >> 21), 1u);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const unsigned x = __shfl_xor_sync(0xffffffffu, top_key, o);
@@ -309,206 +414,210 @@ sample_kernel(const SampleParams p, int ctas) {
   for (int c = 0; c < ctas; ++c) best = max(best, s.tot2[c]);
   const float top = smp_logit((unsigned)(best >> 32));
   at = V - (int)(unsigned)best;
-  if (greedy || top == -INFINITY) {
-    if (rank == 0 && tid == 0) p.out[b] = top == -INFINITY ? -1 : at;
-    return;
+  if (greedy || top == -INFINITY || s.dead) {
+    if (rank == 0 && tid == 0) p.out[b] = top == -INFINITY || s.dead ? -1 : at;
+    if (greedy || top == -INFINITY) return;       // (the cluster agrees on these)
   }
-  const SmpWeight weight = {1.4426950408889634 / T, top, s.table};
-  const double u = fmin(fmax((double)p.u[b], 0.0), 1.0);
+  const SmpWeight weight(T, top, min_p, s.table);
   auto place = [&](u64 total) {                   // the sum that the drawn token's passes
     const u64 x = (u64)(u * (double)total);
-    return x < total ? x : total - 1;
+    return x < total ? x : total - (total > 0);
+  };
+  // Logits for which `wanted` go to the first CTA's list; the number of them, in every CTA.
+  auto gather = [&](auto&& wanted) {
+    u64* const list = smp_peer(s.list, 0);
+    unsigned* const n_list = smp_peer(&s.count, 0);
+    slice.pass(s, p.status, [&](int i, const float* l, int n) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const unsigned key = smp_key(l[e]);
+        if (e < n && wanted(l[e], key)) {
+          const unsigned x = atomicAdd(n_list, 1u);
+          if (x < SMP_CAP) list[x] = (u64)key << 32 | (0xffffffffu - (unsigned)(i + e));
+        }
+      }
+    });
+    smp_cluster_sync();
+    const unsigned n = *n_list;
+    smp_cluster_sync();                           // (the first CTA may leave)
+    return n;
   };
 
   unsigned border = 0;                            // smallest key kept, and how many of it
   u64 of_border = 0;
-  bool few = count;
-  if (count) {
-    // ---- the bins that can matter
-    const bool all_fit = !top_k && V <= SMP_CAP;
-    unsigned lowest = 0;                          // bin
-    if (!all_fit) {
-      smp_find(s, top_k ? top_k : SMP_CAP + 1, rank, ctas);
-      if (top_k) {
-        lowest = (unsigned)s.found[0];
-        few = s.found[1] + s.found[2] <= SMP_CAP;
-      } else {
-        lowest = (unsigned)s.found[0] + 1;
-      }
-    }
-    if (!top_k && min_p > 0.0) {
+  if (top_k || min_p > 0.0) {
+    unsigned least_key = 0;
+    bool few = true;
+    if (min_p > 0.0) {
       float least = __double2float_rd((double)top + log(min_p) * T * (1.0 + 1e-12));
       if (!(least == least)) least = -INFINITY;               // (T is infinite)
       if (fabsf(least) < 1.2e-38f) least = -1.2e-38f;         // (subnormal)
-      const unsigned bin = smp_key(least) >> 21;
-      if (bin < lowest) few = false;
-      else lowest = bin;
+      least_key = smp_key(least);
     }
-    if (few) {
-      const bool need_total = nucleus && !top_k && !(min_p > 0.0);
-      u64 total = 0;
-      u64* const list = smp_peer(s.list, 0);
-      unsigned* const n_list = smp_peer(&s.count, 0);
-      smp_stream<L>(row, begin, end, p.vec, [&](int i, const float* l, int n) {
+    if (top_k) {
+      smp_find(s, rank, ctas, [&](u64 all) { return min((u64)top_k, all + 1); });
+      if (s.found[2] >= (u64)top_k) least_key = max(least_key, (unsigned)s.found[0] << 21);
+      else few = min_p > 0.0 || V <= SMP_CAP;
+    }
+    const unsigned n_list = few ? gather([&](float, unsigned key) { return key >= least_key; }) : SMP_CAP + 1;
+    if (n_list <= SMP_CAP) {
+      if (rank > 0) return;
+      // ---- one CTA sorts them and finishes
+      const int n = (int)n_list;
+      smp_sort(s.list, n);
+      int kept = top_k ? min(n, top_k) : n;
+      u64 below = 0;                              // (this thread's)
+      for (int i = tid; i < n; i += SMP_THREADS) {
+        const float l = smp_logit((unsigned)(s.list[i] >> 32));
+        s.weight[i] = weight(l);
+        below += i < kept && !weight.passes(l);
+      }
+      kept = max(kept - (int)smp_block_sum(below, s.warp), 1);
+      smp_scan(s, n);
+      if (nucleus) {
+        const u64 want = __double2ull_ru(top_p * (double)s.weight[kept - 1]);
+        u64 in = 0;
+        for (int i = tid; i < kept; i += SMP_THREADS) in += i == 0 || s.weight[i - 1] < want;
+        kept = max((int)smp_block_sum(in, s.warp), 1);
+      }
+      const u64 target = place(s.weight[kept - 1]);
+      __syncthreads();
+      for (int i = tid; i < kept; i += SMP_THREADS) {
+        const u64 x = s.list[i];
+        s.list[i] = x << 32 | x >> 32;            // by index now
+      }
+      smp_sort(s.list, kept);
+      for (int i = tid; i < kept; i += SMP_THREADS) s.weight[i] = weight(smp_logit((unsigned)s.list[i]));
+      __syncthreads();
+      smp_scan(s, kept);
+      for (int i = tid; i < kept; i += SMP_THREADS)
+        if (s.weight[i] > target && (i == 0 || s.weight[i - 1] <= target)) p.out[b] = 0xffffffffu - (unsigned)(s.list[i] >> 32);
+      return;
+    }
+  }
+
+  auto clear = [&]() {
+    __syncthreads();
+    for (int i = tid; i < SMP_BINS; i += SMP_THREADS) s.sums[i] = 0;
+    if (tid == 0 && rank == 0) s.count = 0;
+    __syncthreads();
+  };
+  auto add_weight = [&](int bin, u64 w) {         // the carry from the low to the high word is this thread's to see
+    const unsigned low = (unsigned)w, old = atomicAdd(halves + 2 * bin, low), high = (unsigned)(w >> 32) + (old + low < old);
+    if (high) atomicAdd(halves + 2 * bin + 1, high);
+  };
+  // The key at which the sum (of the weights above the border so far, or of ones) reaches `target`, and what lies above it.
+  auto bit_by_bit = [&](bool weights, u64 target, u64& above) {
+    unsigned key_so_far = 0;
+    above = 0;
+    for (int shift = 21;; shift = shift == 21 ? 10 : 0) {
+      const int bits = shift == 0 ? 10 : 11;
+      clear();
+      slice.pass(s, p.status, [&](int i, const float* l, int n) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const unsigned key = smp_key(l[e]);
-          const bool mine = e < n && key >> 21 >= lowest;
-          if (mine) {
-            const unsigned x = atomicAdd(n_list, 1u);
-            if (x < SMP_CAP) list[x] = (u64)key << 32 | (0xffffffffu - (unsigned)(i + e));
-          }
-          if (need_total && e < n) total += weight(l[e]);
+          if (e >= n || (shift < 21 && key >> (shift + bits) != key_so_far >> (shift + bits))) continue;
+          const unsigned bin = key >> shift & ((1u << bits) - 1);
+          if (!weights) atomicAdd(halves + 2 * bin, 1u);
+          else if (key > border && weight.passes(l[e])) add_weight(bin, weight(l[e]));
         }
       });
-      if (need_total) {
-        total = smp_block_sum(total, s.warp);
-        if (tid == 0) smp_peer(s.tot, 0)[rank] = total;
-      }
-      smp_cluster_sync();
-      if (rank == 0) {
-        // ---- one CTA sorts them and finishes
-        const int n = min(s.count, (unsigned)SMP_CAP);
-        smp_sort(s.list, n);
-        int kept = top_k ? min(n, top_k) : n;
-        u64 below = 0;                            // (counts of this thread's)
-        for (int i = tid; i < n; i += SMP_THREADS) {
-          const double w = weight.real(smp_logit((unsigned)(s.list[i] >> 32)));
-          s.weight[i] = SmpWeight::fixed(w);
-          below += i < kept && w < min_p;
-        }
-        kept -= (int)smp_block_sum(below, s.warp);
-        smp_scan(s, n);
-        u64 sum = kept > 0 ? s.weight[kept - 1] : 0;
-        if (need_total) {
-          sum = 0;
-          for (int c = 0; c < ctas; ++c) sum += s.tot[c];
-        }
-        if (nucleus) {
-          const u64 border_sum = __double2ull_ru(top_p * (double)sum);
-          u64 in = 0;
-          for (int i = tid; i < kept; i += SMP_THREADS) in += i == 0 || s.weight[i - 1] < border_sum;
-          const int inside = (int)smp_block_sum(in, s.warp);
-          if (need_total && inside == n && (n == 0 || s.weight[n - 1] < border_sum)) {
-            if (tid < ctas) *smp_peer(&s.bad, tid) = 1;           // the border lies below the list
-          }
-          kept = inside;
-          __syncthreads();
-        }
-        if (!s.bad) {
-          const u64 target = place(s.weight[kept - 1]);
-          __syncthreads();
-          for (int i = tid; i < kept; i += SMP_THREADS) {
-            const u64 x = s.list[i];
-            s.list[i] = x << 32 | x >> 32;        // by index now
-          }
-          smp_sort(s.list, kept);
-          for (int i = tid; i < kept; i += SMP_THREADS) s.weight[i] = weight(smp_logit((unsigned)s.list[i]));
-          __syncthreads();
-          smp_scan(s, kept);
-          for (int i = tid; i < kept; i += SMP_THREADS)
-            if (s.weight[i] > target && (i == 0 || s.weight[i - 1] <= target)) p.out[b] = 0xffffffffu - (unsigned)(s.list[i] >> 32);
-        }
-      }
-      if (!need_total) return;
-      smp_cluster_sync();
-      if (!s.bad) return;
+      smp_find(s, rank, ctas, [&](u64 all) { return min(target - above, all); });
+      key_so_far |= (unsigned)s.found[0] << shift;
+      above += s.found[1];
+      if (shift == 0) return key_so_far;
     }
-
-    // ---- the border by the rest of the order's bits
-    auto refine = [&](bool weights, u64 target, unsigned known, int from) {      // bits below `from` of the border's key
-      u64 above = 0;
-      for (int shift = from == 32 ? 21 : from == 21 ? 10 : 0;;) {
-        const int bits = shift == 21 ? 11 : shift == 10 ? 11 : 10;
-        __syncthreads();
-        for (int i = tid; i < SMP_BINS; i += SMP_THREADS) s.sums[i] = 0;
-        __syncthreads();
-        smp_stream<L>(row, begin, end, p.vec, [&](int i, const float* l, int n) {
+  };
+  auto weight_of_border = [&]() {
+    const float l = smp_logit(border);
+    return border && weight.passes(l) ? weight(l) : 0;
+  };
+  if (top_k) {
+    u64 above;
+    border = bit_by_bit(false, top_k, above);
+    of_border = top_k - above;
+  }
+  if (nucleus) {
+    const u64 each = weight_of_border();
+    clear();
+    slice.pass(s, p.status, [&](int i, const float* l, int n) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const unsigned key = smp_key(l[e]);
-            if (e >= n || (shift < 21 && key >> (shift + bits) != known >> (shift + bits))) continue;
-            const unsigned bin = key >> shift & ((1u << bits) - 1);
-            if (!weights) {
-              atomicAdd(counts + 2 * bin, 1u);
-            } else if (key > border) {
-              const double w = weight.real(l[e]);
-              const u64 f = SmpWeight::fixed(w);
-              if (w >= min_p && f) atomicAdd(s.sums + bin, f);
-            }
-          }
-        });
-        smp_find(s, target - above, rank, ctas);
-        known |= (unsigned)s.found[0] << shift;
-        above += s.found[1];
-        if (shift == 0) break;
-        shift = shift == 21 ? 10 : 0;
-      }
-      of_border = above;                          // what lies above it
-      return known;
-    };
-    if (top_k) {
+      for (int e = 0; e < 4; ++e)
+        if (e < n && smp_key(l[e]) > border && weight.passes(l[e]))
+          if (const u64 w = weight(l[e])) add_weight(weight.bin(l[e]), w);
+    });
+    u64 want = 0;
+    smp_find(s, rank, ctas, [&](u64 all) {
+      want = max(__double2ull_ru(top_p * (double)(all + each * of_border)), 1ULL);
+      if (!each) want = min(want, all);
+      return want;
+    });
+    if (want > s.found[2]) {                      // among those of the border
+      of_border = min(of_border, (want - s.found[2] + each - 1) / max(each, 1ULL));
+    } else {
+      const int bin = (int)s.found[0];
       const u64 above = s.found[1];
-      border = refine(false, top_k - above, (unsigned)s.found[0] << 21, 21);
-      of_border = top_k - above - of_border;
-    }
-    if (nucleus) {
-      // all that is left so far
-      u64 total = 0;
-      smp_stream<L>(row, begin, end, p.vec, [&](int i, const float* l, int n) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (e < n && smp_key(l[e]) > border) {
-            const double w = weight.real(l[e]);
-            if (w >= min_p) total += SmpWeight::fixed(w);
-          }
-      });
-      total = smp_block_sum(total, s.warp);
-      if (tid < ctas) smp_peer(s.tot2, tid)[rank] = total;
-      smp_cluster_sync();
-      total = 0;
-      for (int c = 0; c < ctas; ++c) total += s.tot2[c];
-      u64 each = 0;
-      if (top_k) {
-        const double w = weight.real(smp_logit(border));
-        if (w >= min_p) each = SmpWeight::fixed(w);
-      }
-      const u64 want = max(__double2ull_ru(top_p * (double)(total + each * of_border)), 1ULL);
-      if (want > total && each) {
-        of_border = min(of_border, (want - total + each - 1) / each);
+      const unsigned n_list = gather([&](float l, unsigned key) { return key > border && weight.bin(l) == bin && weight.passes(l); });
+      if (n_list <= SMP_CAP) {
+        if (rank == 0) {
+          const int n = (int)n_list;
+          smp_sort(s.list, n);
+          for (int i = tid; i < n; i += SMP_THREADS) s.weight[i] = weight(smp_logit((unsigned)(s.list[i] >> 32)));
+          __syncthreads();
+          smp_scan(s, n);
+          for (int i = tid; i < n; i += SMP_THREADS)
+            if (above + s.weight[i] >= want && (i == 0 || above + s.weight[i - 1] < want)) {
+              const unsigned key = (unsigned)(s.list[i] >> 32);
+              int of = 1;
+              while (of <= i && (unsigned)(s.list[i - of] >> 32) == key) ++of;
+              for (int c = 0; c < ctas; ++c) *smp_peer(&s.border, c) = key, *smp_peer(&s.of_border, c) = of;
+            }
+        }
+        smp_cluster_sync();
+        border = s.border;
+        of_border = s.of_border;
       } else {
-        const unsigned key = refine(true, min(want, total), 0, 32);
-        const u64 w = weight(smp_logit(key));
-        of_border = (min(want, total) - of_border + w - 1) / w;
+        u64 over;
+        const unsigned key = bit_by_bit(true, want, over);
+        const u64 w = max(weight(smp_logit(key)), 1ULL);
+        of_border = (want - over + w - 1) / w;
         border = key;
       }
     }
   }
 
   // ---- the token: sums of the slices, of the warps' parts of the one it lies in, then along that part
-  const u64 each = border ? [&] { const double w = weight.real(smp_logit(border)); return w >= min_p ? SmpWeight::fixed(w) : 0; }() : 0;
-  const int part = ((end - begin + SMP_WARPS - 1) / SMP_WARPS + 127) / 128 * 128;
-  const int from = min(end, begin + warp * part), to = min(end, from + part);
-  auto add = [&](int i, u64& sum, u64& equal) {   // four logits of a lane
-    float l[4];
-    if (i < to) smp_load<L>(row, i, to, p.vec && (from & 3) == 0, l);
+  const u64 each = weight_of_border();
+  const int part = ((slice.end - slice.begin + SMP_WARPS - 1) / SMP_WARPS + 127) / 128 * 128;
+  const int from = min(slice.end, slice.begin + warp * part), to = min(slice.end, from + part);
+  auto load = [&](int i, float* l) {              // four logits of a lane
+    if (slice.kept && i + 4 <= min(to, slice.copied)) smp_load<L>(reinterpret_cast<const L*>(s.ring), i - slice.begin, to - slice.begin, 1, l);
+    else if (i < to) smp_load<L>(slice.row, i, to, slice.vec && (from & 3) == 0, l);
+  };
+  auto add = [&](int i, const float* l, u64& sum, unsigned& equal) {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (i + e < to) {
         const unsigned key = smp_key(l[e]);
         if (key > border) {
-          const double w = weight.real(l[e]);
-          if (w >= min_p) sum += SmpWeight::fixed(w);
+          if (weight.passes(l[e])) sum += weight(l[e]);
         } else if (key == border) {
           ++equal;
         }
       }
   };
-  u64 sum = 0, equal = 0;
-#pragma unroll 2
-  for (int i = from + lane * 4; i < to; i += 128) add(i, sum, equal);
+  u64 sum = 0;
+  unsigned equal = 0;
+  for (int i = from + lane * 4; i < to; i += 4 * 128) {
+    float l[4][4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) load(i + x * 128, l[x]);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) add(i + x * 128, l[x], sum, equal);
+  }
   sum = smp_warp_sum(sum);
-  equal = smp_warp_sum(equal);
+  equal = __reduce_add_sync(0xffffffffu, equal);
   __syncthreads();
   if (lane == 0) s.warp[warp] = sum, s.warp2[warp] = equal;
   __syncthreads();
@@ -528,33 +637,30 @@ sample_kernel(const SampleParams p, int ctas) {
   for (int w = 0; w < warp; ++w) x += s.warp[w], y += s.warp2[w];
   if (upto(x, y) > target || upto(x + sum, y + equal) <= target) return;
   for (int i0 = from; i0 < to; i0 += 128) {
-    u64 mine = 0, ties = 0;
-    add(i0 + lane * 4, mine, ties);
-    const u64 all = smp_warp_sum(mine), all_ties = smp_warp_sum(ties);
+    const int i = i0 + lane * 4;
+    float l[4];
+    load(i, l);
+    u64 mine = 0;
+    unsigned ties = 0;
+    add(i, l, mine, ties);
+    const u64 all = smp_warp_sum(mine);
+    const unsigned all_ties = __reduce_add_sync(0xffffffffu, ties);
     if (upto(x + all, y + all_ties) > target) {
+      u64 before = mine, before_ties = ties;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const u64 a = __shfl_up_sync(0xffffffffu, mine, o), c = __shfl_up_sync(0xffffffffu, ties, o);
-        if (lane >= o) mine += a, ties += c;
+        const u64 a = __shfl_up_sync(0xffffffffu, before, o), c = __shfl_up_sync(0xffffffffu, before_ties, o);
+        if (lane >= o) before += a, before_ties += c;
       }
-      const unsigned past = __ballot_sync(0xffffffffu, upto(x + mine, y + ties) > target);
-      const int owner = __ffs(past) - 1;
-      u64 before = __shfl_up_sync(0xffffffffu, mine, 1), before_ties = __shfl_up_sync(0xffffffffu, ties, 1);
-      if (lane == 0) before = before_ties = 0;
-      if (lane == owner) {
-        const int i = i0 + lane * 4;
-        float l[4];
-        smp_load<L>(row, i, to, 0, l);
-        u64 a = x + before, c = y + before_ties;
+      const unsigned past = __ballot_sync(0xffffffffu, upto(x + before, y + before_ties) > target);
+      if (lane == __ffs(past) - 1) {
+        x += before - mine;
+        y += before_ties - ties;
         for (int e = 0; e < 4 && i + e < to; ++e) {
           const unsigned key = smp_key(l[e]);
-          if (key > border) {
-            const double w = weight.real(l[e]);
-            if (w >= min_p) a += SmpWeight::fixed(w);
-          } else if (key == border) {
-            ++c;
-          }
-          if (upto(a, c) > target) {
+          if (key > border) x += weight.passes(l[e]) ? weight(l[e]) : 0;
+          else if (key == border) ++y;
+          if (upto(x, y) > target) {
             p.out[b] = i + e;
             break;
           }
@@ -596,8 +702,9 @@ extern "C" int tpb_sample_tokens(const void* logits, int bf16, long long stride,
   while (ctas < 16 && (long long)B * ctas * 2 <= 4LL * sm_count() && V / (ctas * 2) >= 2048) ctas *= 2;
   const int elt = bf16 ? 2 : 4;
   SampleParams p = {logits, stride, u, temperature, top_p, min_p, top_k, temperature0, top_p0, min_p0, top_k0, V,
-                    ((V + ctas - 1) / ctas + 3) / 4 * 4, out, 0};
-  p.vec = reinterpret_cast<uintptr_t>(logits) % (4 * elt) == 0 && stride % 4 == 0;
+                    ((V + ctas - 1) / ctas + 7) / 8 * 8, out, 0, status_block()};
+  p.vec = (reinterpret_cast<uintptr_t>(logits) % (4 * elt) == 0 && stride % 4 == 0) +
+          (reinterpret_cast<uintptr_t>(logits) % 16 == 0 && stride * elt % 16 == 0);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   return bf16 ? launch_sample<__nv_bfloat16>(p, B, ctas, stream) : launch_sample<float>(p, B, ctas, stream);
 }
