@@ -32,7 +32,7 @@ constexpr int SMP_BINS = 2048;          // 11 bits of the order at a time (31-21
 constexpr int SMP_CAP = 2048;           // tokens that one CTA sorts
 constexpr int SMP_FIXED = 44;           // a weight of 1 is 2^44: 2^18 of them stay below 2^63
 constexpr int SMP_TABLE = 1024;         // 2^(j / 1024)
-constexpr int SMP_CHUNK = SMP_THREADS * 4, SMP_RING = 6;       // logits of a bulk copy, copies under way
+constexpr int SMP_CHUNK = SMP_THREADS * 8, SMP_RING = 3;       // logits of a bulk copy, copies under way
 
 using u64 = unsigned long long;
 
@@ -57,11 +57,15 @@ __device__ __forceinline__ T* smp_peer(T* p, int rank) {
   return reinterpret_cast<T*>(a);
 }
 
-// Order of the logits as whole numbers: larger logit, larger key; both zeros alike, subnormal ones as they are.
+// A logit as it counts: -inf for NaN, 0 for -0; subnormal ones as they are (this file is compiled to flush them in fp32 arithmetic).
+__device__ __forceinline__ float smp_clean(float l) {
+  asm("max.f32 %0, %0, 0fFF800000;\n\tadd.rn.f32 %0, %0, 0f00000000;" : "+f"(l));
+  return l;
+}
+// Order of the logits as whole numbers: larger logit, larger key.
 __device__ __forceinline__ unsigned smp_key(float l) {
-  unsigned b = __float_as_uint(l);
-  if (b == 0x80000000u) b = 0;
-  return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
+  const int b = __float_as_int(l);
+  return (unsigned)(b ^ (b >> 31 | (int)0x80000000));
 }
 __device__ __forceinline__ float smp_logit(unsigned key) { return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu)); }
 
@@ -69,17 +73,18 @@ struct SmpWeight {
   double per_unit;        // log2(e) / T
   float top, hi, lo;      // 1024 log2(e) / T as a sum of two floats
   bool slow;              // T, or the logits, near the ends of fp32's range
+  bool some;              // min_p is on
   double min_p;
   float sure, sure_not;   // 1024 log2 of weights that pass min_p, that do not
   const u64* table;       // 2^62 2^(j / 1024), shared
 
   __device__ __forceinline__ SmpWeight(double T, float top_, double min_p_, const u64* table_)
-      : per_unit(1.4426950408889634 / T), top(top_), min_p(min_p_), table(table_) {
+      : per_unit(1.4426950408889634 / T), top(top_), some(min_p_ > 0.0), min_p(min_p_), table(table_) {
     const double c = per_unit * SMP_TABLE;
     hi = (float)c;
     lo = (float)(c - (double)hi);
     slow = !(T > 1e-20 && T < 1e20 && fabsf(top) < 1e18f);
-    const double border = min_p > 0.0 ? log2(min_p) * SMP_TABLE : -1e30;
+    const double border = some ? log2(min_p) * SMP_TABLE : -1e30;
     sure = (float)(border + 0.01 + 1e-6 * fabs(border));
     sure_not = (float)(border - 0.01 - 1e-6 * fabs(border));
   }
@@ -109,11 +114,11 @@ struct SmpWeight {
     const u64 t = table[j & (SMP_TABLE - 1)];
     const u64 w = t + (u64)(((long long)(int)(t >> 32) * qi) >> 1);
     const int down = 62 - SMP_FIXED - (j >> 10);
-    return (w + (1ULL << (down - 1))) >> down;
+    return ((w >> (down - 1)) + 1) >> 1;
   }
   // w >= min_p
   __device__ __forceinline__ bool passes(float l) const {
-    if (!(min_p > 0.0)) return true;
+    if (!some) return true;
     if (!slow) {
       float rest;
       const float x = exponent(l, rest);
@@ -270,7 +275,7 @@ __device__ __forceinline__ float smp_read(const float* p) { return *p; }
 template <>
 __device__ __forceinline__ float smp_read(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
-// Four logits from index i on, -inf for NaN (which is never drawn) and behind `end`.
+// Four logits from index i on, -inf behind `end` (and for NaN: neither is drawn).
 template <typename L>
 __device__ __forceinline__ void smp_load(const L* row, int i, int end, int vec, float* l) {
   if (vec && i + 4 <= end) {
@@ -287,7 +292,7 @@ __device__ __forceinline__ void smp_load(const L* row, int i, int end, int vec, 
     for (int e = 0; e < 4; ++e) l[e] = i + e < end ? smp_read<L>(row + i + e) : -INFINITY;
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) l[e] = l[e] != l[e] ? -INFINITY : l[e];
+  for (int e = 0; e < 4; ++e) l[e] = smp_clean(l[e]);
 }
 
 // The CTA's slice, pass by pass.
@@ -309,23 +314,22 @@ struct SmpSlice {
                    : "r"(smem_u32(reinterpret_cast<L*>(s.ring) + slot * SMP_CHUNK)), "l"(row + at), "r"(n), "r"(smem_u32(&s.full[slot]))
                    : "memory");
   }
-  // f(index, four logits, how many there are) in every thread
+  // f(index, four logits) for all of them; -inf stands behind the end of the row
   template <typename F>
   __device__ __forceinline__ void pass(SmpShared& s, int* status, F&& f) {
     const int chunks = (end - begin + SMP_CHUNK - 1) / SMP_CHUNK, tid = threadIdx.x;
     if (vec < 2) {
-      constexpr int AHEAD = 2;
-      for (int i0 = begin; i0 < end; i0 += AHEAD * SMP_CHUNK) {
-        float l[AHEAD][4];
+      for (int i0 = begin; i0 < end; i0 += SMP_CHUNK) {
+        float l[2][4];
 #pragma unroll
-        for (int x = 0; x < AHEAD; ++x) {
-          const int i = i0 + x * SMP_CHUNK + tid * 4;
+        for (int x = 0; x < 2; ++x) {
+          const int i = i0 + (x * SMP_THREADS + tid) * 4;
           if (i < end) smp_load<L>(row, i, end, vec, l[x]);
         }
 #pragma unroll
-        for (int x = 0; x < AHEAD; ++x) {
-          const int i = i0 + x * SMP_CHUNK + tid * 4;
-          f(i, l[x], min(4, end - i));  // (none: 0 or less)
+        for (int x = 0; x < 2; ++x) {
+          const int i = i0 + (x * SMP_THREADS + tid) * 4;
+          if (i < end) f(i, l[x]);
         }
       }
       return;
@@ -335,21 +339,25 @@ struct SmpSlice {
       if (tid == 0 && !s.dead)
         for (int c = 0; c < min(chunks, SMP_RING); ++c) copy(s, c);
     }
-    for (int c = 0; c < chunks; ++c) {
-      const int slot = c % SMP_RING, i = begin + c * SMP_CHUNK + tid * 4;
+    for (int c = 0, slot = 0; c < chunks; ++c) {
       if (!kept) {
         if (!s.dead && !mbar_wait(&s.full[slot], parity >> slot & 1, status, kTimeoutTmaFull, 76)) s.dead = 1;
         parity ^= 1u << slot;
       }
-      float l[4];
       const L* ring = reinterpret_cast<const L*>(s.ring) + slot * SMP_CHUNK;
-      if (i + 4 <= copied) smp_load<L>(ring, tid * 4, SMP_CHUNK, 1, l);
-      else if (i < end) smp_load<L>(row, i, end, 0, l);
-      f(i, l, min(4, end - i));
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int in = (x * SMP_THREADS + tid) * 4, i = begin + c * SMP_CHUNK + in;
+        float l[4];
+        if (i + 4 <= copied) smp_load<L>(ring, in, SMP_CHUNK, 1, l);
+        else if (i < end) smp_load<L>(row, i, end, 0, l);
+        if (i < end) f(i, l);
+      }
       if (!kept && chunks > SMP_RING) {
         __syncthreads();
         if (tid == 0 && !s.dead && c + SMP_RING < chunks) copy(s, c + SMP_RING);
       }
+      if (++slot == SMP_RING) slot = 0;
     }
     kept = chunks <= SMP_RING;
   }
@@ -387,13 +395,15 @@ sample_kernel(const SampleParams p, int ctas) {
   // ---- the largest logit and its first index
   unsigned top_key = 0;
   int at = V;
-  slice.pass(s, p.status, [&](int i, const float* l, int n) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const unsigned key = smp_key(l[e]);
-      if (e < n && key > top_key) top_key = key, at = i + e;
-    }
+  slice.pass(s, p.status, [&](int i, const float* l) {
+    const unsigned key = max(max(smp_key(l[0]), smp_key(l[1])), max(smp_key(l[2]), smp_key(l[3])));
+    if (key > top_key) top_key = key, at = i;
   });
+  if (greedy && at < V) {                         // which of the four
+    float l[4];
+    smp_load<L>(slice.row, at, slice.end, 0, l);
+    at += smp_key(l[0]) == top_key ? 0 : smp_key(l[1]) == top_key ? 1 : smp_key(l[2]) == top_key ? 2 : 3;
+  }
   if (top_k && !greedy && top_key) atomicAdd(halves + 2 * (top_key >> 21), 1u);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -427,11 +437,11 @@ sample_kernel(const SampleParams p, int ctas) {
   auto gather = [&](auto&& wanted) {
     u64* const list = smp_peer(s.list, 0);
     unsigned* const n_list = smp_peer(&s.count, 0);
-    slice.pass(s, p.status, [&](int i, const float* l, int n) {
+    slice.pass(s, p.status, [&](int i, const float* l) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const unsigned key = smp_key(l[e]);
-        if (e < n && wanted(l[e], key)) {
+        if (wanted(l[e], key)) {
           const unsigned x = atomicAdd(n_list, 1u);
           if (x < SMP_CAP) list[x] = (u64)key << 32 | (0xffffffffu - (unsigned)(i + e));
         }
@@ -513,11 +523,11 @@ sample_kernel(const SampleParams p, int ctas) {
     for (int shift = 21;; shift = shift == 21 ? 10 : 0) {
       const int bits = shift == 0 ? 10 : 11;
       clear();
-      slice.pass(s, p.status, [&](int i, const float* l, int n) {
+      slice.pass(s, p.status, [&](int i, const float* l) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const unsigned key = smp_key(l[e]);
-          if (e >= n || (shift < 21 && key >> (shift + bits) != key_so_far >> (shift + bits))) continue;
+          if (shift < 21 && key >> (shift + bits) != key_so_far >> (shift + bits)) continue;
           const unsigned bin = key >> shift & ((1u << bits) - 1);
           if (!weights) atomicAdd(halves + 2 * bin, 1u);
           else if (key > border && weight.passes(l[e])) add_weight(bin, weight(l[e]));
@@ -541,10 +551,10 @@ sample_kernel(const SampleParams p, int ctas) {
   if (nucleus) {
     const u64 each = weight_of_border();
     clear();
-    slice.pass(s, p.status, [&](int i, const float* l, int n) {
+    slice.pass(s, p.status, [&](int i, const float* l) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (e < n && smp_key(l[e]) > border && weight.passes(l[e]))
+        if (smp_key(l[e]) > border && weight.passes(l[e]))
           if (const u64 w = weight(l[e])) add_weight(weight.bin(l[e]), w);
     });
     u64 want = 0;
