@@ -30,11 +30,34 @@ int sm_count();
 constexpr int SMP_THREADS = 512, SMP_WARPS = SMP_THREADS / 32;
 constexpr int SMP_BINS = 2048;          // 11 bits of the order at a time (31-21, 20-10, 9-0); 64 binary orders of weights in steps of 1/32
 constexpr int SMP_CAP = 2048;           // tokens that one CTA sorts
+#ifndef SMP_FILL
+#define SMP_FILL 4LL
+#endif
+#ifndef SMP_LEAST
+#define SMP_LEAST 2048
+#endif
 constexpr int SMP_FIXED = 44;           // a weight of 1 is 2^44: 2^18 of them stay below 2^63
 constexpr int SMP_TABLE = 1024;         // 2^(j / 1024)
 constexpr int SMP_CHUNK = SMP_THREADS * 8, SMP_RING = 3;       // logits of a bulk copy, copies under way
 
 using u64 = unsigned long long;
+
+// 2^62 2^(j / 1024), to a double's precision.
+struct SmpTable {
+  u64 at[SMP_TABLE];
+  constexpr SmpTable() : at() {
+    for (int j = 0; j < SMP_TABLE; ++j) {
+      const double y = j * (0.69314718055994530942 / SMP_TABLE);
+      double sum = 1, term = 1;
+      for (int k = 1; k < 24; ++k) {
+        term *= y / k;
+        sum += term;
+      }
+      at[j] = (u64)(sum * 4611686018427387904.0);
+    }
+  }
+};
+__device__ const SmpTable smp_table = SmpTable();
 
 struct SampleParams {
   const void* logits;
@@ -64,18 +87,27 @@ __device__ __forceinline__ float smp_clean(float l) {
 }
 // Order of the logits as whole numbers: larger logit, larger key.
 __device__ __forceinline__ unsigned smp_key(float l) {
-  const int b = __float_as_int(l);
+  const int b = __float_as_int(smp_clean(l));
   return (unsigned)(b ^ (b >> 31 | (int)0x80000000));
+}
+// The largest of four logits (no NaN, unless all are).
+__device__ __forceinline__ float smp_max4(const float* l) {
+  float m;
+  asm("max.f32 %0, %1, %2;\n\tmax.f32 %0, %0, %3;\n\tmax.f32 %0, %0, %4;" : "=&f"(m) : "f"(l[0]), "f"(l[1]), "f"(l[2]), "f"(l[3]));
+  return m;
 }
 __device__ __forceinline__ float smp_logit(unsigned key) { return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu)); }
 
 struct SmpWeight {
   double per_unit;        // log2(e) / T
-  float top, hi, lo;      // 1024 log2(e) / T as a sum of two floats
-  bool slow;              // T, or the logits, near the ends of fp32's range
+  float top, hi, lo;      // the largest logit; 1024 log2(e) / T as a sum of two floats
+  float p_top, p_cut;     // 1024 log2 of the largest weight, and 2^-45 of it, before that is made 1: the nearest product
+  int j_top;              // the whole number it is nearest to (with the other bits of the pattern), and what is missing
+  float y_top;
+  bool slow;              // T, or the logits, too far from 1 for that
   bool some;              // min_p is on
   double min_p;
-  float sure, sure_not;   // 1024 log2 of weights that pass min_p, that do not
+  float sure, sure_not;   // p - p_top of weights that pass min_p, that do not
   const u64* table;       // 2^62 2^(j / 1024), shared
 
   __device__ __forceinline__ SmpWeight(double T, float top_, double min_p_, const u64* table_)
@@ -83,56 +115,84 @@ struct SmpWeight {
     const double c = per_unit * SMP_TABLE;
     hi = (float)c;
     lo = (float)(c - (double)hi);
-    slow = !(T > 1e-20 && T < 1e20 && fabsf(top) < 1e18f);
+    slow = !(T > 1e-20 && T < 1e20 && fabsf(top) * hi < 2097152.f);
+    p_top = __fmul_rn(top, hi);
+    p_cut = p_top - 45.f * SMP_TABLE;
+    split(top, p_top, 0.f, j_top, y_top);
     const double border = some ? log2(min_p) * SMP_TABLE : -1e30;
-    sure = (float)(border + 0.01 + 1e-6 * fabs(border));
-    sure_not = (float)(border - 0.01 - 1e-6 * fabs(border));
+    sure = (float)(border + 1.0 + 1e-6 * fabs(border));
+    sure_not = (float)(border - 1.0 - 1e-6 * fabs(border));
+  }
+  // 1024 l log2(e) / T = j + y, j whole (in the low bits of a float's pattern), less y0; p = l * hi
+  __device__ __forceinline__ void split(float l, float p, float y0, int& j, float& y) const {
+    const float shifted = __fadd_rn(p, 12582912.f);             // 1.5 * 2^23 (not as one fma: step() has to see the same)
+    j = __float_as_int(shifted);
+    y = (p - (shifted - 12582912.f)) + (fmaf(l, hi, -p) + fmaf(l, lo, -y0));
   }
   // in 64 bits
   __device__ __noinline__ double real(float l) const {
-    return l == top ? 1.0 : l == -INFINITY ? 0.0 : exp2(((double)l - (double)top) * per_unit);
+    const double x = ((double)l - (double)top) * per_unit;
+    return l == top ? 1.0 : x > -100.0 ? exp2(x) : 0.0;         // (NaN, of infinities: 0)
   }
-  // 1024 log2(w), the nearest float and what is missing
-  __device__ __forceinline__ float exponent(float l, float& rest) const {
-    const float d = l - top, back = d - l;
-    const float err = (l - (d - back)) - (top + back);          // l - top = d + err
-    const float x = d * hi;
-    rest = fmaf(err, hi, fmaf(d, lo, fmaf(d, hi, -x)));
-    return x;
+  __device__ __noinline__ int step_slow(float l) const {
+    return l == top ? 0 : (int)fmax(fmin(rint(((double)l - (double)top) * per_unit * SMP_TABLE), 0.0), -1e9);
   }
-  // in multiples of 2^-44
-  __device__ __forceinline__ u64 operator()(float l) const {
-    if (slow) return __double2ull_rn(real(l) * (double)(1LL << SMP_FIXED));
-    float rest;
-    const float x = exponent(l, rest);
-    if (!(x > -45.0f * SMP_TABLE)) return 0;
-    const float shifted = x + 12582912.f;                       // 1.5 * 2^23: the nearest whole number ends up in the low bits
-    const int j = __float_as_int(shifted) - 0x4b400000;
-    const float y = ((x - (shifted - 12582912.f)) + rest) * (0.69314718056f / SMP_TABLE);
-    const float q = fmaf(0.5f * y, y, y);                       // 2^rest - 1, |q| < 2^-11; the next term is below 2^-37
-    const int qi = __float_as_int(q + 0.00146484375f) - 0x3ac00000;      // 1.5 * 2^-10: in multiples of 2^-33
+  // 1024 log2 of the weight, rounded: does not fall where l grows.
+  __device__ __forceinline__ int step(float l) const {
+    return slow ? step_slow(l) : __float_as_int(__fadd_rn(fmaxf(__fmul_rn(l, hi), p_top - 1048576.f), 12582912.f)) - j_top;
+  }
+  // In multiples of 2^-44: 2^44 for the largest, else with the last bit set, as often above as below what is cut off; 0 below 2^-45 and
+  // for NaN.  j: step(l).
+  __device__ __forceinline__ u64 operator()(float l, int& j) const {
+    if (slow) {
+      j = step_slow(l);
+      return __double2ull_rn(real(l) * (double)(1LL << SMP_FIXED));
+    }
+    const float p = __fmul_rn(l, hi);
+    if (!(p > p_cut)) {
+      j = -0x100000;
+      return 0;
+    }
+    float y;
+    split(l, p, y_top, j, y);
+    j -= j_top;
+    y *= 0.69314718056f / SMP_TABLE;
+    const float q = fmaf(fmaf(y, 1.f / 6, 0.5f) * y, y, y);     // 2^rest - 1, |q| < 2^-10; the next term is below 2^-46
+    const int qi = __float_as_int(q + 0.0029296875f) - 0x3b400000;       // 1.5 * 2^-9: in multiples of 2^-32
     const u64 t = table[j & (SMP_TABLE - 1)];
-    const u64 w = t + (u64)(((long long)(int)(t >> 32) * qi) >> 1);
-    const int down = 62 - SMP_FIXED - (j >> 10);
-    return ((w >> (down - 1)) + 1) >> 1;
+    const u64 w = t + (u64)((long long)(int)(t >> 32) * qi);
+    const u64 x = w >> (62 - SMP_FIXED - (j >> 10));
+    return x | (~x >> SMP_FIXED & 1);
+  }
+  __device__ __forceinline__ u64 operator()(float l) const {
+    int j;
+    return (*this)(l, j);
   }
   // w >= min_p
   __device__ __forceinline__ bool passes(float l) const {
     if (!some) return true;
     if (!slow) {
-      float rest;
-      const float x = exponent(l, rest);
+      const float x = l * hi - p_top;
       if (x > sure) return true;
       if (!(x > sure_not)) return false;
     }
     return real(l) >= min_p;
   }
   // Steps of 1/32 below the largest weight's exponent, the largest weights in the last bin.
-  __device__ __forceinline__ int bin(float l) const {
-    if (l == top) return SMP_BINS - 1;
-    float rest;
-    const float x = slow ? (float)(fmax((double)l - (double)top, -1e38) * per_unit * SMP_TABLE) : exponent(l, rest);
-    return x > -(float)(SMP_BINS - 1) * 32.f ? SMP_BINS - 1 - (int)(-x * 0.03125f) : 0;
+  static __device__ __forceinline__ int bin(int j) { return SMP_BINS - 1 + max(j >> 5, 1 - SMP_BINS); }
+  // The smallest key whose bin is `of` or more; the whole warp calls.
+  __device__ __forceinline__ unsigned first_key(int of) const {
+    unsigned low = 0x007fffffu, high = 0xff800001u;             // -inf (bin 0); behind inf
+    while (high - low > 1) {
+      const unsigned wide = (high - low + 32) / 33, at = low + wide * ((threadIdx.x & 31) + 1);
+      const bool past = at >= high || bin(step(smp_logit(at))) >= of;
+      const unsigned which = __ballot_sync(0xffffffffu, past);
+      const int n = which ? __ffs(which) - 1 : 32;              // lanes in front of the border
+      const unsigned l = low + wide * n, h = low + wide * (n + 1);
+      low = l;
+      high = min(high, h);
+    }
+    return high;
   }
 };
 
@@ -147,6 +207,7 @@ struct SmpShared {
   u64 found[3];                         // bin, sum of the bins above, sum of all
   unsigned count;                       // of the list
   unsigned border, of_border;
+  unsigned staged, base;                // of this CTA's part of the list
   int dead;                             // a copy has not come
 };
 
@@ -198,13 +259,27 @@ template <typename F>
 __device__ __forceinline__ void smp_find(SmpShared& s, int rank, int ctas, F&& target) {
   const int per = SMP_BINS / ctas, b0 = rank * per;
   smp_cluster_sync();
+  // the CTAs' counts of a bin, added up by several threads
+  const int groups = min(SMP_THREADS / min(per, SMP_THREADS), ctas), group = (int)threadIdx.x / per;
+  if (groups > 1) {
+    if (group < groups) {
+      u64 x = 0;
+#pragma unroll 4
+      for (int c = group; c < ctas; c += groups) x += smp_peer(s.sums, c)[b0 + threadIdx.x % per];
+      s.weight[threadIdx.x] = x;
+    }
+    __syncthreads();
+  }
   // four neighbouring bins to a thread, the topmost to thread 0
   u64 v[4] = {}, mine = 0;
   const int high = b0 + per - 1 - (int)threadIdx.x * 4;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     if (high - i >= b0) {
-      for (int c = 0; c < ctas; ++c) v[i] += smp_peer(s.sums, c)[high - i];
+      if (groups > 1)
+        for (int k = 0; k < groups; ++k) v[i] += s.weight[k * per + high - i - b0];
+      else
+        for (int c = 0; c < ctas; ++c) v[i] += smp_peer(s.sums, c)[high - i];
       mine += v[i];
     }
   const u64 sum = smp_block_sum(mine, s.warp), before = smp_block_before(mine, s.warp);
@@ -275,7 +350,7 @@ __device__ __forceinline__ float smp_read(const float* p) { return *p; }
 template <>
 __device__ __forceinline__ float smp_read(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
-// Four logits from index i on, -inf behind `end` (and for NaN: neither is drawn).
+// Four logits from index i on, -inf behind `end`.
 template <typename L>
 __device__ __forceinline__ void smp_load(const L* row, int i, int end, int vec, float* l) {
   if (vec && i + 4 <= end) {
@@ -291,8 +366,6 @@ __device__ __forceinline__ void smp_load(const L* row, int i, int end, int vec, 
 #pragma unroll
     for (int e = 0; e < 4; ++e) l[e] = i + e < end ? smp_read<L>(row + i + e) : -INFINITY;
   }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) l[e] = smp_clean(l[e]);
 }
 
 // The CTA's slice, pass by pass.
@@ -302,6 +375,7 @@ struct SmpSlice {
   int begin, end, vec;
   int copied;                           // what bulk copies can bring ends here: whole 16 bytes
   bool kept = false;                    // all of it lies in the ring
+  bool alive = true;                    // no copy has failed to come
   unsigned parity = 0;                  // of the ring's barriers, a bit each
 
   __device__ __forceinline__ void copy(SmpShared& s, int chunk) const {       // one thread
@@ -336,26 +410,36 @@ struct SmpSlice {
     }
     if (!kept) {
       __syncthreads();
-      if (tid == 0 && !s.dead)
+      if (tid == 0 && alive)
         for (int c = 0; c < min(chunks, SMP_RING); ++c) copy(s, c);
     }
     for (int c = 0, slot = 0; c < chunks; ++c) {
       if (!kept) {
-        if (!s.dead && !mbar_wait(&s.full[slot], parity >> slot & 1, status, kTimeoutTmaFull, 76)) s.dead = 1;
+        if (alive && !mbar_wait(&s.full[slot], parity >> slot & 1, status, kTimeoutTmaFull, 76)) {
+          alive = false;
+          s.dead = 1;
+        }
         parity ^= 1u << slot;
       }
       const L* ring = reinterpret_cast<const L*>(s.ring) + slot * SMP_CHUNK;
+      const int at = begin + c * SMP_CHUNK;
+      if (at + SMP_CHUNK <= copied) {
+        float l[2][4];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int in = (x * SMP_THREADS + tid) * 4, i = begin + c * SMP_CHUNK + in;
-        float l[4];
-        if (i + 4 <= copied) smp_load<L>(ring, in, SMP_CHUNK, 1, l);
-        else if (i < end) smp_load<L>(row, i, end, 0, l);
-        if (i < end) f(i, l);
+        for (int x = 0; x < 2; ++x) smp_load<L>(ring, (x * SMP_THREADS + tid) * 4, SMP_CHUNK, 1, l[x]);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) f(at + (x * SMP_THREADS + tid) * 4, l[x]);
+      } else {
+        for (int in = tid * 4; at + in < end && in < SMP_CHUNK; in += SMP_THREADS * 4) {
+          float l[4];
+          if (at + in + 4 <= copied) smp_load<L>(ring, in, SMP_CHUNK, 1, l);
+          else smp_load<L>(row, at + in, end, 0, l);
+          f(at + in, l);
+        }
       }
       if (!kept && chunks > SMP_RING) {
         __syncthreads();
-        if (tid == 0 && !s.dead && c + SMP_RING < chunks) copy(s, c + SMP_RING);
+        if (tid == 0 && alive && c + SMP_RING < chunks) copy(s, c + SMP_RING);
       }
       if (++slot == SMP_RING) slot = 0;
     }
@@ -369,8 +453,6 @@ sample_kernel(const SampleParams p, int ctas) {
   extern __shared__ __align__(128) uint8_t smp_smem[];
   SmpShared& s = *reinterpret_cast<SmpShared*>(smp_smem);
   const int rank = ctas > 1 ? (int)cluster_ctarank() : 0, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  for (int i = tid; i < SMP_BINS; i += SMP_THREADS) s.sums[i] = 0;
-  for (int i = tid; i < SMP_TABLE; i += SMP_THREADS) s.table[i] = __double2ull_rn(exp2(i / (double)SMP_TABLE) * 4611686018427387904.0);
   if (tid < SMP_RING) mbar_init(&s.full[tid], 1);
   if (tid == 0) s.count = 0, s.dead = 0;
   fence_barrier_init();
@@ -392,11 +474,16 @@ sample_kernel(const SampleParams p, int ctas) {
   const double u = fmin(fmax((double)p.u[b], 0.0), 1.0);
   unsigned* const halves = reinterpret_cast<unsigned*>(s.sums);   // low and high words of the sums
 
+  if (!greedy)
+    for (int i = tid; i < SMP_TABLE; i += SMP_THREADS) s.table[i] = smp_table.at[i];
+  if (top_k && !greedy)
+    for (int i = tid; i < SMP_BINS; i += SMP_THREADS) s.sums[i] = 0;
+
   // ---- the largest logit and its first index
   unsigned top_key = 0;
   int at = V;
   slice.pass(s, p.status, [&](int i, const float* l) {
-    const unsigned key = max(max(smp_key(l[0]), smp_key(l[1])), max(smp_key(l[2]), smp_key(l[3])));
+    const unsigned key = smp_key(smp_max4(l));
     if (key > top_key) top_key = key, at = i;
   });
   if (greedy && at < V) {                         // which of the four
@@ -404,7 +491,10 @@ sample_kernel(const SampleParams p, int ctas) {
     smp_load<L>(slice.row, at, slice.end, 0, l);
     at += smp_key(l[0]) == top_key ? 0 : smp_key(l[1]) == top_key ? 1 : smp_key(l[2]) == top_key ? 2 : 3;
   }
-  if (top_k && !greedy && top_key) atomicAdd(halves + 2 * (top_key >> 21), 1u);
+  if (top_k && !greedy) {
+    __syncthreads();
+    if (top_key) atomicAdd(halves + 2 * (top_key >> 21), 1u);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const unsigned x = __shfl_xor_sync(0xffffffffu, top_key, o);
@@ -433,22 +523,29 @@ sample_kernel(const SampleParams p, int ctas) {
     const u64 x = (u64)(u * (double)total);
     return x < total ? x : total - (total > 0);
   };
-  // Logits for which `wanted` go to the first CTA's list; the number of them, in every CTA.
-  auto gather = [&](auto&& wanted) {
-    u64* const list = smp_peer(s.list, 0);
-    unsigned* const n_list = smp_peer(&s.count, 0);
+  // Logits whose keys are from `least` on and below `past` go to the first CTA's list, by way of one in each CTA; the number of them, in
+  // every CTA.
+  auto gather = [&](unsigned least, unsigned past) {
+    if (tid == 0) s.staged = 0;
+    __syncthreads();
     slice.pass(s, p.status, [&](int i, const float* l) {
+      if (smp_key(smp_max4(l)) < least) return;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const unsigned key = smp_key(l[e]);
-        if (wanted(l[e], key)) {
-          const unsigned x = atomicAdd(n_list, 1u);
-          if (x < SMP_CAP) list[x] = (u64)key << 32 | (0xffffffffu - (unsigned)(i + e));
+        if (key - least < past - least) {
+          const unsigned x = atomicAdd(&s.staged, 1u);
+          if (x < SMP_CAP) s.weight[x] = (u64)key << 32 | (0xffffffffu - (unsigned)(i + e));
         }
       }
     });
+    __syncthreads();
+    if (tid == 0) s.base = atomicAdd(smp_peer(&s.count, 0), s.staged);
+    __syncthreads();
+    u64* const list = smp_peer(s.list, 0);
+    for (unsigned i = tid; i < s.staged && s.base + i < SMP_CAP; i += SMP_THREADS) list[s.base + i] = s.weight[i];
     smp_cluster_sync();
-    const unsigned n = *n_list;
+    const unsigned n = *smp_peer(&s.count, 0);
     smp_cluster_sync();                           // (the first CTA may leave)
     return n;
   };
@@ -469,7 +566,7 @@ sample_kernel(const SampleParams p, int ctas) {
       if (s.found[2] >= (u64)top_k) least_key = max(least_key, (unsigned)s.found[0] << 21);
       else few = min_p > 0.0 || V <= SMP_CAP;
     }
-    const unsigned n_list = few ? gather([&](float, unsigned key) { return key >= least_key; }) : SMP_CAP + 1;
+    const unsigned n_list = few ? gather(least_key, 0xffffffffu) : SMP_CAP + 1;
     if (n_list <= SMP_CAP) {
       if (rank > 0) return;
       // ---- one CTA sorts them and finishes
@@ -554,8 +651,10 @@ sample_kernel(const SampleParams p, int ctas) {
     slice.pass(s, p.status, [&](int i, const float* l) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (smp_key(l[e]) > border && weight.passes(l[e]))
-          if (const u64 w = weight(l[e])) add_weight(weight.bin(l[e]), w);
+        if ((border == 0 || smp_key(l[e]) > border) && weight.passes(l[e])) {
+          int j;
+          if (const u64 w = weight(l[e], j)) add_weight(weight.bin(j), w);
+        }
     });
     u64 want = 0;
     smp_find(s, rank, ctas, [&](u64 all) {
@@ -568,12 +667,16 @@ sample_kernel(const SampleParams p, int ctas) {
     } else {
       const int bin = (int)s.found[0];
       const u64 above = s.found[1];
-      const unsigned n_list = gather([&](float l, unsigned key) { return key > border && weight.bin(l) == bin && weight.passes(l); });
+      const unsigned past = bin + 1 < SMP_BINS ? weight.first_key(bin + 1) : 0xffffffffu;
+      const unsigned n_list = gather(max(weight.first_key(bin), border + 1), past);
       if (n_list <= SMP_CAP) {
         if (rank == 0) {
           const int n = (int)n_list;
           smp_sort(s.list, n);
-          for (int i = tid; i < n; i += SMP_THREADS) s.weight[i] = weight(smp_logit((unsigned)(s.list[i] >> 32)));
+          for (int i = tid; i < n; i += SMP_THREADS) {
+            const float l = smp_logit((unsigned)(s.list[i] >> 32));
+            s.weight[i] = weight.passes(l) ? weight(l) : 0;
+          }
           __syncthreads();
           smp_scan(s, n);
           for (int i = tid; i < n; i += SMP_THREADS)
@@ -605,29 +708,40 @@ sample_kernel(const SampleParams p, int ctas) {
     if (slice.kept && i + 4 <= min(to, slice.copied)) smp_load<L>(reinterpret_cast<const L*>(s.ring), i - slice.begin, to - slice.begin, 1, l);
     else if (i < to) smp_load<L>(slice.row, i, to, slice.vec && (from & 3) == 0, l);
   };
-  auto add = [&](int i, const float* l, u64& sum, unsigned& equal) {
+  auto add = [&](const float* l, u64& sum, unsigned& equal) {      // (-inf, behind the end, weighs nothing)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (i + e < to) {
+    for (int e = 0; e < 4; ++e) {
+      if (border) {
         const unsigned key = smp_key(l[e]);
-        if (key > border) {
-          if (weight.passes(l[e])) sum += weight(l[e]);
-        } else if (key == border) {
-          ++equal;
-        }
+        equal += key == border;
+        if (key <= border) continue;
       }
+      if (weight.passes(l[e])) sum += weight(l[e]);
+    }
   };
+  // A warp's part goes by blocks of 512, whose sums are kept (two for a lane, V / 16 / 512 of them at most).
+  constexpr int BLOCK = 512, MOST = (1 << 18) / SMP_WARPS / BLOCK + 1;
+  static_assert(MOST <= 64 && MOST * SMP_WARPS <= SMP_CAP, "");
+  u64 *const sums = s.weight + warp * MOST, *const ties = s.list + warp * MOST;
   u64 sum = 0;
-  unsigned equal = 0;
-  for (int i = from + lane * 4; i < to; i += 4 * 128) {
+  u64 equal = 0;
+  __syncthreads();                                // (the first CTA's lists have been read)
+  for (int i = from + lane * 4, k = 0; i - lane * 4 < to; i += BLOCK, ++k) {
     float l[4][4];
+    u64 mine = 0;
+    unsigned same = 0;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) load(i + x * 128, l[x]);
+    for (int x = 0; x < 4; ++x)
+      if (i + x * 128 < to) load(i + x * 128, l[x]);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) add(i + x * 128, l[x], sum, equal);
+    for (int x = 0; x < 4; ++x)
+      if (i + x * 128 < to) add(l[x], mine, same);
+    mine = smp_warp_sum(mine);
+    if (border) same = __reduce_add_sync(0xffffffffu, same);
+    sum += mine;
+    equal += same;
+    if (lane == 0) sums[k] = mine, ties[k] = same;
   }
-  sum = smp_warp_sum(sum);
-  equal = __reduce_add_sync(0xffffffffu, equal);
   __syncthreads();
   if (lane == 0) s.warp[warp] = sum, s.warp2[warp] = equal;
   __syncthreads();
@@ -646,30 +760,32 @@ sample_kernel(const SampleParams p, int ctas) {
   for (int c = 0; c < rank; ++c) x += s.tot[c], y += s.tot2[c];
   for (int w = 0; w < warp; ++w) x += s.warp[w], y += s.warp2[w];
   if (upto(x, y) > target || upto(x + sum, y + equal) <= target) return;
-  for (int i0 = from; i0 < to; i0 += 128) {
+  int i0 = from;
+  for (int k = 0; i0 + BLOCK < to && upto(x + sums[k], y + ties[k]) <= target; ++k, i0 += BLOCK) x += sums[k], y += ties[k];
+  for (; i0 < to; i0 += 128) {
     const int i = i0 + lane * 4;
-    float l[4];
+    float l[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
     load(i, l);
     u64 mine = 0;
-    unsigned ties = 0;
-    add(i, l, mine, ties);
+    unsigned same = 0;
+    add(l, mine, same);
     const u64 all = smp_warp_sum(mine);
-    const unsigned all_ties = __reduce_add_sync(0xffffffffu, ties);
-    if (upto(x + all, y + all_ties) > target) {
-      u64 before = mine, before_ties = ties;
+    const unsigned all_same = __reduce_add_sync(0xffffffffu, same);
+    if (upto(x + all, y + all_same) > target) {
+      u64 before = mine, before_same = same;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const u64 a = __shfl_up_sync(0xffffffffu, before, o), c = __shfl_up_sync(0xffffffffu, before_ties, o);
-        if (lane >= o) before += a, before_ties += c;
+        const u64 a = __shfl_up_sync(0xffffffffu, before, o), c = __shfl_up_sync(0xffffffffu, before_same, o);
+        if (lane >= o) before += a, before_same += c;
       }
-      const unsigned past = __ballot_sync(0xffffffffu, upto(x + before, y + before_ties) > target);
+      const unsigned past = __ballot_sync(0xffffffffu, upto(x + before, y + before_same) > target);
       if (lane == __ffs(past) - 1) {
         x += before - mine;
-        y += before_ties - ties;
+        y += before_same - same;
         for (int e = 0; e < 4 && i + e < to; ++e) {
           const unsigned key = smp_key(l[e]);
-          if (key > border) x += weight.passes(l[e]) ? weight(l[e]) : 0;
-          else if (key == border) ++y;
+          if (border && key <= border) y += key == border;
+          else if (weight.passes(l[e])) x += weight(l[e]);
           if (upto(x, y) > target) {
             p.out[b] = i + e;
             break;
@@ -679,7 +795,7 @@ sample_kernel(const SampleParams p, int ctas) {
       return;
     }
     x += all;
-    y += all_ties;
+    y += all_same;
   }
 }
 
@@ -709,7 +825,7 @@ extern "C" int tpb_sample_tokens(const void* logits, int bf16, long long stride,
   if (B > (0x7fffffff >> 4)) return -2;
   // As many CTAs to a row as keep the machine busy, with 2048 logits or more each.
   int ctas = 1;
-  while (ctas < 16 && (long long)B * ctas * 2 <= 4LL * sm_count() && V / (ctas * 2) >= 2048) ctas *= 2;
+  while (ctas < 16 && (long long)B * ctas * 2 <= SMP_FILL * sm_count() && V / (ctas * 2) >= SMP_LEAST) ctas *= 2;
   const int elt = bf16 ? 2 : 4;
   SampleParams p = {logits, stride, u, temperature, top_p, min_p, top_k, temperature0, top_p0, min_p0, top_k0, V,
                     ((V + ctas - 1) / ctas + 7) / 8 * 8, out, 0, status_block()};
