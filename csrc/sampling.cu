@@ -20,6 +20,8 @@
 //     sorts it.  Then two more passes draw the token: sums of slices and of the parts of their warps, and along one of those.
 //   * Where a list is too long for one CTA (thousands of equal logits, large k) the border is found bit by bit of the order.
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "tpb.h"
 
@@ -27,15 +29,9 @@ namespace tpb {
 
 int sm_count();
 
-constexpr int SMP_THREADS = 512, SMP_WARPS = SMP_THREADS / 32;
+constexpr int SMP_THREADS = 512, SMP_WARPS = SMP_THREADS / 32;      // (1024: one row's nucleus 36 -> 41 us)
 constexpr int SMP_BINS = 2048;          // 11 bits of the order at a time (31-21, 20-10, 9-0); 64 binary orders of weights in steps of 1/32
 constexpr int SMP_CAP = 2048;           // tokens that one CTA sorts
-#ifndef SMP_FILL
-#define SMP_FILL 4LL
-#endif
-#ifndef SMP_LEAST
-#define SMP_LEAST 2048
-#endif
 constexpr int SMP_FIXED = 44;           // a weight of 1 is 2^44: 2^18 of them stay below 2^63
 constexpr int SMP_TABLE = 1024;         // 2^(j / 1024)
 constexpr int SMP_CHUNK = SMP_THREADS * 8, SMP_RING = 3;       // logits of a bulk copy, copies under way
@@ -100,28 +96,26 @@ __device__ __forceinline__ float smp_logit(unsigned key) { return __uint_as_floa
 
 struct SmpWeight {
   double per_unit;        // log2(e) / T
-  float top, hi, lo;      // the largest logit; 1024 log2(e) / T as a sum of two floats
+  float hi, lo;           // 1024 log2(e) / T as a sum of two floats
+  const u64* table;       // 2^62 2^(j / 1024), shared
+  float top;              // the largest logit
   float p_top, p_cut;     // 1024 log2 of the largest weight, and 2^-45 of it, before that is made 1: the nearest product
   int j_top;              // the whole number it is nearest to (with the other bits of the pattern), and what is missing
   float y_top;
-  bool slow;              // T, or the logits, too far from 1 for that
-  bool some;              // min_p is on
-  double min_p;
-  float sure, sure_not;   // p - p_top of weights that pass min_p, that do not
-  const u64* table;       // 2^62 2^(j / 1024), shared
+  bool slow;              // T, or the logits, too far from 1 for that: 64 bits
 
-  __device__ __forceinline__ SmpWeight(double T, float top_, double min_p_, const u64* table_)
-      : per_unit(1.4426950408889634 / T), top(top_), some(min_p_ > 0.0), min_p(min_p_), table(table_) {
+  __device__ __forceinline__ SmpWeight(double T, const u64* table_) : per_unit(1.4426950408889634 / T), table(table_) {
     const double c = per_unit * SMP_TABLE;
     hi = (float)c;
     lo = (float)(c - (double)hi);
-    slow = !(T > 1e-20 && T < 1e20 && fabsf(top) * hi < 2097152.f);
+    slow = !(T > 1e-20 && T < 1e20);
+  }
+  __device__ __forceinline__ void begin(float top_) {
+    top = top_;
+    slow |= !(fabsf(top) * hi < 2097152.f);
     p_top = __fmul_rn(top, hi);
     p_cut = p_top - 45.f * SMP_TABLE;
     split(top, p_top, 0.f, j_top, y_top);
-    const double border = some ? log2(min_p) * SMP_TABLE : -1e30;
-    sure = (float)(border + 1.0 + 1e-6 * fabs(border));
-    sure_not = (float)(border - 1.0 - 1e-6 * fabs(border));
   }
   // 1024 l log2(e) / T = j + y, j whole (in the low bits of a float's pattern), less y0; p = l * hi
   __device__ __forceinline__ void split(float l, float p, float y0, int& j, float& y) const {
@@ -139,22 +133,19 @@ struct SmpWeight {
   }
   // 1024 log2 of the weight, rounded: does not fall where l grows.
   __device__ __forceinline__ int step(float l) const {
-    return slow ? step_slow(l) : __float_as_int(__fadd_rn(fmaxf(__fmul_rn(l, hi), p_top - 1048576.f), 12582912.f)) - j_top;
+    return slow ? step_slow(l) : __float_as_int(__fadd_rn(fmaxf(__fmul_rn(l, hi), p_cut), 12582912.f)) - j_top;
   }
   // In multiples of 2^-44: 2^44 for the largest, else with the last bit set, as often above as below what is cut off; 0 below 2^-45 and
   // for NaN.  j: step(l).
-  __device__ __forceinline__ u64 operator()(float l, int& j) const {
-    if (slow) {
+  template <bool SLOW>
+  __device__ __forceinline__ u64 of(float l, int& j) const {
+    if (SLOW) {
       j = step_slow(l);
       return __double2ull_rn(real(l) * (double)(1LL << SMP_FIXED));
     }
     const float p = __fmul_rn(l, hi);
-    if (!(p > p_cut)) {
-      j = -0x100000;
-      return 0;
-    }
     float y;
-    split(l, p, y_top, j, y);
+    split(l, fmaxf(p, p_cut), y_top, j, y);
     j -= j_top;
     y *= 0.69314718056f / SMP_TABLE;
     const float q = fmaf(fmaf(y, 1.f / 6, 0.5f) * y, y, y);     // 2^rest - 1, |q| < 2^-10; the next term is below 2^-46
@@ -162,39 +153,35 @@ struct SmpWeight {
     const u64 t = table[j & (SMP_TABLE - 1)];
     const u64 w = t + (u64)((long long)(int)(t >> 32) * qi);
     const u64 x = w >> (62 - SMP_FIXED - (j >> 10));
-    return x | (~x >> SMP_FIXED & 1);
+    return p > p_cut ? x | (~x >> SMP_FIXED & 1) : 0;
   }
   __device__ __forceinline__ u64 operator()(float l) const {
     int j;
-    return (*this)(l, j);
+    return slow ? of<true>(l, j) : of<false>(l, j);
   }
-  // w >= min_p
-  __device__ __forceinline__ bool passes(float l) const {
-    if (!some) return true;
-    if (!slow) {
-      const float x = l * hi - p_top;
-      if (x > sure) return true;
-      if (!(x > sure_not)) return false;
-    }
-    return real(l) >= min_p;
+  // f(std::true_type) where weights are slow, else f(std::false_type)
+  template <typename F>
+  __device__ __forceinline__ void either(F&& f) const {
+    if (slow) f(std::true_type());
+    else f(std::false_type());
   }
   // Steps of 1/32 below the largest weight's exponent, the largest weights in the last bin.
   static __device__ __forceinline__ int bin(int j) { return SMP_BINS - 1 + max(j >> 5, 1 - SMP_BINS); }
-  // The smallest key whose bin is `of` or more; the whole warp calls.
-  __device__ __forceinline__ unsigned first_key(int of) const {
-    unsigned low = 0x007fffffu, high = 0xff800001u;             // -inf (bin 0); behind inf
-    while (high - low > 1) {
-      const unsigned wide = (high - low + 32) / 33, at = low + wide * ((threadIdx.x & 31) + 1);
-      const bool past = at >= high || bin(step(smp_logit(at))) >= of;
-      const unsigned which = __ballot_sync(0xffffffffu, past);
-      const int n = which ? __ffs(which) - 1 : 32;              // lanes in front of the border
-      const unsigned l = low + wide * n, h = low + wide * (n + 1);
-      low = l;
-      high = min(high, h);
-    }
-    return high;
-  }
 };
+
+// The smallest key in (low, high] for which `past` holds, as it does for `high` and for all behind; the whole warp calls.
+template <typename F>
+__device__ __forceinline__ unsigned smp_first_key(unsigned low, unsigned high, F&& past) {
+  while (high - low > 1) {
+    const unsigned wide = (high - low + 32) / 33, at = low + wide * ((threadIdx.x & 31) + 1);
+    const unsigned which = __ballot_sync(0xffffffffu, at >= high || past(at));
+    const int n = which ? __ffs(which) - 1 : 32;                // lanes in front of the border
+    high = min(high, low + wide * (n + 1));
+    low += wide * n;
+  }
+  return high;
+}
+constexpr unsigned SMP_LOWEST = 0x007fffffu, SMP_HIGHEST = 0xff800000u;      // keys of -inf and inf
 
 struct SmpShared {
   float ring[SMP_RING * SMP_CHUNK];     // bf16 logits take half of it
@@ -205,9 +192,8 @@ struct SmpShared {
   u64 tot[16], tot2[16];                // of the cluster's CTAs
   uint64_t full[SMP_RING];              // barriers of the copies
   u64 found[3];                         // bin, sum of the bins above, sum of all
-  unsigned count;                       // of the list
   unsigned border, of_border;
-  unsigned staged, base;                // of this CTA's part of the list
+  unsigned staged;                      // of this CTA's part of the list
   int dead;                             // a copy has not come
 };
 
@@ -254,55 +240,46 @@ __device__ __forceinline__ void smp_cluster_sync() {
 }
 
 // Every CTA's s.sums, added up, from the last bin down: the bin in which the sum reaches target(sum of all), in s.found; the
-// sum of all alone where that is more.
+// sum of all alone where that is more.  (s.list and s.weight are used.)
 template <typename F>
 __device__ __forceinline__ void smp_find(SmpShared& s, int rank, int ctas, F&& target) {
-  const int per = SMP_BINS / ctas, b0 = rank * per;
-  smp_cluster_sync();
-  // the CTAs' counts of a bin, added up by several threads
-  const int groups = min(SMP_THREADS / min(per, SMP_THREADS), ctas), group = (int)threadIdx.x / per;
-  if (groups > 1) {
-    if (group < groups) {
-      u64 x = 0;
+  const int per = SMP_BINS / ctas, b0 = rank * per, tid = threadIdx.x;
+  const u64* total = s.sums;
+  if (ctas > 1) {                       // each CTA adds up its share of the bins, for all
+    smp_cluster_sync();
+    const int groups = max(1, min(SMP_THREADS / per, ctas));
+    for (int x = tid; x < per * groups; x += SMP_THREADS) {
+      u64 sum = 0;
 #pragma unroll 4
-      for (int c = group; c < ctas; c += groups) x += smp_peer(s.sums, c)[b0 + threadIdx.x % per];
-      s.weight[threadIdx.x] = x;
+      for (int c = x / per; c < ctas; c += groups) sum += smp_peer(s.sums, c)[b0 + x % per];
+      s.weight[x] = sum;
     }
     __syncthreads();
-  }
-  // four neighbouring bins to a thread, the topmost to thread 0
-  u64 v[4] = {}, mine = 0;
-  const int high = b0 + per - 1 - (int)threadIdx.x * 4;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (high - i >= b0) {
-      if (groups > 1)
-        for (int k = 0; k < groups; ++k) v[i] += s.weight[k * per + high - i - b0];
-      else
-        for (int c = 0; c < ctas; ++c) v[i] += smp_peer(s.sums, c)[high - i];
-      mine += v[i];
+    for (int x = tid; x < per * ctas; x += SMP_THREADS) {
+      u64 sum = 0;
+      for (int g = 0; g < groups; ++g) sum += s.weight[g * per + x % per];
+      smp_peer(s.list, x / per)[b0 + x % per] = sum;
     }
-  const u64 sum = smp_block_sum(mine, s.warp), before = smp_block_before(mine, s.warp);
-  if ((int)threadIdx.x < ctas) smp_peer(s.tot, threadIdx.x)[rank] = sum;
-  smp_cluster_sync();
-  u64 above = before, all = 0;
-  for (int c = 0; c < ctas; ++c) {
-    all += s.tot[c];
-    if (c > rank) above += s.tot[c];
+    smp_cluster_sync();
+    total = s.list;
+  } else {
+    __syncthreads();
   }
+  constexpr int N = SMP_BINS / SMP_THREADS;     // neighbouring bins to a thread, the topmost to thread 0
+  u64 v[N], mine = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) mine += v[i] = total[SMP_BINS - 1 - (tid * N + i)];
+  u64 above = smp_block_before(mine, s.warp), all = 0;
+#pragma unroll
+  for (int w = 0; w < SMP_WARPS; ++w) all += s.warp[w];
   const u64 t = target(all);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (high - i >= b0 && above < t && above + v[i] >= t)
-      for (int c = 0; c < ctas; ++c) {
-        u64* f = smp_peer(s.found, c);
-        f[0] = high - i;
-        f[1] = above;
-      }
+  for (int i = 0; i < N; ++i) {
+    if (above < t && above + v[i] >= t) s.found[0] = SMP_BINS - 1 - (tid * N + i), s.found[1] = above;
     above += v[i];
   }
-  if (threadIdx.x == 0) s.found[2] = all;
-  smp_cluster_sync();
+  if (tid == 0) s.found[2] = all;
+  __syncthreads();
 }
 
 // s.list[0 .. n) in descending order; n is padded with zeros to a power of two.
@@ -326,17 +303,17 @@ __device__ __forceinline__ void smp_sort(u64* list, int n) {
 }
 // s.weight[0 .. n) becomes the sums up to and with each.
 __device__ __forceinline__ void smp_scan(SmpShared& s, int n) {
-  u64 v[4], mine = 0;
+  constexpr int N = SMP_CAP / SMP_THREADS;
+  u64 v[N], mine = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int x = threadIdx.x * 4 + i;
-    v[i] = x < n ? s.weight[x] : 0;
-    mine += v[i];
+  for (int i = 0; i < N; ++i) {
+    const int x = threadIdx.x * N + i;
+    mine += v[i] = x < n ? s.weight[x] : 0;
   }
   u64 sum = smp_block_before(mine, s.warp);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int x = threadIdx.x * 4 + i;
+  for (int i = 0; i < N; ++i) {
+    const int x = threadIdx.x * N + i;
     sum += v[i];
     if (x < n) s.weight[x] = sum;
   }
@@ -448,13 +425,13 @@ struct SmpSlice {
 };
 
 template <typename L>
-__global__ void __launch_bounds__(SMP_THREADS, 2)
+__global__ void __launch_bounds__(SMP_THREADS, 1024 / SMP_THREADS)
 sample_kernel(const SampleParams p, int ctas) {
   extern __shared__ __align__(128) uint8_t smp_smem[];
   SmpShared& s = *reinterpret_cast<SmpShared*>(smp_smem);
   const int rank = ctas > 1 ? (int)cluster_ctarank() : 0, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid < SMP_RING) mbar_init(&s.full[tid], 1);
-  if (tid == 0) s.count = 0, s.dead = 0;
+  if (tid == 0) s.dead = 0;
   fence_barrier_init();
   __syncthreads();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // (nobody writes to a CTA that has not begun)
@@ -473,6 +450,7 @@ sample_kernel(const SampleParams p, int ctas) {
   min_p = min_p > 0.0 ? fmin(min_p, 1.0) : 0.0;
   const double u = fmin(fmax((double)p.u[b], 0.0), 1.0);
   unsigned* const halves = reinterpret_cast<unsigned*>(s.sums);   // low and high words of the sums
+  SmpWeight weight(greedy ? 1.0 : T, s.table);
 
   if (!greedy)
     for (int i = tid; i < SMP_TABLE; i += SMP_THREADS) s.table[i] = smp_table.at[i];
@@ -518,7 +496,7 @@ sample_kernel(const SampleParams p, int ctas) {
     if (rank == 0 && tid == 0) p.out[b] = top == -INFINITY || s.dead ? -1 : at;
     if (greedy || top == -INFINITY) return;       // (the cluster agrees on these)
   }
-  const SmpWeight weight(T, top, min_p, s.table);
+  weight.begin(top);
   auto place = [&](u64 total) {                   // the sum that the drawn token's passes
     const u64 x = (u64)(u * (double)total);
     return x < total ? x : total - (total > 0);
@@ -540,47 +518,50 @@ sample_kernel(const SampleParams p, int ctas) {
       }
     });
     __syncthreads();
-    if (tid == 0) s.base = atomicAdd(smp_peer(&s.count, 0), s.staged);
-    __syncthreads();
-    u64* const list = smp_peer(s.list, 0);
-    for (unsigned i = tid; i < s.staged && s.base + i < SMP_CAP; i += SMP_THREADS) list[s.base + i] = s.weight[i];
+    if (tid < ctas) smp_peer(s.tot, tid)[rank] = s.staged;
     smp_cluster_sync();
-    const unsigned n = *smp_peer(&s.count, 0);
-    smp_cluster_sync();                           // (the first CTA may leave)
+    u64 n = 0, base = 0;
+    for (int c = 0; c < ctas; ++c) {
+      if (c == rank) base = n;
+      n += s.tot[c];
+    }
+    u64* const list = smp_peer(s.list, 0);
+    if (n <= SMP_CAP)
+      for (unsigned i = tid; i < s.staged; i += SMP_THREADS) list[base + i] = s.weight[i];
+    smp_cluster_sync();
     return n;
   };
 
-  unsigned border = 0;                            // smallest key kept, and how many of it
+  unsigned least_key = 0;                         // smallest key that min_p leaves
+  if (min_p > 0.0) {
+    const float guess = __double2float_rd((double)top + log(min_p) * T);
+    const unsigned at_guess = min(max(smp_key(guess), SMP_LOWEST + 20), (unsigned)(best >> 32));
+    auto passes = [&](unsigned key) { return weight.real(smp_logit(key)) >= min_p; };
+    unsigned low = at_guess - 16, high = min(at_guess + 16, (unsigned)(best >> 32));
+    if (!passes(high)) high = (unsigned)(best >> 32);
+    if (passes(low)) low = SMP_LOWEST - 1;
+    least_key = smp_first_key(low, high, passes);
+  }
+  unsigned border = 0;                            // smallest key kept, and how many of it (those above it all)
   u64 of_border = 0;
   if (top_k || min_p > 0.0) {
-    unsigned least_key = 0;
+    unsigned from = least_key;
     bool few = true;
-    if (min_p > 0.0) {
-      float least = __double2float_rd((double)top + log(min_p) * T * (1.0 + 1e-12));
-      if (!(least == least)) least = -INFINITY;               // (T is infinite)
-      if (fabsf(least) < 1.2e-38f) least = -1.2e-38f;         // (subnormal)
-      least_key = smp_key(least);
-    }
     if (top_k) {
       smp_find(s, rank, ctas, [&](u64 all) { return min((u64)top_k, all + 1); });
-      if (s.found[2] >= (u64)top_k) least_key = max(least_key, (unsigned)s.found[0] << 21);
+      if (s.found[2] >= (u64)top_k) from = max(from, (unsigned)s.found[0] << 21);
       else few = min_p > 0.0 || V <= SMP_CAP;
     }
-    const unsigned n_list = few ? gather(least_key, 0xffffffffu) : SMP_CAP + 1;
+    const u64 n_list = few ? gather(from, 0xffffffffu) : SMP_CAP + 1;
     if (n_list <= SMP_CAP) {
       if (rank > 0) return;
       // ---- one CTA sorts them and finishes
       const int n = (int)n_list;
       smp_sort(s.list, n);
-      int kept = top_k ? min(n, top_k) : n;
-      u64 below = 0;                              // (this thread's)
-      for (int i = tid; i < n; i += SMP_THREADS) {
-        const float l = smp_logit((unsigned)(s.list[i] >> 32));
-        s.weight[i] = weight(l);
-        below += i < kept && !weight.passes(l);
-      }
-      kept = max(kept - (int)smp_block_sum(below, s.warp), 1);
-      smp_scan(s, n);
+      int kept = max(top_k ? min(n, top_k) : n, 1);
+      for (int i = tid; i < kept; i += SMP_THREADS) s.weight[i] = weight(smp_logit((unsigned)(s.list[i] >> 32)));
+      __syncthreads();
+      smp_scan(s, kept);
       if (nucleus) {
         const u64 want = __double2ull_ru(top_p * (double)s.weight[kept - 1]);
         u64 in = 0;
@@ -606,7 +587,6 @@ sample_kernel(const SampleParams p, int ctas) {
   auto clear = [&]() {
     __syncthreads();
     for (int i = tid; i < SMP_BINS; i += SMP_THREADS) s.sums[i] = 0;
-    if (tid == 0 && rank == 0) s.count = 0;
     __syncthreads();
   };
   auto add_weight = [&](int bin, u64 w) {         // the carry from the low to the high word is this thread's to see
@@ -627,7 +607,7 @@ sample_kernel(const SampleParams p, int ctas) {
           if (shift < 21 && key >> (shift + bits) != key_so_far >> (shift + bits)) continue;
           const unsigned bin = key >> shift & ((1u << bits) - 1);
           if (!weights) atomicAdd(halves + 2 * bin, 1u);
-          else if (key > border && weight.passes(l[e])) add_weight(bin, weight(l[e]));
+          else if (key > border) add_weight(bin, weight(l[e]));
         }
       });
       smp_find(s, rank, ctas, [&](u64 all) { return min(target - above, all); });
@@ -636,25 +616,28 @@ sample_kernel(const SampleParams p, int ctas) {
       if (shift == 0) return key_so_far;
     }
   };
-  auto weight_of_border = [&]() {
-    const float l = smp_logit(border);
-    return border && weight.passes(l) ? weight(l) : 0;
-  };
   if (top_k) {
     u64 above;
     border = bit_by_bit(false, top_k, above);
     of_border = top_k - above;
   }
+  if (least_key > border) {                       // (the border's own do not pass min_p)
+    border = least_key - 1;
+    of_border = 0;
+  }
   if (nucleus) {
-    const u64 each = weight_of_border();
+    const u64 each = of_border ? weight(smp_logit(border)) : 0;
     clear();
-    slice.pass(s, p.status, [&](int i, const float* l) {
+    weight.either([&](auto slow) {
+      slice.pass(s, p.status, [&](int i, const float* l) {
+        u64 w[4];
+        int j[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if ((border == 0 || smp_key(l[e]) > border) && weight.passes(l[e])) {
-          int j;
-          if (const u64 w = weight(l[e], j)) add_weight(weight.bin(j), w);
-        }
+        for (int e = 0; e < 4; ++e) w[e] = weight.of<decltype(slow)::value>(l[e], j[e]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (w[e] && (border == 0 || smp_key(l[e]) > border)) add_weight(weight.bin(j[e]), w[e]);
+      });
     });
     u64 want = 0;
     smp_find(s, rank, ctas, [&](u64 all) {
@@ -667,16 +650,15 @@ sample_kernel(const SampleParams p, int ctas) {
     } else {
       const int bin = (int)s.found[0];
       const u64 above = s.found[1];
-      const unsigned past = bin + 1 < SMP_BINS ? weight.first_key(bin + 1) : 0xffffffffu;
-      const unsigned n_list = gather(max(weight.first_key(bin), border + 1), past);
+      auto first_of = [&](int of) {
+        return smp_first_key(SMP_LOWEST, SMP_HIGHEST, [&](unsigned key) { return weight.bin(weight.step(smp_logit(key))) >= of; });
+      };
+      const u64 n_list = gather(max(first_of(bin), border + 1), bin + 1 < SMP_BINS ? first_of(bin + 1) : 0xffffffffu);
       if (n_list <= SMP_CAP) {
         if (rank == 0) {
           const int n = (int)n_list;
           smp_sort(s.list, n);
-          for (int i = tid; i < n; i += SMP_THREADS) {
-            const float l = smp_logit((unsigned)(s.list[i] >> 32));
-            s.weight[i] = weight.passes(l) ? weight(l) : 0;
-          }
+          for (int i = tid; i < n; i += SMP_THREADS) s.weight[i] = weight(smp_logit((unsigned)(s.list[i] >> 32)));
           __syncthreads();
           smp_scan(s, n);
           for (int i = tid; i < n; i += SMP_THREADS)
@@ -701,22 +683,21 @@ sample_kernel(const SampleParams p, int ctas) {
   }
 
   // ---- the token: sums of the slices, of the warps' parts of the one it lies in, then along that part
-  const u64 each = weight_of_border();
+  const u64 each = of_border ? weight(smp_logit(border)) : 0;
   const int part = ((slice.end - slice.begin + SMP_WARPS - 1) / SMP_WARPS + 127) / 128 * 128;
   const int from = min(slice.end, slice.begin + warp * part), to = min(slice.end, from + part);
   auto load = [&](int i, float* l) {              // four logits of a lane
     if (slice.kept && i + 4 <= min(to, slice.copied)) smp_load<L>(reinterpret_cast<const L*>(s.ring), i - slice.begin, to - slice.begin, 1, l);
     else if (i < to) smp_load<L>(slice.row, i, to, slice.vec && (from & 3) == 0, l);
   };
-  auto add = [&](const float* l, u64& sum, unsigned& equal) {      // (-inf, behind the end, weighs nothing)
+  auto add = [&](auto slow, const float* l, u64& sum, unsigned& equal) {      // (-inf, behind the end, weighs nothing)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (border) {
-        const unsigned key = smp_key(l[e]);
-        equal += key == border;
-        if (key <= border) continue;
-      }
-      if (weight.passes(l[e])) sum += weight(l[e]);
+      int j;
+      const u64 w = weight.of<decltype(slow)::value>(l[e], j);
+      const unsigned key = border ? smp_key(l[e]) : 1;
+      sum += key > border ? w : 0;
+      equal += key == border;
     }
   };
   // A warp's part goes by blocks of 512, whose sums are kept (two for a lane, V / 16 / 512 of them at most).
@@ -726,22 +707,25 @@ sample_kernel(const SampleParams p, int ctas) {
   u64 sum = 0;
   u64 equal = 0;
   __syncthreads();                                // (the first CTA's lists have been read)
-  for (int i = from + lane * 4, k = 0; i - lane * 4 < to; i += BLOCK, ++k) {
-    float l[4][4];
-    u64 mine = 0;
-    unsigned same = 0;
+  weight.either([&](auto slow) {
+    for (int i = from + lane * 4, k = 0; i - lane * 4 < to; i += BLOCK, ++k) {
+      float l[4][4];
+      u64 mine = 0;
+      unsigned same = 0;
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-      if (i + x * 128 < to) load(i + x * 128, l[x]);
+      for (int x = 0; x < 4; ++x) {
+        l[x][0] = l[x][1] = l[x][2] = l[x][3] = -INFINITY;
+        load(i + x * 128, l[x]);
+      }
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-      if (i + x * 128 < to) add(l[x], mine, same);
-    mine = smp_warp_sum(mine);
-    if (border) same = __reduce_add_sync(0xffffffffu, same);
-    sum += mine;
-    equal += same;
-    if (lane == 0) sums[k] = mine, ties[k] = same;
-  }
+      for (int x = 0; x < 4; ++x) add(slow, l[x], mine, same);
+      mine = smp_warp_sum(mine);
+      if (border) same = __reduce_add_sync(0xffffffffu, same);
+      sum += mine;
+      equal += same;
+      if (lane == 0) sums[k] = mine, ties[k] = same;
+    }
+  });
   __syncthreads();
   if (lane == 0) s.warp[warp] = sum, s.warp2[warp] = equal;
   __syncthreads();
@@ -768,7 +752,7 @@ sample_kernel(const SampleParams p, int ctas) {
     load(i, l);
     u64 mine = 0;
     unsigned same = 0;
-    add(l, mine, same);
+    weight.either([&](auto slow) { add(slow, l, mine, same); });
     const u64 all = smp_warp_sum(mine);
     const unsigned all_same = __reduce_add_sync(0xffffffffu, same);
     if (upto(x + all, y + all_same) > target) {
@@ -785,7 +769,7 @@ sample_kernel(const SampleParams p, int ctas) {
         for (int e = 0; e < 4 && i + e < to; ++e) {
           const unsigned key = smp_key(l[e]);
           if (border && key <= border) y += key == border;
-          else if (weight.passes(l[e])) x += weight(l[e]);
+          else x += weight(l[e]);
           if (upto(x, y) > target) {
             p.out[b] = i + e;
             break;
@@ -823,9 +807,12 @@ extern "C" int tpb_sample_tokens(const void* logits, int bf16, long long stride,
   if (B < 0 || V < 1 || V > (1 << 18)) return -2;
   if (B == 0) return 0;
   if (B > (0x7fffffff >> 4)) return -2;
-  // As many CTAs to a row as keep the machine busy, with 2048 logits or more each.
+  // CTAs to a row: as many as the SMs hold at once (two each), with 2048 logits or more to a CTA.  Rows with settings of their own take
+  // unequal times, a nucleus of a flat distribution ten times a greedy row's, and get twice as many.  us, once / twice as many: 64 rows
+  // of 128256, nucleus 91 / 118, 50 largest 34 / 58; 256 rows of 102400, nucleus 193 / 226, 50 largest 51 / 78, mixed 174 / 138.
+  const long long room = (temperature || top_k || top_p || min_p ? 4LL : 2LL) * sm_count();
   int ctas = 1;
-  while (ctas < 16 && (long long)B * ctas * 2 <= SMP_FILL * sm_count() && V / (ctas * 2) >= SMP_LEAST) ctas *= 2;
+  while (ctas < 16 && (long long)B * ctas * 2 <= room && V / (ctas * 2) >= 2048) ctas *= 2;
   const int elt = bf16 ? 2 : 4;
   SampleParams p = {logits, stride, u, temperature, top_p, min_p, top_k, temperature0, top_p0, min_p0, top_k0, V,
                     ((V + ctas - 1) / ctas + 7) / 8 * 8, out, 0, status_block()};
