@@ -52,48 +52,59 @@ paged_rows_kernel(PagedRows k, PagedRows v, const long long* __restrict__ slots,
   const PagedRows p = blockIdx.y ? v : k;
   const int per_warp = 32 / LANES, lane = threadIdx.x & 31, in_row = lane % LANES;
   const unsigned warp = (blockIdx.x * PAGED_THREADS + threadIdx.x) >> 5;
-  const unsigned first = warp * (per_warp * PAGED_ROWS) + lane / LANES;      // (rows < 2^31)
+  // A lane finds a row's places for the lanes that move it.  (Every lane for its own rows: 50 us instead of 41 for 30011 tokens of 8
+  // heads to e4m3, bound by those instructions.)
+  const unsigned r = warp * (per_warp * PAGED_ROWS) + lane, t = r / H, h = r - t * H;      // (rows < 2^31)
+  const bool live = lane < per_warp * PAGED_ROWS && r < rows;
+  __nv_bfloat16* const my_x = live ? p.x + (long long)t * p.x_token + (long long)h * p.x_head : nullptr;
+  const long long my_slot = live ? slots[t] : -1;
+  auto of_row = [&](auto* mine, int i) {
+    return reinterpret_cast<decltype(mine)>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), i * per_warp + lane / LANES));
+  };
   uint4 d[PAGED_ROWS][V];
-  long long slot[PAGED_ROWS];
-  uint8_t* at[PAGED_ROWS];
-  uint8_t* sc[PAGED_ROWS];
   __nv_bfloat16* x[PAGED_ROWS];
 #pragma unroll
   for (int i = 0; i < PAGED_ROWS; ++i) {
-    const unsigned r = first + i * per_warp;
-    slot[i] = -1;
-    at[i] = sc[i] = nullptr;
-    x[i] = nullptr;
-    if (r < rows) {
-      const unsigned t = r / H, h = r - t * H;
-      slot[i] = slots[t];
-      x[i] = p.x + (long long)t * p.x_token + (long long)h * p.x_head;
-      if (slot[i] < 0 || slot[i] >= n_slots) {
-        if (slot[i] != -1 && in_row == 0) report(st, kBadArgument, 70);
-        slot[i] = -1;
-      } else {
-        const unsigned s = (unsigned)slot[i], pg = s / page, off = s - pg * page;
-        at[i] = p.pool + pg * p.page_bytes + off * p.row_bytes + h * p.head_bytes;
-        if (HELD8) sc[i] = p.scale + pg * p.s_page + off * p.s_row + h * p.s_head;
+    x[i] = of_row(my_x, i);
+    if (WRITE) {                        // (without waiting for the slot)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int c = in_row + j * LANES;        // 8 values
+        d[i][j] = x[i] != nullptr && c * 8 < p.D ? reinterpret_cast<const uint4*>(x[i])[c] : make_uint4(0, 0, 0, 0);
       }
     }
   }
+  uint8_t *my_at = nullptr, *my_sc = nullptr;
+  if (my_slot >= 0 && my_slot < n_slots) {
+    const unsigned s = (unsigned)my_slot, pg = s / page, off = s - pg * page;
+    my_at = p.pool + pg * p.page_bytes + off * p.row_bytes + h * p.head_bytes;
+    if (HELD8) my_sc = p.scale + pg * p.s_page + off * p.s_row + h * p.s_head;
+  } else if (my_slot != -1) {
+    report(st, kBadArgument, 70);
+  }
+  uint8_t* at[PAGED_ROWS];
+  uint8_t* sc[PAGED_ROWS];
 #pragma unroll
-  for (int i = 0; i < PAGED_ROWS; ++i)
+  for (int i = 0; i < PAGED_ROWS; ++i) {
+    at[i] = of_row(my_at, i);
+    sc[i] = HELD8 ? of_row(my_sc, i) : nullptr;
+    if (!WRITE) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = in_row + j * LANES;      // 8 values
-      d[i][j] = make_uint4(0, 0, 0, 0);
-      if (slot[i] < 0 || c * 8 >= p.D) continue;
-      if (WRITE) d[i][j] = reinterpret_cast<const uint4*>(x[i])[c];
-      else if (!HELD8) d[i][j] = reinterpret_cast<const uint4*>(at[i])[c];
-      else {
-        const uint2 u = reinterpret_cast<const uint2*>(at[i])[c];
-        d[i][j].x = u.x;
-        d[i][j].y = u.y;
-        d[i][j].z = *sc[i];
+      for (int j = 0; j < V; ++j) {
+        const int c = in_row + j * LANES;
+        d[i][j] = make_uint4(0, 0, 0, 0);
+        if (at[i] == nullptr || c * 8 >= p.D) continue;
+        if (!HELD8) {
+          d[i][j] = reinterpret_cast<const uint4*>(at[i])[c];
+        } else {
+          const uint2 u = reinterpret_cast<const uint2*>(at[i])[c];
+          d[i][j].x = u.x;
+          d[i][j].y = u.y;
+          d[i][j].z = *sc[i];
+        }
       }
     }
+  }
 #pragma unroll
   for (int i = 0; i < PAGED_ROWS; ++i) {
     if (WRITE && HELD8) {
@@ -103,7 +114,7 @@ paged_rows_kernel(PagedRows k, PagedRows v, const long long* __restrict__ slots,
       m = max(m & 0xffffu, m >> 16);
 #pragma unroll
       for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      if (slot[i] < 0) continue;
+      if (at[i] == nullptr) continue;
       const int e = row_exponent(m);
       const float f = __int_as_float((127 - e) << 23);
 #pragma unroll
@@ -118,14 +129,14 @@ paged_rows_kernel(PagedRows k, PagedRows v, const long long* __restrict__ slots,
       }
       if (in_row == 0) *sc[i] = (uint8_t)(e + 127);
     } else {
-      if (x[i] == nullptr || (WRITE && slot[i] < 0)) continue;      // (a read of no slot gives zeros)
+      if (x[i] == nullptr || (WRITE && at[i] == nullptr)) continue;      // (a read of no slot gives zeros)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const int c = in_row + j * LANES;
         if (c * 8 >= p.D) continue;
         uint4 o = d[i][j];
         if (!WRITE && HELD8) {
-          const float f = __int_as_float(slot[i] < 0 ? 0 : d[i][j].z << 23);
+          const float f = __int_as_float(d[i][j].z << 23);
           const float2 a = from_e4m3x2(d[i][j].x), b = from_e4m3x2(d[i][j].x >> 16), g = from_e4m3x2(d[i][j].y), h = from_e4m3x2(d[i][j].y >> 16);
           o.x = pack_bf16(a.x * f, a.y * f);
           o.y = pack_bf16(b.x * f, b.y * f);
