@@ -146,3 +146,74 @@ def test_debug_mode_names_lengths_beyond_the_table(monkeypatch):
   c = PagedKV.allocate(4, 16, 2, 8)
   with pytest.raises(IndexError, match="lengths"):
     paged_kv.decode_attention(torch.randn(1, 4, 8).bfloat16(), c, torch.zeros(1, 2, dtype=torch.int32), torch.tensor([33], dtype=torch.int32))
+
+
+# ----------------------------------------------------------------------------- in the inference engine
+def _tiny():
+  from torchprime_b200.config import compose
+  from torchprime_b200.models.model_utils import initialize_model_class
+  cfg = compose("default", ["model=deepseek-tiny"]).model
+  torch.manual_seed(0)
+  return cfg, initialize_model_class(cfg).eval()
+
+
+def test_paged_engine_matches_the_training_model():
+  from torchprime_b200.experimental.deepseek_inference.engine import DeepseekInferenceEngine, full_forward_last_logits
+  cfg, model = _tiny()
+  eng = DeepseekInferenceEngine(model, max_batch_size=2, max_seq_len=32, attn_impl="paged", page_size=4)
+  ids = torch.randint(0, cfg.vocab_size, (2, 12))
+  full = lambda n: full_forward_last_logits(model, ids[:, :n])  # noqa: E731
+  assert torch.allclose(eng.forward(ids, 0), full(12), atol=2e-4)
+  assert torch.allclose(eng.forward(ids[:, :5], 0), full(5), atol=2e-4)          # anew
+  assert torch.allclose(eng.forward(ids[:, 5:8], 5), full(8), atol=2e-4)         # the next part of the prompts
+  for t in range(8, 12):
+    assert torch.allclose(eng.forward(ids[:, t:t + 1], t), full(t + 1), atol=2e-4)
+  eng.forward(ids[:1, :3], 0, rows=[1])                                           # sequences at positions of their own
+  got = eng.forward(torch.stack([ids[0, 3:4], ids[0, :1]]), [3, 12], rows=[1, 0])
+  assert torch.allclose(got[0], full_forward_last_logits(model, ids[:1, :4])[0], atol=2e-4)
+
+
+def test_paged_engine_takes_and_gives_back_pages():
+  from torchprime_b200.experimental.deepseek_inference.engine import DeepseekInferenceEngine
+  cfg, model = _tiny()
+  eng = DeepseekInferenceEngine(model, max_batch_size=3, max_seq_len=16, attn_impl="paged", page_size=4, num_pages=5)
+  ids = torch.randint(0, cfg.vocab_size, (1, 9))
+  eng.forward(ids, 0, rows=[2])
+  assert len(eng._free) == 2
+  with pytest.raises(RuntimeError, match="full"):
+    eng.forward(ids, 0, rows=[0])
+  assert len(eng._free) == 2 and len(eng._owned[2]) == 3                          # a refusal changes nothing
+  eng.forward(ids, 0, rows=[2])
+  eng.release([2])
+  assert sorted(eng._free) == list(range(5))
+  with pytest.raises(AssertionError):
+    eng.forward(ids[:, :1], 4, rows=[0])                                          # nothing in front of it
+
+
+@pytest.mark.parametrize("dtype", [None, E4M3])
+def test_paged_generation(dtype):
+  from torchprime_b200.experimental.deepseek_inference.engine import DeepseekInferenceEngine, full_forward_last_logits
+  from torchprime_b200.experimental.deepseek_inference.generate import generate
+  cfg, model = _tiny()
+  eng = DeepseekInferenceEngine(model, 2, 32, "paged", cache_dtype=dtype, page_size=4)
+  prompts = [[5, 9, 17, 3], [7, 2]]
+  outs = generate(eng, prompts, max_new_tokens=5, eos_id=-5, temperature=0.0)
+  assert [len(o) for o in outs] == [5, 5] and sorted(eng._free) == list(range(16))
+  if dtype is None:
+    for p, o in zip(prompts, outs):
+      for i, tok in enumerate(o):
+        assert tok == int(full_forward_last_logits(model, torch.tensor([p + o[:i]])).argmax())
+  stop = outs[0][2]
+  assert generate(eng, prompts[:1], 5, stop, 0.0)[0] == outs[0][: outs[0].index(stop)]
+  g = torch.Generator().manual_seed(0)
+  assert generate(eng, prompts, 5, -5, 1.0, g, top_k=1) == outs                  # one token left to draw
+  assert all(0 <= t < cfg.vocab_size for o in generate(eng, prompts, 4, -5, 1.0, g, top_p=0.9, min_p=0.01) for t in o)
+
+
+def test_filters_with_the_other_caches():
+  from torchprime_b200.experimental.deepseek_inference.engine import DeepseekInferenceEngine
+  from torchprime_b200.experimental.deepseek_inference.generate import generate
+  _, model = _tiny()
+  eng = DeepseekInferenceEngine(model, 2, 32, "absorb")
+  prompts = [[5, 9, 17, 3], [7, 2]]
+  assert generate(eng, prompts, 5, -5, 1.0, torch.Generator().manual_seed(1), top_k=1) == generate(eng, prompts, 5, -5, 0.0)

@@ -2,7 +2,7 @@
 
   python -m torchprime_b200.experimental.deepseek_inference.generate --ckpt-path <export dir> \
       --model deepseek-v2-lite [--input-file prompts.txt | --interactive] [--max-new-tokens 100] \
-      [--temperature 1.0] [--attn-impl absorb]
+      [--temperature 1.0] [--top-k 50] [--top-p 0.95] [--min-p 0.05] [--attn-impl absorb] [--cache-dtype e4m3]
 
 Capability reference: torchprime/experimental/torchax_models/deepseek_v3/generate.py:11-234
 (``sample`` = Gumbel-max over temperature-scaled logits, ``generate`` = prompt-aware incremental
@@ -15,6 +15,7 @@ import argparse
 
 import torch
 
+from ...ops.sampling import sample_tokens
 from .engine import DeepseekInferenceEngine
 
 
@@ -25,13 +26,32 @@ def sample(logits: torch.Tensor, temperature: float = 1.0, generator=None) -> to
   return (probs / noise).argmax(dim=-1)
 
 
+def next_tokens(logits, temperature, generator=None, top_k=None, top_p=None, min_p=None) -> torch.Tensor:
+  """A token for every row: the largest logit at temperature 0, else drawn, among the tokens that the filters leave
+  (``ops.sampling.sample_tokens``) if there are any."""
+  if not temperature > 0:
+    return logits.argmax(dim=-1)
+  if top_k is None and top_p is None and min_p is None:
+    return sample(logits, temperature, generator)
+  u = torch.rand(logits.shape[0], generator=generator, device=logits.device if generator is None else generator.device)
+  return sample_tokens(logits, u.to(logits.device), temperature, top_k, top_p, min_p)
+
+
+def _cut(row, eos_id):
+  return row[: row.index(eos_id)] if eos_id in row else row
+
+
 @torch.no_grad()
 def generate(engine: DeepseekInferenceEngine, prompt_tokens: list[list[int]], max_new_tokens: int, eos_id: int,
-             temperature: float = 1.0, generator=None) -> list[list[int]]:
+             temperature: float = 1.0, generator=None, top_k=None, top_p=None, min_p=None) -> list[list[int]]:
   """Complete every prompt by up to ``max_new_tokens`` tokens.  Prompts of different lengths
-  share the batch: positions still inside a prompt keep the prompt's token."""
+  share the batch: positions still inside a prompt keep the prompt's token, or, with the engine's paged cache, every
+  sequence stands at its own position."""
   lens = [len(t) for t in prompt_tokens]
   assert prompt_tokens and min(lens) > 0 and max(lens) <= engine.max_seq_len
+  draw = lambda logits: next_tokens(logits, temperature, generator, top_k, top_p, min_p)  # noqa: E731
+  if engine.attn_impl == "paged":
+    return _generate_paged(engine, prompt_tokens, max_new_tokens, eos_id, draw)
   total = min(engine.max_seq_len, max_new_tokens + max(lens))
   dev = engine.device
   tokens = torch.full((len(prompt_tokens), total), -1, dtype=torch.long, device=dev)
@@ -42,20 +62,33 @@ def generate(engine: DeepseekInferenceEngine, prompt_tokens: list[list[int]], ma
   prev = 0
   for cur in range(min(lens), total):
     logits = engine.forward(tokens[:, prev:cur].clamp_min(0), prev)
-    nxt = sample(logits, temperature, generator) if temperature > 0 else logits.argmax(dim=-1)
+    nxt = draw(logits)
     nxt = torch.where(prompt_mask[:, cur], tokens[:, cur], nxt)
     tokens[:, cur] = nxt
     finished |= (~prompt_mask[:, cur]) & (nxt == eos_id)
     prev = cur
     if bool(finished.all()):
       break
-  out = []
-  for i, row in enumerate(tokens.tolist()):
-    row = [t for t in row[lens[i]: lens[i] + max_new_tokens] if t >= 0]
-    if eos_id in row:
-      row = row[: row.index(eos_id)]
-    out.append(row)
-  return out
+  return [_cut([t for t in row[n: n + max_new_tokens] if t >= 0], eos_id) for row, n in zip(tokens.tolist(), lens)]
+
+
+def _generate_paged(engine, prompt_tokens, max_new_tokens, eos_id, draw):
+  """Prompts one after the other, then a step for all sequences that have not ended, each at its own position."""
+  n = len(prompt_tokens)
+  lens = [len(t) for t in prompt_tokens]
+  most = [min(max_new_tokens, engine.max_seq_len - k) for k in lens]
+  out = [[] for _ in range(n)]
+  rows = [i for i in range(n) if most[i] > 0]
+  if rows:
+    nxt = draw(torch.cat([engine.forward(torch.tensor([prompt_tokens[i]]), 0, rows=[i]) for i in rows]))
+  while rows:
+    for i, t in zip(rows, nxt.tolist()):
+      out[i].append(t)
+    rows = [i for i in rows if out[i][-1] != eos_id and len(out[i]) < most[i]]
+    if rows:
+      nxt = draw(engine.forward(torch.tensor([[out[i][-1]] for i in rows]), [lens[i] + len(out[i]) - 1 for i in rows], rows=rows))
+  engine.release(range(n))
+  return [_cut(row, eos_id) for row in out]
 
 
 def main(argv=None):
@@ -68,8 +101,15 @@ def main(argv=None):
   ap.add_argument("--max-new-tokens", type=int, default=100)
   ap.add_argument("--max-seq-len", type=int, default=4096)
   ap.add_argument("--temperature", type=float, default=1.0)
-  ap.add_argument("--attn-impl", choices=["naive", "absorb"], default="absorb")
+  ap.add_argument("--top-k", type=int, default=None, help="draw among the k largest logits")
+  ap.add_argument("--top-p", type=float, default=None, help="draw among the likeliest tokens of this probability together")
+  ap.add_argument("--min-p", type=float, default=None, help="draw among tokens at least this likely, the likeliest being 1")
+  ap.add_argument("--attn-impl", choices=["naive", "absorb", "paged"], default="absorb")
+  ap.add_argument("--cache-dtype", choices=["model", "e4m3"], default="model", help="e4m3: 8-bit keys and values (paged cache)")
+  ap.add_argument("--page-size", type=int, default=64, help="tokens to a page (paged cache)")
   args = ap.parse_args(argv)
+  if args.cache_dtype == "e4m3" and args.attn_impl != "paged":
+    ap.error("--cache-dtype e4m3 needs --attn-impl paged")
   from transformers import AutoTokenizer
 
   from ...config import compose
@@ -84,7 +124,9 @@ def main(argv=None):
     with open(args.input_file) as f:
       prompts = [line.strip() for line in f if line.strip()]
   engine = DeepseekInferenceEngine(model, max_batch_size=max(1, len(prompts)), max_seq_len=args.max_seq_len,
-                                   attn_impl=args.attn_impl)
+                                   attn_impl=args.attn_impl, page_size=args.page_size,
+                                   cache_dtype=torch.float8_e4m3fn if args.cache_dtype == "e4m3" else None)
+  filters = dict(top_k=args.top_k, top_p=args.top_p, min_p=args.min_p)
 
   def encode(text):
     if getattr(tok, "chat_template", None):
@@ -92,7 +134,7 @@ def main(argv=None):
     return tok.encode(text)
 
   if prompts:
-    outs = generate(engine, [encode(p) for p in prompts], args.max_new_tokens, tok.eos_token_id, args.temperature)
+    outs = generate(engine, [encode(p) for p in prompts], args.max_new_tokens, tok.eos_token_id, args.temperature, **filters)
     for p, o in zip(prompts, outs):
       print("Prompt:", p)
       print("Completion:", tok.decode(o, skip_special_tokens=True))
@@ -105,7 +147,7 @@ def main(argv=None):
         break
       if text in ("/exit", "/quit"):
         break
-      out = generate(engine, [encode(text)], args.max_new_tokens, tok.eos_token_id, args.temperature)[0]
+      out = generate(engine, [encode(text)], args.max_new_tokens, tok.eos_token_id, args.temperature, **filters)[0]
       print(tok.decode(out, skip_special_tokens=True))
 
 

@@ -69,7 +69,7 @@ if __name__ == "__main__":
   ap.add_argument("--layers", type=int, default=None)
   ap.add_argument("--seqlen", type=int, default=2048)
   ap.add_argument("--batch-size", type=int, default=1)
-  ap.add_argument("--attn-impl", choices=["naive", "absorb"], default="naive")
+  ap.add_argument("--attn-impl", choices=["naive", "absorb", "paged"], default="naive")
   ap.add_argument("--decode-steps", type=int, default=0)
   ap.add_argument("--iters", type=int, default=5)
   a = ap.parse_args()
