@@ -26,6 +26,8 @@
 //   - m) v_i / sum_i 2^(s_i - m) with m the maximum of s_i + e_i.  K's columns go to the product in another order than Q's would
 //   (four neighbouring bytes to a lane instead of two and two); the queries are loaded in the same one.
 
+#include <atomic>
+
 #include "common.cuh"
 #include "tpb.h"
 
@@ -50,7 +52,7 @@ struct PagedDecode {
   int* status;
   int B, Hkv, G, blocks, rows;             // blocks of up to 16 query heads to a key head; rows of the largest block
   int pages, page, width, capacity;        // entries of a row of the table, tokens that it can name
-  int window, stages;
+  int window, stages, aligned;
   float scale_log2, cap_log2;              // cap_log2: the cap in log2 units, 0 for none
 };
 
@@ -231,24 +233,31 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     }
     return running;
   };
-  int all = 0;
-  for (int base = 0; base < p.B; base += THREADS) all = add_up(base, all);
-  cta_share = pd_share(all * HB, gridDim.x);
-  cta_first = blockIdx.x * cta_share;
-  cta_steps = min(cta_share, all * HB - cta_first);
-  share = pd_share(cta_steps, NW);
-  for (int base = 0, running = 0; base < p.B; base += THREADS) {
-    if (p.B > THREADS) running = add_up(base, running);      // (else as it was left)
-    if (n > 0)
+  if (p.aligned) {                         // a CTA for each (sequence, head block)
+    const int b = blockIdx.x / HB, own = pd_visible<KEYS>(p, b).steps;
+    cta_share = cta_steps = own;
+    share = pd_share(own, NW);
+    if (lane == 0) s_at[warp][0] = b, s_at[warp][1] = blockIdx.x % HB, s_at[warp][2] = warp * share;
+  } else {
+    int all = 0;
+    for (int base = 0; base < p.B; base += THREADS) all = add_up(base, all);
+    cta_share = pd_share(all * HB, gridDim.x);
+    cta_first = blockIdx.x * cta_share;
+    cta_steps = min(cta_share, all * HB - cta_first);
+    share = pd_share(cta_steps, NW);
+    for (int base = 0, running = 0; base < p.B; base += THREADS) {
+      if (p.B > THREADS) running = add_up(base, running);      // (else as it was left)
+      if (n > 0)
 #pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const int in = cta_first + w * share - before * HB;
-        if (w * share < cta_steps && in >= 0 && in < n * HB) {
-          s_at[w][0] = base + threadIdx.x;
-          s_at[w][1] = in / n;
-          s_at[w][2] = in % n;
+        for (int w = 0; w < NW; ++w) {
+          const int in = cta_first + w * share - before * HB;
+          if (w * share < cta_steps && in >= 0 && in < n * HB) {
+            s_at[w][0] = base + threadIdx.x;
+            s_at[w][1] = in / n;
+            s_at[w][2] = in % n;
+          }
         }
-      }
+    }
   }
   __syncthreads();
   const int steps = min(share, cta_steps - warp * share);      // (none: 0 or less)
@@ -306,7 +315,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   if (blockIdx.x == 0)
     for (int b = threadIdx.x; b < p.B; b += THREADS)
       if (p.lengths[b] < 0 || p.lengths[b] > p.capacity) report(p.status, kBadArgument, 71);
-  if (threadIdx.x == 0) p.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  if (threadIdx.x == 0 && !p.aligned) p.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
   for (int b = blockIdx.x; b < p.B; b += gridDim.x)        // sequences of no visible token
     if (pd_visible<KEYS>(p, b).steps == 0) {
       uint4* dst = reinterpret_cast<uint4*>(p.out + (long long)b * p.Hkv * p.G * DV);
@@ -341,14 +350,25 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         }
       }
   };
-  auto put_part = [&](int slot) {
+  // A part that another warp or the kernel behind this one joins: results, then maximum and sum of each row.
+  struct Part {
+    float* o;
+    float2* ml;
+  };
+  auto part_at = [&](int slot) { return Part{p.part_o + (long long)slot * p.rows * DV, reinterpret_cast<float2*>(p.part_ml) + slot * p.rows}; };
+  auto warp_part = [&](int w) {            // of a warp of this CTA: in its ring, if it has nothing else to do
+    float* o = reinterpret_cast<float*>(pd_smem + (size_t)w * ST * T::STAGE);
+    return p.aligned ? Part{o, reinterpret_cast<float2*>(o + (WIDE ? 16 : 8) * DV)} : part_at(2 * gridDim.x + blockIdx.x * NW + w);
+  };
+  static_assert((WIDE ? 16 : 8) * DV * 4 <= T::STAGE - 16 * 8, "a part fits into a stage");
+  auto put_part = [&](const Part& part) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int r = 8 * nt + 2 * t + x;
         if (r >= rows) continue;
-        float* dst = p.part_o + (long long)(slot * p.rows + r) * DV;
+        float* dst = part.o + r * DV;
 #pragma unroll
         for (int cb = 0; cb < DV / 16; ++cb) {
           if constexpr (F8) {
@@ -358,7 +378,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
             dst[column(cb, 1)] = o[nt][cb][2 + x];
           }
         }
-        if (g == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * p.rows + r) * 2) = make_float2(m[nt][x], l[nt][x]);
+        if (g == 0) part.ml[r] = make_float2(m[nt][x], l[nt][x]);
       }
   };
   while (done < steps) {
@@ -583,10 +603,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
     if (starts && ends) {
       put_result();
     } else if (!starts && warp > 0) {      // for the warp that began it, or began this CTA's part of it
-      put_part(2 * gridDim.x + blockIdx.x * NW + warp);
+      put_part(warp_part(warp));
       if (lane == 0) s_ends[warp] = ends;
     } else if (ends) {
-      put_part(2 * blockIdx.x);
+      put_part(part_at(2 * blockIdx.x));
     } else {
       joins = true;                        // (the list's part of this warp ends here)
       break;
@@ -598,7 +618,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   if (joins) {
     bool ends = false;
     for (int w = warp + 1; w < NW && w * share < cta_steps && !ends; ++w) {
-      const int at = 2 * gridDim.x + blockIdx.x * NW + w;
+      const Part part = warp_part(w);
       ends = s_ends[w];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -606,8 +626,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         for (int x = 0; x < 2; ++x) {
           const int r = 8 * nt + 2 * t + x;
           if (r >= rows) continue;
-          const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (at * p.rows + r) * 2);
-          const float* src = p.part_o + (long long)(at * p.rows + r) * DV;
+          const float2 ml = part.ml[r];
+          const float* src = part.o + r * DV;
           const float top = fmaxf(m[nt][x], ml.x);
           const float fa = m[nt][x] == -INFINITY ? 0.f : ex2_approx(m[nt][x] - top), fb = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
           m[nt][x] = top;
@@ -624,7 +644,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       put_result();
     } else {
       const int slot = 2 * blockIdx.x + (warp == 0 && done == seg ? 0 : 1);
-      put_part(slot);
+      put_part(part_at(slot));
       if (c.at == 0 && lane == 0)
         p.split[blockIdx.x] = make_int4((cta_first + warp * share + done - seg + c.s.steps - 1) / cta_share, slot, c.b, c.hb);
     }
@@ -691,6 +711,13 @@ static int pd_grid(long long most_steps) {
   return (int)(most_steps < 1 ? 1 : most_steps < sms ? most_steps : sms);
 }
 
+// Whether a CTA takes a whole (sequence, head block), with nothing to add up before and to join behind: short sequences, or as many of
+// them as there are SMs.  us in a graph, list / CTA each: 1 sequence of 32 / 8 heads of 128 in bf16, 64 tokens 6.4 / 3.7, 256 6.7 / 6.2,
+// 512 7.0 / 7.7; 16 sequences 512 10.9 / 8.0, 1024 11.9 / 10.6, 2048 15.3 / 15.4; 8 of 16 heads of 192 / 128, 1024 12.0 / 10.8, 2048 15.1 / 16.9.
+static bool pd_aligned(long long jobs, long long capacity) {
+  return jobs <= sm_count() && capacity <= (2 * jobs >= sm_count() ? 1024 : 256);
+}
+
 template <int DK, int DV, bool F8, bool WIDE>
 static int launch_paged_decode(PagedDecode p, int grid, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t stream) {
   using T = PagedTile<DK, DV, F8, WIDE>;
@@ -700,10 +727,16 @@ static int launch_paged_decode(PagedDecode p, int grid, const CUtensorMap& km, c
   if (p.stages > 8) p.stages = 8;
   const int smem = 1024 + T::WARPS * p.stages * (T::STAGE + T::SCALES + 8);
   auto* f = paged_decode_kernel<DK, DV, F8, WIDE>;
-  cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<unsigned> ready{0};              // a bit for each device
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess && (device > 31 || !(ready.load(std::memory_order_relaxed) >> device & 1))) {
+    e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess && device <= 31) ready.fetch_or(1u << device, std::memory_order_relaxed);
+  }
   if (e != cudaSuccess) return 1000 + (int)e;
   chain(f, grid, T::WARPS * 32, smem, stream, km, vm, p);
-  if (grid > 1) chain(paged_join_kernel<DV>, dim3(grid, p.rows), 256, 0, stream, p);
+  if (grid > 1 && !p.aligned) chain(paged_join_kernel<DV>, dim3(grid, p.rows), 256, 0, stream, p);
   e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 1000 + (int)e;
 }
@@ -715,8 +748,8 @@ using namespace tpb;
 // Bytes of scratch for tpb_paged_decode.
 extern "C" int tpb_paged_decode_scratch(int B, int Hkv, int G, int DK, int DV, int held8, int capacity) {
   const PagedShape shape = pd_shape(held8 != 0, G > 8, DK + DV);
-  const long long steps = (long long)B * Hkv * ((G + 15) / 16) * (((long long)capacity + shape.keys - 1) / shape.keys);
-  return pd_grid(steps) * ((2 + shape.warps) * (G < 16 ? G : 16) * (DV + 2) * 4 + 16);
+  const long long jobs = (long long)B * Hkv * ((G + 15) / 16), steps = jobs * (((long long)capacity + shape.keys - 1) / shape.keys);
+  return pd_aligned(jobs, capacity) ? 0 : pd_grid(steps) * ((2 + shape.warps) * (G < 16 ? G : 16) * (DV + 2) * 4 + 16);
 }
 
 // q [B, Hkv * G, DK] bf16 (strides q_b, q_h), pools as in tpb_paged_rows (strides of pages, tokens, heads; scales contiguous over
@@ -760,7 +793,8 @@ extern "C" int tpb_paged_decode(const void* q, long long q_b, long long q_h, con
   p.ks_head = strides[5];
   p.vs_page = strides[9];
   p.vs_head = strides[11];
-  const int grid = pd_grid(steps);
+  p.aligned = pd_aligned((long long)B * Hkv * blocks, capacity);
+  const int grid = p.aligned ? B * Hkv * blocks : pd_grid(steps);
   p.rows = G < 16 ? G : 16;
   const long long part_rows = (long long)grid * (2 + shape.warps) * p.rows;
   p.split = static_cast<int4*>(scratch);

@@ -20,6 +20,7 @@
 //     sorts it.  Then two more passes draw the token: sums of slices and of the parts of their warps, and along one of those.
 //   * Where a list is too long for one CTA (thousands of equal logits, large k) the border is found bit by bit of the order.
 
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -786,8 +787,14 @@ sample_kernel(const SampleParams p, int ctas) {
 template <typename L>
 static int launch_sample(const SampleParams& p, int B, int ctas, cudaStream_t stream) {
   auto* f = sample_kernel<L>;
-  cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SmpShared));
-  if (e == cudaSuccess && ctas > 8) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  static std::atomic<unsigned> ready{0};              // a bit for each device
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess && (device > 31 || !(ready.load(std::memory_order_relaxed) >> device & 1))) {
+    e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SmpShared));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess && device <= 31) ready.fetch_or(1u << device, std::memory_order_relaxed);
+  }
   if (e == cudaSuccess) e = chain_clusters(f, ctas, dim3(B * ctas), SMP_THREADS, sizeof(SmpShared), stream, p, ctas);
   const cudaError_t last = cudaGetLastError();
   if (e == cudaSuccess) e = last;

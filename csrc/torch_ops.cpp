@@ -1068,7 +1068,7 @@ struct Pools {
         v.get_device() != k.get_device() || held8 != ks.defined() || held8 != vs.defined())
       return false;
     pages = k.size(0), page = k.size(1), heads = k.size(2), dk = k.size(3), dv = v.size(3);
-    if (v.size(0) != pages || v.size(1) != page || v.size(2) != heads || page < 1 || heads < 1 || pages * page > 0x7fffffff) return false;
+    if (v.size(0) != pages || v.size(1) != page || v.size(2) != heads || pages < 1 || page < 1 || heads < 1 || pages * page > 0x7fffffff) return false;
     const int64_t unit = held8 ? 16 : 8;
     for (int i = 0; i < 2; ++i) {
       const Tensor &t = i ? v : k, &s = i ? vs : ks;
@@ -1131,11 +1131,13 @@ py::object paged_read(py::handle k_, py::handle v_, py::handle ks_, py::handle v
 
 // Attention of one token per sequence over a cache; see paged_kv.decode_attention.
 py::object paged_decode(py::handle q_, py::handle k_, py::handle v_, py::handle ks_, py::handle vs_, py::handle table_, py::handle lens_,
-                        double scale, int64_t window, double softcap) {
+                        py::handle scale_, py::handle window_, py::handle softcap_) {
   Pools c;
   Tensor q, table, lens, out;
-  if (!unobserved() || !unpack(q_, q) || !plain(q) || q.dim() != 3 || !c.take(k_, v_, ks_, vs_) || !unpack(table_, table) ||
-      !unpack(lens_, lens) || (at::GradMode::is_enabled() && recording(q)))
+  double scale, softcap;
+  int64_t window;
+  if (!whole(window_, 0, window) || !real(softcap_, 0.0, softcap) || !unobserved() || !unpack(q_, q) || !plain(q) || q.dim() != 3 || !c.take(k_, v_, ks_, vs_) || !unpack(table_, table) ||
+      !unpack(lens_, lens) || (at::GradMode::is_enabled() && recording(q)) || !real(scale_, 1.0 / std::sqrt((double)q.size(2)), scale))
     return py::none();
   const int64_t b = q.size(0), hq = q.size(1);
   if (b < 1 || b > (1 << 24) || hq < 1 || hq > 65535 || hq % c.heads || q.size(2) != c.dk || c.pages < 1 || c.page % 16 ||

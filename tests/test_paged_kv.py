@@ -89,6 +89,9 @@ def test_refusals():
     paged_kv.append(PagedKV(c.k, c.v.to(E4M3)), x, x, s)
   with pytest.raises(ValueError):
     paged_kv.read(PagedKV(c.k.to(E4M3), c.v.to(E4M3)), s)
+  for empty in (PagedKV.allocate(0, 16, 1, 8), PagedKV.allocate(2, 0, 1, 8), PagedKV(c.k[0], c.v[0])):
+    with pytest.raises(ValueError):
+      paged_kv.read(empty, s)
   q = PagedKV.allocate(2, 16, 1, 16, dtype=E4M3)
   with pytest.raises(ValueError):
     paged_kv.read(PagedKV(q.k, q.v, q.k_scale, q.v_scale.view(torch.uint8)), s)

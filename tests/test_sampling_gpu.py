@@ -116,6 +116,13 @@ def test_strided_rows(cuda_lib):
     _same(x, u[: x.shape[0]], temperature=2.5, top_k=30)
 
 
+def test_settings_out_of_wider_tensors(cuda_lib):
+  g = torch.Generator(device="cuda").manual_seed(15)
+  x, u = _logits(g, 16, 9000, "peaks"), torch.rand(32, generator=g, device="cuda")[::2]
+  both = torch.stack([torch.linspace(0, 2, 16, device="cuda"), torch.linspace(0.3, 1, 16, device="cuda")], 1)
+  _same(x, u, temperature=both[:, 0], top_p=both[:, 1], min_p=(both * 0.01)[:, 0], top_k=torch.arange(0, 64, 2, dtype=torch.int32, device="cuda")[::2])
+
+
 def test_same_token_every_time_and_from_python(cuda_lib, monkeypatch):
   g = torch.Generator(device="cuda").manual_seed(11)
   x, u = _logits(g, 40, 30000, "normal"), torch.rand(40, generator=g, device="cuda")

@@ -16,8 +16,9 @@ from typing import NamedTuple
 
 import torch
 
-from . import _debug, _lib, reference as ref
+from . import _debug, _lib, functional, reference as ref
 from ._lib import check, lib, ptr, stream_ptr
+from .functional import inference_only, use_kernels
 
 P, I, LL, F = c_void_p, c_int, c_longlong, c_float
 _lib.register_signature("tpb_paged_rows", [I, P, P, P, P, P, P, P, LL, I, I, I, I, I, P, P, P])
@@ -52,6 +53,8 @@ class PagedKV(NamedTuple):
 
 
 def _check_cache(c: PagedKV):
+  if c.k.dim() != 4 or c.v.dim() != 4 or 0 in c.k.shape or 0 in c.v.shape:
+    raise ValueError(f"pools are [pages, page, heads, columns], got {tuple(c.k.shape)} and {tuple(c.v.shape)}")
   pages, page, h, _ = c.k.shape
   if c.v.shape[:3] != c.k.shape[:3] or c.v.dtype != c.k.dtype:
     raise ValueError(f"pools of keys {tuple(c.k.shape)} {c.k.dtype} and values {tuple(c.v.shape)} {c.v.dtype} differ")
@@ -105,8 +108,7 @@ def append(cache: PagedKV, k, v, slots):
   """Writes keys [T, H, Dk] and values [T, H, Dv] to the rows ``slots`` [T] (int64) of the cache, quantised where it is
   e4m3; a token of slot -1 (padding) is not written, and neither is one whose slot lies outside the pool, which the kernel
   reports (``_lib.raise_on_device_timeout``).  No slot may come twice: which of its tokens a row of it holds is not defined."""
-  from .functional import _native, use_kernels
-  if not _debug.bounds_enabled() and (nat := _native()) is not None and nat.paged_append(*cache, k, v, slots):
+  if not _debug.bounds_enabled() and (nat := functional._native()) is not None and nat.paged_append(*cache, k, v, slots):
     return
   _check_cache(cache)
   _check_slots("paged_append", cache, slots)
@@ -131,8 +133,7 @@ def append(cache: PagedKV, k, v, slots):
 def read(cache: PagedKV, slots, dtype=torch.bfloat16):
   """The rows ``slots`` [T] of the cache as (keys [T, H, Dk], values [T, H, Dv]) of ``dtype``; zeros for slot -1 and, reported as in
   :func:`append`, for slots outside the pool."""
-  from .functional import _native, use_kernels
-  if dtype == torch.bfloat16 and not _debug.bounds_enabled() and (nat := _native()) is not None:
+  if dtype == torch.bfloat16 and not _debug.bounds_enabled() and (nat := functional._native()) is not None:
     rows = nat.paged_read(*cache, slots)
     if rows is not None:
       return rows
@@ -169,10 +170,7 @@ def decode_attention(q, cache: PagedKV, block_table, lengths, scale=None, window
   64 columns.  It reads nothing of the table and of the pages behind a sequence's last token (what a page holds there may be
   anything); a page outside the pool counts as zeros, a length beyond the table as the whole table, a negative one as none, and all three are
   reported (``_lib.raise_on_device_timeout``)."""
-  from .functional import _native, inference_only, use_kernels
-  window, softcap = int(window or 0), float(softcap or 0.0)
-  scale = float(scale) if scale is not None else q.shape[-1] ** -0.5
-  if not _debug.bounds_enabled() and (nat := _native()) is not None:
+  if not _debug.bounds_enabled() and (nat := functional._native()) is not None:
     o = nat.paged_decode(q, *cache, block_table, lengths, scale, window, softcap)
     if o is not None:
       return o
@@ -186,11 +184,13 @@ def decode_attention(q, cache: PagedKV, block_table, lengths, scale=None, window
     raise ValueError("decode_attention: block_table and lengths must be int32")
   if any(t.device != cache.k.device for t in (q, block_table, lengths)):
     raise ValueError("decode_attention: queries, block_table and lengths must be on the cache's device")
+  window, softcap = int(window or 0), float(softcap or 0.0)
+  scale = float(scale) if scale is not None else dk ** -0.5
   if window < 0 or not softcap >= 0.0:
     raise ValueError(f"decode_attention: window {window}, softcap {softcap}")
   _debug.check_index("decode_attention", "lengths", lengths, 0, block_table.shape[1] * cache.page + 1)
-  if (use_kernels(q) and q.is_cuda and _decode_ok(q, cache) and (inference_only() or not q.requires_grad)):
-    q = _vectors(q)
+  if (use_kernels(q) and q.is_cuda and _decode_ok(q, cache) and block_table.shape[1] * cache.page <= 0x7fffff00 and (inference_only() or not q.requires_grad)):
+    q, lengths = _vectors(q), lengths.contiguous()
     block_table = block_table if block_table.stride(1) == 1 else block_table.contiguous()
     pages, page, hkv, _ = cache.k.shape
     dv, width = cache.v.shape[3], block_table.shape[1]
@@ -199,7 +199,7 @@ def decode_attention(q, cache: PagedKV, block_table, lengths, scale=None, window
       n = lib().tpb_paged_decode_scratch(b, hkv, hq // hkv, dk, dv, int(cache.k.dtype == E4M3), width * page)
       scratch = torch.empty(n, dtype=torch.uint8, device=q.device)
       rc = lib().tpb_paged_decode(ptr(q), q.stride(0), q.stride(1), ptr(cache.k), ptr(cache.v), ptr(cache.k_scale), ptr(cache.v_scale),
-                                  _c_strides(cache), ptr(block_table), block_table.stride(0), width, ptr(lengths.contiguous()), ptr(out),
+                                  _c_strides(cache), ptr(block_table), block_table.stride(0), width, ptr(lengths), ptr(out),
                                   ptr(scratch), b, hkv, hq // hkv, dk, dv, pages, page, window, scale, softcap, stream_ptr())
     check(rc, f"paged_decode q{tuple(q.shape)} pool{tuple(cache.k.shape)}")
     return out

@@ -6,7 +6,7 @@ from ctypes import c_double, c_int, c_longlong, c_void_p
 
 import torch
 
-from . import _lib, reference as ref
+from . import _lib, functional, reference as ref
 from ._lib import check, lib, ptr, stream_ptr
 
 P, I, LL, D = c_void_p, c_int, c_longlong, c_double
@@ -34,9 +34,8 @@ def sample_tokens(logits, u, temperature=1.0, top_k=None, top_p=None, min_p=None
   logit.  NaN counts as -inf; a row without a logit above -inf gives -1.
 
   The four settings are numbers or one for each row (fp32, ``top_k`` int32).  Rows of up to 2^18 logits in fp32 or bf16 run in
-  one kernel, whose sums of weights are exact to 2^-44 of the largest and do not depend on the machine's load."""
-  from .functional import _native, get_backend
-  if (nat := _native()) is not None:
+  one kernel, whose weights are good to 2^-34 and whose sums of them are exact: the same call draws the same tokens."""
+  if (nat := functional._native()) is not None:
     y = nat.sample_tokens(logits, u, temperature, top_k, top_p, min_p)
     if y is not None:
       return y
@@ -50,17 +49,17 @@ def sample_tokens(logits, u, temperature=1.0, top_k=None, top_p=None, min_p=None
   top_p = _setting("top_p", 1.0 if top_p is None else top_p, b, logits.device, torch.float32)
   min_p = _setting("min_p", 0.0 if min_p is None else min_p, b, logits.device, torch.float32)
   logits = logits.detach()
-  if logits.is_cuda and get_backend() != "torch" and logits.dtype in (torch.float32, torch.bfloat16) and v <= MAX_VOCAB and b < 1 << 26:
+  if logits.is_cuda and functional.get_backend() != "torch" and logits.dtype in (torch.float32, torch.bfloat16) and v <= MAX_VOCAB and b < 1 << 26:
     _lib.lib()
     logits = logits if logits.stride(1) == 1 else logits.contiguous()
     out = torch.empty(b, dtype=torch.int64, device=logits.device)
-    row = lambda t: ptr(t.contiguous()) if torch.is_tensor(t) else None  # noqa: E731
+    # (held until the launch: a copy that is let go is the next one's memory)
+    rows = [t.contiguous() if torch.is_tensor(t) else None for t in (u, temperature, top_k, top_p, min_p)]
     num = lambda t, other: other if torch.is_tensor(t) else t  # noqa: E731
-    u = u.contiguous()
     with torch.cuda.device(logits.device):
-      rc = lib().tpb_sample_tokens(ptr(logits), int(logits.dtype == torch.bfloat16), logits.stride(0), ptr(u), row(temperature), row(top_k),
-                                   row(top_p), row(min_p), float(num(temperature, 1.0)), min(max(int(num(top_k, 0)), 0), v),
-                                   float(num(top_p, 1.0)), float(num(min_p, 0.0)), ptr(out), b, v, stream_ptr())
+      rc = lib().tpb_sample_tokens(ptr(logits), int(logits.dtype == torch.bfloat16), logits.stride(0), *map(ptr, rows),
+                                   float(num(temperature, 1.0)), min(max(int(num(top_k, 0)), 0), v), float(num(top_p, 1.0)),
+                                   float(num(min_p, 0.0)), ptr(out), b, v, stream_ptr())
     check(rc, f"sample_tokens {b}x{v}")
     return out
   return ref.sample_tokens(logits, u, temperature, top_k, top_p, min_p)
