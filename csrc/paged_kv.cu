@@ -15,8 +15,6 @@
 
 namespace tpb {
 
-int sm_count();
-
 // One pool and the rows that go there or come from there (strides in elements; scales: null for bf16).
 struct PagedRows {
   __nv_bfloat16* x;

@@ -16,7 +16,7 @@
 //   * The first pass finds m.
 //   * top-k: the k-th largest of the threads' own largest logits is a lower bound of the k-th largest of all; min-p has a bound of its
 //     own.  The logits from the bound on, usually little more than k, go to one CTA, which sorts them and finishes alone.
-//   * nucleus: a histogram of the weights over their exponents in steps of 1/32; the bin with the border goes to one CTA, which
+//   * nucleus: a histogram of the weights over their exponents in steps of 1/64; the bin with the border goes to one CTA, which
 //     sorts it.  Then two more passes draw the token: sums of slices and of the parts of their warps, and along one of those.
 //   * Where a list is too long for one CTA (thousands of equal logits, large k) the border is found bit by bit of the order.
 
@@ -28,10 +28,8 @@
 
 namespace tpb {
 
-int sm_count();
-
 constexpr int SMP_THREADS = 512, SMP_WARPS = SMP_THREADS / 32;      // (1024: one row's nucleus 36 -> 41 us)
-constexpr int SMP_BINS = 2048;          // 11 bits of the order at a time (31-21, 20-10, 9-0); 64 binary orders of weights in steps of 1/32
+constexpr int SMP_BINS = 2048;          // 11 bits of the order at a time (31-21, 20-10, 9-0); 32 binary orders of weights in steps of 1/64
 constexpr int SMP_CAP = 2048;           // tokens that one CTA sorts
 constexpr int SMP_FIXED = 44;           // a weight of 1 is 2^44: 2^18 of them stay below 2^63
 constexpr int SMP_TABLE = 1024;         // 2^(j / 1024)
@@ -63,7 +61,7 @@ struct SampleParams {
   const float *temperature, *top_p, *min_p;      // one a row, or null: the numbers below
   const int* top_k;
   double temperature0, top_p0, min_p0;
-  int top_k0, V, slice;                          // slice: logits of a CTA, a multiple of 8
+  int top_k0, B, V, slice;                       // slice: logits of a CTA, a multiple of 8
   long long* out;
   int vec;                                       // rows can be read four logits at a time: 2, also by bulk copies (16-byte aligned)
   int* status;
@@ -166,8 +164,8 @@ struct SmpWeight {
     if (slow) f(std::true_type());
     else f(std::false_type());
   }
-  // Steps of 1/32 below the largest weight's exponent, the largest weights in the last bin.
-  static __device__ __forceinline__ int bin(int j) { return SMP_BINS - 1 + max(j >> 5, 1 - SMP_BINS); }
+  // Steps of 1/64 below the largest weight's exponent, the largest weights in the last bin, all below 2^-32 in the first.
+  static __device__ __forceinline__ int bin(int j) { return SMP_BINS - 1 + max(j >> 4, 1 - SMP_BINS); }
 };
 
 // The smallest key in (low, high] for which `past` holds, as it does for `high` and for all behind; the whole warp calls.
@@ -194,6 +192,8 @@ struct SmpShared {
   uint64_t full[SMP_RING];              // barriers of the copies
   u64 found[3];                         // bin, sum of the bins above, sum of all
   unsigned border, of_border;
+  unsigned range[2];                    // of keys
+  int row;
   unsigned staged;                      // of this CTA's part of the list
   int dead;                             // a copy has not come
 };
@@ -283,8 +283,22 @@ __device__ __forceinline__ void smp_find(SmpShared& s, int rank, int ctas, F&& t
   __syncthreads();
 }
 
-// s.list[0 .. n) in descending order; n is padded with zeros to a power of two.
+// s.list[0 .. n) in descending order: no two are the same.  Few go to where the larger ones leave them room; more are padded with zeros
+// to a power of two and merged.
 __device__ __forceinline__ void smp_sort(u64* list, int n) {
+  if (n <= SMP_THREADS) {
+    __syncthreads();
+    const u64 mine = (int)threadIdx.x < n ? list[threadIdx.x] : 0;
+    int larger = 0;
+    if ((int)threadIdx.x < n) {
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) larger += list[i] > mine;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < n) list[larger] = mine;
+    __syncthreads();
+    return;
+  }
   int size = 32;
   while (size < n) size <<= 1;
   for (int i = n + threadIdx.x; i < size; i += SMP_THREADS) list[i] = 0;
@@ -438,7 +452,27 @@ sample_kernel(const SampleParams p, int ctas) {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // (nobody writes to a CTA that has not begun)
   chain_launch();
   if (!chain_wait()) return;
-  const int b = blockIdx.x / ctas, V = p.V;
+  const int V = p.V;
+  int b = blockIdx.x / ctas;
+  if ((p.temperature || p.top_k || p.min_p) && p.B <= SMP_THREADS) {
+    // Rows whose sums take all their logits come first: they take longest.  (256 rows of 102400, settings of their own, one in
+    // seventeen of that kind: 114 us instead of 123.)
+    const int k = tid < p.B && p.top_k ? p.top_k[tid] : p.top_k0;
+    const bool here = tid < p.B, long_ = here && (p.temperature ? (double)p.temperature[tid] : p.temperature0) > 0.0 && (k <= 0 || k >= V) &&
+                                         !((p.min_p ? (double)p.min_p[tid] : p.min_p0) > 0.0);
+    const unsigned longs = __ballot_sync(0xffffffffu, long_), before = (1u << lane) - 1;
+    if (lane == 0) s.warp[warp] = __popc(longs);
+    __syncthreads();
+    int at = 0, all = 0;
+    for (int w = 0; w < SMP_WARPS; ++w) {
+      if (w < warp) at += (int)s.warp[w];
+      all += (int)s.warp[w];
+    }
+    at += __popc(longs & before);
+    if (here && (long_ ? at : all + tid - at) == b) s.row = tid;
+    __syncthreads();
+    b = s.row;
+  }
   SmpSlice<L> slice = {static_cast<const L*>(p.logits) + b * p.stride, min(V, rank * p.slice), min(V, (rank + 1) * p.slice), p.vec};
   slice.copied = slice.end - (slice.end - slice.begin) % (16 / (int)sizeof(L));
   const double T = p.temperature ? (double)p.temperature[b] : p.temperature0;
@@ -651,10 +685,15 @@ sample_kernel(const SampleParams p, int ctas) {
     } else {
       const int bin = (int)s.found[0];
       const u64 above = s.found[1];
-      auto first_of = [&](int of) {
-        return smp_first_key(SMP_LOWEST, SMP_HIGHEST, [&](unsigned key) { return weight.bin(weight.step(smp_logit(key))) >= of; });
-      };
-      const u64 n_list = gather(max(first_of(bin), border + 1), bin + 1 < SMP_BINS ? first_of(bin + 1) : 0xffffffffu);
+      if (warp < 2) {                             // the bin's smallest key, and the next one's
+        const int of = bin + warp;
+        const unsigned key = of >= SMP_BINS ? 0xffffffffu : smp_first_key(SMP_LOWEST, SMP_HIGHEST, [&](unsigned k) {
+          return weight.bin(weight.step(smp_logit(k))) >= of;
+        });
+        if (lane == 0) s.range[warp] = key;
+      }
+      __syncthreads();
+      const u64 n_list = gather(max(s.range[0], border + 1), s.range[1]);
       if (n_list <= SMP_CAP) {
         if (rank == 0) {
           const int n = (int)n_list;
@@ -784,8 +823,29 @@ sample_kernel(const SampleParams p, int ctas) {
   }
 }
 
+// How many clusters of that many CTAs the current device holds at once.
 template <typename L>
-static int launch_sample(const SampleParams& p, int B, int ctas, cudaStream_t stream) {
+static cudaError_t sample_clusters(int device, int ctas, int* most) {
+  static std::atomic<int> known[32][5];               // by device and ctas / 4 (0, 1, 2, 4); 0: not asked yet
+  std::atomic<int>* const at = device < 32 ? &known[device][ctas / 4] : nullptr;
+  if (at && (*most = at->load(std::memory_order_relaxed)) > 0) return cudaSuccess;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(SMP_THREADS);
+  cfg.dynamicSmemBytes = sizeof(SmpShared);
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaOccupancyMaxActiveClusters(most, sample_kernel<L>, &cfg);
+  if (at && e == cudaSuccess) at->store(*most, std::memory_order_relaxed);
+  return e;
+}
+
+template <typename L>
+static int launch_sample(SampleParams p, cudaStream_t stream) {
   auto* f = sample_kernel<L>;
   static std::atomic<unsigned> ready{0};              // a bit for each device
   int device = 0;
@@ -795,7 +855,21 @@ static int launch_sample(const SampleParams& p, int B, int ctas, cudaStream_t st
     if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e == cudaSuccess && device <= 31) ready.fetch_or(1u << device, std::memory_order_relaxed);
   }
-  if (e == cudaSuccess) e = chain_clusters(f, ctas, dim3(B * ctas), SMP_THREADS, sizeof(SmpShared), stream, p, ctas);
+  // CTAs to a row: as many as leave all rows under way at once, with 2048 logits or more to a CTA.  A GPC's SMs bound what clusters fit:
+  // 16 rows of 16 CTAs or 37 of 8 do not, though the SMs hold 296 CTAs.  us, by this rule / with twice the CTAs, rows of 128256: 16 rows,
+  // 50 largest 24 / 32, nucleus 51 / 63; 37 rows, 30 / 39, 82 / 89; 64 rows, 31 / 55, 84 / 108.  Rows with settings of their own take
+  // unequal times, a nucleus of a flat distribution ten times a greedy row's: two waves of clusters even that out (256 rows of 102400:
+  // 114 us, by the rule of the others 156, with four 122).
+  const int waves = p.temperature || p.top_k || p.top_p || p.min_p ? 2 : 1;
+  int ctas = 1;
+  while (e == cudaSuccess && ctas < 16 && p.V / (ctas * 2) >= 2048) {
+    int most = 0;
+    e = sample_clusters<L>(device, ctas * 2, &most);
+    if (p.B > (long long)waves * most) break;
+    ctas *= 2;
+  }
+  p.slice = ((p.V + ctas - 1) / ctas + 7) / 8 * 8;
+  if (e == cudaSuccess) e = chain_clusters(f, ctas, dim3(p.B * ctas), SMP_THREADS, sizeof(SmpShared), stream, p, ctas);
   const cudaError_t last = cudaGetLastError();
   if (e == cudaSuccess) e = last;
   return e == cudaSuccess ? 0 : 1000 + (int)e;
@@ -814,17 +888,11 @@ extern "C" int tpb_sample_tokens(const void* logits, int bf16, long long stride,
   if (B < 0 || V < 1 || V > (1 << 18)) return -2;
   if (B == 0) return 0;
   if (B > (0x7fffffff >> 4)) return -2;
-  // CTAs to a row: as many as the SMs hold at once (two each), with 2048 logits or more to a CTA.  Rows with settings of their own take
-  // unequal times, a nucleus of a flat distribution ten times a greedy row's, and get twice as many.  us, once / twice as many: 64 rows
-  // of 128256, nucleus 91 / 118, 50 largest 34 / 58; 256 rows of 102400, nucleus 193 / 226, 50 largest 51 / 78, mixed 174 / 138.
-  const long long room = (temperature || top_k || top_p || min_p ? 4LL : 2LL) * sm_count();
-  int ctas = 1;
-  while (ctas < 16 && (long long)B * ctas * 2 <= room && V / (ctas * 2) >= 2048) ctas *= 2;
   const int elt = bf16 ? 2 : 4;
-  SampleParams p = {logits, stride, u, temperature, top_p, min_p, top_k, temperature0, top_p0, min_p0, top_k0, V,
-                    ((V + ctas - 1) / ctas + 7) / 8 * 8, out, 0, status_block()};
+  SampleParams p = {logits, stride, u, temperature, top_p, min_p, top_k, temperature0, top_p0, min_p0, top_k0, B, V,
+                    0, out, 0, status_block()};
   p.vec = (reinterpret_cast<uintptr_t>(logits) % (4 * elt) == 0 && stride % 4 == 0) +
           (reinterpret_cast<uintptr_t>(logits) % 16 == 0 && stride * elt % 16 == 0);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  return bf16 ? launch_sample<__nv_bfloat16>(p, B, ctas, stream) : launch_sample<float>(p, B, ctas, stream);
+  return bf16 ? launch_sample<__nv_bfloat16>(p, stream) : launch_sample<float>(p, stream);
 }
