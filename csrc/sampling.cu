@@ -93,6 +93,18 @@ __device__ __forceinline__ float smp_max4(const float* l) {
 }
 __device__ __forceinline__ float smp_logit(unsigned key) { return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu)); }
 
+// Larger, and the same, in that order, with subnormal numbers.
+__device__ __forceinline__ bool smp_above(float a, float b) {
+  int x;
+  asm("{\n\t.reg .pred p;\n\tsetp.gt.f32 p, %1, %2;\n\tselp.s32 %0, 1, 0, p;\n\t}" : "=r"(x) : "f"(a), "f"(b));
+  return x;
+}
+__device__ __forceinline__ bool smp_same(float a, float b) {
+  int x;
+  asm("{\n\t.reg .pred p;\n\tsetp.eq.f32 p, %1, %2;\n\tselp.s32 %0, 1, 0, p;\n\t}" : "=r"(x) : "f"(a), "f"(b));
+  return x;
+}
+
 struct SmpWeight {
   double per_unit;        // log2(e) / T
   float hi, lo;           // 1024 log2(e) / T as a sum of two floats
@@ -135,12 +147,12 @@ struct SmpWeight {
     return slow ? step_slow(l) : __float_as_int(__fadd_rn(fmaxf(__fmul_rn(l, hi), p_cut), 12582912.f)) - j_top;
   }
   // In multiples of 2^-44: 2^44 for the largest, else with the last bit set, as often above as below what is cut off; 0 below 2^-45 and
-  // for NaN.  j: step(l).
+  // for NaN and where it is not wanted.  j: step(l).
   template <bool SLOW>
-  __device__ __forceinline__ u64 of(float l, int& j) const {
+  __device__ __forceinline__ u64 of(float l, int& j, bool wanted = true) const {
     if (SLOW) {
       j = step_slow(l);
-      return __double2ull_rn(real(l) * (double)(1LL << SMP_FIXED));
+      return wanted ? __double2ull_rn(real(l) * (double)(1LL << SMP_FIXED)) : 0;
     }
     const float p = __fmul_rn(l, hi);
     float y;
@@ -152,7 +164,7 @@ struct SmpWeight {
     const u64 t = table[j & (SMP_TABLE - 1)];
     const u64 w = t + (u64)((long long)(int)(t >> 32) * qi);
     const u64 x = w >> (62 - SMP_FIXED - (j >> 10));
-    return p > p_cut ? x | (~x >> SMP_FIXED & 1) : 0;
+    return wanted & (p > p_cut) ? x | (~x >> SMP_FIXED & 1) : 0;
   }
   __device__ __forceinline__ u64 operator()(float l) const {
     int j;
@@ -625,7 +637,7 @@ sample_kernel(const SampleParams p, int ctas) {
     __syncthreads();
   };
   auto add_weight = [&](int bin, u64 w) {         // the carry from the low to the high word is this thread's to see
-    const unsigned low = (unsigned)w, old = atomicAdd(halves + 2 * bin, low), high = (unsigned)(w >> 32) + (old + low < old);
+    const unsigned high = (unsigned)((w + atomicAdd(halves + 2 * bin, (unsigned)w)) >> 32);
     if (high) atomicAdd(halves + 2 * bin + 1, high);
   };
   // The key at which the sum (of the weights above the border so far, or of ones) reaches `target`, and what lies above it.
@@ -662,16 +674,25 @@ sample_kernel(const SampleParams p, int ctas) {
   }
   if (nucleus) {
     const u64 each = of_border ? weight(smp_logit(border)) : 0;
+    const float border_logit = border ? smp_logit(border) : -INFINITY;
     clear();
     weight.either([&](auto slow) {
       slice.pass(s, p.status, [&](int i, const float* l) {
         u64 w[4];
-        int j[4];
+        int bin[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = weight.of<decltype(slow)::value>(l[e], j[e]);
+        for (int e = 0; e < 4; ++e) {
+          w[e] = weight.of<decltype(slow)::value>(l[e], bin[e], smp_above(l[e], border_logit));
+          bin[e] = weight.bin(bin[e]);
+        }
+        unsigned old[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (w[e] && (border == 0 || smp_key(l[e]) > border)) add_weight(weight.bin(j[e]), w[e]);
+        for (int e = 0; e < 4; ++e) old[e] = w[e] ? atomicAdd(halves + 2 * bin[e], (unsigned)w[e]) : 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned high = (unsigned)((w[e] + old[e]) >> 32);
+          if (high) atomicAdd(halves + 2 * bin[e] + 1, high);
+        }
       });
     });
     u64 want = 0;
@@ -730,15 +751,16 @@ sample_kernel(const SampleParams p, int ctas) {
     if (slice.kept && i + 4 <= min(to, slice.copied)) smp_load<L>(reinterpret_cast<const L*>(s.ring), i - slice.begin, to - slice.begin, 1, l);
     else if (i < to) smp_load<L>(slice.row, i, to, slice.vec && (from & 3) == 0, l);
   };
+  const float border_logit = border ? smp_logit(border) : -INFINITY;
   auto add = [&](auto slow, const float* l, u64& sum, unsigned& equal) {      // (-inf, behind the end, weighs nothing)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       int j;
-      const u64 w = weight.of<decltype(slow)::value>(l[e], j);
-      const unsigned key = border ? smp_key(l[e]) : 1;
-      sum += key > border ? w : 0;
-      equal += key == border;
+      sum += weight.of<decltype(slow)::value>(l[e], j, smp_above(l[e], border_logit));
     }
+    if (of_border)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) equal += smp_same(l[e], border_logit);
   };
   // A warp's part goes by blocks of 512, whose sums are kept (two for a lane, V / 16 / 512 of them at most).
   constexpr int BLOCK = 512, MOST = (1 << 18) / SMP_WARPS / BLOCK + 1;
@@ -760,7 +782,7 @@ sample_kernel(const SampleParams p, int ctas) {
 #pragma unroll
       for (int x = 0; x < 4; ++x) add(slow, l[x], mine, same);
       mine = smp_warp_sum(mine);
-      if (border) same = __reduce_add_sync(0xffffffffu, same);
+      if (of_border) same = __reduce_add_sync(0xffffffffu, same);
       sum += mine;
       equal += same;
       if (lane == 0) sums[k] = mine, ties[k] = same;
@@ -857,7 +879,7 @@ static int launch_sample(SampleParams p, cudaStream_t stream) {
   }
   // CTAs to a row: as many as leave all rows under way at once, with 2048 logits or more to a CTA.  A GPC's SMs bound what clusters fit:
   // 16 rows of 16 CTAs or 37 of 8 do not, though the SMs hold 296 CTAs.  us, by this rule / with twice the CTAs, rows of 128256: 16 rows,
-  // 50 largest 24 / 32, nucleus 51 / 63; 37 rows, 30 / 39, 82 / 89; 64 rows, 31 / 55, 84 / 108.  Rows with settings of their own take
+  // 50 largest 24 / 32, nucleus 50 / 63; 37 rows, 30 / 39, 82 / 89; 64 rows, 31 / 55, 82 / 108.  Rows with settings of their own take
   // unequal times, a nucleus of a flat distribution ten times a greedy row's: two waves of clusters even that out (256 rows of 102400:
   // 114 us, by the rule of the others 156, with four 122).
   const int waves = p.temperature || p.top_k || p.top_p || p.min_p ? 2 : 1;
