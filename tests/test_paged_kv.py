@@ -213,6 +213,17 @@ def test_paged_generation(dtype):
   assert all(0 <= t < cfg.vocab_size for o in generate(eng, prompts, 4, -5, 1.0, g, top_p=0.9, min_p=0.01) for t in o)
 
 
+def test_generation_that_the_pages_do_not_suffice_for_gives_them_back():
+  from torchprime_b200.experimental.deepseek_inference.engine import DeepseekInferenceEngine
+  from torchprime_b200.experimental.deepseek_inference.generate import generate
+  _, model = _tiny()
+  eng = DeepseekInferenceEngine(model, 2, 32, "paged", page_size=4, num_pages=3)
+  with pytest.raises(RuntimeError, match="full"):
+    generate(eng, [[5, 9, 17, 3], [7, 2]], max_new_tokens=9, eos_id=-5, temperature=0.0)
+  assert sorted(eng._free) == [0, 1, 2]
+  assert len(generate(eng, [[5, 9, 17, 3]], max_new_tokens=7, eos_id=-5, temperature=0.0)[0]) == 7
+
+
 def test_filters_with_the_other_caches():
   from torchprime_b200.experimental.deepseek_inference.engine import DeepseekInferenceEngine
   from torchprime_b200.experimental.deepseek_inference.generate import generate

@@ -79,15 +79,17 @@ def _generate_paged(engine, prompt_tokens, max_new_tokens, eos_id, draw):
   most = [min(max_new_tokens, engine.max_seq_len - k) for k in lens]
   out = [[] for _ in range(n)]
   rows = [i for i in range(n) if most[i] > 0]
-  if rows:
-    nxt = draw(torch.cat([engine.forward(torch.tensor([prompt_tokens[i]]), 0, rows=[i]) for i in rows]))
-  while rows:
-    for i, t in zip(rows, nxt.tolist()):
-      out[i].append(t)
-    rows = [i for i in rows if out[i][-1] != eos_id and len(out[i]) < most[i]]
+  try:
     if rows:
-      nxt = draw(engine.forward(torch.tensor([[out[i][-1]] for i in rows]), [lens[i] + len(out[i]) - 1 for i in rows], rows=rows))
-  engine.release(range(n))
+      nxt = draw(torch.cat([engine.forward(torch.tensor([prompt_tokens[i]]), 0, rows=[i]) for i in rows]))
+    while rows:
+      for i, t in zip(rows, nxt.tolist()):
+        out[i].append(t)
+      rows = [i for i in rows if out[i][-1] != eos_id and len(out[i]) < most[i]]
+      if rows:
+        nxt = draw(engine.forward(torch.tensor([[out[i][-1]] for i in rows]), [lens[i] + len(out[i]) - 1 for i in rows], rows=rows))
+  finally:                    # (where the pages do not suffice, too)
+    engine.release(range(min(n, engine.max_batch_size)))
   return [_cut(row, eos_id) for row in out]
 
 
