@@ -18,7 +18,7 @@
 //   for as soon as it has used a stage up, across the borders of sequences.
 // * Scores and weighted sums are mma.sync m16n8k16: the query heads of a key head are its 16 rows.  (A tcgen05 tile would be
 //   seven eighths empty, and its operands would still come through shared memory once.)  Statistics and sums are fp32; the
-//   weights of the sum are rounded to the operand type of the product, half a step of 2^-9 (bf16) or 2^-12 (f16) each, to
+//   weights of the sum are rounded to the operand type of the product, by up to 2^-8 (bf16) or 2^-11 (f16) of each, to
 //   either side, against a result that is rounded to bf16 itself; the sum of the weights is not rounded.
 // * An e4m3 cache is turned into f16 in registers, exactly; queries become f16 with a power of two for each head that puts the
 //   largest at 2^14 (f16 has more bits than bf16; what falls below 2^-38 of the largest is lost).  The keys' powers of two
@@ -131,6 +131,13 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
+}
+
+// To 2^-19 of itself: below 1/8, where the other form cancels, by its series (the next term is below 2^-29 of it).
+__device__ __forceinline__ float pd_tanh(float x) {
+  const float x2 = x * x, small = fmaf(fmaf(fmaf(x2, -17.f / 315, 2.f / 15), x2, -1.f / 3) * x2, x, x);
+  const float large = 1.f - __fdividef(2.f, ex2_approx(x * 2.8853900817779268f) + 1.f);
+  return fabsf(x) < 0.125f ? small : large;
 }
 
 // What is visible of a sequence, in tokens and in steps.
@@ -324,6 +331,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 
   const int g = lane >> 2, t = lane & 3;
   constexpr int NT = WIDE ? 2 : 1;         // blocks of eight query heads
+  constexpr int F16_UP = 15;               // f16 weights are 2^15 times as large: of a long sequence's small ones those from 2^-39 on count
   int done = 0, seg = 0, h0 = 0, rows = 0;
   // Of heads 8 nt + 2t and the one after: columns 16 c + (0 .. 15), two of them to a lane (see column()), maxima and sums.
   float o[NT][DV / 16][4], m[NT][2], l[NT][2];
@@ -447,13 +455,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
           __syncwarp();
         }
         float s[MT][NT][4] = {};
-        float factor[MT][2], add[MT][2];     // e4m3: powers of two of the keys, exponents of the values
+        float factor[MT][2], add[MT][2];     // e4m3: powers of two of the keys, exponents of the values and F16_UP (so m, too)
         if constexpr (F8) {
           const uint8_t* sc = scales + stage * T::SCALES;
 #pragma unroll
           for (int x = 0; x < 2 * MT; ++x) {
             factor[x >> 1][x & 1] = __int_as_float((int)sc[x * 8 + g] << 23);
-            add[x >> 1][x & 1] = (float)((int)sc[KEYS + x * 8 + g] - 127);
+            add[x >> 1][x & 1] = (float)((int)sc[KEYS + x * 8 + g] - 127 + F16_UP);
           }
         }
         // ---- scores, transposed: 16 tokens by 8 heads each; s[mt][nt] = (token g: heads 2t, 2t + 1; token g + 8: the same)
@@ -501,7 +509,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 #pragma unroll
               for (int x = 0; x < 2; ++x) {
                 float v = s[mt][nt][2 * hi + x] * (F8 ? qs[nt][x] * factor[mt][hi] : qs[nt][x]);
-                if (p.cap_log2 > 0.f) v = p.cap_log2 * (1.f - __fdividef(2.f, ex2_approx(v / p.cap_log2 * 2.8853900817779268f) + 1.f));
+                if (p.cap_log2 > 0.f) v = p.cap_log2 * pd_tanh(v / p.cap_log2);
                 v = dead ? -INFINITY : v;
                 s[mt][nt][2 * hi + x] = v;
                 top[nt][x] = fmaxf(top[nt][x], F8 ? v + add[mt][hi] : v);
@@ -537,7 +545,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         for (int nt = 0; nt < NT; ++nt) {
           float from[2];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) from[x] = m[nt][x] == -INFINITY ? 0.f : m[nt][x];      // (all scores so far are NaN or -inf)
+          for (int x = 0; x < 2; ++x) from[x] = m[nt][x] == -INFINITY ? 0.f : F8 ? m[nt][x] - F16_UP : m[nt][x];      // (all scores so far are NaN or -inf)
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -593,11 +601,18 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 
     // ---- the result, or this warp's part of it
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], off);
+      if constexpr (F8) {
+#pragma unroll
+        for (int cb = 0; cb < DV / 16; ++cb)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[nt][cb][x] *= 1.f / (1 << F16_UP);
+      }
+    }
     const bool starts = c.at == 0, ends = c.at + seg == c.s.steps;
     done += seg;
     if (starts && ends) {

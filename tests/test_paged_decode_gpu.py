@@ -158,6 +158,52 @@ def test_values_whose_sizes_differ_by_far(cuda_lib):
   _check(paged_kv.decode_attention(q, c, table, lens), q, c, table, lens)
 
 
+def _check_scores(got, q, c, table, lengths, scale, softcap=0.0):
+  """Within: half a step of bf16 on the result; half a step of bf16 or f16 on every weight; 2^-19 of their size on scores, capped or
+  not, and 2^-20 on exponentials and sums."""
+  for i, n in enumerate(lengths.tolist()):
+    pos = torch.arange(n, device=q.device)
+    k, v = _held(c, table[i].long()[pos // c.page] * c.page + pos % c.page)
+    q1 = q[i].double().view(k.shape[1], -1, q.shape[2])
+    s = torch.einsum("hgd,shd->hgs", q1, k) * scale
+    size = torch.einsum("hgd,shd->hgs", q1.abs(), k.abs()).amax(-1, keepdim=True) * scale
+    p = (softcap * torch.tanh(s / softcap) if softcap else s).softmax(-1)
+    o, a = torch.einsum("hgs,shd->hgd", p, v), torch.einsum("hgs,shd->hgd", p, v.abs())
+    tol = 2.0 ** -8 * o.abs() + a * ((2.0 ** -11 if c.k.dtype == E4M3 else 2.0 ** -8) + 2.0 ** -19 * (2 * size + 2))
+    off = (got[i].double().view(o.shape) - o).abs()
+    assert bool((off <= tol).all()), (i, n, (off / tol).max().item())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("lens", [[30000], [900, 17]])
+def test_many_small_weights_count(cuda_lib, dtype, lens):
+  """A first token that outweighs each of the others 2^26 times, but holds nothing."""
+  q, c, table, lengths = _problem(lens, 4, 1, 64, 64, 64, dtype)
+  q.zero_()[:, :, 0] = 1
+  first = table[:, 0].long() * 64
+  every = torch.cat([table[i].long()[(r := torch.arange(n, device="cuda")) // 64] * 64 + r % 64 for i, n in enumerate(lens)])
+  k = torch.zeros(every.numel(), 1, 64, device="cuda").bfloat16()
+  v = torch.rand(every.numel(), 1, 64, device="cuda").bfloat16() + 1
+  begins = torch.isin(every, first)
+  k[begins, 0, 0] = 26
+  v[begins] = 0
+  paged_kv.append(c, k, v, every)
+  scale = 0.6931471805599453
+  _check_scores(paged_kv.decode_attention(q, c, table, lengths, scale=scale), q, c, table, lengths, scale)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("softcap", [1.0, 50.0, 3e4, 1e7])
+def test_caps_far_above_the_scores(cuda_lib, dtype, softcap):
+  p = _problem([700, 33], 8, 2, 128, 128, 32, dtype, seed=3)
+  _check_scores(paged_kv.decode_attention(*p, scale=0.3, softcap=softcap), *p, 0.3, softcap)
+
+
+def test_a_window_beyond_32_bits_is_none(cuda_lib):
+  p = _problem([700, 33], 8, 2, 128, 128, 32, torch.bfloat16)
+  assert torch.equal(paged_kv.decode_attention(*p, window=(1 << 32) + 5), paged_kv.decode_attention(*p))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
 @pytest.mark.parametrize("size", [0.0, 2.0 ** -60, 2.0 ** 30])
 def test_queries_of_any_size(cuda_lib, dtype, size):

@@ -167,7 +167,8 @@ def decode_attention(q, cache: PagedKV, block_table, lengths, scale=None, window
   ``softcap`` makes scores ``softcap * tanh(score / softcap)``.  Returns [B, Hq, Dv] in q's type; a sequence of no token gives zeros.
 
   The kernel takes bf16 queries, pools of bf16 or e4m3 whose pages are multiples of 16 tokens, and heads of 128, 192 / 128 or
-  64 columns.  It reads nothing of the table and of the pages behind a sequence's last token (what a page holds there may be
+  64 columns; sequences x key heads x the tokens that a row of the table can name may come to 2^35 (2^36 of 128 columns in all and
+  fewer).  It reads nothing of the table and of the pages behind a sequence's last token (what a page holds there may be
   anything); a page outside the pool counts as zeros, a length beyond the table as the whole table, a negative one as none, and all three are
   reported (``_lib.raise_on_device_timeout``)."""
   if not _debug.bounds_enabled() and (nat := functional._native()) is not None:
@@ -200,7 +201,7 @@ def decode_attention(q, cache: PagedKV, block_table, lengths, scale=None, window
       scratch = torch.empty(n, dtype=torch.uint8, device=q.device)
       rc = lib().tpb_paged_decode(ptr(q), q.stride(0), q.stride(1), ptr(cache.k), ptr(cache.v), ptr(cache.k_scale), ptr(cache.v_scale),
                                   _c_strides(cache), ptr(block_table), block_table.stride(0), width, ptr(lengths), ptr(out),
-                                  ptr(scratch), b, hkv, hq // hkv, dk, dv, pages, page, window, scale, softcap, stream_ptr())
+                                  ptr(scratch), b, hkv, hq // hkv, dk, dv, pages, page, min(window, 2 ** 31 - 1), scale, softcap, stream_ptr())
     check(rc, f"paged_decode q{tuple(q.shape)} pool{tuple(cache.k.shape)}")
     return out
   return ref.paged_attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, lengths, scale, window, softcap)
