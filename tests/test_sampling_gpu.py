@@ -81,6 +81,18 @@ def test_settings_for_each_row(cuda_lib):
   _same(x, u, temperature=(i % 5).float() * 0.4, top_k=((i % 7) * 700).int(), top_p=0.5 + (i % 6).float() * 0.1, min_p=(i % 3).float() * 0.03)
 
 
+@pytest.mark.parametrize("b", [17, 300, 512, 513])
+def test_rows_of_unequal_work(cuda_lib, b):
+  """Some rows take all their logits, some a few, some one; their order in the batch is no order of the work."""
+  g = torch.Generator(device="cuda").manual_seed(b)
+  x, u = _logits(g, b, 9001, "few values"), torch.rand(b, generator=g, device="cuda")
+  i = torch.randperm(b, generator=g, device="cuda")
+  kw = dict(temperature=torch.where(i % 4 == 0, 0.0, 0.9), top_k=torch.where(i % 3 == 0, 0, i % 9000 + 1).int(),
+            top_p=torch.where(i % 5 == 0, 1.0, 0.93))
+  _same(x, u, **kw)
+  _same(x, u, **kw, min_p=torch.where(i % 2 == 0, 0.0, 0.2))
+
+
 @pytest.mark.parametrize("kind", ["huge", "tiny", "normal"])
 def test_extreme_logits(cuda_lib, kind):
   g = torch.Generator(device="cuda").manual_seed(8)
