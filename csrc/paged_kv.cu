@@ -29,10 +29,22 @@ struct PagedRows {
 constexpr int PAGED_THREADS = 256;
 constexpr int PAGED_ROWS = 4;        // sets of rows per warp under way together
 
-// The larger magnitude of each 16-bit half among finite bf16 values, as bits.
-__device__ __forceinline__ uint32_t finite_max(uint32_t m, uint32_t v) {
+// The larger magnitude of each 16-bit half, as bits; FINITE: among finite bf16 values.
+template <bool FINITE>
+__device__ __forceinline__ uint32_t max_of(uint32_t m, uint32_t v) {
   v &= 0x7fff7fffu;
-  return __vmaxu2(m, v & __vcmpltu2(v, 0x7f807f80u));
+  return __vmaxu2(m, FINITE ? v & __vcmpltu2(v, 0x7f807f80u) : v);
+}
+// Of all values of a row, which LANES lanes hold.
+template <bool FINITE, int LANES, int V>
+__device__ __forceinline__ uint32_t row_max(const uint4* d) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    m = max_of<FINITE>(max_of<FINITE>(max_of<FINITE>(max_of<FINITE>(m, d[j].x), d[j].y), d[j].z), d[j].w);
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return max(m & 0xffffu, m >> 16);
 }
 // Exponent e of a row whose largest finite magnitude has these bf16 bits; 448 = 1.75 * 2^8.
 __device__ __forceinline__ int row_exponent(uint32_t amax) {
@@ -106,12 +118,8 @@ paged_rows_kernel(PagedRows k, PagedRows v, const long long* __restrict__ slots,
 #pragma unroll
   for (int i = 0; i < PAGED_ROWS; ++i) {
     if (WRITE && HELD8) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int j = 0; j < V; ++j) m = finite_max(finite_max(finite_max(finite_max(m, d[i][j].x), d[i][j].y), d[i][j].z), d[i][j].w);
-      m = max(m & 0xffffu, m >> 16);
-#pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      uint32_t m = row_max<false, LANES, V>(d[i]);
+      if (__any_sync(0xffffffffu, m >= 0x7f80u)) m = row_max<true, LANES, V>(d[i]);      // (an infinity or NaN)
       if (at[i] == nullptr) continue;
       const int e = row_exponent(m);
       const float f = __int_as_float((127 - e) << 23);

@@ -19,6 +19,7 @@
 
 #include <atomic>
 #include <cmath>
+#include <cstdlib>
 #include <optional>
 
 #include "tpb.h"
@@ -1052,6 +1053,12 @@ py::object grouped_mlp_few_rows(py::handle x_, py::handle rw_, py::handle idx_, 
   return py::cast(y);
 }
 
+// The checks of indices on the host are on: the Python definitions do them.
+bool bounds_checked() {
+  const char* v = std::getenv("TPB_DEBUG_BOUNDS");
+  return v && v[0] == '1' && !v[1];
+}
+
 // The pools of a paged cache and, where they are e4m3, their scales: layouts that the kernels take, on the current device; see
 // paged_kv.PagedKV.
 struct Pools {
@@ -1107,7 +1114,7 @@ bool slots_of(const Pools& c, py::handle h, Tensor& slots) {
 py::object paged_append(py::handle k_, py::handle v_, py::handle ks_, py::handle vs_, py::handle xk_, py::handle xv_, py::handle slots_) {
   Pools c;
   Tensor xk, xv, slots;
-  if (!unobserved() || !c.take(k_, v_, ks_, vs_) || !unpack(xk_, xk) || !unpack(xv_, xv) || !slots_of(c, slots_, slots) ||
+  if (bounds_checked() || !unobserved() || !c.take(k_, v_, ks_, vs_) || !unpack(xk_, xk) || !unpack(xv_, xv) || !slots_of(c, slots_, slots) ||
       !c.rows(xk, slots.size(0), c.dk) || !c.rows(xv, slots.size(0), c.dv))
     return py::none();
   {
@@ -1119,7 +1126,7 @@ py::object paged_append(py::handle k_, py::handle v_, py::handle ks_, py::handle
 py::object paged_read(py::handle k_, py::handle v_, py::handle ks_, py::handle vs_, py::handle slots_) {
   Pools c;
   Tensor xk, xv, slots;
-  if (!unobserved() || !c.take(k_, v_, ks_, vs_) || !slots_of(c, slots_, slots)) return py::none();
+  if (bounds_checked() || !unobserved() || !c.take(k_, v_, ks_, vs_) || !slots_of(c, slots_, slots)) return py::none();
   {
     py::gil_scoped_release nogil;
     xk = empty_like_type(c.k, {slots.size(0), c.heads, c.dk}, at::kBFloat16);
@@ -1136,8 +1143,9 @@ py::object paged_decode(py::handle q_, py::handle k_, py::handle v_, py::handle 
   Tensor q, table, lens, out;
   double scale, softcap;
   int64_t window;
-  if (!whole(window_, 0, window) || !real(softcap_, 0.0, softcap) || !unobserved() || !unpack(q_, q) || !plain(q) || q.dim() != 3 || !c.take(k_, v_, ks_, vs_) || !unpack(table_, table) ||
-      !unpack(lens_, lens) || (at::GradMode::is_enabled() && recording(q)) || !real(scale_, 1.0 / std::sqrt((double)q.size(2)), scale))
+  if (bounds_checked() || !whole(window_, 0, window) || !real(softcap_, 0.0, softcap) || !unobserved() || !unpack(q_, q) || !plain(q) ||
+      q.dim() != 3 || !c.take(k_, v_, ks_, vs_) || !unpack(table_, table) || !unpack(lens_, lens) ||
+      (at::GradMode::is_enabled() && recording(q)) || !real(scale_, 1.0 / std::sqrt((double)q.size(2)), scale))
     return py::none();
   const int64_t b = q.size(0), hq = q.size(1);
   if (b < 1 || b > (1 << 24) || hq < 1 || hq > 65535 || hq % c.heads || q.size(2) != c.dk || c.pages < 1 || c.page % 16 ||

@@ -108,7 +108,7 @@ def append(cache: PagedKV, k, v, slots):
   """Writes keys [T, H, Dk] and values [T, H, Dv] to the rows ``slots`` [T] (int64) of the cache, quantised where it is
   e4m3; a token of slot -1 (padding) is not written, and neither is one whose slot lies outside the pool, which the kernel
   reports (``_lib.raise_on_device_timeout``).  No slot may come twice: which of its tokens a row of it holds is not defined."""
-  if not _debug.bounds_enabled() and (nat := functional._native()) is not None and nat.paged_append(*cache, k, v, slots):
+  if (nat := functional._native()) is not None and nat.paged_append(*cache, k, v, slots):
     return
   _check_cache(cache)
   _check_slots("paged_append", cache, slots)
@@ -133,7 +133,7 @@ def append(cache: PagedKV, k, v, slots):
 def read(cache: PagedKV, slots, dtype=torch.bfloat16):
   """The rows ``slots`` [T] of the cache as (keys [T, H, Dk], values [T, H, Dv]) of ``dtype``; zeros for slot -1 and, reported as in
   :func:`append`, for slots outside the pool."""
-  if dtype == torch.bfloat16 and not _debug.bounds_enabled() and (nat := functional._native()) is not None:
+  if dtype == torch.bfloat16 and (nat := functional._native()) is not None:
     rows = nat.paged_read(*cache, slots)
     if rows is not None:
       return rows
@@ -171,7 +171,7 @@ def decode_attention(q, cache: PagedKV, block_table, lengths, scale=None, window
   fewer).  It reads nothing of the table and of the pages behind a sequence's last token (what a page holds there may be
   anything); a page outside the pool counts as zeros, a length beyond the table as the whole table, a negative one as none, and all three are
   reported (``_lib.raise_on_device_timeout``)."""
-  if not _debug.bounds_enabled() and (nat := functional._native()) is not None:
+  if (nat := functional._native()) is not None:
     o = nat.paged_decode(q, *cache, block_table, lengths, scale, window, softcap)
     if o is not None:
       return o
