@@ -27,7 +27,8 @@ struct PagedRows {
 };
 
 constexpr int PAGED_THREADS = 256;
-constexpr int PAGED_ROWS = 4;        // sets of rows per warp under way together
+// Sets of rows per warp under way together.  (2 / 4 / 8: 30011 tokens of 8 heads to e4m3 40 / 36 / 36 us, a read in bf16 66 / 53 / 62.)
+constexpr int PAGED_ROWS = 4;
 
 // The larger magnitude of each 16-bit half, as bits; FINITE: among finite bf16 values.
 template <bool FINITE>
@@ -63,7 +64,7 @@ paged_rows_kernel(PagedRows k, PagedRows v, const long long* __restrict__ slots,
   const int per_warp = 32 / LANES, lane = threadIdx.x & 31, in_row = lane % LANES;
   const unsigned warp = blockIdx.x * (PAGED_THREADS / 32) + (threadIdx.x >> 5);
   // A lane finds a row's places for the lanes that move it.  (Every lane for its own rows: 50 us instead of 41 for 30011 tokens of 8
-  // heads to e4m3, bound by those instructions.)
+  // heads to e4m3.  Eight tokens of one head to a warp, which lie together, instead of eight heads of one token: 37 instead of 36.)
   const unsigned r = warp * (per_warp * PAGED_ROWS) + lane, t = r / H, h = r - t * H;      // (rows < 2^31)
   const bool live = lane < per_warp * PAGED_ROWS && r < rows;
   __nv_bfloat16* const my_x = live ? p.x + (long long)t * p.x_token + (long long)h * p.x_head : nullptr;
