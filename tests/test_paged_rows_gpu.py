@@ -138,3 +138,19 @@ def test_captured_step_on_a_side_stream(cuda_lib):
     graph.replay()
     assert bool((out[0] == i + 1).all()) and bool((out[1] == i + 1).all())
   assert bool((paged_kv.read(c, torch.tensor([5, 6, 7], device="cuda"))[0][:, 0, 0] == torch.tensor([1.0, 2, 3], device="cuda")).all())
+
+
+def test_debug_mode_is_asked_at_every_call(cuda_lib, monkeypatch):
+  c = PagedKV.allocate(2, 16, 1, 64, 64, device="cuda")
+  k, slots = torch.ones(2, 1, 64, device="cuda").bfloat16(), torch.tensor([3, 3], device="cuda")
+  paged_kv.append(c, k, k, slots)
+  monkeypatch.setenv("TPB_DEBUG_BOUNDS", "1")
+  with pytest.raises(IndexError, match="twice"):
+    paged_kv.append(c, k, k, slots)
+  with pytest.raises(IndexError, match="slots"):
+    paged_kv.read(c, slots + 40)
+  with pytest.raises(IndexError, match="lengths"):
+    paged_kv.decode_attention(torch.ones(1, 1, 64, device="cuda").bfloat16(), c, torch.zeros(1, 1, dtype=torch.int32, device="cuda"),
+                              torch.tensor([17], dtype=torch.int32, device="cuda"))
+  monkeypatch.delenv("TPB_DEBUG_BOUNDS")
+  paged_kv.append(c, k, k, slots)
