@@ -7,8 +7,10 @@
 // move the values within their steps and not the steps, and a row that was read back and written again is the same.  Scale
 // bytes are e + 127, the form of e8m0.
 //
-// Both directions are bound by memory: every value is moved once.  A row is held by 8 to 32 lanes, 16 bytes each, and a warp
-// takes four sets of rows at once so that their loads are all in flight.
+// Both directions are bound by memory: every value is moved once.  A row is held by 4 to 32 lanes, two or three 16-byte vectors
+// each, and a warp takes four sets of rows at once so that their loads are all in flight.  (One vector to a lane, with twice the lanes:
+// finding places and the largest value cost twice as many instructions for a byte, 30011 tokens of 8 heads of 128 to e4m3 36 us instead
+// of 30, 20000 of 16 of 192 / 128 82 instead of 50, at the memory's rate 28 and 47.)
 
 #include "common.cuh"
 #include "tpb.h"
@@ -27,7 +29,7 @@ struct PagedRows {
 };
 
 constexpr int PAGED_THREADS = 256;
-// Sets of rows per warp under way together.  (2 / 4 / 8: 30011 tokens of 8 heads to e4m3 40 / 36 / 36 us, a read in bf16 66 / 53 / 62.)
+// Sets of rows per warp under way together.  (2 / 4: 30011 tokens of 8 heads to e4m3 33 / 31 us.)
 constexpr int PAGED_ROWS = 4;
 
 // The larger magnitude of each 16-bit half, as bits; FINITE: among finite bf16 values.
@@ -56,7 +58,7 @@ __device__ __forceinline__ int row_exponent(uint32_t amax) {
 // LANES lanes hold a row, V 16-byte vectors of bf16 each.  Grid y: keys, values.
 // WRITE: x -> pool, else pool -> x.  HELD8: the pool is e4m3.
 template <int LANES, int V, bool WRITE, bool HELD8>
-__global__ void __launch_bounds__(PAGED_THREADS)
+__global__ void __launch_bounds__(PAGED_THREADS, V > 2 ? 3 : 4)
 paged_rows_kernel(PagedRows k, PagedRows v, const long long* __restrict__ slots, unsigned rows, unsigned H, unsigned page,
                   long long n_slots, int* st) {
   if (!chain_begin()) return;
@@ -200,7 +202,8 @@ extern "C" int tpb_paged_rows(int write, void* k, void* v, void* k_pool, void* v
   const int most = Dk > Dv ? Dk : Dv;
   const long long n_slots = (long long)pages * page;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  auto* launch = most <= 64 ? launch_paged_rows<8, 1> : most <= 128 ? launch_paged_rows<16, 1> : most <= 256 ? launch_paged_rows<32, 1> : launch_paged_rows<32, 2>;
+  auto* launch = most <= 64 ? launch_paged_rows<4, 2> : most <= 128 ? launch_paged_rows<8, 2>
+                                            : most <= 192 ? launch_paged_rows<8, 3> : most <= 256 ? launch_paged_rows<16, 2> : launch_paged_rows<32, 2>;
   launch(r[0], r[1], slots, (unsigned)(T * H), H, page, n_slots, write != 0, held8, stream);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 1000 + (int)e;
