@@ -9,6 +9,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/TracerMode.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAStream.h>
@@ -1053,6 +1054,11 @@ py::object grouped_mlp_few_rows(py::handle x_, py::handle rw_, py::handle idx_, 
   return py::cast(y);
 }
 
+// Memory on t's device, for operators that record nothing: straight from the allocator, ahead of every dispatch.
+Tensor fresh(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::detail::empty_cuda(sizes, type, t.device(), std::nullopt);
+}
+
 // The checks of indices on the host are on: the Python definitions do them.
 bool bounds_checked() {
   const char* v = std::getenv("TPB_DEBUG_BOUNDS");
@@ -1129,8 +1135,8 @@ py::object paged_read(py::handle k_, py::handle v_, py::handle ks_, py::handle v
   if (bounds_checked() || !unobserved() || !c.take(k_, v_, ks_, vs_) || !slots_of(c, slots_, slots)) return py::none();
   {
     py::gil_scoped_release nogil;
-    xk = empty_like_type(c.k, {slots.size(0), c.heads, c.dk}, at::kBFloat16);
-    xv = empty_like_type(c.k, {slots.size(0), c.heads, c.dv}, at::kBFloat16);
+    xk = fresh(c.k, {slots.size(0), c.heads, c.dk}, at::kBFloat16);
+    xv = fresh(c.k, {slots.size(0), c.heads, c.dv}, at::kBFloat16);
     c.move(false, xk, xv, slots);
   }
   return py::make_tuple(xk, xv);
@@ -1165,9 +1171,9 @@ py::object paged_decode(py::handle q_, py::handle k_, py::handle v_, py::handle 
   if (width * c.page > 0x7fffff00) return py::none();
   {
     py::gil_scoped_release nogil;
-    out = empty_as(q, {b, hq, c.dv});
+    out = fresh(q, {b, hq, c.dv}, at::kBFloat16);
     const int g = (int)(hq / c.heads);
-    Tensor scratch = empty_like_type(
+    Tensor scratch = fresh(
         q, {tpb_paged_decode_scratch((int)b, (int)c.heads, g, (int)c.dk, (int)c.dv, c.held8, (int)(width * c.page))}, at::kByte);
     check(tpb_paged_decode(cptr(q), q.stride(0), q.stride(1), cptr(c.k), cptr(c.v), cptr(c.ks), cptr(c.vs), c.strides, iptr(table),
                            table.stride(0), (int)width, iptr(lens), mptr(out), mptr(scratch), (int)b, (int)c.heads, g, (int)c.dk,
@@ -1205,7 +1211,7 @@ py::object sample_tokens(py::handle x_, py::handle u_, py::handle t_, py::handle
   }
   {
     py::gil_scoped_release nogil;
-    out = empty_like_type(x, {b}, at::kLong);
+    out = fresh(x, {b}, at::kLong);
     check(tpb_sample_tokens(cptr(x), x.scalar_type() == at::kBFloat16, x.stride(0), static_cast<const float*>(cptr(u)),
                             static_cast<const float*>(cptr(each[0])), iptr(each[1]), static_cast<const float*>(cptr(each[2])),
                             static_cast<const float*>(cptr(each[3])), number[0], (int)number[1], number[2], number[3],

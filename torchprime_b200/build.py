@@ -79,7 +79,7 @@ def _build_torch_ops(path: str) -> None:
          os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
   cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in inc), OPS_SRC, "-o", path,
-         f"-L{LIB_DIR}", "-ltpb200", f"-L{os.path.join(root, 'lib')}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
+         f"-L{LIB_DIR}", "-ltpb200", f"-L{os.path.join(root, 'lib')}", "-lc10", "-lc10_cuda", "-ltorch_cuda", "-ltorch_cpu", "-ltorch",
          "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
   res = subprocess.run(cmd, capture_output=True, text=True)
   if res.returncode != 0:
