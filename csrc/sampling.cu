@@ -61,7 +61,9 @@ struct SampleParams {
   const float *temperature, *top_p, *min_p;      // one a row, or null: the numbers below
   const int* top_k;
   double temperature0, top_p0, min_p0;
-  int top_k0, B, V, slice;                       // slice: logits of a CTA, a multiple of 8
+  int top_k0, B, V, slice;                       // slice: logits of a CTA of several, a multiple of 8
+  int unequal, whole;                            // rows take unequal times; of them, how many take a whole cluster, the others a CTA each
+                                                 // (0: every row takes a cluster)
   long long* out;
   int vec;                                       // rows can be read four logits at a time: 2, also by bulk copies (16-byte aligned)
   int* status;
@@ -246,34 +248,40 @@ __device__ __forceinline__ u64 smp_block_before(u64 v, u64* part) {
   return before;
 }
 
-// All threads of the cluster, which come together warp by warp first (the cluster's barrier is the aligned one).
-__device__ __forceinline__ void smp_cluster_sync() {
-  __syncthreads();
-  cluster_sync_all();
-}
+// The CTAs that share a row: a cluster, or one CTA of it.
+struct SmpGroup {
+  int first, rank, ctas;
+  template <typename T>
+  __device__ __forceinline__ T* peer(T* p, int of) const { return smp_peer(p, first + of); }
+  // All threads, which come together warp by warp first (the cluster's barrier is the aligned one).
+  __device__ __forceinline__ void sync() const {
+    __syncthreads();
+    if (ctas > 1) cluster_sync_all();
+  }
+};
 
 // Every CTA's s.sums, added up, from the last bin down: the bin in which the sum reaches target(sum of all), in s.found; the
 // sum of all alone where that is more.  (s.list and s.weight are used.)
 template <typename F>
-__device__ __forceinline__ void smp_find(SmpShared& s, int rank, int ctas, F&& target) {
-  const int per = SMP_BINS / ctas, b0 = rank * per, tid = threadIdx.x;
+__device__ __forceinline__ void smp_find(SmpShared& s, const SmpGroup& group, F&& target) {
+  const int rank = group.rank, ctas = group.ctas, per = SMP_BINS / ctas, b0 = rank * per, tid = threadIdx.x;
   const u64* total = s.sums;
   if (ctas > 1) {                       // each CTA adds up its share of the bins, for all
-    smp_cluster_sync();
+    group.sync();
     const int groups = max(1, min(SMP_THREADS / per, ctas));
     for (int x = tid; x < per * groups; x += SMP_THREADS) {
       u64 sum = 0;
 #pragma unroll 4
-      for (int c = x / per; c < ctas; c += groups) sum += smp_peer(s.sums, c)[b0 + x % per];
+      for (int c = x / per; c < ctas; c += groups) sum += group.peer(s.sums, c)[b0 + x % per];
       s.weight[x] = sum;
     }
     __syncthreads();
     for (int x = tid; x < per * ctas; x += SMP_THREADS) {
       u64 sum = 0;
       for (int g = 0; g < groups; ++g) sum += s.weight[g * per + x % per];
-      smp_peer(s.list, x / per)[b0 + x % per] = sum;
+      group.peer(s.list, x / per)[b0 + x % per] = sum;
     }
-    smp_cluster_sync();
+    group.sync();
     total = s.list;
   } else {
     __syncthreads();
@@ -456,9 +464,9 @@ __global__ void __launch_bounds__(SMP_THREADS, 1024 / SMP_THREADS)
 sample_kernel(const SampleParams p, int ctas) {
   extern __shared__ __align__(128) uint8_t smp_smem[];
   SmpShared& s = *reinterpret_cast<SmpShared*>(smp_smem);
-  const int rank = ctas > 1 ? (int)cluster_ctarank() : 0, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid < SMP_RING) mbar_init(&s.full[tid], 1);
-  if (tid == 0) s.dead = 0;
+  if (tid == 0) s.dead = 0, s.row = -1;
   fence_barrier_init();
   __syncthreads();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // (nobody writes to a CTA that has not begun)
@@ -466,26 +474,33 @@ sample_kernel(const SampleParams p, int ctas) {
   if (!chain_wait()) return;
   const int V = p.V;
   int b = blockIdx.x / ctas;
-  if ((p.temperature || p.top_k || p.min_p) && p.B <= SMP_THREADS) {
-    // Rows whose sums take all their logits come first: they take longest.  (256 rows of 102400, settings of their own, one in
-    // seventeen of that kind: 114 us instead of 123.)
-    const int k = tid < p.B && p.top_k ? p.top_k[tid] : p.top_k0;
-    const bool here = tid < p.B, long_ = here && (p.temperature ? (double)p.temperature[tid] : p.temperature0) > 0.0 && (k <= 0 || k >= V) &&
-                                         !((p.min_p ? (double)p.min_p[tid] : p.min_p0) > 0.0);
-    const unsigned longs = __ballot_sync(0xffffffffu, long_), before = (1u << lane) - 1;
-    if (lane == 0) s.warp[warp] = __popc(longs);
-    __syncthreads();
-    int at = 0, all = 0;
-    for (int w = 0; w < SMP_WARPS; ++w) {
-      if (w < warp) at += (int)s.warp[w];
-      all += (int)s.warp[w];
+  SmpGroup group = {0, ctas > 1 ? (int)cluster_ctarank() : 0, ctas};
+  if (p.unequal) {
+    // Rows whose sums take all their logits come first, and get the whole clusters that there are: they take longest.  The rows are
+    // numbered thread by thread, those rows and then the others.  (In the batch's order: 123 us instead of 114 where all take two CTAs.)
+    auto is_long = [&](int i) {
+      const int k = p.top_k ? p.top_k[i] : p.top_k0;
+      return (p.temperature ? (double)p.temperature[i] : p.temperature0) > 0.0 && (k <= 0 || k >= V) &&
+             !((p.min_p ? (double)p.min_p[i] : p.min_p0) > 0.0);
+    };
+    int mine = 0, longs = 0;
+    for (int i = tid; i < p.B; i += SMP_THREADS) mine += is_long(i);
+    int at_long = (int)smp_block_before(mine, s.warp), at_short = tid * (p.B / SMP_THREADS) + min(tid, p.B % SMP_THREADS) - at_long;
+    for (int w = 0; w < SMP_WARPS; ++w) longs += (int)s.warp[w];
+    const int whole = p.whole ? min(longs, p.whole) : p.B;
+    if (b >= whole) {
+      b = whole + (b - whole) * ctas + group.rank;
+      group = {group.rank, 0, 1};
     }
-    at += __popc(longs & before);
-    if (here && (long_ ? at : all + tid - at) == b) s.row = tid;
+    for (int i = tid; i < p.B; i += SMP_THREADS)
+      if ((is_long(i) ? at_long++ : longs + at_short++) == b) s.row = i;
     __syncthreads();
     b = s.row;
+    if (b < 0) return;                            // (more CTAs than rows)
   }
-  SmpSlice<L> slice = {static_cast<const L*>(p.logits) + b * p.stride, min(V, rank * p.slice), min(V, (rank + 1) * p.slice), p.vec};
+  ctas = group.ctas;
+  const int rank = group.rank, per_cta = ctas > 1 ? p.slice : V;
+  SmpSlice<L> slice = {static_cast<const L*>(p.logits) + b * p.stride, min(V, rank * per_cta), min(V, (rank + 1) * per_cta), p.vec};
   slice.copied = slice.end - (slice.end - slice.begin) % (16 / (int)sizeof(L));
   const double T = p.temperature ? (double)p.temperature[b] : p.temperature0;
   double top_p = p.top_p ? (double)p.top_p[b] : p.top_p0, min_p = p.min_p ? (double)p.min_p[b] : p.min_p0;
@@ -532,9 +547,9 @@ sample_kernel(const SampleParams p, int ctas) {
   if (tid < ctas) {
     u64 best = 0;
     for (int w = 0; w < SMP_WARPS; ++w) best = max(best, s.warp[w]);
-    smp_peer(s.tot2, tid)[rank] = best;
+    group.peer(s.tot2, tid)[rank] = best;
   }
-  smp_cluster_sync();
+  group.sync();
   u64 best = 0;
   for (int c = 0; c < ctas; ++c) best = max(best, s.tot2[c]);
   const float top = smp_logit((unsigned)(best >> 32));
@@ -565,17 +580,17 @@ sample_kernel(const SampleParams p, int ctas) {
       }
     });
     __syncthreads();
-    if (tid < ctas) smp_peer(s.tot, tid)[rank] = s.staged;
-    smp_cluster_sync();
+    if (tid < ctas) group.peer(s.tot, tid)[rank] = s.staged;
+    group.sync();
     u64 n = 0, base = 0;
     for (int c = 0; c < ctas; ++c) {
       if (c == rank) base = n;
       n += s.tot[c];
     }
-    u64* const list = smp_peer(s.list, 0);
+    u64* const list = group.peer(s.list, 0);
     if (n <= SMP_CAP)
       for (unsigned i = tid; i < s.staged; i += SMP_THREADS) list[base + i] = s.weight[i];
-    smp_cluster_sync();
+    group.sync();
     return n;
   };
 
@@ -595,7 +610,7 @@ sample_kernel(const SampleParams p, int ctas) {
     unsigned from = least_key;
     bool few = true;
     if (top_k) {
-      smp_find(s, rank, ctas, [&](u64 all) { return min((u64)top_k, all + 1); });
+      smp_find(s, group, [&](u64 all) { return min((u64)top_k, all + 1); });
       if (s.found[2] >= (u64)top_k) from = max(from, (unsigned)s.found[0] << 21);
       else few = min_p > 0.0 || V <= SMP_CAP;
     }
@@ -657,7 +672,7 @@ sample_kernel(const SampleParams p, int ctas) {
           else if (key > border) add_weight(bin, weight(l[e]));
         }
       });
-      smp_find(s, rank, ctas, [&](u64 all) { return min(target - above, all); });
+      smp_find(s, group, [&](u64 all) { return min(target - above, all); });
       key_so_far |= (unsigned)s.found[0] << shift;
       above += s.found[1];
       if (shift == 0) return key_so_far;
@@ -696,7 +711,7 @@ sample_kernel(const SampleParams p, int ctas) {
       });
     });
     u64 want = 0;
-    smp_find(s, rank, ctas, [&](u64 all) {
+    smp_find(s, group, [&](u64 all) {
       want = max(__double2ull_ru(top_p * (double)(all + each * of_border)), 1ULL);
       if (!each) want = min(want, all);
       return want;
@@ -727,10 +742,10 @@ sample_kernel(const SampleParams p, int ctas) {
               const unsigned key = (unsigned)(s.list[i] >> 32);
               int of = 1;
               while (of <= i && (unsigned)(s.list[i - of] >> 32) == key) ++of;
-              for (int c = 0; c < ctas; ++c) *smp_peer(&s.border, c) = key, *smp_peer(&s.of_border, c) = of;
+              for (int c = 0; c < ctas; ++c) *group.peer(&s.border, c) = key, *group.peer(&s.of_border, c) = of;
             }
         }
-        smp_cluster_sync();
+        group.sync();
         border = s.border;
         of_border = s.of_border;
       } else {
@@ -794,10 +809,10 @@ sample_kernel(const SampleParams p, int ctas) {
   if (tid < ctas) {
     u64 x = 0, y = 0;
     for (int w = 0; w < SMP_WARPS; ++w) x += s.warp[w], y += s.warp2[w];
-    smp_peer(s.tot, tid)[rank] = x;
-    smp_peer(s.tot2, tid)[rank] = y;
+    group.peer(s.tot, tid)[rank] = x;
+    group.peer(s.tot2, tid)[rank] = y;
   }
-  smp_cluster_sync();
+  group.sync();
   auto upto = [&](u64 x, u64 y) { return x + each * min(y, of_border); };
   u64 x = 0, y = 0;
   for (int c = 0; c < ctas; ++c) x += s.tot[c], y += s.tot2[c];
@@ -879,19 +894,29 @@ static int launch_sample(SampleParams p, cudaStream_t stream) {
   }
   // CTAs to a row: as many as leave all rows under way at once, with 2048 logits or more to a CTA.  A GPC's SMs bound what clusters fit:
   // 16 rows of 16 CTAs or 37 of 8 do not, though the SMs hold 296 CTAs.  us, by this rule / with twice the CTAs, rows of 128256: 16 rows,
-  // 50 largest 24 / 32, nucleus 50 / 63; 37 rows, 30 / 39, 82 / 89; 64 rows, 31 / 55, 82 / 108.  Rows with settings of their own take
-  // unequal times, a nucleus of a flat distribution ten times a greedy row's: two waves of clusters even that out (256 rows of 102400:
-  // 114 us, by the rule of the others 156, with four 122).
-  const int waves = p.temperature || p.top_k || p.top_p || p.min_p ? 2 : 1;
-  int ctas = 1;
-  while (e == cudaSuccess && ctas < 16 && p.V / (ctas * 2) >= 2048) {
+  // 50 largest 24 / 32, nucleus 50 / 63; 37 rows, 30 / 39, 82 / 89; 64 rows, 31 / 55, 82 / 108.
+  // Rows with settings of their own take unequal times, a nucleus of a flat distribution ten times a greedy row's.  Two waves of
+  // clusters even that out a little (256 rows of 102400, one in seventeen of the long kind, 114 us, one wave 156).  Where the batch nearly
+  // fills the SMs with a CTA to a row, long rows take clusters of four and the others a CTA each: that mix 88 us instead of 111, 256 rows of
+  // 128256 50 largest 58 instead of 83, but a nucleus for every row 297 instead of 254; the mix with 128 rows of 128256 114 instead of 85.
+  auto fit = [&](int n) {
     int most = 0;
-    e = sample_clusters<L>(device, ctas * 2, &most);
-    if (p.B > (long long)waves * most) break;
-    ctas *= 2;
+    if (e == cudaSuccess) e = sample_clusters<L>(device, n, &most);
+    return (long long)most;
+  };
+  p.unequal = p.temperature || p.top_k || p.min_p;
+  int ctas = 1;
+  long long clusters = p.B;
+  const long long pairs = p.unequal && p.V >= 4 * 2048 ? fit(2) : 0;
+  if (3 * p.B > 4 * pairs && p.B <= 4 * pairs) {
+    ctas = 4;
+    p.whole = (int)min(max(fit(4), 1LL), (long long)p.B);
+    clusters = p.whole + (p.B - p.whole + ctas - 1) / ctas;
+  } else {
+    while (ctas < 16 && p.V / (ctas * 2) >= 2048 && p.B <= (p.unequal ? 2 : 1) * fit(ctas * 2)) ctas *= 2;
   }
   p.slice = ((p.V + ctas - 1) / ctas + 7) / 8 * 8;
-  if (e == cudaSuccess) e = chain_clusters(f, ctas, dim3(p.B * ctas), SMP_THREADS, sizeof(SmpShared), stream, p, ctas);
+  if (e == cudaSuccess) e = chain_clusters(f, ctas, dim3((unsigned)(clusters * ctas)), SMP_THREADS, sizeof(SmpShared), stream, p, ctas);
   const cudaError_t last = cudaGetLastError();
   if (e == cudaSuccess) e = last;
   return e == cudaSuccess ? 0 : 1000 + (int)e;
@@ -912,7 +937,7 @@ extern "C" int tpb_sample_tokens(const void* logits, int bf16, long long stride,
   if (B > (0x7fffffff >> 4)) return -2;
   const int elt = bf16 ? 2 : 4;
   SampleParams p = {logits, stride, u, temperature, top_p, min_p, top_k, temperature0, top_p0, min_p0, top_k0, B, V,
-                    0, out, 0, status_block()};
+                    0, 0, 0, out, 0, status_block()};
   p.vec = (reinterpret_cast<uintptr_t>(logits) % (4 * elt) == 0 && stride % 4 == 0) +
           (reinterpret_cast<uintptr_t>(logits) % 16 == 0 && stride * elt % 16 == 0);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
