@@ -15,7 +15,8 @@
 // rows there are.  A slice comes through a ring of bulk copies, or stays in it where it fits.
 //   * The first pass finds m.
 //   * top-k: the k-th largest of the threads' own largest logits is a lower bound of the k-th largest of all; min-p has a bound of its
-//     own.  The logits from the bound on, usually little more than k, go to one CTA, which sorts them and finishes alone.
+//     own.  The logits from the bound on, usually little more than k, go to one CTA, which sorts them and finishes alone.  A long slice
+//     with a small k has them staged by the first pass.
 //   * nucleus: a histogram of the weights over their exponents in steps of 1/64; the bin with the border goes to one CTA, which
 //     sorts it.  Then two more passes draw the token: sums of slices and of the parts of their warps, and along one of those.
 //   * Where a list is too long for one CTA (thousands of equal logits, large k) the border is found bit by bit of the order.
@@ -203,12 +204,13 @@ struct SmpShared {
   u64 table[SMP_TABLE];
   u64 warp[SMP_WARPS], warp2[SMP_WARPS];
   u64 tot[16], tot2[16];                // of the cluster's CTAs
+  unsigned bounds[16];                  // the same: all that belongs to the list is staged from there on; 0: it is not
   uint64_t full[SMP_RING];              // barriers of the copies
   u64 found[3];                         // bin, sum of the bins above, sum of all
   unsigned border, of_border;
   unsigned range[2];                    // of keys
   int row;
-  unsigned staged;                      // of this CTA's part of the list
+  unsigned staged, listed;              // tokens of this CTA that may belong to the list, and that do
   int dead;                             // a copy has not come
 };
 
@@ -400,9 +402,15 @@ struct SmpSlice {
                    : "r"(smem_u32(reinterpret_cast<L*>(s.ring) + slot * SMP_CHUNK)), "l"(row + at), "r"(n), "r"(smem_u32(&s.full[slot]))
                    : "memory");
   }
+  __device__ __forceinline__ bool streams() const { return vec == 2 && end - begin > SMP_RING * SMP_CHUNK; }
   // f(index, four logits) for all of them; -inf stands behind the end of the row
   template <typename F>
   __device__ __forceinline__ void pass(SmpShared& s, int* status, F&& f) {
+    pass(s, status, f, [](int, auto&&) {});
+  }
+  // Where it streams, between(chunk, sweep) follows each chunk, and sweep(g) goes over that chunk again.
+  template <typename F, typename G>
+  __device__ __forceinline__ void pass(SmpShared& s, int* status, F&& f, G&& between) {
     const int chunks = (end - begin + SMP_CHUNK - 1) / SMP_CHUNK, tid = threadIdx.x;
     if (vec < 2) {
       for (int i0 = begin; i0 < end; i0 += SMP_CHUNK) {
@@ -435,20 +443,24 @@ struct SmpSlice {
       }
       const L* ring = reinterpret_cast<const L*>(s.ring) + slot * SMP_CHUNK;
       const int at = begin + c * SMP_CHUNK;
-      if (at + SMP_CHUNK <= copied) {
-        float l[2][4];
+      auto sweep = [&](auto&& g) {
+        if (at + SMP_CHUNK <= copied) {
+          float l[2][4];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) smp_load<L>(ring, (x * SMP_THREADS + tid) * 4, SMP_CHUNK, 1, l[x]);
+          for (int x = 0; x < 2; ++x) smp_load<L>(ring, (x * SMP_THREADS + tid) * 4, SMP_CHUNK, 1, l[x]);
 #pragma unroll
-        for (int x = 0; x < 2; ++x) f(at + (x * SMP_THREADS + tid) * 4, l[x]);
-      } else {
-        for (int in = tid * 4; at + in < end && in < SMP_CHUNK; in += SMP_THREADS * 4) {
-          float l[4];
-          if (at + in + 4 <= copied) smp_load<L>(ring, in, SMP_CHUNK, 1, l);
-          else smp_load<L>(row, at + in, end, 0, l);
-          f(at + in, l);
+          for (int x = 0; x < 2; ++x) g(at + (x * SMP_THREADS + tid) * 4, l[x]);
+        } else {
+          for (int in = tid * 4; at + in < end && in < SMP_CHUNK; in += SMP_THREADS * 4) {
+            float l[4];
+            if (at + in + 4 <= copied) smp_load<L>(ring, in, SMP_CHUNK, 1, l);
+            else smp_load<L>(row, at + in, end, 0, l);
+            g(at + in, l);
+          }
         }
-      }
+      };
+      sweep(f);
+      between(c, sweep);
       if (!kept && chunks > SMP_RING) {
         __syncthreads();
         if (tid == 0 && alive && c + SMP_RING < chunks) copy(s, c + SMP_RING);
@@ -522,10 +534,49 @@ sample_kernel(const SampleParams p, int ctas) {
   // ---- the largest logit and its first index
   unsigned top_key = 0;
   int at = V;
-  slice.pass(s, p.status, [&](int i, const float* l) {
+  auto largest = [&](int i, const float* l) {
     const unsigned key = smp_key(smp_max4(l));
     if (key > top_key) top_key = key, at = i;
-  });
+    return key;
+  };
+  auto stage = [&](int i, const float* l, unsigned least, unsigned past) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const unsigned key = smp_key(l[e]);
+      if (key - least < past - least) {
+        const unsigned x = atomicAdd(&s.staged, 1u);
+        if (x < SMP_CAP) s.weight[x] = (u64)key << 32 | (0xffffffffu - (unsigned)(i + e));
+      }
+    }
+  };
+  // Where few are kept of a slice that would have to be read from memory again, candidates for the list are staged at once: as many
+  // threads as top_k have seen a logit from `bound` on so far.  (50 largest, with a pass of its own for the list / without: 256 rows of
+  // 102400 48 / 41 us, 512 of 128256 109 / 88.  With more than a fourth of the threads that bound is low, and so is min_p of the largest
+  // logit so far: 60 / 62 for 256 rows with that alone.)
+  const bool streams = !greedy && top_k > 0 && top_k <= SMP_THREADS / 4 && slice.streams();
+  unsigned bound = SMP_LOWEST + 1;
+  if (!streams) {
+    slice.pass(s, p.status, largest);
+  } else {
+    if (tid == 0) s.staged = 0;
+    __syncthreads();
+    slice.pass(
+        s, p.status,
+        [&](int i, const float* l) {
+          if (largest(i, l) >= bound && i >= slice.begin + SMP_CHUNK) stage(i, l, bound, 0xffffffffu);
+        },
+        [&](int chunk, auto&& sweep) {
+          if (chunk & (chunk + 1)) return;        // 0, 1, 3, 7, ...
+          unsigned seen = 0;                      // the key that enough threads have seen, but for its last 14 bits
+          for (int bit = 31; bit >= 14; --bit)
+            if (__syncthreads_count(top_key >= (seen | 1u << bit)) >= top_k) seen |= 1u << bit;
+          bound = max(bound, seen);
+          if (chunk == 0)
+            sweep([&](int i, const float* l) {
+              if (smp_key(smp_max4(l)) >= bound) stage(i, l, bound, 0xffffffffu);
+            });
+        });
+  }
   if (greedy && at < V) {                         // which of the four
     float l[4];
     smp_load<L>(slice.row, at, slice.end, 0, l);
@@ -548,10 +599,20 @@ sample_kernel(const SampleParams p, int ctas) {
     u64 best = 0;
     for (int w = 0; w < SMP_WARPS; ++w) best = max(best, s.warp[w]);
     group.peer(s.tot2, tid)[rank] = best;
+    group.peer(s.bounds, tid)[rank] = streams && s.staged <= SMP_CAP ? bound : 0;
   }
   group.sync();
   u64 best = 0;
   for (int c = 0; c < ctas; ++c) best = max(best, s.tot2[c]);
+  unsigned staged_from = 0;                       // all candidates from this key on are staged: 0, they are not
+  if (streams) {
+    bool all = true;
+    for (int c = 0; c < ctas; ++c) {
+      all &= s.bounds[c] > 0;
+      staged_from = max(staged_from, s.bounds[c]);
+    }
+    if (!all) staged_from = 0;
+  }
   const float top = smp_logit((unsigned)(best >> 32));
   at = V - (int)(unsigned)best;
   if (greedy || top == -INFINITY || s.dead) {
@@ -565,22 +626,28 @@ sample_kernel(const SampleParams p, int ctas) {
   };
   // Logits whose keys are from `least` on and below `past` go to the first CTA's list, by way of one in each CTA; the number of them, in
   // every CTA.
-  auto gather = [&](unsigned least, unsigned past) {
-    if (tid == 0) s.staged = 0;
+  auto gather = [&](unsigned least, unsigned past, bool staged) {
+    if (!staged) {
+      if (tid == 0) s.staged = 0;
+      __syncthreads();
+      slice.pass(s, p.status, [&](int i, const float* l) {
+        if (smp_key(smp_max4(l)) >= least) stage(i, l, least, past);
+      });
+    }
+    if (tid == 0) s.listed = 0;
     __syncthreads();
-    slice.pass(s, p.status, [&](int i, const float* l) {
-      if (smp_key(smp_max4(l)) < least) return;
+    constexpr int EACH = SMP_CAP / SMP_THREADS;
+    u64 mine[EACH];
+    unsigned place[EACH];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const unsigned key = smp_key(l[e]);
-        if (key - least < past - least) {
-          const unsigned x = atomicAdd(&s.staged, 1u);
-          if (x < SMP_CAP) s.weight[x] = (u64)key << 32 | (0xffffffffu - (unsigned)(i + e));
-        }
-      }
-    });
+    for (int x = 0; x < EACH; ++x) {
+      const unsigned i = x * SMP_THREADS + tid;
+      mine[x] = i < s.staged ? s.weight[i] : 0;
+      if (mine[x] >> 32 < least) mine[x] = 0;     // (staged from a lower bound)
+      if (mine[x]) place[x] = atomicAdd(&s.listed, 1u);
+    }
     __syncthreads();
-    if (tid < ctas) group.peer(s.tot, tid)[rank] = s.staged;
+    if (tid < ctas) group.peer(s.tot, tid)[rank] = s.staged > SMP_CAP ? s.staged : s.listed;
     group.sync();
     u64 n = 0, base = 0;
     for (int c = 0; c < ctas; ++c) {
@@ -588,8 +655,11 @@ sample_kernel(const SampleParams p, int ctas) {
       n += s.tot[c];
     }
     u64* const list = group.peer(s.list, 0);
-    if (n <= SMP_CAP)
-      for (unsigned i = tid; i < s.staged; i += SMP_THREADS) list[base + i] = s.weight[i];
+    if (n <= SMP_CAP) {
+#pragma unroll
+      for (int x = 0; x < EACH; ++x)
+        if (mine[x]) list[base + place[x]] = mine[x];
+    }
     group.sync();
     return n;
   };
@@ -609,12 +679,14 @@ sample_kernel(const SampleParams p, int ctas) {
   if (top_k || min_p > 0.0) {
     unsigned from = least_key;
     bool few = true;
-    if (top_k) {
+    if (staged_from) {
+      from = max(from, staged_from);
+    } else if (top_k) {
       smp_find(s, group, [&](u64 all) { return min((u64)top_k, all + 1); });
       if (s.found[2] >= (u64)top_k) from = max(from, (unsigned)s.found[0] << 21);
       else few = min_p > 0.0 || V <= SMP_CAP;
     }
-    const u64 n_list = few ? gather(from, 0xffffffffu) : SMP_CAP + 1;
+    const u64 n_list = few ? gather(from, 0xffffffffu, staged_from > 0) : SMP_CAP + 1;
     if (n_list <= SMP_CAP) {
       if (rank > 0) return;
       // ---- one CTA sorts them and finishes
@@ -729,7 +801,7 @@ sample_kernel(const SampleParams p, int ctas) {
         if (lane == 0) s.range[warp] = key;
       }
       __syncthreads();
-      const u64 n_list = gather(max(s.range[0], border + 1), s.range[1]);
+      const u64 n_list = gather(max(s.range[0], border + 1), s.range[1], false);
       if (n_list <= SMP_CAP) {
         if (rank == 0) {
           const int n = (int)n_list;

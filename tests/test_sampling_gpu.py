@@ -177,3 +177,22 @@ def test_empty_batch_and_wide_rows(cuda_lib):
   g = torch.Generator(device="cuda").manual_seed(14)
   x, u = _logits(g, 2, (1 << 18) + 3, "peaks"), torch.rand(2, generator=g, device="cuda")
   _same(x, u, top_p=0.9)                       # (more than the kernel takes: the definition)
+
+
+@pytest.mark.parametrize("order", ["random", "rising", "falling", "few finite", "equal"])
+@pytest.mark.parametrize("k", [1, 50, 128, 129])
+def test_long_slices_in_any_order(cuda_lib, order, k):
+  """So many rows that a CTA reads its slice in pieces: what the k largest may be is known better and better, or worst at first."""
+  g = torch.Generator(device="cuda").manual_seed(k)
+  b, v = 160, 40003
+  x, u = torch.randn(b, v, generator=g, device="cuda") * 2, torch.rand(b, generator=g, device="cuda")
+  if order in ("rising", "falling"):
+    x = x.sort(1, descending=order == "falling").values
+  elif order == "few finite":
+    x[torch.rand(b, v, generator=g, device="cuda") > 100 / v] = -math.inf
+  elif order == "equal":
+    x = x.round()
+  x = torch.nn.functional.pad(x, (0, 5))[:, :v]      # rows that bulk copies can take
+  _same(x, u, top_k=k, temperature=0.8)
+  _same(x, u, top_k=k, top_p=0.9, min_p=0.01)
+  _same(x.bfloat16(), u, top_k=k, top_p=0.9)
