@@ -627,6 +627,10 @@ sample_kernel(const SampleParams p, int ctas) {
   // Logits whose keys are from `least` on and below `past` go to the first CTA's list, by way of one in each CTA; the number of them, in
   // every CTA.
   auto gather = [&](unsigned least, unsigned past, bool staged) {
+    constexpr int EACH = SMP_CAP / SMP_THREADS;
+    u64 mine[EACH];
+    unsigned place[EACH];
+    if (tid == 0) s.listed = 0;
     if (!staged) {
       if (tid == 0) s.staged = 0;
       __syncthreads();
@@ -634,20 +638,21 @@ sample_kernel(const SampleParams p, int ctas) {
         if (smp_key(smp_max4(l)) >= least) stage(i, l, least, past);
       });
     }
-    if (tid == 0) s.listed = 0;
     __syncthreads();
-    constexpr int EACH = SMP_CAP / SMP_THREADS;
-    u64 mine[EACH];
-    unsigned place[EACH];
 #pragma unroll
     for (int x = 0; x < EACH; ++x) {
-      const unsigned i = x * SMP_THREADS + tid;
-      mine[x] = i < s.staged ? s.weight[i] : 0;
-      if (mine[x] >> 32 < least) mine[x] = 0;     // (staged from a lower bound)
-      if (mine[x]) place[x] = atomicAdd(&s.listed, 1u);
+      place[x] = x * SMP_THREADS + tid;
+      mine[x] = place[x] < s.staged ? s.weight[place[x]] : 0;
     }
-    __syncthreads();
-    if (tid < ctas) group.peer(s.tot, tid)[rank] = s.staged > SMP_CAP ? s.staged : s.listed;
+    if (staged) {                                 // from a lower bound
+#pragma unroll
+      for (int x = 0; x < EACH; ++x) {
+        if (mine[x] >> 32 < least) mine[x] = 0;
+        if (mine[x]) place[x] = atomicAdd(&s.listed, 1u);
+      }
+      __syncthreads();
+    }
+    if (tid < ctas) group.peer(s.tot, tid)[rank] = staged ? s.listed : s.staged;
     group.sync();
     u64 n = 0, base = 0;
     for (int c = 0; c < ctas; ++c) {
@@ -976,7 +981,7 @@ static int launch_sample(SampleParams p, cudaStream_t stream) {
     if (e == cudaSuccess) e = sample_clusters<L>(device, n, &most);
     return (long long)most;
   };
-  p.unequal = p.temperature || p.top_k || p.min_p;
+  p.unequal = (p.temperature || p.top_k || p.min_p) && p.B <= 1024;      // (each CTA looks at every row's settings)
   int ctas = 1;
   long long clusters = p.B;
   const long long pairs = p.unequal && p.V >= 4 * 2048 ? fit(2) : 0;

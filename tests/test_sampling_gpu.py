@@ -81,7 +81,7 @@ def test_settings_for_each_row(cuda_lib):
   _same(x, u, temperature=(i % 5).float() * 0.4, top_k=((i % 7) * 700).int(), top_p=0.5 + (i % 6).float() * 0.1, min_p=(i % 3).float() * 0.03)
 
 
-@pytest.mark.parametrize("b", [17, 100, 300, 513, 700])
+@pytest.mark.parametrize("b", [17, 100, 300, 513, 700, 1500])
 def test_rows_of_unequal_work(cuda_lib, b):
   """Some rows take all their logits, some a few, some one; their order in the batch is no order of the work."""
   g = torch.Generator(device="cuda").manual_seed(b)
