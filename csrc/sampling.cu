@@ -32,6 +32,7 @@ namespace tpb {
 constexpr int SMP_THREADS = 512, SMP_WARPS = SMP_THREADS / 32;      // (1024: one row's nucleus 36 -> 41 us)
 constexpr int SMP_BINS = 2048;          // 11 bits of the order at a time (31-21, 20-10, 9-0); 32 binary orders of weights in steps of 1/64
 constexpr int SMP_CAP = 2048;           // tokens that one CTA sorts
+constexpr int SMP_FEW = SMP_THREADS / 4;        // largest k whose candidates are found while a row is read
 constexpr int SMP_FIXED = 44;           // a weight of 1 is 2^44: 2^18 of them stay below 2^63
 constexpr int SMP_TABLE = 1024;         // 2^(j / 1024)
 constexpr int SMP_CHUNK = SMP_THREADS * 8, SMP_RING = 3;       // logits of a bulk copy, copies under way
@@ -488,24 +489,31 @@ sample_kernel(const SampleParams p, int ctas) {
   int b = blockIdx.x / ctas;
   SmpGroup group = {0, ctas > 1 ? (int)cluster_ctarank() : 0, ctas};
   if (p.unequal) {
-    // Rows whose sums take all their logits come first, and get the whole clusters that there are: they take longest.  The rows are
-    // numbered thread by thread, those rows and then the others.  (In the batch's order: 123 us instead of 114 where all take two CTAs.)
-    auto is_long = [&](int i) {
+    // Rows in order of how long they take: those whose sums take all their logits; those that may, with more tokens than a list holds;
+    // those with a small k; greedy ones.  The first two kinds get the whole clusters that there are.  Rows of a kind are numbered thread
+    // by thread, in quarters of 64 bits.  (In the batch's order: 123 us instead of 114 where all take two CTAs.)
+    auto kind = [&](int i) {
       const int k = p.top_k ? p.top_k[i] : p.top_k0;
-      return (p.temperature ? (double)p.temperature[i] : p.temperature0) > 0.0 && (k <= 0 || k >= V) &&
-             !((p.min_p ? (double)p.min_p[i] : p.min_p0) > 0.0);
+      if (!((p.temperature ? (double)p.temperature[i] : p.temperature0) > 0.0)) return 48;
+      if (k > 0 && k <= SMP_FEW) return 32;
+      return (k > 0 && k < V) || (p.min_p ? (double)p.min_p[i] : p.min_p0) > 0.0 ? 16 : 0;
     };
-    int mine = 0, longs = 0;
-    for (int i = tid; i < p.B; i += SMP_THREADS) mine += is_long(i);
-    int at_long = (int)smp_block_before(mine, s.warp), at_short = tid * (p.B / SMP_THREADS) + min(tid, p.B % SMP_THREADS) - at_long;
-    for (int w = 0; w < SMP_WARPS; ++w) longs += (int)s.warp[w];
-    const int whole = p.whole ? min(longs, p.whole) : p.B;
+    u64 mine = 0, all = 0;
+    for (int i = tid; i < p.B; i += SMP_THREADS) mine += 1ULL << kind(i);
+    u64 at = smp_block_before(mine, s.warp);
+    for (int w = 0; w < SMP_WARPS; ++w) all += s.warp[w];
+    const u64 begins = (all << 16) + (all << 32) + (all << 48);
+    at += begins;
+    const int whole = p.whole ? min((int)(begins >> 32 & 0xffff), p.whole) : p.B;
     if (b >= whole) {
       b = whole + (b - whole) * ctas + group.rank;
       group = {group.rank, 0, 1};
     }
-    for (int i = tid; i < p.B; i += SMP_THREADS)
-      if ((is_long(i) ? at_long++ : longs + at_short++) == b) s.row = i;
+    for (int i = tid; i < p.B; i += SMP_THREADS) {
+      const int of = kind(i);
+      if ((int)(at >> of & 0xffff) == b) s.row = i;
+      at += 1ULL << of;
+    }
     __syncthreads();
     b = s.row;
     if (b < 0) return;                            // (more CTAs than rows)
@@ -553,7 +561,7 @@ sample_kernel(const SampleParams p, int ctas) {
   // threads as top_k have seen a logit from `bound` on so far.  (50 largest, with a pass of its own for the list / without: 256 rows of
   // 102400 48 / 41 us, 512 of 128256 109 / 88.  With more than a fourth of the threads that bound is low, and so is min_p of the largest
   // logit so far: 60 / 62 for 256 rows with that alone.)
-  const bool streams = !greedy && top_k > 0 && top_k <= SMP_THREADS / 4 && slice.streams();
+  const bool streams = !greedy && top_k > 0 && top_k <= SMP_FEW && slice.streams();
   unsigned bound = SMP_LOWEST + 1;
   if (!streams) {
     slice.pass(s, p.status, largest);
