@@ -981,9 +981,11 @@ static int launch_sample(SampleParams p, cudaStream_t stream) {
   // 16 rows of 16 CTAs or 37 of 8 do not, though the SMs hold 296 CTAs.  us, by this rule / with twice the CTAs, rows of 128256: 16 rows,
   // 50 largest 24 / 32, nucleus 50 / 63; 37 rows, 30 / 39, 82 / 89; 64 rows, 31 / 55, 82 / 108.
   // Rows with settings of their own take unequal times, a nucleus of a flat distribution ten times a greedy row's.  Two waves of
-  // clusters even that out a little (256 rows of 102400, one in seventeen of the long kind, 114 us, one wave 156).  Where the batch nearly
-  // fills the SMs with a CTA to a row, long rows take clusters of four and the others a CTA each: that mix 88 us instead of 111, 256 rows of
-  // 128256 50 largest 58 instead of 83, but a nucleus for every row 297 instead of 254; the mix with 128 rows of 128256 114 instead of 85.
+  // clusters even that out a little (256 rows of 102400, a third without a small k, some of them without a filter, 114 us, one wave 156).
+  // Where a batch fills the SMs with clusters of four, or with a CTA to a row, long rows take clusters of four and the others a CTA
+  // each.  us, such a mix, 50 largest, a nucleus for every row; that way and by waves, of 128256 logits:
+  //   64 rows 69 / 57, 45 / 59, 83 / 108;  192 rows 87 / 121, 47 / 61, 284 / 209;  256 rows 91 / 127, 47 / 83, 300 / 254;
+  //   and not 96 rows 72 / 72, 42 / 53, 218 / 132;  512 rows 198 / 193, 92 / 91, 522 / 444.
   auto fit = [&](int n) {
     int most = 0;
     if (e == cudaSuccess) e = sample_clusters<L>(device, n, &most);
@@ -992,8 +994,7 @@ static int launch_sample(SampleParams p, cudaStream_t stream) {
   p.unequal = (p.temperature || p.top_k || p.min_p) && p.B <= 1024;      // (each CTA looks at every row's settings)
   int ctas = 1;
   long long clusters = p.B;
-  const long long pairs = p.unequal && p.V >= 4 * 2048 ? fit(2) : 0;
-  if (3 * p.B > 4 * pairs && p.B <= 4 * pairs) {
+  if (p.unequal && p.V >= 4 * 2048 && p.B > fit(8) && p.B <= 3 * fit(2) && (p.B <= fit(4) || p.B > fit(2))) {
     ctas = 4;
     p.whole = (int)min(max(fit(4), 1LL), (long long)p.B);
     clusters = p.whole + (p.B - p.whole + ctas - 1) / ctas;
