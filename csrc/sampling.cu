@@ -204,7 +204,8 @@ struct SmpShared {
   u64 list[SMP_CAP], weight[SMP_CAP];
   u64 table[SMP_TABLE];
   u64 warp[SMP_WARPS], warp2[SMP_WARPS];
-  u64 tot[16], tot2[16];                // of the cluster's CTAs
+  u64 tops[16], tot[16], ties[16];      // of the cluster's CTAs: largest logits, sums, equal logits.  (Not one array for the first and the
+                                        // last: a row without a filter meets no barrier of the cluster between them)
   unsigned bounds[16];                  // the same: all that belongs to the list is staged from there on; 0: it is not
   uint64_t full[SMP_RING];              // barriers of the copies
   u64 found[3];                         // bin, sum of the bins above, sum of all
@@ -606,12 +607,12 @@ sample_kernel(const SampleParams p, int ctas) {
   if (tid < ctas) {
     u64 best = 0;
     for (int w = 0; w < SMP_WARPS; ++w) best = max(best, s.warp[w]);
-    group.peer(s.tot2, tid)[rank] = best;
+    group.peer(s.tops, tid)[rank] = best;
     group.peer(s.bounds, tid)[rank] = streams && s.staged <= SMP_CAP ? bound : 0;
   }
   group.sync();
   u64 best = 0;
-  for (int c = 0; c < ctas; ++c) best = max(best, s.tot2[c]);
+  for (int c = 0; c < ctas; ++c) best = max(best, s.tops[c]);
   unsigned staged_from = 0;                       // all candidates from this key on are staged: 0, they are not
   if (streams) {
     bool all = true;
@@ -895,15 +896,15 @@ sample_kernel(const SampleParams p, int ctas) {
     u64 x = 0, y = 0;
     for (int w = 0; w < SMP_WARPS; ++w) x += s.warp[w], y += s.warp2[w];
     group.peer(s.tot, tid)[rank] = x;
-    group.peer(s.tot2, tid)[rank] = y;
+    group.peer(s.ties, tid)[rank] = y;
   }
   group.sync();
   auto upto = [&](u64 x, u64 y) { return x + each * min(y, of_border); };
   u64 x = 0, y = 0;
-  for (int c = 0; c < ctas; ++c) x += s.tot[c], y += s.tot2[c];
+  for (int c = 0; c < ctas; ++c) x += s.tot[c], y += s.ties[c];
   const u64 target = place(upto(x, y));
   x = y = 0;
-  for (int c = 0; c < rank; ++c) x += s.tot[c], y += s.tot2[c];
+  for (int c = 0; c < rank; ++c) x += s.tot[c], y += s.ties[c];
   for (int w = 0; w < warp; ++w) x += s.warp[w], y += s.warp2[w];
   if (upto(x, y) > target || upto(x + sum, y + equal) <= target) return;
   int i0 = from;

@@ -128,6 +128,18 @@ def test_strided_rows(cuda_lib):
     _same(x, u[: x.shape[0]], temperature=2.5, top_k=30)
 
 
+@pytest.mark.parametrize("b,v", [(1, 32768), (1, 262144), (3, 40007), (16, 128256), (40, 8200), (70, 60000)])
+def test_rows_without_a_filter_over_and_over(cuda_lib, b, v):
+  """The CTAs of a row meet after the largest logits and then not before the sums: all of them work with the same largest logit,
+  however far apart they are (rows whose slices weigh nothing but for one, and slices of unequal length)."""
+  g = torch.Generator(device="cuda").manual_seed(v)
+  x, u = _logits(g, b, v, "peaks"), torch.rand(b, generator=g, device="cuda")
+  x[0, v // 2:] = -math.inf
+  want = ref.sample_tokens(x, u)
+  got = torch.stack([sample_tokens(x, u) for _ in range(200)])
+  assert bool((got == want).all())
+
+
 def test_settings_out_of_wider_tensors(cuda_lib):
   g = torch.Generator(device="cuda").manual_seed(15)
   x, u = _logits(g, 16, 9000, "peaks"), torch.rand(32, generator=g, device="cuda")[::2]
