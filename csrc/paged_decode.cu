@@ -82,6 +82,9 @@ struct PagedTile {
   static constexpr int WARPS = pd_shape(F8, WIDE, DK + DV).warps;
 };
 
+// Powers of two of 1, for the rows of pages that are not there.
+__device__ const uint8_t __align__(16) pd_ones[16] = {127, 127, 127, 127, 127, 127, 127, 127, 127, 127, 127, 127, 127, 127, 127, 127};
+
 __device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int row, int head, int page) {
   asm volatile(
       "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %3, %5, %6}], [%2];"
@@ -294,9 +297,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   auto ask = [&]() {
     uint64_t* bar = &bars[ask_stage];
     const bool inside = seen && pg >= 0 && pg < p.pages;
-    if (seen && !inside) report(p.status, kBadArgument, 72);      // a box outside the pool reads as zeros
-    const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, seen)) * (T::K_BOX + T::V_BOX) +
-                           (F8 ? __popc(__ballot_sync(0xffffffffu, inside)) * 32 : 0);
+    if (seen && !inside) report(p.status, kBadArgument, 72);      // a box outside the pool reads as zeros, of the size 1
+    const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, seen)) * (T::K_BOX + T::V_BOX + (F8 ? 32 : 0));
     if (lane == 0) mbar_expect_tx(bar, bytes);
     __syncwarp();
     if (seen) {
@@ -305,10 +307,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       fence_proxy_async();
       tma_load_page(at + lane * T::K_BOX, &k_map, bar, row, head, inside ? pg : -1);
       tma_load_page(at + MT * T::K_BOX + lane * T::V_BOX, &v_map, bar, row, head, inside ? pg : -1);
-      if (F8 && inside) {
+      if (F8) {
         const uint32_t sc = scales_at + ask_stage * T::SCALES + lane * 16;
-        bulk_load_16(sc, p.k_scale + pg * p.ks_page + head * p.ks_head + row, bar);
-        bulk_load_16(sc + KEYS, p.v_scale + pg * p.vs_page + head * p.vs_head + row, bar);
+        bulk_load_16(sc, inside ? p.k_scale + pg * p.ks_page + head * p.ks_head + row : pd_ones, bar);
+        bulk_load_16(sc + KEYS, inside ? p.v_scale + pg * p.vs_page + head * p.vs_head + row : pd_ones, bar);
       }
     }
     __syncwarp();

@@ -256,6 +256,31 @@ def test_pages_and_lengths_that_do_not_exist_are_reported(cuda_lib):
       assert not got[1].any() if bad_lens < 0 else bool(got[1].isfinite().all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("bad", [BAD, -1])
+@pytest.mark.parametrize("dims", [(8, 2, 128, 128), (32, 2, 128, 128), (4, 4, 192, 128), (12, 4, 64, 64)])
+def test_pages_outside_the_pool_count_as_zeros(cuda_lib, dtype, bad, dims):
+  """Whatever keys, values and powers of two the places held that such a page would have come to: every other sequence has the largest
+  values there are, and a warp has steps of several sequences."""
+  heads, kv_heads, dk, dv = dims
+  lens = [290, 130] * 500
+  q, c, table, lengths = _problem(lens, heads, kv_heads, dk, dv, 16, dtype)
+  pos = torch.arange(290, device="cuda")
+  slots = (table[::2].long()[:, pos // 16] * 16 + pos % 16).reshape(-1)
+  paged_kv.append(c, torch.zeros(slots.numel(), kv_heads, dk, device="cuda").bfloat16(),
+                  torch.full((slots.numel(), kv_heads, dv), 3e38, device="cuda").bfloat16(), slots)
+  good = paged_kv.decode_attention(q, c, table, lengths)
+  table[1::2, 2] = bad
+  table[1::4, 6:8] = bad
+  got = paged_kv.decode_attention(q, c, table, lengths)
+  torch.cuda.synchronize()
+  with pytest.raises(_lib.KernelError, match="bad argument"):
+    _lib.raise_on_device_timeout()
+  assert torch.equal(got[::2], good[::2])
+  few = list(range(1, 1000, 38))
+  _check(got[few], q[few], c, table[few], lengths[few])
+
+
 def test_streams_and_graphs_with_scratch_of_their_own(cuda_lib):
   """Two captured steps replayed on two streams at once, lengths and pages changing between replays."""
   problems = [_problem(ls, 8, 2, 128, 128, 16, dt, seed=i) for i, (ls, dt) in
