@@ -281,12 +281,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
   PagedCursor<KEYS> ahead = c;
   int asked = 0, ask_stage = 0, stage = 0, parity = 0;
   bool alive = true;
-  // A lane for each box.  The pages of the step that is asked for next are on their way from the table since the one before was.
+  // A lane for each box that holds a visible token: the pages in front of a window may have been given back.  The pages of the step
+  // that is asked for next are on their way from the table since the one before was.
   int pg = -1, row = 0;
   bool seen = false;
   auto look_up = [&]() {
     const int key = ahead.key0() + 16 * lane;
-    seen = lane < MT && key < ahead.s.len;
+    seen = lane < MT && key < ahead.s.len && key + 16 > ahead.s.lo;
     const unsigned at = (unsigned)key / (unsigned)p.page;
     row = key - at * p.page;
     if (seen) pg = p.table[ahead.b * p.table_b + at];

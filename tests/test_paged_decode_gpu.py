@@ -281,6 +281,25 @@ def test_pages_outside_the_pool_count_as_zeros(cuda_lib, dtype, bad, dims):
   _check(got[few], q[few], c, table[few], lengths[few])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("page", [16, 32, 48])
+@pytest.mark.parametrize("heads,kv_heads,dk,dv", [(8, 2, 128, 128), (12, 4, 64, 64), (32, 2, 64, 64)])
+@pytest.mark.parametrize("window", [1, 17, 40, 100])
+@pytest.mark.parametrize("bad", [BAD, -1])
+def test_pages_in_front_of_a_window_are_not_looked_at(cuda_lib, dtype, page, heads, kv_heads, dk, dv, window, bad):
+  """They may have been given back: nothing is reported, and the result is the same."""
+  lens = [1, 16, 63, 64, 65, 112, 129, 200, 333, 700]
+  q, c, table, lengths = _problem(lens, heads, kv_heads, dk, dv, page, dtype, seed=window)
+  want = paged_kv.decode_attention(q, c, table, lengths, window=window)
+  _check(want, q, c, table, lengths, window=window)
+  for i, n in enumerate(lens):
+    table[i, : max(0, n - window) // page] = bad
+  got = paged_kv.decode_attention(q, c, table, lengths, window=window)
+  torch.cuda.synchronize()
+  _lib.raise_on_device_timeout()
+  assert torch.equal(got, want)
+
+
 def test_streams_and_graphs_with_scratch_of_their_own(cuda_lib):
   """Two captured steps replayed on two streams at once, lengths and pages changing between replays."""
   problems = [_problem(ls, 8, 2, 128, 128, 16, dt, seed=i) for i, (ls, dt) in

@@ -167,10 +167,10 @@ def decode_attention(q, cache: PagedKV, block_table, lengths, scale=None, window
   ``softcap`` makes scores ``softcap * tanh(score / softcap)``.  Returns [B, Hq, Dv] in q's type; a sequence of no token gives zeros.
 
   The kernel takes bf16 queries, pools of bf16 or e4m3 whose pages are multiples of 16 tokens, and heads of 128, 192 / 128 or
-  64 columns; sequences x key heads x the tokens that a row of the table can name may come to 2^35 (2^36 of 128 columns in all and
-  fewer).  It reads nothing of the table and of the pages behind a sequence's last token (what a page holds there may be
-  anything); a page outside the pool counts as zeros, a length beyond the table as the whole table, a negative one as none, and all three are
-  reported (``_lib.raise_on_device_timeout``)."""
+  64 columns; sequences x key heads (one for each sixteen of its query heads) x the tokens that a row of the table can name may come to
+  2^35 (2^36 of 128 columns in all and fewer).  It looks only at entries of the table and pages that hold a visible token, and what a
+  page holds beside them may be anything; a page outside the pool counts as zeros, a length beyond the table as the whole table, a
+  negative one as none, and all three are reported (``_lib.raise_on_device_timeout``)."""
   if (nat := functional._native()) is not None:
     o = nat.paged_decode(q, *cache, block_table, lengths, scale, window, softcap)
     if o is not None:
