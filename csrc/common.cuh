@@ -547,6 +547,19 @@ __device__ __forceinline__ float2 from_e4m3x2(uint32_t v) {
   return f;
 }
 
+// The powers of two (or NaN) of two e8m0 bytes.  The smallest, 2^-127, is subnormal: mul_exact does not flush it.
+__device__ __forceinline__ void from_e8m0x2(uint32_t v, float& lo, float& hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.ue8m0x2 %0, %1;" : "=r"(r) : "h"((uint16_t)v));
+  lo = __uint_as_float(r << 16);
+  hi = __uint_as_float(r & 0xffff0000u);
+}
+__device__ __forceinline__ float mul_exact(float a, float b) {
+  float r;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // ---- packed fp32 pairs (sm_100: one FMA-pipe instruction works on two floats held in an aligned
 // 64-bit register pair), the three-input maximum and the bare MUFU exponential.  The softmax loops
 // of the attention kernels are bound by instruction issue, not by any one pipe; these halve the

@@ -23,8 +23,9 @@
 // * An e4m3 cache is turned into f16 in registers, exactly; queries become f16 with a power of two for each head that puts the
 //   largest at 2^14 (f16 has more bits than bf16; what falls below 2^-38 of the largest is lost).  The keys' powers of two
 //   multiply the scores, the values' are added to the exponent of the weights, so that no weight overflows: o = sum_i 2^(s_i + e_i
-//   - m) v_i / sum_i 2^(s_i - m) with m the maximum of s_i + e_i.  K's columns go to the product in another order than Q's would
-//   (four neighbouring bytes to a lane instead of two and two); the queries are loaded in the same one.
+//   - m) v_i / sum_i 2^(s_i - m) with m the maximum of s_i + max(e_i, -100), so that a token adds 2^100 at most to the
+//   lower sum.  K's columns go to the product in another order than Q's would (four neighbouring bytes to a lane instead of two and two);
+//   the queries are loaded in the same one.
 
 #include <atomic>
 
@@ -449,12 +450,15 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
       const bool edge = key0 < c.s.lo || key0 + KEYS > c.s.len;
       if (alive) {
         if (edge) {
-          // Rows behind the end (or in front of the window) hold anything, NaN too: zeros in the values, -inf in the scores.
+          // Rows behind the end (or in front of the window) hold anything, NaN too: zeros of the size 1 in the values, -inf in the scores.
           uint4* v = reinterpret_cast<uint4*>(ring + stage * T::STAGE + MT * T::K_BOX);
           for (int x = lane; x < MT * T::V_BOX / 16; x += 32) {
             const int key = key0 + x / (T::V_BOX / 16) * 16 + x % (T::BLOCK / 16) / (T::ROW / 16);
             if (key < c.s.lo || key >= c.s.len) v[x] = make_uint4(0, 0, 0, 0);
           }
+          if constexpr (F8)
+            for (int x = lane; x < KEYS; x += 32)
+              if (key0 + x < c.s.lo || key0 + x >= c.s.len) scales[stage * T::SCALES + KEYS + x] = 127;
           __syncwarp();
         }
         float s[MT][NT][4] = {};
@@ -462,9 +466,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
         if constexpr (F8) {
           const uint8_t* sc = scales + stage * T::SCALES;
 #pragma unroll
-          for (int x = 0; x < 2 * MT; ++x) {
-            factor[x >> 1][x & 1] = __int_as_float((int)sc[x * 8 + g] << 23);
-            add[x >> 1][x & 1] = (float)((int)sc[KEYS + x * 8 + g] - 127 + F16_UP);
+          for (int mt = 0; mt < MT; ++mt) {
+            from_e8m0x2(sc[mt * 16 + g] | (uint32_t)sc[mt * 16 + 8 + g] << 8, factor[mt][0], factor[mt][1]);
+#pragma unroll
+            for (int hi = 0; hi < 2; ++hi)       // (as a multiple of 2^104; 255, NaN: infinity, which makes all results NaN)
+              add[mt][hi] = fmaf(__uint_as_float(0x7f7fff01u + sc[KEYS + mt * 16 + hi * 8 + g]), 1.f / (1ULL << 52) / (1ULL << 52),
+                                 -(float)((1 << 24) - 255 + 127 - F16_UP));
           }
         }
         // ---- scores, transposed: 16 tokens by 8 heads each; s[mt][nt] = (token g: heads 2t, 2t + 1; token g + 8: the same)
@@ -507,15 +514,16 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
           for (int hi = 0; hi < 2; ++hi) {
             const int in = mt * 16 + hi * 8 + g;
             const bool dead = edge && (key0 + in < c.s.lo || key0 + in >= c.s.len);
+            const float up = F8 ? fmaxf(add[mt][hi], F16_UP - 100.f) : 0.f;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int x = 0; x < 2; ++x) {
-                float v = s[mt][nt][2 * hi + x] * (F8 ? qs[nt][x] * factor[mt][hi] : qs[nt][x]);
+                float v = s[mt][nt][2 * hi + x] * (F8 ? mul_exact(qs[nt][x], factor[mt][hi]) : qs[nt][x]);
                 if (p.cap_log2 > 0.f) v = p.cap_log2 * pd_tanh(v / p.cap_log2);
                 v = dead ? -INFINITY : v;
                 s[mt][nt][2 * hi + x] = v;
-                top[nt][x] = fmaxf(top[nt][x], F8 ? v + add[mt][hi] : v);
+                top[nt][x] = fmaxf(top[nt][x], F8 ? v + up : v);
               }
           }
         bool grown = false;

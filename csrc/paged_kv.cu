@@ -145,12 +145,13 @@ paged_rows_kernel(PagedRows k, PagedRows v, const long long* __restrict__ slots,
         if (c * 8 >= p.D) continue;
         uint4 o = d[i][j];
         if (!WRITE && HELD8) {
-          const float f = __int_as_float(d[i][j].z << 23);
+          float f, none;
+          from_e8m0x2(d[i][j].z, f, none);
           const float2 a = from_e4m3x2(d[i][j].x), b = from_e4m3x2(d[i][j].x >> 16), g = from_e4m3x2(d[i][j].y), h = from_e4m3x2(d[i][j].y >> 16);
-          o.x = pack_bf16(a.x * f, a.y * f);
-          o.y = pack_bf16(b.x * f, b.y * f);
-          o.z = pack_bf16(g.x * f, g.y * f);
-          o.w = pack_bf16(h.x * f, h.y * f);
+          o.x = pack_bf16(mul_exact(a.x, f), mul_exact(a.y, f));
+          o.y = pack_bf16(mul_exact(b.x, f), mul_exact(b.y, f));
+          o.z = pack_bf16(mul_exact(g.x, f), mul_exact(g.y, f));
+          o.w = pack_bf16(mul_exact(h.x, f), mul_exact(h.y, f));
         }
         reinterpret_cast<uint4*>(WRITE ? (void*)at[i] : (void*)x[i])[c] = o;
       }

@@ -223,6 +223,49 @@ def test_nan_of_a_visible_row_reaches_its_sequence_alone(cuda_lib, dtype):
   assert not got[0, :4].isnan().any() and not got[1].isnan().any()
 
 
+@pytest.mark.parametrize("dims", [(8, 2, 128, 128), (32, 2, 128, 128), (4, 4, 192, 128), (12, 4, 64, 64)])
+@pytest.mark.parametrize("lens", [[200, 130, 90, 77], [4000, 130, 900, 61]])
+def test_powers_of_two_at_the_ends_of_their_type(cuda_lib, dims, lens):
+  """A NaN for a power of two reaches its sequence and head, and no other from rows that cannot be seen; 2^-127 counts as that."""
+  heads, kv_heads, dk, dv = dims
+  q, c, table, lengths = _problem(lens, heads, kv_heads, dk, dv, 16, E4M3)
+  group = heads // kv_heads
+  good = paged_kv.decode_attention(q, c, table, lengths)
+  k8, v8 = c.k_scale.view(torch.uint8), c.v_scale.view(torch.uint8)
+  for i in range(4):
+    end = lens[i]                          # behind the last token, on its page
+    if end % 16:
+      page = table[i, end // 16].long()
+      for s in (k8, v8):
+        s[page, end % 16:] = 255
+  assert torch.equal(paged_kv.decode_attention(q, c, table, lengths), good)
+  k8[table[0, 3].long(), 5, 1] = 255
+  v8[table[1, 2].long(), 9, 0] = 255
+  got = paged_kv.decode_attention(q, c, table, lengths)
+  bad = torch.zeros(4, heads, dtype=torch.bool, device="cuda")
+  bad[0, group:2 * group] = True
+  bad[1, :group] = True
+  assert torch.equal(got.isnan().all(-1), bad) and torch.equal(got.isnan().any(-1), bad) and torch.equal(got[~bad], good[~bad])
+  # the smallest power of two, under keys that huge queries see, with values of the same, then of 1
+  q[2] = (q[2].float() * 2.0 ** 122).bfloat16()
+  pos = torch.arange(lens[2], device="cuda")
+  at = (table[2].long()[pos // 16], pos % 16)
+  k8[at] = 0
+  q1 = q[2].double().view(kv_heads, group, dk)
+  s = torch.einsum("hgd,shd->hgs", q1, c.k[at].float().double() * 2.0 ** -127) * 2.0 ** 3
+  size = torch.einsum("hgd,shd->hgs", q1.abs(), c.k[at].float().double().abs() * 2.0 ** -124).amax()
+  p = s.softmax(-1)
+  assert float(s.abs().max()) > 1
+  for byte in (0, 127):
+    v8[at] = byte
+    got = paged_kv.decode_attention(q[2:3], c, table[2:3], lengths[2:3], scale=2.0 ** 3)[0]
+    v = c.v[at].float().double() * 2.0 ** (byte - 127)
+    o, a = torch.einsum("hgs,shd->hgd", p, v).reshape(heads, dv), torch.einsum("hgs,shd->hgd", p, v.abs()).reshape(heads, dv)
+    # as in _check; results and terms below 2^-126 are flushed
+    tol = 2.0 ** -8 * o.abs() + a * (2.0 ** -11 + 2.0 ** -20 * (2 * size + 2)) + pos.numel() * 2.0 ** -25 * v.abs().max() + 2.0 ** -126
+    assert bool(((got.double() - o).abs() <= tol).all())
+
+
 def test_addresses_past_32_bits(cuda_lib):
   c = PagedKV.allocate(70000, 16, 16, 128, dtype=E4M3, device="cuda")        # 2.3e9 values a pool
   table = torch.tensor([[69999, 0, 69998], [35000, 69997, 1]], dtype=torch.int32, device="cuda")

@@ -17,6 +17,19 @@ def test_quantised_rows_take_the_smallest_power_of_two_that_fits():
   assert bool(((held - x).abs() <= torch.maximum(x.abs() * 2.0 ** -4, scale * 2.0 ** -10))[:5].all())
 
 
+def test_powers_of_two_are_those_of_their_type():
+  """All 256 bytes of e8m0, the ends too: 2^-127 and NaN."""
+  c = PagedKV.allocate(16, 16, 1, 16, dtype=E4M3)
+  c.k.view(torch.uint8).fill_(0x40), c.v.view(torch.uint8).fill_(0x00)                  # 2, 0
+  every = torch.arange(256, dtype=torch.uint8)
+  for s in (c.k_scale, c.v_scale):
+    s.view(torch.uint8).copy_(every.view(16, 16, 1))
+  k, v = paged_kv.read(c, torch.arange(256), dtype=torch.float32)
+  want = torch.tensor([2.0 * 2.0 ** (i - 127) for i in range(255)], dtype=torch.float64).float()      # (2^128 is infinity)
+  assert torch.equal(k[:255, 0, 0], want) and bool(k[255].isnan().all())
+  assert not v[:255].any() and bool(v[255].isnan().all())
+
+
 def test_quantising_twice_changes_nothing():
   torch.manual_seed(0)
   x = torch.randn(200, 64) * torch.exp2(torch.randn(200, 1) * 8)

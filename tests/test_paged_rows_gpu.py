@@ -76,6 +76,23 @@ def test_every_finite_value_is_rounded_as_defined(cuda_lib, dtype):
     assert torch.equal(paged_kv.read(c, slots)[0], ek)
 
 
+def test_every_byte_is_read_as_defined(cuda_lib):
+  """All values under all powers of two, down to bf16's subnormal numbers, and the type's NaN."""
+  c = PagedKV.allocate(16, 16, 1, 256, dtype=E4M3, device="cuda")
+  every = torch.arange(256, dtype=torch.uint8, device="cuda")
+  for t, s in ((c.k, c.k_scale), (c.v, c.v_scale)):
+    t.view(torch.uint8).copy_(every.expand(16, 16, 1, 256))
+    s.view(torch.uint8).copy_(every.view(16, 16, 1))
+  slots = torch.arange(256, device="cuda")
+  with ops.backend("torch"):
+    want = paged_kv.read(c, slots)
+  for got, w in zip(paged_kv.read(c, slots), want):
+    assert torch.equal(got.isnan(), w.isnan()) and torch.equal(got.nan_to_num(), w.nan_to_num())
+  # and by arithmetic: magnitudes below NaN's, in 64 bits, rounded once
+  x = c.k.reshape(256, 256).float().double() * torch.exp2(torch.arange(256, device="cuda").double() - 127)[:, None]
+  assert torch.equal(want[0].view(256, 256)[:255].nan_to_num(), x[:255].float().bfloat16().nan_to_num())
+
+
 def test_strided_inputs_and_pools(cuda_lib):
   torch.manual_seed(0)
   pool = torch.zeros(6, 2, 16, 4, 128, dtype=torch.bfloat16, device="cuda")      # keys and values of a page side by side

@@ -242,8 +242,8 @@ def adamw_step(p32, g, m, v, lr, beta1, beta2, eps, wd, step, grad_scale=1.0):
 
 # ----------------------------------------------------------------------------- paged cache
 def power_of_two(e: torch.Tensor) -> torch.Tensor:
-  """2^e in fp32 for whole numbers e in [-126, 127], exactly."""
-  return ((e.to(torch.int32) + 127) << 23).view(torch.float32)
+  """2^e in fp32 for whole numbers e in [-127, 127], exactly (fp64's power is right to far more than fp32 holds)."""
+  return torch.pow(2.0, e.double()).float()
 
 
 def quantise_e4m3(x: torch.Tensor):
@@ -255,7 +255,7 @@ def quantise_e4m3(x: torch.Tensor):
   e = torch.where(m <= 0.875, e - 9, e - 8).clamp(-100, 120)
   e = torch.where(amax > 0, e, torch.zeros_like(e))
   q = (x * power_of_two(-e)[..., None]).clamp(-448.0, 448.0).to(torch.float8_e4m3fn)
-  return q, (e + 127).to(torch.uint8).view(torch.float8_e8m0fnu)
+  return q, power_of_two(e).to(torch.float8_e8m0fnu)
 
 
 def paged_append(pool, scale, x, slots):
@@ -281,8 +281,7 @@ def paged_read(pool, scale, slots):
   if scale is None:
     rows = pool[at]
   else:
-    e = scale.view(torch.uint8)[at].to(torch.int32) - 127
-    rows = pool.view(torch.uint8)[at].view(torch.float8_e4m3fn).float() * power_of_two(e)[..., None]
+    rows = pool[at].float() * scale[at].float()[..., None]
   return torch.where(inside[..., None, None], rows, torch.zeros_like(rows))
 
 
