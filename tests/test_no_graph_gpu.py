@@ -67,3 +67,47 @@ def test_traces_follow_their_input(cuda_lib, op):
   with torch.no_grad():
     traced = torch.jit.trace(fn, (first,), check_trace=False)
     assert torch.equal(traced(second), fn(second)) and torch.equal(traced(first), fn(first))
+
+
+def _cache(dtype=torch.bfloat16):
+  """Two sequences of 40 and 17 tokens in pages of 16."""
+  from torchprime_b200.ops import paged_kv
+  g = torch.Generator(device="cuda").manual_seed(0)
+  c = paged_kv.PagedKV.allocate(6, 16, 2, 64, dtype=dtype, device="cuda")
+  paged_kv.append(c, *(torch.randn(96, 2, 64, generator=g, device="cuda").bfloat16() for _ in range(2)), torch.arange(96, device="cuda"))
+  return c, torch.tensor([[4, 0, 2], [1, 5, 3]], dtype=torch.int32, device="cuda"), torch.tensor([40, 17], dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("op", ["sample", "read", "append", "decode"])
+def test_traces_of_serving_operators_follow_their_input(cuda_lib, op, dtype):
+  """Traced, they are their definitions."""
+  from torchprime_b200.ops import paged_kv
+  from torchprime_b200.ops.sampling import sample_tokens
+  c, table, lens = _cache(dtype)
+  u = torch.tensor([0.3, 0.8], device="cuda")
+  slots = torch.tensor([7, 90, 33], device="cuda")
+  pools = [t for t in c if t is not None]
+  def written(x):
+    paged_kv.append(c, x, -x, slots)
+    return paged_kv.read(c, slots)
+  g = torch.Generator(device="cuda").manual_seed(1)
+  r = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()  # noqa: E731
+  fn, first, second = {
+    "sample": (lambda x: sample_tokens(x, u, 0.8, top_p=0.9), r(2, 500), r(2, 500)),
+    "read": (lambda s: paged_kv.read(c, s), slots, slots - 5),
+    "append": (written, r(3, 2, 64), r(3, 2, 64)),
+    "decode": (lambda q: paged_kv.decode_attention(q, c, table, lens), r(2, 4, 64), r(2, 4, 64)),
+  }[op]
+  same = lambda a, b: torch.equal(a, b) if torch.is_tensor(a) else all(torch.equal(x, y) for x, y in zip(a, b))  # noqa: E731
+  with torch.no_grad():
+    with ops.backend("torch"):
+      want = fn(second), fn(first)
+    traced = torch.jit.trace(fn, (first,), check_trace=False)
+    for x, w in zip((second, first) * 3, want * 3):      # (fused from the third time on)
+      for t in pools:                  # (memory that was let go is what an unwritten result shows)
+        t.clone()
+      if op == "append":
+        for t in pools:
+          t.view(torch.uint8).zero_()
+      assert same(traced(x), w)

@@ -64,6 +64,13 @@ def inference_only() -> bool:
           and not torch._C._is_tracing())
 
 
+def unobserved() -> bool:
+  """Nothing follows or rewrites the operators that run (a trace, a dispatch mode, a ``torch.func`` transform), so one without an
+  autograd function may launch its kernel by hand."""
+  return (not torch._C._is_tracing() and not torch._C._len_torch_dispatch_stack()
+          and torch._C._functorch.peek_interpreter_stack() is None)
+
+
 def batched(*tensors) -> bool:
   """Whether a backward pass runs for several gradients at once (``is_grads_batched``, ``vmap`` over ``grad``): kernels
   cannot be given such tensors, torch operators can."""

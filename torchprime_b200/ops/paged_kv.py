@@ -6,7 +6,7 @@ A cache is a pool of pages of ``page`` tokens each.  Which pages hold a sequence
 *slot* is ``block_table[b, i // page] * page + i % page``.  Pools are bf16, or e4m3 with one power of two (e8m0) for each
 token and head: the smallest under which the row's finite values fit into +-448, at least 2^-100.
 
-On CUDA/bf16 these run as sm_100a kernels; elsewhere the same math runs in plain PyTorch (``reference.py``).
+On CUDA/bf16 these run as sm_100a kernels; elsewhere, and under a trace, the same math runs in plain PyTorch (``reference.py``).
 """
 
 from __future__ import annotations
@@ -18,7 +18,7 @@ import torch
 
 from . import _debug, _lib, functional, reference as ref
 from ._lib import check, lib, ptr, stream_ptr
-from .functional import inference_only, use_kernels
+from .functional import unobserved, use_kernels
 
 P, I, LL, F = c_void_p, c_int, c_longlong, c_float
 _lib.register_signature("tpb_paged_rows", [I, P, P, P, P, P, P, P, LL, I, I, I, I, I, P, P, P])
@@ -122,7 +122,7 @@ def append(cache: PagedKV, k, v, slots):
     used = slots[slots >= 0]
     if used.unique().numel() != used.numel():
       raise IndexError("paged_append: a slot comes twice")
-  if use_kernels(k, v) and k.is_cuda and _rows_ok(cache, h, k.shape[2], v.shape[2]):
+  if use_kernels(k, v) and k.is_cuda and unobserved() and _rows_ok(cache, h, k.shape[2], v.shape[2]):
     _move(True, _vectors(k.detach()), _vectors(v.detach()), cache, slots.contiguous())
     return
   with torch.no_grad():
@@ -140,7 +140,7 @@ def read(cache: PagedKV, slots, dtype=torch.bfloat16):
   _check_cache(cache)
   _check_slots("paged_read", cache, slots)
   h, dk, dv = cache.k.shape[2], cache.k.shape[3], cache.v.shape[3]
-  if slots.is_cuda and dtype == torch.bfloat16 and use_kernels() and _rows_ok(cache, h, dk, dv):
+  if slots.is_cuda and dtype == torch.bfloat16 and use_kernels() and unobserved() and _rows_ok(cache, h, dk, dv):
     k = torch.empty(slots.shape[0], h, dk, dtype=dtype, device=slots.device)
     v = torch.empty(slots.shape[0], h, dv, dtype=dtype, device=slots.device)
     _move(False, k, v, cache, slots.contiguous())
@@ -190,7 +190,8 @@ def decode_attention(q, cache: PagedKV, block_table, lengths, scale=None, window
   if window < 0 or not softcap >= 0.0:
     raise ValueError(f"decode_attention: window {window}, softcap {softcap}")
   _debug.check_index("decode_attention", "lengths", lengths, 0, block_table.shape[1] * cache.page + 1)
-  if (use_kernels(q) and q.is_cuda and _decode_ok(q, cache) and block_table.shape[1] * cache.page <= 0x7fffff00 and (inference_only() or not q.requires_grad)):
+  if (use_kernels(q) and q.is_cuda and _decode_ok(q, cache) and block_table.shape[1] * cache.page <= 0x7fffff00 and unobserved()
+      and not (torch.is_grad_enabled() and q.requires_grad)):
     q, lengths = _vectors(q), lengths.contiguous()
     block_table = block_table if block_table.stride(1) == 1 else block_table.contiguous()
     pages, page, hkv, _ = cache.k.shape

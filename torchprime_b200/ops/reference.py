@@ -254,8 +254,9 @@ def quantise_e4m3(x: torch.Tensor):
   m, e = torch.frexp(amax)                          # 448 = 0.875 * 2^9
   e = torch.where(m <= 0.875, e - 9, e - 8).clamp(-100, 120)
   e = torch.where(amax > 0, e, torch.zeros_like(e))
-  q = (x * power_of_two(-e)[..., None]).clamp(-448.0, 448.0).to(torch.float8_e4m3fn)
-  return q, power_of_two(e).to(torch.float8_e8m0fnu)
+  # (the reshapes keep the conversions out of what the script compiler fuses: it knows no 8-bit types)
+  q = (x * power_of_two(-e)[..., None]).clamp(-448.0, 448.0).reshape(x.shape).to(torch.float8_e4m3fn)
+  return q, power_of_two(e).reshape(x.shape[:-1]).to(torch.float8_e8m0fnu)
 
 
 def paged_append(pool, scale, x, slots):
@@ -268,8 +269,11 @@ def paged_append(pool, scale, x, slots):
     pool[at] = x[keep].to(pool.dtype)
     return
   q, e = quantise_e4m3(x[keep])
-  pool.view(torch.uint8)[at] = q.view(torch.uint8)
-  scale.view(torch.uint8)[at] = e.view(torch.uint8)
+  pool[at] = q
+  if scale.is_cuda:              # (a trace does not take views of another type)
+    scale[at] = e
+  else:                          # (on the host rows of e8m0 are not written)
+    scale.view(torch.uint8)[at] = e.view(torch.uint8)
 
 
 def paged_read(pool, scale, slots):
@@ -281,7 +285,8 @@ def paged_read(pool, scale, slots):
   if scale is None:
     rows = pool[at]
   else:
-    rows = pool[at].float() * scale[at].float()[..., None]
+    # (reshapes as above)
+    rows = pool[at].float().reshape(*slots.shape, *pool.shape[2:]) * scale[at].float().reshape(*slots.shape, -1, 1)
   return torch.where(inside[..., None, None], rows, torch.zeros_like(rows))
 
 

@@ -49,7 +49,8 @@ def sample_tokens(logits, u, temperature=1.0, top_k=None, top_p=None, min_p=None
   top_p = _setting("top_p", 1.0 if top_p is None else top_p, b, logits.device, torch.float32)
   min_p = _setting("min_p", 0.0 if min_p is None else min_p, b, logits.device, torch.float32)
   logits = logits.detach()
-  if logits.is_cuda and functional.get_backend() != "torch" and logits.dtype in (torch.float32, torch.bfloat16) and v <= MAX_VOCAB and b < 1 << 26:
+  if (logits.is_cuda and functional.get_backend() != "torch" and functional.unobserved() and logits.dtype in (torch.float32, torch.bfloat16)
+      and v <= MAX_VOCAB and b < 1 << 26):
     _lib.lib()
     logits = logits if logits.stride(1) == 1 else logits.contiguous()
     out = torch.empty(b, dtype=torch.int64, device=logits.device)
