@@ -111,3 +111,27 @@ def test_traces_of_serving_operators_follow_their_input(cuda_lib, op, dtype):
         for t in pools:
           t.view(torch.uint8).zero_()
       assert same(traced(x), w)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_tangents_pass_the_cache(cuda_lib, dtype):
+  """Of queries and of bf16 pools, as the definitions give them."""
+  import torch.autograd.forward_ad as fwd
+  from torchprime_b200.ops import paged_kv
+  c, table, lens = _cache(dtype)
+  g = torch.Generator(device="cuda").manual_seed(2)
+  q, tq = (torch.randn(2, 4, 64, generator=g, device="cuda").bfloat16() for _ in range(2))
+  slots = torch.tensor([7, 90, 33], device="cuda")
+  tk, tv = (torch.randn(6, 2, 16, 64, generator=g, device="cuda").bfloat16().transpose(1, 2) for _ in range(2))
+  def call(pools):
+    with torch.no_grad(), fwd.dual_level():
+      cache = c if not pools else c._replace(k=fwd.make_dual(c.k, tk), v=fwd.make_dual(c.v, tv))
+      o = paged_kv.decode_attention(fwd.make_dual(q, tq), cache, table, lens)
+      return [fwd.unpack_dual(t).tangent for t in (o, *paged_kv.read(cache, slots))]
+  for pools in [False] + [True] * (dtype == torch.bfloat16):
+    got = call(pools)
+    with ops.backend("torch"):
+      want = call(pools)
+    assert got[0] is not None and torch.equal(got[0], want[0])
+    for a, b in zip(got[1:], want[1:]):
+      assert (a is None) == (b is None) == (not pools) and (a is None or torch.equal(a, b))

@@ -23,3 +23,9 @@ def test_traces_dispatch_modes_and_transforms_are_seen():
   torch.func.grad(lambda t: fn(t).sum())(x)
   fn(x)
   assert seen == [True, False, False, False, False, True]
+
+
+def test_forward_mode_is_seen():
+  with torch.autograd.forward_ad.dual_level():
+    assert not functional.unobserved()
+  assert functional.unobserved()

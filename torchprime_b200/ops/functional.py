@@ -65,9 +65,9 @@ def inference_only() -> bool:
 
 
 def unobserved() -> bool:
-  """Nothing follows or rewrites the operators that run (a trace, a dispatch mode, a ``torch.func`` transform), so one without an
-  autograd function may launch its kernel by hand."""
-  return (not torch._C._is_tracing() and not torch._C._len_torch_dispatch_stack()
+  """Nothing follows or rewrites the operators that run but reverse-mode autograd (no trace, no forward-mode derivative, no dispatch
+  mode, no ``torch.func`` transform), so one without an autograd function may launch its kernel by hand."""
+  return (torch.autograd.forward_ad._current_level < 0 and not torch._C._is_tracing() and not torch._C._len_torch_dispatch_stack()
           and torch._C._functorch.peek_interpreter_stack() is None)
 
 

@@ -6,7 +6,7 @@ A cache is a pool of pages of ``page`` tokens each.  Which pages hold a sequence
 *slot* is ``block_table[b, i // page] * page + i % page``.  Pools are bf16, or e4m3 with one power of two (e8m0) for each
 token and head: the smallest under which the row's finite values fit into +-448, at least 2^-100.
 
-On CUDA/bf16 these run as sm_100a kernels; elsewhere, and under a trace, the same math runs in plain PyTorch (``reference.py``).
+On CUDA/bf16 these run as sm_100a kernels; elsewhere, and under a trace or a forward-mode derivative, the same math runs in plain PyTorch (``reference.py``).
 """
 
 from __future__ import annotations
