@@ -1099,6 +1099,12 @@ struct Pools {
     }
     return true;
   }
+  bool recording() const {              // what is read of them has a gradient
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor* t : {&k, &v, &ks, &vs})
+      if (t->defined() && t->requires_grad()) return true;
+    return false;
+  }
   bool rows(const Tensor& x, int64_t t, int64_t d) const {     // [t, heads, d] as the kernel reads it
     return plain(x) && x.dim() == 3 && x.size(0) == t && x.size(1) == heads && x.size(2) == d && x.get_device() == k.get_device() &&
            x.stride(2) == 1 && x.stride(0) % 8 == 0 && x.stride(1) % 8 == 0 && aligned(x);
@@ -1132,7 +1138,7 @@ py::object paged_append(py::handle k_, py::handle v_, py::handle ks_, py::handle
 py::object paged_read(py::handle k_, py::handle v_, py::handle ks_, py::handle vs_, py::handle slots_) {
   Pools c;
   Tensor xk, xv, slots;
-  if (bounds_checked() || !unobserved() || !c.take(k_, v_, ks_, vs_) || !slots_of(c, slots_, slots)) return py::none();
+  if (bounds_checked() || !unobserved() || !c.take(k_, v_, ks_, vs_) || !slots_of(c, slots_, slots) || c.recording()) return py::none();
   {
     py::gil_scoped_release nogil;
     xk = fresh(c.k, {slots.size(0), c.heads, c.dk}, at::kBFloat16);
@@ -1151,7 +1157,7 @@ py::object paged_decode(py::handle q_, py::handle k_, py::handle v_, py::handle 
   int64_t window;
   if (bounds_checked() || !whole(window_, 0, window) || !real(softcap_, 0.0, softcap) || !unobserved() || !unpack(q_, q) || !plain(q) ||
       q.dim() != 3 || !c.take(k_, v_, ks_, vs_) || !unpack(table_, table) || !unpack(lens_, lens) ||
-      (at::GradMode::is_enabled() && recording(q)) || !real(scale_, 1.0 / std::sqrt((double)q.size(2)), scale))
+      (at::GradMode::is_enabled() && recording(q)) || c.recording() || !real(scale_, 1.0 / std::sqrt((double)q.size(2)), scale))
     return py::none();
   const int64_t b = q.size(0), hq = q.size(1);
   if (b < 1 || b > (1 << 24) || hq < 1 || hq > 65535 || hq % c.heads || q.size(2) != c.dk || c.pages < 1 || c.page % 16 ||

@@ -135,3 +135,33 @@ def test_tangents_pass_the_cache(cuda_lib, dtype):
     assert got[0] is not None and torch.equal(got[0], want[0])
     for a, b in zip(got[1:], want[1:]):
       assert (a is None) == (b is None) == (not pools) and (a is None or torch.equal(a, b))
+
+
+@pytest.mark.parametrize("which", ["k", "v", "q"])
+def test_gradients_of_the_pools(cuda_lib, which):
+  """Pools that require a gradient get the one of the definition, from attention and from reads."""
+  from torchprime_b200.ops import paged_kv
+  c, table, lens = _cache()
+  g = torch.Generator(device="cuda").manual_seed(3)
+  q, do = (torch.randn(2, 4, 64, generator=g, device="cuda").bfloat16() for _ in range(2))
+  slots = torch.tensor([7, 90, 33], device="cuda")
+  dr = torch.randn(3, 2, 64, generator=g, device="cuda").bfloat16()
+  def call():
+    leaf = {"q": q, "k": c.k, "v": c.v}[which].detach().clone().requires_grad_()
+    cache = c._replace(**{which: leaf}) if which != "q" else c
+    o = paged_kv.decode_attention(leaf if which == "q" else q, cache, table, lens)
+    assert o.requires_grad
+    grads = [torch.autograd.grad(o, leaf, do)[0]]
+    if which != "q":
+      rows = paged_kv.read(cache, slots)["kv".index(which)]
+      assert rows.requires_grad
+      grads.append(torch.autograd.grad(rows, leaf, dr)[0])
+      with torch.no_grad():            # nothing is recorded: the kernels
+        assert not paged_kv.read(cache, slots)[0].requires_grad
+        assert not paged_kv.decode_attention(q, cache, table, lens).requires_grad
+    return grads
+  got = call()
+  with ops.backend("torch"):
+    want = call()
+  for a, b in zip(got, want):
+    assert bool(b.any()) and torch.allclose(a, b, rtol=2.0 ** -7, atol=2.0 ** -7 * float(b.abs().max()))      # (sums by atomics, in bf16)

@@ -244,3 +244,35 @@ def test_filters_with_the_other_caches():
   eng = DeepseekInferenceEngine(model, 2, 32, "absorb")
   prompts = [[5, 9, 17, 3], [7, 2]]
   assert generate(eng, prompts, 5, -5, 1.0, torch.Generator().manual_seed(1), top_k=1) == generate(eng, prompts, 5, -5, 0.0)
+
+
+@pytest.mark.parametrize("window,softcap", [(0, 0.0), (7, 0.0), (0, 2.0)])
+def test_gradients_of_attention_over_the_pages(window, softcap):
+  """Of queries and pools, against the formula in 64 bits over dense rows, and along one direction against differences."""
+  torch.manual_seed(4)
+  lens, table = [21, 0, 5], torch.tensor([[3, 1], [0, 0], [2, 0]], dtype=torch.int32)
+  c = PagedKV.allocate(4, 16, 2, 8, dtype=torch.float32)
+  leaves = [torch.randn(3, 4, 8), torch.randn(4, 16, 2, 8), torch.randn(4, 16, 2, 8)]
+  do = torch.randn(3, 4, 8)
+  n = torch.tensor(lens, dtype=torch.int32)
+  def f(q, k, v):
+    return (paged_kv.decode_attention(q, c._replace(k=k, v=v), table, n, window=window, softcap=softcap) * do).sum()
+  def formula(q, k, v):
+    total = 0
+    for b, m in enumerate(lens):
+      pos = torch.arange(max(0, m - window) if window else 0, m)
+      kb, vb = (t[table[b].long()[pos // 16], pos % 16].repeat_interleave(2, 1) for t in (k, v))
+      s = torch.einsum("hd,shd->hs", q[b], kb) * 8 ** -0.5
+      if softcap:
+        s = softcap * torch.tanh(s / softcap)
+      total = total + (torch.einsum("hs,shd->hd", s.softmax(-1), vb) * do[b].double()).sum()
+    return total
+  a, b = [t.clone().requires_grad_() for t in leaves], [t.double().requires_grad_() for t in leaves]
+  got, want = torch.autograd.grad(f(*a), a), torch.autograd.grad(formula(*b), b)
+  for x, y in zip(got, want):
+    assert bool(y.any()) and torch.allclose(x.double(), y, atol=1e-5)                # (sums of up to 21 terms near 1 in fp32)
+  way = [torch.randn_like(t) for t in leaves]
+  step = 2.0 ** -7                       # rest of the series: step^2 by a third derivative along a way of length ~20; rounding 2^-24 / step
+  ends = [f(*[t + s * step * w for t, w in zip(leaves, way)]) for s in (1, -1)]
+  along = sum((x * w).sum() for x, w in zip(got, way))
+  assert abs(float((ends[0] - ends[1]) / (2 * step) - along)) < 2.0 ** -6 * (1 + abs(float(along)))

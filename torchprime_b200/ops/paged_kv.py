@@ -6,7 +6,8 @@ A cache is a pool of pages of ``page`` tokens each.  Which pages hold a sequence
 *slot* is ``block_table[b, i // page] * page + i % page``.  Pools are bf16, or e4m3 with one power of two (e8m0) for each
 token and head: the smallest under which the row's finite values fit into +-448, at least 2^-100.
 
-On CUDA/bf16 these run as sm_100a kernels; elsewhere, and under a trace or a forward-mode derivative, the same math runs in plain PyTorch (``reference.py``).
+On CUDA/bf16 these run as sm_100a kernels; elsewhere, under a trace and where a gradient is recorded the same math runs in plain
+PyTorch (``reference.py``).
 """
 
 from __future__ import annotations
@@ -76,6 +77,11 @@ def _rows_ok(c: PagedKV, h: int, *ds) -> bool:
           and all(t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % unit == 0 for s in t.stride()[:3]) for t in c[:2]))
 
 
+def _recorded(*tensors) -> bool:
+  """What is computed of them has a gradient, which the kernels do not give."""
+  return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def _c_strides(c: PagedKV):
   out = []
   for t, s in ((c.k, c.k_scale), (c.v, c.v_scale)):
@@ -140,7 +146,8 @@ def read(cache: PagedKV, slots, dtype=torch.bfloat16):
   _check_cache(cache)
   _check_slots("paged_read", cache, slots)
   h, dk, dv = cache.k.shape[2], cache.k.shape[3], cache.v.shape[3]
-  if slots.is_cuda and dtype == torch.bfloat16 and use_kernels() and unobserved() and _rows_ok(cache, h, dk, dv):
+  if (slots.is_cuda and dtype == torch.bfloat16 and use_kernels() and unobserved() and not _recorded(*cache)
+      and _rows_ok(cache, h, dk, dv)):
     k = torch.empty(slots.shape[0], h, dk, dtype=dtype, device=slots.device)
     v = torch.empty(slots.shape[0], h, dv, dtype=dtype, device=slots.device)
     _move(False, k, v, cache, slots.contiguous())
@@ -191,7 +198,7 @@ def decode_attention(q, cache: PagedKV, block_table, lengths, scale=None, window
     raise ValueError(f"decode_attention: window {window}, softcap {softcap}")
   _debug.check_index("decode_attention", "lengths", lengths, 0, block_table.shape[1] * cache.page + 1)
   if (use_kernels(q) and q.is_cuda and _decode_ok(q, cache) and block_table.shape[1] * cache.page <= 0x7fffff00 and unobserved()
-      and not (torch.is_grad_enabled() and q.requires_grad)):
+      and not _recorded(q, *cache)):
     q, lengths = _vectors(q), lengths.contiguous()
     block_table = block_table if block_table.stride(1) == 1 else block_table.contiguous()
     pages, page, hkv, _ = cache.k.shape
