@@ -1132,6 +1132,8 @@ py::object paged_append(py::handle k_, py::handle v_, py::handle ks_, py::handle
   {
     py::gil_scoped_release nogil;
     c.move(true, xk, xv, slots);
+    for (const Tensor* t : {&c.k, &c.v, &c.ks, &c.vs})           // an earlier graph that saved a pool has to notice
+      if (t->defined() && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   }
   return py::bool_(true);
 }

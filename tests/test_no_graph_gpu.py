@@ -165,3 +165,32 @@ def test_gradients_of_the_pools(cuda_lib, which):
     want = call()
   for a, b in zip(got, want):
     assert bool(b.any()) and torch.allclose(a, b, rtol=2.0 ** -7, atol=2.0 ** -7 * float(b.abs().max()))      # (sums by atomics, in bf16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("native", [True, False])
+def test_append_counts_as_a_write(cuda_lib, monkeypatch, dtype, native):
+  """A graph that saved a pool notices, as it does where the definition writes; pools made for inference have no versions."""
+  from torchprime_b200.ops import paged_kv
+  if not native:
+    monkeypatch.setattr(ops, "_native", lambda: None)
+  c, _, _ = _cache(dtype)
+  x = torch.randn(2, 2, 64, device="cuda").bfloat16()
+  slots = torch.tensor([3, 50], device="cuda")
+  pools = [t for t in c if t is not None]
+  for backend in ("torch", "auto"):
+    with ops.backend(backend):
+      before = [t._version for t in pools]
+      paged_kv.append(c, x, x, slots)
+      assert all(t._version > v for t, v in zip(pools, before))
+  if dtype == torch.bfloat16:
+    w = torch.ones(64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    loss = (c.k * w).sum()             # saves the pool
+    paged_kv.append(c, x, x, slots)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+      loss.backward()
+  with torch.inference_mode():
+    c, _, _ = _cache(dtype)
+    paged_kv.append(c, x, x, slots)
+  paged_kv.append(c, x, x, slots)
+  assert torch.equal(paged_kv.read(c, slots)[0][0].isnan(), torch.zeros(2, 64, dtype=torch.bool, device="cuda"))

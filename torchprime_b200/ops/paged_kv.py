@@ -130,6 +130,7 @@ def append(cache: PagedKV, k, v, slots):
       raise IndexError("paged_append: a slot comes twice")
   if use_kernels(k, v) and k.is_cuda and unobserved() and _rows_ok(cache, h, k.shape[2], v.shape[2]):
     _move(True, _vectors(k.detach()), _vectors(v.detach()), cache, slots.contiguous())
+    torch.autograd.graph.increment_version([t for t in cache if t is not None])      # an earlier graph that saved a pool has to notice
     return
   with torch.no_grad():
     for pool, scale, x in ((cache.k, cache.k_scale, k), (cache.v, cache.v_scale, v)):
