@@ -237,6 +237,19 @@ def test_generation_that_the_pages_do_not_suffice_for_gives_them_back():
   assert len(generate(eng, [[5, 9, 17, 3]], max_new_tokens=7, eos_id=-5, temperature=0.0)[0]) == 7
 
 
+def test_sequences_that_have_ended_give_their_pages_to_the_others():
+  from torchprime_b200.experimental.deepseek_inference.engine import DeepseekInferenceEngine
+  from torchprime_b200.experimental.deepseek_inference.generate import generate
+  _, model = _tiny()
+  prompts = [[5, 9, 17, 3], [7, 2]]
+  outs = generate(DeepseekInferenceEngine(model, 2, 32, "paged", page_size=4), prompts, 9, -5, 0.0)
+  eos = outs[1][0]                                                                # the second ends at once
+  assert eos not in outs[0]
+  eng = DeepseekInferenceEngine(model, 2, 32, "paged", page_size=4, num_pages=3)  # what the first takes to its end
+  assert generate(eng, prompts, 9, eos, 0.0) == [outs[0], []]
+  assert sorted(eng._free) == [0, 1, 2]
+
+
 def test_filters_with_the_other_caches():
   from torchprime_b200.experimental.deepseek_inference.engine import DeepseekInferenceEngine
   from torchprime_b200.experimental.deepseek_inference.generate import generate

@@ -73,7 +73,8 @@ def generate(engine: DeepseekInferenceEngine, prompt_tokens: list[list[int]], ma
 
 
 def _generate_paged(engine, prompt_tokens, max_new_tokens, eos_id, draw):
-  """Prompts one after the other, then a step for all sequences that have not ended, each at its own position."""
+  """Prompts one after the other, then a step for all sequences that have not ended, each at its own position.  Sequences give back
+  their pages as they end."""
   n = len(prompt_tokens)
   lens = [len(t) for t in prompt_tokens]
   most = [min(max_new_tokens, engine.max_seq_len - k) for k in lens]
@@ -85,7 +86,9 @@ def _generate_paged(engine, prompt_tokens, max_new_tokens, eos_id, draw):
     while rows:
       for i, t in zip(rows, nxt.tolist()):
         out[i].append(t)
-      rows = [i for i in rows if out[i][-1] != eos_id and len(out[i]) < most[i]]
+      ended = [i for i in rows if out[i][-1] == eos_id or len(out[i]) == most[i]]
+      engine.release(ended)   # for the others to grow
+      rows = [i for i in rows if i not in ended]
       if rows:
         nxt = draw(engine.forward(torch.tensor([[out[i][-1]] for i in rows]), [lens[i] + len(out[i]) - 1 for i in rows], rows=rows))
   finally:                    # (where the pages do not suffice, too)
