@@ -19,7 +19,10 @@
 // * Scores and weighted sums are mma.sync m16n8k16: the query heads of a key head are its 16 rows.  (A tcgen05 tile would be
 //   seven eighths empty, and its operands would still come through shared memory once.)  Statistics and sums are fp32; the
 //   weights of the sum are rounded to the operand type of the product, by up to 2^-8 (bf16) or 2^-11 (f16) of each, to
-//   either side, against a result that is rounded to bf16 itself; the sum of the weights is not rounded.
+//   either side, against a result that is rounded to bf16 itself; the sum of the weights is not rounded.  f16 ends sooner: weights
+//   below 2^-29 of the largest are rounded by up to 2^-40 of that.  (What counts is weight times power of two of the values.  A row
+//   of zeros is held with the power 1, others of ordinary size with 2^-7 or so: beside a token of zeros that has nearly all the
+//   weight, others of 2^-26 of it are off by up to 2^-7 of themselves.)
 // * An e4m3 cache is turned into f16 in registers, exactly; queries become f16 with a power of two for each head that puts the
 //   largest at 2^14 (f16 has more bits than bf16; what falls below 2^-38 of the largest is lost).  The keys' powers of two
 //   multiply the scores, the values' are added to the exponent of the weights, so that no weight overflows: o = sum_i 2^(s_i + e_i
@@ -335,7 +338,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_cons
 
   const int g = lane >> 2, t = lane & 3;
   constexpr int NT = WIDE ? 2 : 1;         // blocks of eight query heads
-  constexpr int F16_UP = 15;               // f16 weights are 2^15 times as large: of a long sequence's small ones those from 2^-39 on count
+  constexpr int F16_UP = 15;               // f16 weights are 2^15 times as large: of a long sequence's small ones those from 2^-40 on count
   int done = 0, seg = 0, h0 = 0, rows = 0;
   // Of heads 8 nt + 2t and the one after: columns 16 c + (0 .. 15), two of them to a lane (see column()), maxima and sums.
   float o[NT][DV / 16][4], m[NT][2], l[NT][2];

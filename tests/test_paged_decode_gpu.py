@@ -192,6 +192,40 @@ def test_many_small_weights_count(cuda_lib, dtype, lens):
   _check_scores(paged_kv.decode_attention(q, c, table, lengths, scale=scale), q, c, table, lengths, scale)
 
 
+@pytest.mark.parametrize("lens", [[5, 17], [2], [30], [900, 64]])
+@pytest.mark.parametrize("below", [10, 22, 26, 30])
+def test_small_weights_of_any_fraction(cuda_lib, lens, below):
+  """As above, with an 8-bit cache, few tokens and scores at fractions of an octave: a weight below 2^-29 of the largest, each times its
+  power of two of the values, is off by up to 2^-40 of that instead of 2^-11 of itself."""
+  q, c, table, lengths = _problem(lens, 4, 1, 64, 64, 64, E4M3)
+  q.zero_()[:, :, 0] = 1
+  g = torch.Generator(device="cuda").manual_seed(below)
+  scale = 0.6931471805599453             # scores in octaves
+  for i, n in enumerate(lens):
+    pos = torch.arange(n, device="cuda")
+    slots = table[i].long()[pos // 64] * 64 + pos % 64
+    k = torch.zeros(n, 1, 64, device="cuda")
+    k[:, 0, 0] = -below - torch.rand(n, generator=g, device="cuda") * 2
+    k[0, 0, 0] = 0
+    v = torch.rand(n, 1, 64, generator=g, device="cuda") + 1
+    v[0] = 0
+    paged_kv.append(c, k.bfloat16(), v.bfloat16(), slots)
+  got = paged_kv.decode_attention(q, c, table, lengths, scale=scale)
+  for i, n in enumerate(lens):
+    pos = torch.arange(n, device="cuda")
+    slots = table[i].long()[pos // 64] * 64 + pos % 64
+    k, v = _held(c, slots)
+    power = c.v_scale[slots // 64, slots % 64].double()[:, 0]
+    s = torch.einsum("hd,sd->hs", q[i].double(), k[:, 0]) * scale
+    p = s.softmax(-1)
+    o, a = p @ v[:, 0], p @ v[:, 0].abs()
+    size = s.abs().amax()
+    subnormal = 2.0 ** -40 * (p * power).amax(-1, keepdim=True) * (v[:, 0].abs() / power[:, None]).sum(0)
+    tol = 2.0 ** -8 * o.abs() + a * (2.0 ** -11 + 2.0 ** -19 * (2 * size + 2)) + subnormal
+    off = (got[i].double() - o).abs()
+    assert bool((off <= tol).all()), (i, n, (off / tol).max().item())
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
 @pytest.mark.parametrize("softcap", [1.0, 50.0, 3e4, 1e7])
 def test_caps_far_above_the_scores(cuda_lib, dtype, softcap):
