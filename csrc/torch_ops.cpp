@@ -1166,7 +1166,7 @@ py::object paged_decode(py::handle q_, py::handle k_, py::handle v_, py::handle 
       q.get_device() != c.k.get_device() || q.stride(2) != 1 || q.stride(0) % 8 || q.stride(1) % 8 || !aligned(q) ||
       !plain(table, at::kInt) || !plain(lens, at::kInt) || table.dim() != 2 || lens.dim() != 1 || table.size(0) != b || lens.size(0) != b ||
       table.get_device() != q.get_device() || lens.get_device() != q.get_device() || (table.size(1) > 1 && table.stride(1) != 1) ||
-      !lens.is_contiguous() || window < 0 || window > 0x7fffffff || !(softcap >= 0))
+      !lens.is_contiguous() || window < 0 || window > 0x7fffffff || !(softcap == 0 || (softcap >= 0x1p-60 && softcap <= 0x1p60)))
     return py::none();
   if (!((c.dk == 128 && c.dv == 128) || (c.dk == 192 && c.dv == 128) || (c.dk == 64 && c.dv == 64))) return py::none();
   for (int i = 0; i < 2; ++i) {

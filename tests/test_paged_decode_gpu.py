@@ -233,6 +233,14 @@ def test_caps_far_above_the_scores(cuda_lib, dtype, softcap):
   _check_scores(paged_kv.decode_attention(*p, scale=0.3, softcap=softcap), *p, 0.3, softcap)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("softcap", [1e-42, 1e-37, 1e-25, 1e-6, 1e25, 1e33, 1e37, 3e38])
+def test_caps_of_any_size(cuda_lib, dtype, softcap):
+  """Far below the scores all tokens weigh the same, far above them they weigh as without a cap."""
+  p = _problem([700, 33], 8, 2, 128, 128, 32, dtype, seed=3)
+  _check_scores(paged_kv.decode_attention(*p, scale=0.3, softcap=softcap), *p, 0.3, softcap)
+
+
 def test_a_window_beyond_32_bits_is_none(cuda_lib):
   p = _problem([700, 33], 8, 2, 128, 128, 32, torch.bfloat16)
   assert torch.equal(paged_kv.decode_attention(*p, window=(1 << 32) + 5), paged_kv.decode_attention(*p))

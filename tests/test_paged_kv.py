@@ -157,6 +157,13 @@ def test_decode_attention_refusals():
       paged_kv.decode_attention(q, c, table, lens, **kw)
 
 
+def test_an_infinite_cap_is_refused():
+  c = PagedKV.allocate(4, 16, 2, 8)
+  with pytest.raises(ValueError, match="softcap"):
+    paged_kv.decode_attention(torch.randn(1, 4, 8).bfloat16(), c, torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32),
+                              softcap=float("inf"))
+
+
 def test_debug_mode_names_lengths_beyond_the_table(monkeypatch):
   monkeypatch.setenv("TPB_DEBUG_BOUNDS", "1")
   c = PagedKV.allocate(4, 16, 2, 8)

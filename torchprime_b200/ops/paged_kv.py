@@ -195,11 +195,13 @@ def decode_attention(q, cache: PagedKV, block_table, lengths, scale=None, window
     raise ValueError("decode_attention: queries, block_table and lengths must be on the cache's device")
   window, softcap = int(window or 0), float(softcap or 0.0)
   scale = float(scale) if scale is not None else dk ** -0.5
-  if window < 0 or not softcap >= 0.0:
+  if window < 0 or not 0.0 <= softcap < float("inf"):
     raise ValueError(f"decode_attention: window {window}, softcap {softcap}")
+  if softcap:
+    softcap = max(softcap, 2.0 ** -60)       # (no score is told from another by less, and fp32 holds what it is divided by)
   _debug.check_index("decode_attention", "lengths", lengths, 0, block_table.shape[1] * cache.page + 1)
   if (use_kernels(q) and q.is_cuda and _decode_ok(q, cache) and block_table.shape[1] * cache.page <= 0x7fffff00 and unobserved()
-      and not _recorded(q, *cache)):
+      and not _recorded(q, *cache) and softcap <= 2.0 ** 60):      # (quotients by more would be flushed)
     q, lengths = _vectors(q), lengths.contiguous()
     block_table = block_table if block_table.stride(1) == 1 else block_table.contiguous()
     pages, page, hkv, _ = cache.k.shape
