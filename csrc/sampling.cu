@@ -97,6 +97,12 @@ __device__ __forceinline__ float smp_max4(const float* l) {
 }
 __device__ __forceinline__ float smp_logit(unsigned key) { return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu)); }
 
+// To 64 bits, with subnormal numbers.
+__device__ __forceinline__ double smp_double(float a) {
+  double r;
+  asm("cvt.f64.f32 %0, %1;" : "=d"(r) : "f"(a));
+  return r;
+}
 // Larger, and the same, in that order, with subnormal numbers.
 __device__ __forceinline__ bool smp_above(float a, float b) {
   int x;
@@ -140,11 +146,11 @@ struct SmpWeight {
   }
   // in 64 bits
   __device__ __noinline__ double real(float l) const {
-    const double x = ((double)l - (double)top) * per_unit;
-    return l == top ? 1.0 : x > -100.0 ? exp2(x) : 0.0;         // (NaN, of infinities: 0)
+    const double x = (smp_double(l) - smp_double(top)) * per_unit;
+    return smp_same(l, top) ? 1.0 : x > -100.0 ? exp2(x) : 0.0;         // (NaN, of infinities: 0)
   }
   __device__ __noinline__ int step_slow(float l) const {
-    return l == top ? 0 : (int)fmax(fmin(rint(((double)l - (double)top) * per_unit * SMP_TABLE), 0.0), -1e9);
+    return smp_same(l, top) ? 0 : (int)fmax(fmin(rint((smp_double(l) - smp_double(top)) * per_unit * SMP_TABLE), 0.0), -1e9);
   }
   // 1024 log2 of the weight, rounded: does not fall where l grows.
   __device__ __forceinline__ int step(float l) const {
@@ -495,9 +501,9 @@ sample_kernel(const SampleParams p, int ctas) {
     // by thread, in quarters of 64 bits.  (In the batch's order: 123 us instead of 114 where all take two CTAs.)
     auto kind = [&](int i) {
       const int k = p.top_k ? p.top_k[i] : p.top_k0;
-      if (!((p.temperature ? (double)p.temperature[i] : p.temperature0) > 0.0)) return 48;
+      if (!((p.temperature ? smp_double(p.temperature[i]) : p.temperature0) > 0.0)) return 48;
       if (k > 0 && k <= SMP_FEW) return 32;
-      return (k > 0 && k < V) || (p.min_p ? (double)p.min_p[i] : p.min_p0) > 0.0 ? 16 : 0;
+      return (k > 0 && k < V) || (p.min_p ? smp_double(p.min_p[i]) : p.min_p0) > 0.0 ? 16 : 0;
     };
     u64 mine = 0, all = 0;
     for (int i = tid; i < p.B; i += SMP_THREADS) mine += 1ULL << kind(i);
@@ -523,15 +529,15 @@ sample_kernel(const SampleParams p, int ctas) {
   const int rank = group.rank, per_cta = ctas > 1 ? p.slice : V;
   SmpSlice<L> slice = {static_cast<const L*>(p.logits) + b * p.stride, min(V, rank * per_cta), min(V, (rank + 1) * per_cta), p.vec};
   slice.copied = slice.end - (slice.end - slice.begin) % (16 / (int)sizeof(L));
-  const double T = p.temperature ? (double)p.temperature[b] : p.temperature0;
-  double top_p = p.top_p ? (double)p.top_p[b] : p.top_p0, min_p = p.min_p ? (double)p.min_p[b] : p.min_p0;
+  const double T = p.temperature ? smp_double(p.temperature[b]) : p.temperature0;
+  double top_p = p.top_p ? smp_double(p.top_p[b]) : p.top_p0, min_p = p.min_p ? smp_double(p.min_p[b]) : p.min_p0;
   int top_k = p.top_k ? p.top_k[b] : p.top_k0;
   const bool greedy = !(T > 0.0);
   if (top_k <= 0 || top_k >= V) top_k = 0;
   const bool nucleus = top_p < 1.0;               // (NaN: off)
   top_p = fmax(top_p, 0.0);
   min_p = min_p > 0.0 ? fmin(min_p, 1.0) : 0.0;
-  const double u = fmin(fmax((double)p.u[b], 0.0), 1.0);
+  const double u = fmin(fmax(smp_double(p.u[b]), 0.0), 1.0);
   unsigned* const halves = reinterpret_cast<unsigned*>(s.sums);   // low and high words of the sums
   SmpWeight weight(greedy ? 1.0 : T, s.table);
 
@@ -680,7 +686,7 @@ sample_kernel(const SampleParams p, int ctas) {
 
   unsigned least_key = 0;                         // smallest key that min_p leaves
   if (min_p > 0.0) {
-    const float guess = __double2float_rd((double)top + log(min_p) * T);
+    const float guess = __double2float_rd(smp_double(top) + log(min_p) * T);
     const unsigned at_guess = min(max(smp_key(guess), SMP_LOWEST + 20), (unsigned)(best >> 32));
     auto passes = [&](unsigned key) { return weight.real(smp_logit(key)) >= min_p; };
     unsigned low = at_guess - 16, high = min(at_guess + 16, (unsigned)(best >> 32));

@@ -108,6 +108,19 @@ def test_extreme_logits(cuda_lib, kind):
     _same(x, u, **kw)
 
 
+def test_temperatures_too_small_for_normal_numbers(cuda_lib):
+  """Above 0 all the same: drawn among the largest logits, given for all rows or for each."""
+  g = torch.Generator(device="cuda").manual_seed(16)
+  x, u = _logits(g, 40, 9000, "few values"), torch.rand(40, generator=g, device="cuda")
+  _same(x, u, temperature=1e-42)
+  _same(x, u, temperature=torch.full((40,), 1e-42, device="cuda"))
+  _same(x, u, temperature=torch.full((40,), 1e-42, device="cuda"), top_k=700, top_p=torch.full((40,), 1e-40, device="cuda"))
+  tiny = _logits(g, 40, 9000, "tiny")                # of the same size as the temperature
+  for kw in (dict(), dict(top_p=0.9), dict(top_k=50), dict(min_p=0.1), dict(top_k=3000, top_p=0.8, min_p=0.01)):
+    _same(tiny, u, temperature=1e-42, **kw)
+    _same(tiny, u, temperature=torch.full((40,), 2e-42, device="cuda"), **kw)
+
+
 def test_first_and_last_numbers(cuda_lib):
   g = torch.Generator(device="cuda").manual_seed(9)
   x = _logits(g, 6, 40000, "peaks")
