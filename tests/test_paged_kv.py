@@ -213,6 +213,26 @@ def test_paged_engine_takes_and_gives_back_pages():
     eng.forward(ids[:, :1], 4, rows=[0])                                          # nothing in front of it
 
 
+def test_paged_engine_refuses_positions_that_nothing_was_written_in_front_of():
+  """A page holds what its last sequence left behind the tokens of this one."""
+  from torchprime_b200.experimental.deepseek_inference.engine import DeepseekInferenceEngine, full_forward_last_logits
+  cfg, model = _tiny()
+  eng = DeepseekInferenceEngine(model, max_batch_size=2, max_seq_len=32, attn_impl="paged", page_size=16)
+  ids = torch.randint(0, cfg.vocab_size, (1, 9))
+  eng.forward(ids[:, :4], 0)
+  with pytest.raises(AssertionError, match="position 6"):
+    eng.forward(ids[:, 6:7], 6)
+  eng.forward(ids[:, 4:8], 4)                                                     # (the refusal changed nothing)
+  assert torch.allclose(eng.forward(ids[:, 3:4], 3), full_forward_last_logits(model, ids[:, :4]), atol=2e-4)      # back, and on again
+  assert torch.allclose(eng.forward(ids[:, 8:9], 8), full_forward_last_logits(model, ids[:, :9]), atol=2e-4)
+  eng.forward(ids[:, :2], 0)                                                      # anew
+  with pytest.raises(AssertionError, match="position 3"):
+    eng.forward(ids[:, 3:4], 3)
+  eng.release()
+  with pytest.raises(AssertionError, match="position 1"):
+    eng.forward(ids[:, 1:2], 1)
+
+
 @pytest.mark.parametrize("dtype", [None, E4M3])
 def test_paged_generation(dtype):
   from torchprime_b200.experimental.deepseek_inference.engine import DeepseekInferenceEngine, full_forward_last_logits

@@ -60,6 +60,7 @@ class DeepseekInferenceEngine:
       self.page_size, self.pages = page_size, [
         paged_kv.PagedKV.allocate(num_pages, page_size, h, dn + dr, dv, dtype=self.dtype, device=self.device) for _ in range(n)]
       self._free, self._owned = list(range(num_pages))[::-1], [[] for _ in range(max_batch_size)]
+      self._written = [0] * max_batch_size         # tokens of each sequence
       self._table = torch.zeros(max_batch_size, width, dtype=torch.int32)      # on the host; a step takes the rows that it needs
     else:
       self.kv_cache = [mk(max_batch_size, max_seq_len, c) for _ in range(n)]
@@ -78,6 +79,7 @@ class DeepseekInferenceEngine:
     for r in range(self.max_batch_size) if rows is None else rows:
       self._free += self._owned[r][::-1]
       self._owned[r] = []
+      self._written[r] = 0
 
   def _step(self, rows, starts, s: int):
     """Pages for ``s`` tokens more of each sequence, and where a step finds them: slots of the new tokens [B * s], table [B, pages]
@@ -85,15 +87,16 @@ class DeepseekInferenceEngine:
     p, ends = self.page_size, [st + s for st in starts]
     need = [max(0, -(-e // p) - (len(self._owned[r]) if st else 0)) for r, st, e in zip(rows, starts, ends)]
     for r, st in zip(rows, starts):
-      assert st <= len(self._owned[r]) * p, f"sequence {r} has no token in front of position {st}"
+      assert st <= self._written[r], f"sequence {r} has {self._written[r]} tokens, not all in front of position {st}"
     spare = len(self._free) + sum(len(self._owned[r]) for r, st in zip(rows, starts) if not st)
     if sum(need) > spare:
       raise RuntimeError(f"the cache is full: {sum(need)} pages are needed, {spare} are free")
     self.release(r for r, st in zip(rows, starts) if not st)
-    for r, n in zip(rows, need):
+    for r, n, e in zip(rows, need, ends):
       for _ in range(n):
         self._table[r, len(self._owned[r])] = self._free[-1]
         self._owned[r].append(self._free.pop())
+      self._written[r] = max(self._written[r], e)
     pos = torch.tensor(starts)[:, None] + torch.arange(s)
     table = self._table[rows, : max(len(self._owned[r]) for r in rows)]
     slots = table.long().gather(1, pos // p) * p + pos % p
