@@ -65,11 +65,12 @@ struct PagedShape {
   int keys, warps;         // tokens of a warp's step, warps to a CTA
 };
 // One CTA takes the SM's shared memory, a warp at least one stage of it: many warps with one stage each keep as many bytes under way
-// as few with several, and hide the conversions of an 8-bit cache better.  us, 64 sequences of up to 8192 tokens, 64 / 8 heads of 128
-// in e4m3: 4 warps 159, 8 118, 16 (scores transposed) 90; 128 of 32 / 8 heads in bf16: 4 warps 277, 6 266, 8 261.  Narrow heads take 64
-// tokens to a step (8 / 8 heads of 64 columns, 64 sequences, bf16 50 -> 44 us, e4m3 60 -> 57), which costs wide ones their
-// registers or stages; with more than 8 query heads to a key head eight warps have registers (64 / 2 heads of 192 / 128 in e4m3:
-// 8 warps 35 us, 10 45, 12 40).
+// as few with several, and hide the conversions of an 8-bit cache better.  us, as the kernel grew, 64 sequences of up to 8192 tokens, 64 / 8
+// heads of 128 in e4m3: 4 warps 159, 8 118, 16 (scores transposed) 90; 128 of 32 / 8 heads in bf16: 4 warps 277, 6 266, 8 261.  Narrow
+// heads take 64 tokens to a step, 32 / 64: 64 sequences of 8 / 8 heads of 64 columns, up to 8192 tokens, bf16 82 / 76 us, e4m3 65 / 58, up
+// to 4096 50 / 44 and 42 / 37.  That costs wide ones their registers or stages, but an 8-bit cache with more than 8 query heads to
+// a key head has to: a part of a result would not fit into a stage of 32.  With more than 8 query heads eight warps have registers
+// (64 / 2 heads of 192 / 128 in e4m3: 8 warps 35 us, 10 45, 12 40).
 constexpr PagedShape pd_shape(bool held8, bool wide, int width) {
   return {width <= 128 || (held8 && wide && width <= 256) ? 64 : 32, held8 && !wide ? 16 : 8};
 }

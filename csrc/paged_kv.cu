@@ -10,7 +10,7 @@
 // Both directions are bound by memory: every value is moved once.  A row is held by 4 to 32 lanes, two or three 16-byte vectors
 // each, and a warp takes four sets of rows at once so that their loads are all in flight.  (One vector to a lane, with twice the lanes:
 // finding places and the largest value cost twice as many instructions for a byte, 30011 tokens of 8 heads of 128 to e4m3 36 us instead
-// of 30, 20000 of 16 of 192 / 128 82 instead of 50, at the memory's rate 28 and 47.)
+// of 31, 20000 of 16 of 192 / 128 82 instead of 53, at a copy's rate 28 and 47.)
 
 #include "common.cuh"
 #include "tpb.h"
@@ -65,8 +65,9 @@ paged_rows_kernel(PagedRows k, PagedRows v, const long long* __restrict__ slots,
   const PagedRows p = blockIdx.y ? v : k;
   const int per_warp = 32 / LANES, lane = threadIdx.x & 31, in_row = lane % LANES;
   const unsigned warp = blockIdx.x * (PAGED_THREADS / 32) + (threadIdx.x >> 5);
-  // A lane finds a row's places for the lanes that move it.  (Every lane for its own rows: 50 us instead of 41 for 30011 tokens of 8
-  // heads to e4m3.  Eight tokens of one head to a warp, which lie together, instead of eight heads of one token: 37 instead of 36.)
+  // A lane finds a row's places for the lanes that move it.  (Both in the form with one vector to a lane, 30011 tokens of 8 heads to e4m3:
+  // every lane for its own rows, 50 us instead of 41; eight tokens of one head to a warp, which lie together, instead of eight heads of
+  // one token, 37 instead of 36.)
   const unsigned r = warp * (per_warp * PAGED_ROWS) + lane, t = r / H, h = r - t * H;      // (rows < 2^31)
   const bool live = lane < per_warp * PAGED_ROWS && r < rows;
   __nv_bfloat16* const my_x = live ? p.x + (long long)t * p.x_token + (long long)h * p.x_head : nullptr;

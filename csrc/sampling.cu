@@ -8,7 +8,7 @@
 //
 // Which token comes out hangs on sums of up to 2^18 weights that are compared with a border, so fp32 exponentials will not do: a
 // weight is a table's 2^(j / 1024) times the series of the rest, with the exponent as an unevaluated sum of two floats, good to 2^-34
-// (in fp64 throughout, the same 65 M weights took five times as long), and weights are added as whole multiples of 2^-44: sums are
+// (in fp64 throughout, an early form took five times as long for 65 M weights), and weights are added as whole multiples of 2^-44: sums are
 // exact, and the same in any order.
 //
 // Memory bounds it: a row has to be read once.  A cluster of 1 to 16 CTAs takes a row, each a contiguous slice; more CTAs the fewer
@@ -29,7 +29,7 @@
 
 namespace tpb {
 
-constexpr int SMP_THREADS = 512, SMP_WARPS = SMP_THREADS / 32;      // (1024: one row's nucleus 36 -> 41 us)
+constexpr int SMP_THREADS = 512, SMP_WARPS = SMP_THREADS / 32;      // (1024, when one row's nucleus took 36 us instead of 33: 41)
 constexpr int SMP_BINS = 2048;          // 11 bits of the order at a time (31-21, 20-10, 9-0); 32 binary orders of weights in steps of 1/64
 constexpr int SMP_CAP = 2048;           // tokens that one CTA sorts
 constexpr int SMP_FEW = SMP_THREADS / 4;        // largest k whose candidates are found while a row is read
@@ -498,7 +498,7 @@ sample_kernel(const SampleParams p, int ctas) {
   if (p.unequal) {
     // Rows in order of how long they take: those whose sums take all their logits; those that may, with more tokens than a list holds;
     // those with a small k; greedy ones.  The first two kinds get the whole clusters that there are.  Rows of a kind are numbered thread
-    // by thread, in quarters of 64 bits.  (In the batch's order: 123 us instead of 114 where all take two CTAs.)
+    // by thread, in quarters of 64 bits.  (In the batch's order: 123 us instead of 114, in the form that gave every row two CTAs.)
     auto kind = [&](int i) {
       const int k = p.top_k ? p.top_k[i] : p.top_k0;
       if (!((p.temperature ? smp_double(p.temperature[i]) : p.temperature0) > 0.0)) return 48;
@@ -985,14 +985,17 @@ static int launch_sample(SampleParams p, cudaStream_t stream) {
     if (e == cudaSuccess && device <= 31) ready.fetch_or(1u << device, std::memory_order_relaxed);
   }
   // CTAs to a row: as many as leave all rows under way at once, with 2048 logits or more to a CTA.  A GPC's SMs bound what clusters fit:
-  // 16 rows of 16 CTAs or 37 of 8 do not, though the SMs hold 296 CTAs.  us, by this rule / with twice the CTAs, rows of 128256: 16 rows,
-  // 50 largest 24 / 32, nucleus 50 / 63; 37 rows, 30 / 39, 82 / 89; 64 rows, 31 / 55, 82 / 108.
+  // 16 rows of 16 CTAs or 37 of 8 do not, though the SMs hold 296 CTAs.  us after a flushed L2, by this rule / with twice the CTAs, rows
+  // of 128256: 16 rows, 50 largest 35 / 41, nucleus 70 / 92; 37 rows, 35 / 47, 90 / 116; 64 rows, 37 / 61, 94 / 127.
   // Rows with settings of their own take unequal times, a nucleus of a flat distribution ten times a greedy row's.  Two waves of
-  // clusters even that out a little (256 rows of 102400, a third without a small k, some of them without a filter, 114 us, one wave 156).
+  // clusters even that out (64 rows of 128256, a third without a small k, some of them without a filter, 76 us, one wave 92; 256 rows 131
+  // and 191).
   // Where a batch fills the SMs with clusters of four, or with a CTA to a row, long rows take clusters of four and the others a CTA
-  // each.  us, such a mix, 50 largest, a nucleus for every row; that way and by waves, of 128256 logits:
-  //   64 rows 69 / 57, 45 / 59, 83 / 108;  192 rows 87 / 121, 47 / 61, 284 / 209;  256 rows 91 / 127, 47 / 83, 300 / 254;
-  //   and not 96 rows 72 / 72, 42 / 53, 218 / 132;  512 rows 198 / 193, 92 / 91, 522 / 444.
+  // each.  us after a flushed L2, such a mix, 50 largest, a nucleus for every row; that way and by waves, of 128256 logits:
+  //   64 rows 88 / 76, 43 / 64, 94 / 119;  192 rows 92 / 128, 53 / 70, 305 / 239;  256 rows 99 / 131, 55 / 79, 317 / 266;
+  // of 32000: 64 rows 57 / 54, 29 / 51, 53 / 80;  192 rows 57 / 70, 35 / 48, 120 / 102;  256 rows 57 / 70, 35 / 53, 123 / 116;
+  // and not (measured in an earlier form) 96 rows of 128256 72 / 72, 42 / 53, 218 / 132;  512 rows 198 / 193, 92 / 91, 522 / 444.
+  // It loses where every row is long, by 28 % at 192 rows of a nucleus each: how many are is on the device.
   auto fit = [&](int n) {
     int most = 0;
     if (e == cudaSuccess) e = sample_clusters<L>(device, n, &most);
