@@ -6,7 +6,7 @@
 // Every cached row is read once per 16 query heads that share it: 2 * 16 operations a byte at most, so memory bounds it, and
 // what the kernel is built for is to keep loads under way on every SM from the first to the last token.
 //
-// * The work is cut into steps: 32 tokens of one sequence, for one key head and up to 16 of its query heads.  In the order
+// * The work is cut into steps: 32 or 64 tokens of one sequence, for one key head and up to 16 of its query heads.  In the order
 //   sequence, head, token they form one list, of which every CTA (one per SM) takes an equal, contiguous part, and every warp of
 //   it an equal part of that; how long the sequences are only the device knows, so each CTA adds up the lengths itself.  Where a
 //   (sequence, head) goes on in the next warps, the warp that began it waits for them at the kernel's end and joins their
@@ -14,7 +14,7 @@
 //   has at most two of the latter, so the scratch is bounded by the grid and not by the batch.  Nothing is added by atomics: the
 //   order of every sum follows from the lengths.  (Eight warps sharing units of 256 tokens met in a block barrier wherever a
 //   sequence ended: 24 sequences of up to 3001 tokens, 16 heads of 192 / 128 in e4m3, 69 us, the SMs idle for half of it.)
-// * A warp has a ring of stages of its own, filled by TMA boxes of 16 tokens (a page is a multiple of 16) that its elected lane asks
+// * A warp has a ring of stages of its own, filled by TMA boxes of 16 tokens (a page is a multiple of 16) that a lane each asks
 //   for as soon as it has used a stage up, across the borders of sequences.
 // * Scores and weighted sums are mma.sync m16n8k16: the query heads of a key head are its 16 rows.  (A tcgen05 tile would be
 //   seven eighths empty, and its operands would still come through shared memory once.)  Statistics and sums are fp32; the
