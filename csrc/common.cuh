@@ -559,6 +559,11 @@ __device__ __forceinline__ float mul_exact(float a, float b) {
   asm("mul.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ float add_exact(float a, float b) {
+  float r;
+  asm("add.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
 // ---- packed fp32 pairs (sm_100: one FMA-pipe instruction works on two floats held in an aligned
 // 64-bit register pair), the three-input maximum and the bare MUFU exponential.  The softmax loops

@@ -1,8 +1,7 @@
 // Bandwidth-bound kernels of the training step: RMSNorm (+residual) fwd/bwd, RoPE,
-// SwiGLU, softmax cross-entropy (fused forward + gradient), embedding gather /
-// scatter-add, fused AdamW and the gradient-norm reduction.  All of them move
-// 16-byte vectors, keep a row in registers between its passes and run on grids
-// sized from the SM count.
+// SwiGLU, softmax cross-entropy (fused forward + gradient), fused AdamW and the
+// gradient-norm reduction.  All of them move 16-byte vectors, keep a row in
+// registers between its passes and run on grids sized from the SM count.
 
 #include "common.cuh"
 #include "tpb.h"
@@ -751,44 +750,6 @@ ce_kernel(__nv_bfloat16* __restrict__ logits, long long ld, const long long* __r
 }
 
 // ----------------------------------------------------------------------------
-// Embedding
-// ----------------------------------------------------------------------------
-__global__ void embedding_fwd_kernel(const uint4* __restrict__ table, const long long* __restrict__ ids,
-                                     uint4* __restrict__ out, long long tokens, int nvec, long long vocab,
-                                     long long row0) {
-  if (!chain_begin()) return;
-  const long long total = tokens * nvec;
-  for (long long idx = blockIdx.x * (long long)blockDim.x + threadIdx.x; idx < total;
-       idx += (long long)gridDim.x * blockDim.x) {
-    const long long t = idx / nvec;
-    const int c = (int)(idx % nvec);
-    const long long id = ids[t] - row0;
-    out[idx] = (id >= 0 && id < vocab) ? table[id * nvec + c] : make_uint4(0, 0, 0, 0);
-  }
-}
-template <bool F32>
-__global__ void embedding_bwd_kernel(const __nv_bfloat162* __restrict__ dout, const long long* __restrict__ ids,
-                                     void* __restrict__ dtable, long long tokens, int dim2, long long rows_local,
-                                     long long row0) {
-  const long long total = tokens * dim2;
-  for (long long idx = blockIdx.x * (long long)blockDim.x + threadIdx.x; idx < total;
-       idx += (long long)gridDim.x * blockDim.x) {
-    const long long t = idx / dim2;
-    const int c = (int)(idx % dim2);
-    const long long id = ids[t] - row0;
-    if (id < 0 || id >= rows_local) continue;
-    const __nv_bfloat162 g = dout[idx];
-    if (F32) {
-      float* d = reinterpret_cast<float*>(dtable) + (id * dim2 + c) * 2;
-      atomicAdd(d, __low2float(g));
-      atomicAdd(d + 1, __high2float(g));
-    } else {
-      atomicAdd(reinterpret_cast<__nv_bfloat162*>(dtable) + id * dim2 + c, g);
-    }
-  }
-}
-
-// ----------------------------------------------------------------------------
 // Optimizer
 // ----------------------------------------------------------------------------
 template <bool GBF16>
@@ -1103,28 +1064,6 @@ extern "C" int tpb_sumsq(const void* g, long long n, int is_bf16, float* out, vo
 
 extern "C" int tpb_clip_coef(const float* sumsq, float max_norm, float* coef, float* norm_out, void* stream) {
   clip_coef_kernel<<<1, 1, 0, STREAM(stream)>>>(sumsq, max_norm, coef, norm_out);
-  return rc(cudaGetLastError());
-}
-
-extern "C" int tpb_embedding_fwd(const void* table, const long long* ids, void* out, int tokens, int dim,
-                                 long long vocab, long long row0, void* stream) {
-  if (dim % 8) return -2;
-  if (tokens <= 0) return 0;
-  chain(embedding_fwd_kernel, grid_for((long long)tokens * (dim / 8), 256), 256, 0, STREAM(stream),
-        (const uint4*)table, ids, (uint4*)out, tokens, dim / 8, vocab, row0);
-  return rc(cudaGetLastError());
-}
-extern "C" int tpb_embedding_bwd(const void* dout, const long long* ids, void* dtable, int tokens, int dim,
-                                 long long rows_local, long long row0, int dtable_is_f32, void* stream) {
-  if (dim % 2) return -2;
-  if (tokens <= 0) return 0;
-  const int grid = grid_for((long long)tokens * (dim / 2), 256);
-  if (dtable_is_f32)
-    embedding_bwd_kernel<true><<<grid, 256, 0, STREAM(stream)>>>((const __nv_bfloat162*)dout, ids, dtable, tokens,
-                                                                 dim / 2, rows_local, row0);
-  else
-    embedding_bwd_kernel<false><<<grid, 256, 0, STREAM(stream)>>>((const __nv_bfloat162*)dout, ids, dtable, tokens,
-                                                                  dim / 2, rows_local, row0);
   return rc(cudaGetLastError());
 }
 

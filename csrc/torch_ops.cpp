@@ -919,7 +919,7 @@ py::object embedding(py::handle ids_, py::handle table_) {
     sizes.push_back(table.size(1));
     y = empty_as(table, sizes);
     check(tpb_embedding_fwd(cptr(table), static_cast<const long long*>(cptr(ids)), mptr(y), (int)ids.numel(), (int)table.size(1),
-                            table.size(0), 0, stream()),
+                            table.size(0), 0, 1.f, stream()),
           "embedding_fwd");
   }
   return py::cast(y);

@@ -93,12 +93,13 @@ int tpb_sumsq(const void* g, long long n, int is_bf16, float* out, void* stream)
 // coef = min(1, max_norm / (sqrt(*sumsq) + 1e-6)); norm_out = sqrt(*sumsq)
 int tpb_clip_coef(const float* sumsq, float max_norm, float* coef, float* norm_out, void* stream);
 
-// out[t,:] = table[ids[t],:]
+// out[t,:] = scale * table[ids[t] - row0,:]; zeros for ids without a row here (embedding.cu)
 int tpb_embedding_fwd(const void* table, const long long* ids, void* out, int tokens, int dim,
-                      long long vocab, long long row0, void* stream);
-// dtable[ids[t]-row0,:] += dout[t,:] for rows owned by this shard
-int tpb_embedding_bwd(const void* dout, const long long* ids, void* dtable, int tokens, int dim,
-                      long long rows_local, long long row0, int dtable_is_f32, void* stream);
+                      long long vocab, long long row0, float scale, void* stream);
+// dtable[v,:] = (`add`: dtable[v,:] +) scale * sum of dout[t,:] over ids[t] - row0 = v, in the order of t
+long long tpb_embedding_bwd_scratch(int tokens, int rows_local, int dim);     // bytes
+int tpb_embedding_bwd(const void* dout, const long long* ids, void* dtable, void* scratch, int tokens, int dim,
+                      int rows_local, long long row0, int dtable_is_f32, int add, float scale, void* stream);
 
 // bf16 <- fp32 with scale, and fp32 accumulate into bf16 destinations
 int tpb_cast_f32_to_bf16(const float* src, void* dst, long long n, float scale, int accumulate, void* stream);
@@ -288,6 +289,19 @@ int tpb_paged_decode(const void* q, long long q_b, long long q_h, const void* k_
 int tpb_sample_tokens(const void* logits, int bf16, long long stride, const float* u, const float* temperature, const int* top_k,
                       const float* top_p, const float* min_p, double temperature0, int top_k0, double top_p0, double min_p0,
                       long long* out, int B, int V, void* stream);
+
+// ---- norms of query and key heads with the rotation, and their gradient (qk_norm.cu)
+int tpb_qk_norm_fwd(const void* x, long long ld, const void* wq, const void* wk, const float* cos, const float* sin, int table,
+                    const int* pos, int seq, void* q, void* k, int tokens, int hq, int hkv, int d, int rot, float eps,
+                    int interleaved, void* stream);
+long long tpb_qk_norm_bwd_scratch(int tokens, int d);     // floats
+int tpb_qk_norm_bwd(const void* x, long long ld, const void* wq, const void* wk, const float* cos, const float* sin, int table,
+                    const int* pos, int seq, const void* dq, const void* dk, const void* dv, void* dx, float* sums, void* dwq,
+                    void* dwk, int tokens, int hq, int hkv, int d, int rot, float eps, int interleaved, void* stream);
+
+// ---- dropout from a counter-based generator, with the residual's sum (dropout.cu)
+int tpb_dropout(const void* x, const void* residual, void* y, const long long* seed, long long n, int threshold, unsigned site,
+                void* stream);
 
 #ifdef __cplusplus
 }

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_float, c_int, c_longlong, c_void_p
+from ctypes import c_float, c_int, c_longlong, c_uint, c_void_p
 
 import torch
 
@@ -81,7 +81,7 @@ def native():
 
 
 def _declare(L):
-  P, I, LL, F = c_void_p, c_int, c_longlong, c_float
+  P, I, LL, F, U = c_void_p, c_int, c_longlong, c_float, c_uint
   sigs = {
     "tpb_status": [P],
     "tpb_sm_count": [],
@@ -102,11 +102,14 @@ def _declare(L):
     "tpb_adamw": [P, P, P, P, P, LL, F, F, F, F, F, F, F, P, I, P],
     "tpb_sumsq": [P, LL, I, P, P],
     "tpb_clip_coef": [P, F, P, P, P],
-    "tpb_embedding_fwd": [P, P, P, I, I, LL, LL, P],
-    "tpb_embedding_bwd": [P, P, P, I, I, LL, LL, I, P],
+    "tpb_embedding_fwd": [P, P, P, I, I, LL, LL, F, P],
+    "tpb_embedding_bwd": [P, P, P, P, I, I, I, LL, I, I, F, P],
     "tpb_cast_f32_to_bf16": [P, P, LL, F, I, P],
     "tpb_scale_cast_bf16": [P, P, LL, P, P],
     "tpb_linear_f32": [P, P, P, I, I, I, LL, LL, LL, P],
+    "tpb_qk_norm_fwd": [P, LL, P, P, P, P, I, P, I, P, P, I, I, I, I, I, F, I, P],
+    "tpb_qk_norm_bwd": [P, LL, P, P, P, P, I, P, I, P, P, P, P, P, P, P, I, I, I, I, I, F, I, P],
+    "tpb_dropout": [P, P, P, P, LL, I, U, P],
     "tpb_mla_pack": [P, P, LL, P, P, LL, I, I, I, I, P],
     "tpb_mla_unpack": [P, P, P, P, LL, I, I, I, I, P],
   }
@@ -116,6 +119,8 @@ def _declare(L):
       continue
     fn.argtypes = args
     fn.restype = c_int
+  for name, args in {"tpb_embedding_bwd_scratch": [I, I, I], "tpb_qk_norm_bwd_scratch": [I, I]}.items():
+    getattr(L, name).argtypes, getattr(L, name).restype = args, LL
   L.tpb_status_clear.argtypes = []
   L.tpb_status_clear.restype = None
   _declare_optional(L)

@@ -722,6 +722,139 @@ def rope_inplace(qkv, cos_half, sin_half, heads, dim, seq_len, pos=None, interle
   return torch.cat([rot.to(qkv.dtype).reshape(b, s, heads * dim), qkv[..., heads * dim:]], dim=-1)
 
 
+# --------------------------------------------------------------------------- norms of query and key heads
+def _dense(t):
+  """Contiguous and 16-byte aligned."""
+  t = t.contiguous()
+  return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _qk_norm_ok(qkv, q_weight, k_weight, cos, sin, d, eps) -> bool:
+  """What the kernels take: see :func:`qk_norm_rope`."""
+  rot = 2 * cos.shape[1]
+  return (use_kernels(qkv, q_weight, k_weight) and d % 16 == 0 and d <= 512 and rot % 16 == 0 and eps >= 2.0 ** -126
+          and all(t.is_cuda and t.dtype == torch.float32 and t.is_contiguous() and t.data_ptr() % 16 == 0 for t in (cos, sin))
+          and all(w is None or (w.is_contiguous() and w.data_ptr() % 16 == 0) for w in (q_weight, k_weight))
+          and qkv.shape[0] * qkv.shape[1] * (qkv.shape[2] // d) < 2 ** 31)
+
+
+class _QkNormRopeFn(torch.autograd.Function):
+  """One node for queries, keys and values, so that the projection's gradient is one tensor, written once."""
+
+  @staticmethod
+  def forward(ctx, qkv, q_weight, k_weight, cos, sin, pos, args):
+    from . import kernels as k
+    hq, hkv, d, seq_len, eps, interleaved = args
+    ctx.save_for_backward(qkv, q_weight, k_weight, cos, sin, pos)
+    ctx.args = args
+    q, kk = k.qk_norm_fwd(qkv, hq, hkv, d, q_weight, k_weight, cos, sin, seq_len, pos, eps, interleaved)
+    return q, kk, qkv[..., (hq + hkv) * d:].unflatten(-1, (hkv, d))
+
+  @staticmethod
+  def backward(ctx, dq, dk, dv):
+    from . import kernels as k
+    qkv, q_weight, k_weight, cos, sin, pos = ctx.saved_tensors
+    hq, hkv, d, seq_len, eps, interleaved = ctx.args
+    need = ctx.needs_input_grad[:3]
+    # a gradient that is recorded itself, or several at once, and what saved-tensor hooks gave back otherwise take torch's operators
+    if (torch.is_grad_enabled() or batched(dq, dk, dv) or not use_kernels(dq, dk, dv)
+        or not _qk_norm_ok(qkv, q_weight, k_weight, cos, sin, d, eps)):
+      out = ref.qk_norm_rope_grad(dq, dk, dv, qkv, cos, sin, hq, hkv, d, seq_len, q_weight, k_weight, eps, pos, interleaved)
+      return (*(g if n else None for g, n in zip(out, need)), None, None, None, None)
+    dx, dw = k.qk_norm_bwd(_dense(dq), _dense(dk), _dense(dv), qkv, hq, hkv, d, q_weight, k_weight, cos, sin, seq_len, pos, eps, interleaved,
+                           need[1] or need[2])
+    return (dx if need[0] else None, _norm_wgrad(q_weight, dw[0]) if need[1] else None,
+            _norm_wgrad(k_weight, dw[1]) if need[2] else None, None, None, None, None)
+
+
+def qk_norm_rope(qkv, cos_half, sin_half, hq, hkv, d, seq_len, q_weight=None, k_weight=None, eps=1e-6, pos=None, interleaved=False):
+  """Queries [B, S, hq, d], keys and values [B, S, hkv, d] of a fused projection ``qkv`` [B, S, (hq + 2 hkv) * d].  Every query and key
+  head becomes ``x / sqrt(mean(x^2) + eps)``, times ``q_weight`` or ``k_weight`` [d] where there is one, and its leading
+  ``2 * cos_half.shape[1]`` columns are rotated (by pairs (i, i + half), ``interleaved`` (2i, 2i + 1)) to the token's position ``pos`` [B, S], or
+  token % ``seq_len``; all in fp32, rounded once.  Values are a view of ``qkv``.  cos/sin: fp32 [positions, columns / 2]; a position
+  outside of them counts as the nearest one and is reported (``_lib.raise_on_device_timeout``).
+
+  The kernels take bf16, heads and rotated parts of multiples of 16 columns, heads of up to 512, and ``eps`` from 2^-126 on."""
+  if qkv.dim() != 3 or hq < 1 or hkv < 1 or d < 1 or qkv.shape[2] != (hq + 2 * hkv) * d:
+    raise ValueError(f"qk_norm_rope: {tuple(qkv.shape)} is not [B, S, (hq + 2 hkv) * d] of {hq} and {hkv} heads of {d}")
+  if cos_half.dim() != 2 or cos_half.shape != sin_half.shape or not 0 < 2 * cos_half.shape[1] <= d or cos_half.shape[0] == 0:
+    raise ValueError(f"qk_norm_rope: tables {tuple(cos_half.shape)} and {tuple(sin_half.shape)} for heads of {d}")
+  tokens = qkv.shape[0] * qkv.shape[1]
+  for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+    if w is not None and w.shape != (d,):
+      raise ValueError(f"qk_norm_rope: {name} {tuple(w.shape)} for heads of {d}")
+  if pos is None and not 0 < seq_len <= cos_half.shape[0]:
+    raise ValueError(f"qk_norm_rope: seq_len {seq_len} for {cos_half.shape[0]} positions")
+  if pos is not None and (pos.numel() != tokens or pos.dtype not in (torch.int32, torch.int64)):
+    raise ValueError(f"qk_norm_rope: pos must be int32 or int64 of {tokens} tokens, got {pos.dtype} {tuple(pos.shape)}")
+  if any(t is not None and t.device != qkv.device for t in (cos_half, sin_half, q_weight, k_weight, pos)):
+    raise ValueError("qk_norm_rope: everything must be on the projection's device")
+  eps = float(eps)
+  if not 0.0 <= eps < float("inf"):
+    raise ValueError(f"qk_norm_rope: eps {eps}")
+  _debug.check_index("qk_norm_rope", "pos", pos, 0, cos_half.shape[0])
+  if (unobserved() and _qk_norm_ok(qkv, q_weight, k_weight, cos_half, sin_half, d, eps)
+      and not (torch.is_grad_enabled() and (cos_half.requires_grad or sin_half.requires_grad))):
+    if pos is not None:
+      pos = pos.clamp(-1, 2 ** 31 - 1).to(torch.int32) if pos.dtype == torch.int64 else pos
+      pos = pos.contiguous()
+    return _QkNormRopeFn.apply(qkv, q_weight, k_weight, cos_half, sin_half, pos, (hq, hkv, d, seq_len, eps, bool(interleaved)))
+  return ref.qk_norm_rope(qkv, cos_half, sin_half, hq, hkv, d, seq_len, q_weight, k_weight, eps, pos, interleaved)
+
+
+# --------------------------------------------------------------------------- dropout
+class _DropoutFn(torch.autograd.Function):
+  @staticmethod
+  def forward(ctx, x, residual, seed, threshold, site):
+    from . import kernels as k
+    ctx.save_for_backward(seed)
+    ctx.args = (threshold, site, x.shape)
+    return k.dropout(_dense(x), threshold, seed, site, None if residual is None else _dense(residual))
+
+  @staticmethod
+  def backward(ctx, dy):
+    (seed,) = ctx.saved_tensors
+    threshold, site, shape = ctx.args
+    dx = None
+    if ctx.needs_input_grad[0]:
+      if batched(dy) or not use_kernels(dy) or not _seed_ok(seed):
+        dx = ref.dropout(dy, ref.dropout_keep(shape, threshold, seed, site), threshold)
+      else:
+        dx = _DropoutFn.apply(dy, None, seed, threshold, site)      # (a gradient that is recorded itself follows)
+    return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
+
+
+def _seed_ok(seed) -> bool:
+  return seed.is_cuda and seed.dtype == torch.int64 and seed.shape == (2,) and seed.is_contiguous()
+
+
+def dropout(x, p, seed, site=0, residual=None, training=True):
+  """``residual`` (if given) plus ``x`` with each element kept with probability 1 - p and divided by it, else 0; rounded once.
+
+  What is kept follows from ``seed``, an int64 tensor {seed, step} on ``x``'s device, from ``site``, a number below 2^32 for the place
+  in the model, and from the element's place in ``x``: the same call, in the backward pass or a recomputed layer too, drops the same ones,
+  and nothing is stored for it.  Of the step the lower 32 bits count.  ``p`` counts in steps of 2^-16, to the nearest (the
+  elements that stay are divided by what that leaves).  A step that is counted up in place between forward and backward is an error of the
+  backward pass; give the next step's calls a new tensor, or count up behind the backward pass."""
+  p = float(p)
+  if not 0.0 <= p <= 1.0:
+    raise ValueError(f"dropout: p {p}")
+  if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+    raise ValueError(f"dropout: residual {residual.dtype} {tuple(residual.shape)} for {x.dtype} {tuple(x.shape)}")
+  if not x.is_floating_point():
+    raise ValueError(f"dropout: {x.dtype}")
+  threshold = round(p * 65536)
+  if not training or threshold == 0:
+    return x if residual is None else x + residual
+  if seed.shape != (2,) or seed.dtype != torch.int64 or seed.device != x.device:
+    raise ValueError(f"dropout: seed must be two int64 on the device of x, got {seed.dtype} {tuple(seed.shape)}")
+  if not 0 <= site < 2 ** 32:
+    raise ValueError(f"dropout: site {site}")
+  if use_kernels(x, residual) and unobserved():
+    return _DropoutFn.apply(x, residual, seed.contiguous(), threshold, site)
+  return ref.dropout(x, ref.dropout_keep(x.shape, threshold, seed, site), threshold, residual)
+
+
 # --------------------------------------------------------------------------- swiglu
 class _SwigluFn(torch.autograd.Function):
   @staticmethod
@@ -745,12 +878,33 @@ def swiglu(gate_up):
 
 
 # --------------------------------------------------------------------------- embedding
+def _embedding_grad(ids, table, dout, scale):
+  """The table's gradient in torch operations."""
+  ok = (ids >= 0) & (ids < table.shape[0])
+  rows = torch.where(ok[..., None], ref.wide(dout) * scale, 0.0).reshape(-1, table.shape[1])
+  sums = torch.zeros(table.shape, dtype=rows.dtype, device=table.device)
+  return sums.index_add(0, torch.where(ok, ids, 0).reshape(-1), rows).to(table.dtype)
+
+
+def _embedding_collect(ids, mg, dout, scale, overwrite):
+  """The gradient of a table that collects it in ``mg``."""
+  from . import kernels as k
+  dout, ids = dout.contiguous(), ids.contiguous()
+  if mg.data_ptr() % 16 == 0 and dout.data_ptr() % 16 == 0:
+    k.embedding_bwd_(dout, ids, mg, scale=scale, overwrite=overwrite)
+  else:
+    g = torch.empty(mg.shape, dtype=mg.dtype, device=mg.device)
+    k.embedding_bwd_(dout.clone(), ids, g, scale=scale, overwrite=True)
+    mg.copy_(g) if overwrite else mg.add_(g)
+
+
 class _EmbeddingFn(torch.autograd.Function):
   @staticmethod
-  def forward(ctx, ids, table):
+  def forward(ctx, ids, table, scale):
     from . import kernels as k
     ctx.save_for_backward(ids, table)
-    return k.embedding_fwd(table, ids.contiguous())
+    ctx.scale = scale
+    return k.embedding_fwd(table, ids.contiguous(), scale=scale)
 
   @staticmethod
   def backward(ctx, dout):
@@ -758,14 +912,14 @@ class _EmbeddingFn(torch.autograd.Function):
     ids, table = ctx.saved_tensors
     mg = getattr(table, "main_grad", None)
     if mg is not None:
-      if getattr(table, "grad_overwrite", False):
-        mg.zero_()
-        table.grad_overwrite = False
-      k.embedding_bwd_(dout.contiguous(), ids.contiguous(), mg)
-      return None, None
-    g = torch.zeros(table.shape, dtype=torch.float32, device=table.device)
-    k.embedding_bwd_(dout.contiguous(), ids.contiguous(), g)
-    return None, g.to(table.dtype)
+      _embedding_collect(ids, mg, dout, ctx.scale, bool(getattr(table, "grad_overwrite", False)))
+      table.grad_overwrite = False
+      return None, None, None
+    if batched(dout) or (torch.is_grad_enabled() and dout.requires_grad) or not use_kernels(dout, table):
+      return None, _embedding_grad(ids, table, dout, ctx.scale), None
+    dout = dout.contiguous()
+    g = torch.empty(table.shape, dtype=table.dtype, device=table.device)
+    return None, k.embedding_bwd_(dout if dout.data_ptr() % 16 == 0 else dout.clone(), ids.contiguous(), g, scale=ctx.scale, overwrite=True), None
 
 
 class _EmbeddingPeerFn(torch.autograd.Function):
@@ -784,14 +938,12 @@ class _EmbeddingPeerFn(torch.autograd.Function):
 
   @staticmethod
   def backward(ctx, dout):
-    from . import kernels as k
     (ids,) = ctx.saved_tensors
     table = ctx.table
-    mg = table.main_grad
-    if overwrites_grad(table):
-      mg.zero_()
+    overwrite = overwrites_grad(table)
+    _embedding_collect(ids, table.main_grad, dout, 1.0, overwrite)
+    if overwrite:
       table.grad_overwrite = False
-    k.embedding_bwd_(dout.contiguous(), ids.contiguous(), mg)
     return None, None, None
 
 
@@ -799,14 +951,21 @@ def embedding_peer(ids, table, peer):
   return _EmbeddingPeerFn.apply(ids, table, peer)
 
 
-def embedding(ids, table):
-  if (nat := _native()) is not None:
+def embedding(ids, table, scale=None):
+  """Rows ``ids`` of the table, times the number ``scale`` (rounded once; None: as they are).  On the kernels an id without a row gives
+  zeros and no gradient, and the table's gradient adds up each id's tokens in their order: it is the same in every run."""
+  if scale is not None:
+    scale = float(scale)
+    if not math.isfinite(scale):
+      raise ValueError(f"embedding: scale {scale}")
+  if (nat := _native()) is not None and scale is None:
     y = nat.embedding(ids, table)
     if y is not None:
       return y
-  if use_kernels(table) and table.shape[1] % 8 == 0:
-    return _EmbeddingFn.apply(ids, table)
-  return F.embedding(ids, table)
+  if use_kernels(table) and table.shape[1] % 8 == 0 and (scale is None or unobserved()):
+    return _EmbeddingFn.apply(ids, table, 1.0 if scale is None else scale)
+  y = F.embedding(ids, table)
+  return y if scale is None else (ref.wide(y) * scale).to(table.dtype)
 
 
 # --------------------------------------------------------------------------- attention

@@ -14,7 +14,7 @@ from ._lib import (EPI_BF16, EPI_BF16_ACC, EPI_BF16_RES, EPI_F32, EPI_F32_ACC, E
 
 __all__ = [
   "gemm", "rmsnorm_fwd", "rmsnorm_bwd", "rope_", "swiglu_fwd", "swiglu_bwd", "ce_fwd_bwd_", "adamw_",
-  "sumsq_", "clip_coef_", "embedding_fwd", "embedding_bwd_", "cast_f32_to_bf16_",
+  "sumsq_", "clip_coef_", "embedding_fwd", "embedding_bwd_", "qk_norm_fwd", "qk_norm_bwd", "dropout", "cast_f32_to_bf16_",
   "EPI_BF16", "EPI_F32", "EPI_F32_ACC", "EPI_BF16_ACC", "EPI_BF16_RES", "EPI_SWIGLU", "EPI_SWIGLU_BWD",
 ]
 
@@ -181,22 +181,81 @@ def clip_coef_(sumsq, max_norm, coef, norm_out):
   check(lib().tpb_clip_coef(ptr(sumsq), float(max_norm or 0.0), ptr(coef), ptr(norm_out), stream_ptr()), "clip_coef")
 
 
-def embedding_fwd(table, ids, row0=0):
+def embedding_fwd(table, ids, row0=0, scale=1.0):
+  """``scale`` times rows ``ids - row0`` of the table; zeros for ids without a row in it."""
   flat = ids.reshape(-1)
   assert flat.dtype == torch.int64 and flat.is_contiguous() and table.is_contiguous()
   out = torch.empty(flat.numel(), table.shape[1], dtype=table.dtype, device=table.device)
-  check(lib().tpb_embedding_fwd(ptr(table), ptr(flat), ptr(out), flat.numel(), table.shape[1], table.shape[0], row0,
-                                stream_ptr()), "embedding_fwd")
+  with torch.cuda.device(table.device):
+    check(lib().tpb_embedding_fwd(ptr(table), ptr(flat), ptr(out), flat.numel(), table.shape[1], table.shape[0], row0,
+                                  float(scale), stream_ptr()), "embedding_fwd")
   return out.view(*ids.shape, table.shape[1])
 
 
-def embedding_bwd_(dout, ids, dtable, row0=0):
+def embedding_bwd_(dout, ids, dtable, row0=0, scale=1.0, overwrite=False):
+  """Adds ``scale`` times the sum of every id's rows of ``dout``, in the tokens' order, to ``dtable`` (fp32 or bf16, row 0 of which
+  is id ``row0``); with ``overwrite`` it becomes that sum, rows without a token zeros."""
   flat = ids.reshape(-1)
-  d2 = dout.reshape(flat.numel(), -1)
+  d2 = dout.reshape(flat.numel(), dtable.shape[1])
+  assert flat.is_contiguous() and flat.dtype == torch.int64
   assert d2.is_contiguous() and dtable.is_contiguous() and d2.dtype == torch.bfloat16
-  check(lib().tpb_embedding_bwd(ptr(d2), ptr(flat), ptr(dtable), flat.numel(), d2.shape[1], dtable.shape[0], row0,
-                                int(dtable.dtype == torch.float32), stream_ptr()), "embedding_bwd")
+  t, (v, d) = flat.numel(), dtable.shape
+  with torch.cuda.device(dtable.device):
+    scratch = torch.empty(lib().tpb_embedding_bwd_scratch(t, v, d), dtype=torch.uint8, device=dtable.device)
+    check(lib().tpb_embedding_bwd(ptr(d2), ptr(flat), ptr(dtable), ptr(scratch), t, d, v, row0, int(dtable.dtype == torch.float32),
+                                  int(not overwrite), float(scale), stream_ptr()), "embedding_bwd")
   return dtable
+
+
+def _row_pitch(x):
+  """Distance of the rows of a [B, S, C] tensor if it is one, else None."""
+  b, s, c = x.shape
+  pitch = c if b * s <= 1 else x.stride(1) if s > 1 else x.stride(0)
+  return pitch if x.stride(2) == 1 and (b == 1 or s == 1 or x.stride(0) == s * pitch) else None
+
+
+def _qk_norm_rows(qkv):
+  """The projection as rows of 16-byte vectors, and their distance."""
+  pitch = _row_pitch(qkv)
+  if pitch is None or pitch % 8 or qkv.data_ptr() % 16:
+    return qkv.clone(memory_format=torch.contiguous_format), qkv.shape[2]
+  return qkv, pitch
+
+
+def qk_norm_fwd(qkv, hq, hkv, d, q_weight, k_weight, cos, sin, seq_len, pos, eps, interleaved):
+  """Normalised and rotated queries [B, S, hq, d] and keys [B, S, hkv, d] of ``qkv`` [B, S, (hq + 2 hkv) * d]."""
+  x, pitch = _qk_norm_rows(qkv)
+  b, s, _ = x.shape
+  q = torch.empty(b, s, hq, d, dtype=x.dtype, device=x.device)
+  k = torch.empty(b, s, hkv, d, dtype=x.dtype, device=x.device)
+  with torch.cuda.device(x.device):
+    check(lib().tpb_qk_norm_fwd(ptr(x), pitch, ptr(q_weight), ptr(k_weight), ptr(cos), ptr(sin), cos.shape[0], ptr(pos), seq_len,
+                                ptr(q), ptr(k), b * s, hq, hkv, d, 2 * cos.shape[1], float(eps), int(interleaved), stream_ptr()),
+          f"qk_norm_fwd {tuple(qkv.shape)}")
+  return q, k
+
+
+def qk_norm_bwd(dq, dk, dv, qkv, hq, hkv, d, q_weight, k_weight, cos, sin, seq_len, pos, eps, interleaved, want_dw):
+  """Gradients (of ``qkv``, fp32 [2, d] of the two weights or None)."""
+  x, pitch = _qk_norm_rows(qkv)
+  b, s, c = x.shape
+  assert all(t.is_contiguous() for t in (dq, dk, dv))
+  dx = torch.empty(b, s, c, dtype=x.dtype, device=x.device)
+  with torch.cuda.device(x.device):
+    sums = torch.empty(lib().tpb_qk_norm_bwd_scratch(b * s, d), dtype=torch.float32, device=x.device) if want_dw else None
+    check(lib().tpb_qk_norm_bwd(ptr(x), pitch, ptr(q_weight), ptr(k_weight), ptr(cos), ptr(sin), cos.shape[0], ptr(pos), seq_len,
+                                ptr(dq), ptr(dk), ptr(dv), ptr(dx), ptr(sums), None, None, b * s, hq, hkv, d, 2 * cos.shape[1],
+                                float(eps), int(interleaved), stream_ptr()), f"qk_norm_bwd {tuple(qkv.shape)}")
+  return dx, (sums[: 2 * d].view(2, d) if want_dw else None)
+
+
+def dropout(x, threshold, seed, site, residual=None):
+  """See :func:`functional.dropout`; ``threshold`` is the probability in steps of 2^-16."""
+  assert x.is_contiguous() and (residual is None or residual.is_contiguous())
+  y = torch.empty_like(x)
+  with torch.cuda.device(x.device):
+    check(lib().tpb_dropout(ptr(x), ptr(residual), ptr(y), ptr(seed), x.numel(), threshold, site, stream_ptr()), "dropout")
+  return y
 
 
 def cast_f32_to_bf16_(src, dst, scale=1.0, accumulate=False):

@@ -66,6 +66,92 @@ def rope_apply_complex(x, freqs_cis):
   return torch.view_as_real(xc * f).flatten(3).type_as(x)
 
 
+def wide(t: torch.Tensor) -> torch.Tensor:
+  """In fp32, or in 64 bits where it is."""
+  return t if t.dtype == torch.float64 else t.float()
+
+
+def _qk_tables(qkv, cos_half, sin_half, seq_len, pos):
+  """cos and sin of every token, [B, S, 1, columns / 2]; positions outside the tables count as their nearest."""
+  b, s = qkv.shape[:2]
+  p = pos.reshape(b, s).long() if pos is not None else (torch.arange(b * s, device=qkv.device) % seq_len).view(b, s)
+  p = p.clamp(0, cos_half.shape[0] - 1)
+  return cos_half[p][:, :, None], sin_half[p][:, :, None]
+
+
+def _turn(y, cos, sin, interleaved):
+  """The leading columns of [..., D] rotated by pairs (i, i + half), or (2i, 2i + 1)."""
+  n = 2 * cos.shape[-1]
+  u, v = (y[..., 0:n:2], y[..., 1:n:2]) if interleaved else (y[..., : n // 2], y[..., n // 2: n])
+  turned = u * cos - v * sin, v * cos + u * sin
+  turned = torch.stack(turned, -1).reshape(*u.shape[:-1], n) if interleaved else torch.cat(turned, -1)
+  return torch.cat([turned, y[..., n:]], -1)
+
+
+def qk_norm_rope(qkv, cos_half, sin_half, hq, hkv, d, seq_len, q_weight=None, k_weight=None, eps=1e-6, pos=None, interleaved=False):
+  """Queries and keys of a fused [B, S, (hq + 2 hkv) * d] projection, each head normalised (and weighted), its leading
+  2 * cos_half.shape[1] columns rotated, rounded once; and the values as they are."""
+  b, s, _ = qkv.shape
+  x = qkv.reshape(b, s, hq + 2 * hkv, d)
+  cos, sin = _qk_tables(qkv, cos_half, sin_half, seq_len, pos)
+
+  def head(t, w):
+    y = wide(t)
+    y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + eps)
+    return _turn(y if w is None else y * wide(w), cos, sin, interleaved).to(qkv.dtype)
+
+  return head(x[:, :, :hq], q_weight), head(x[:, :, hq: hq + hkv], k_weight), x[:, :, hq + hkv:]
+
+
+def qk_norm_rope_grad(dq, dk, dv, qkv, cos_half, sin_half, hq, hkv, d, seq_len, q_weight=None, k_weight=None, eps=1e-6, pos=None,
+                      interleaved=False):
+  """Gradients of :func:`qk_norm_rope` (of the projection and the two weights) by their formulas."""
+  b, s, _ = qkv.shape
+  x = qkv.reshape(b, s, hq + 2 * hkv, d)
+  cos, sin = _qk_tables(qkv, cos_half, sin_half, seq_len, pos)
+
+  def head(dy, t, w):
+    t = wide(t)
+    r = torch.rsqrt(t.square().mean(-1, keepdim=True) + eps)
+    g = _turn(wide(dy), cos, -sin, interleaved)
+    dw = None if w is None else (g * (t * r)).sum((0, 1, 2)).to(w.dtype)
+    g = g if w is None else g * wide(w)
+    return (r * g - t * (r * r * r * (g * t).mean(-1, keepdim=True))).to(qkv.dtype), dw
+
+  gq, dwq = head(dq, x[:, :, :hq], q_weight)
+  gk, dwk = head(dk, x[:, :, hq: hq + hkv], k_weight)
+  return torch.cat([gq, gk, dv.to(qkv.dtype)], 2).reshape(b, s, (hq + 2 * hkv) * d), dwq, dwk
+
+
+def philox(counter, key):
+  """Philox4x32-10 (Salmon et al., 2011): four 32-bit words of a counter and two of a key, as int64 tensors (or numbers), to four
+  random words."""
+  low = 0xFFFFFFFF
+  c0, c1, c2, c3 = counter
+  k0, k1 = key
+  for _ in range(10):
+    p, q = c0 * 0xD2511F53, c2 * 0xCD9E8D57            # (the low 64 bits of a product are the same with a sign)
+    c0, c1, c2, c3 = (q >> 32 & low) ^ c1 ^ k0, q & low, (p >> 32 & low) ^ c3 ^ k1, p & low
+    k0, k1 = k0 + 0x9E3779B9 & low, k1 + 0xBB67AE85 & low
+  return c0, c1, c2, c3
+
+
+def dropout_keep(shape, threshold, seed, site):
+  """Whether each element of a tensor of this shape stays."""
+  n = math.prod(shape)
+  i = torch.arange((n + 7) // 8, device=seed.device)
+  low = 0xFFFFFFFF
+  words = philox((i & low, i >> 32, (seed[1] & low).expand_as(i), torch.full_like(i, site)), (seed[0] & low, seed[0] >> 32 & low))
+  bits = torch.stack([half for w in words for half in (w & 0xFFFF, w >> 16)], -1).reshape(-1)[:n]
+  return (bits >= threshold).view(shape)
+
+
+def dropout(x, keep, threshold, residual=None):
+  """``x`` scaled where it stays, zeros elsewhere, and the residual's sum, rounded once."""
+  y = torch.where(keep, wide(x) * (65536 / (65536 - threshold) if threshold < 65536 else 0.0), 0.0)
+  return (y if residual is None else y + wide(residual)).to(x.dtype)
+
+
 def swiglu(gate_up: torch.Tensor) -> torch.Tensor:
   """silu(gate) * up for a fused ``[..., 2F]`` tensor laid out as [gate | up]."""
   g, u = gate_up.chunk(2, dim=-1)
