@@ -38,6 +38,9 @@ std::atomic<long long> g_launches{0};
 PyObject* g_check = nullptr;         // _lib.check: raises KernelError for a non-zero code
 PyObject* g_late_wgrads = nullptr;   // functional._deliver_wgrads: weights that got a main_grad after their forward
 PyObject* g_late_norm = nullptr;     // functional._norm_wgrad
+PyObject* g_embedding_backward = nullptr;   // functional._embedding_backward, _qk_norm_backward and _dropout_backward: gradients that are
+PyObject* g_qk_norm_backward = nullptr;     // recorded themselves, several at once, collected in a main_grad that came late, or of saved
+PyObject* g_dropout_backward = nullptr;     // tensors that hooks gave back in another form
 PyObject* g_main_grad = nullptr;     // "main_grad"
 
 void check(int rc, const char* what) {
@@ -82,6 +85,12 @@ Tensor empty_as(const Tensor& t, at::IntArrayRef sizes) { return empty_like_type
 const void* cptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* mptr(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 const int* iptr(const Tensor& t) { return static_cast<const int*>(cptr(t)); }
+
+// The checks of indices on the host are on: the Python definitions do them.
+bool bounds_checked() {
+  const char* v = std::getenv("TPB_DEBUG_BOUNDS");
+  return v && v[0] == '1' && !v[1];
+}
 
 std::vector<int64_t> with_last(const Tensor& t, int64_t last) {
   auto s = t.sizes().vec();
@@ -908,19 +917,238 @@ bool mla_pack_into(py::handle kv_, py::handle rot_, int64_t heads, int64_t dn, i
 }
 
 // ------------------------------------------------------------------------------------------- without gradients only
-py::object embedding(py::handle ids_, py::handle table_) {
+// A tensor as an argument of a Python function.
+py::object to_python(const Tensor& t) {
+  return t.defined() ? py::reinterpret_steal<py::object>(THPVariable_Wrap(t)) : py::object(py::none());
+}
+Tensor from_python(const py::object& o) { return o.is_none() ? Tensor() : o.cast<Tensor>(); }
+// A gradient as the kernels read it, or nothing: it is of another kind, or recorded itself.
+Tensor dense_grad(const Tensor& g) {
+  if (!plain(g) || (at::GradMode::is_enabled() && g.requires_grad())) return Tensor();
+  const Tensor d = g.contiguous();
+  return aligned(d) ? d : d.clone();
+}
+
+bool ids_of(const Tensor& ids, const Tensor& table) {
+  return plain_rows(ids, at::kLong) && small(ids.numel()) && ids.get_device() == table.get_device();
+}
+Tensor embedding_fwd(const Tensor& ids, const Tensor& table, double scale) {
+  auto sizes = ids.sizes().vec();
+  sizes.push_back(table.size(1));
+  Tensor y = empty_as(table, sizes);
+  check(tpb_embedding_fwd(cptr(table), static_cast<const long long*>(cptr(ids)), mptr(y), (int)ids.numel(), (int)table.size(1),
+                          table.size(0), 0, (float)scale, stream()),
+        "embedding_fwd");
+  return y;
+}
+
+struct EmbeddingFn : Function<EmbeddingFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& table, const Tensor& ids, double scale) {
+    ctx->save_for_backward({table, ids});
+    ctx->saved_data["s"] = scale;
+    return embedding_fwd(ids, table, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &table = saved[0], &ids = saved[1];
+    const double scale = ctx->saved_data["s"].toDouble();
+    const Tensor dout = dense_grad(grads[0]);
+    if (!dout.defined() || !plain_rows(table) || !ids_of(ids, table) || any_main_grad(&table, 1)) {
+      py::gil_scoped_acquire gil;
+      return {from_python(py::reinterpret_borrow<py::object>(g_embedding_backward)(to_python(ids), to_python(table), to_python(grads[0]), scale)),
+              Tensor(), Tensor()};
+    }
+    const int tokens = (int)ids.numel(), rows = (int)table.size(0), dim = (int)table.size(1);
+    Tensor dtable = empty_as(table, table.sizes());
+    Tensor scratch = empty_like_type(table, {tpb_embedding_bwd_scratch(tokens, rows, dim)}, at::kByte);
+    check(tpb_embedding_bwd(cptr(dout), static_cast<const long long*>(cptr(ids)), mptr(dtable), mptr(scratch), tokens, dim, rows, 0, 0, 0,
+                            (float)scale, stream()),
+          "embedding_bwd");
+    return {dtable, Tensor(), Tensor()};
+  }
+};
+
+py::object embedding(py::handle ids_, py::handle table_, double scale) {
   Tensor ids, table, y;
-  if (at::GradMode::is_enabled() || !unobserved() || !unpack(ids_, ids) || !unpack(table_, table) || !plain_rows(ids, at::kLong) ||
-      !plain_rows(table) || table.dim() != 2 || table.size(1) % 8 || ids.get_device() != table.get_device() || !small(ids.numel()))
+  if (!unobserved() || !unpack(ids_, ids) || !unpack(table_, table) || !plain_rows(table) || table.dim() != 2 || table.size(1) % 8 ||
+      !aligned(table) || !small(table.size(0)) || !small(table.size(1)) || !ids_of(ids, table) ||
+      table.get_device() != c10::cuda::current_device())
     return py::none();
+  const bool rec = at::GradMode::is_enabled() && recording(table);
+  if (rec && has_main_grad(table_.ptr())) return py::none();
   {
     py::gil_scoped_release nogil;
-    auto sizes = ids.sizes().vec();
-    sizes.push_back(table.size(1));
-    y = empty_as(table, sizes);
-    check(tpb_embedding_fwd(cptr(table), static_cast<const long long*>(cptr(ids)), mptr(y), (int)ids.numel(), (int)table.size(1),
-                            table.size(0), 0, 1.f, stream()),
-          "embedding_fwd");
+    y = rec ? EmbeddingFn::apply(table, ids, scale) : embedding_fwd(ids, table, scale);
+  }
+  return py::cast(y);
+}
+
+// ------------------------------------------------------------------------------------------- norms of query and key heads
+struct QkArgs {
+  int64_t hq, hkv, d, seq;
+  bool interleaved;
+  double eps;
+};
+
+// Distance of a projection's rows; 0: it has none, or they are not what the kernels read.
+int64_t row_pitch(const Tensor& x) {
+  const int64_t b = x.size(0), s = x.size(1), pitch = b * s <= 1 ? x.size(2) : s > 1 ? x.stride(1) : x.stride(0);
+  return x.stride(2) == 1 && (b == 1 || s == 1 || x.stride(0) == s * pitch) && pitch > 0 && pitch % 8 == 0 && aligned(x) ? pitch : 0;
+}
+bool qk_tensors(const QkArgs& a, const Tensor& x, const Tensor& qw, const Tensor& kw, const Tensor& cos, const Tensor& sin, const Tensor& pos) {
+  if (!plain(x) || x.dim() != 3 || x.numel() == 0 || x.size(2) != (a.hq + 2 * a.hkv) * a.d || !small(x.size(0) * x.size(1) * (a.hq + a.hkv)) ||
+      row_pitch(x) == 0)
+    return false;
+  for (const Tensor* w : {&qw, &kw})
+    if (w->defined() &&
+        (!plain_rows(*w) || w->dim() != 1 || w->size(0) != a.d || !aligned(*w) || w->get_device() != x.get_device()))
+      return false;
+  for (const Tensor* t : {&cos, &sin})
+    if (!plain_rows(*t, at::kFloat) || t->dim() != 2 || t->sizes() != cos.sizes() || t->size(1) % 8 || 2 * t->size(1) > a.d ||
+        !small(t->size(0)) || !aligned(*t) || t->get_device() != x.get_device() || recording(*t))
+      return false;
+  if (!pos.defined()) return a.seq > 0 && a.seq <= cos.size(0);
+  return plain_rows(pos, at::kInt) && pos.numel() == x.size(0) * x.size(1) && pos.get_device() == x.get_device();
+}
+
+variable_list qk_fwd(const QkArgs& a, const Tensor& x, const Tensor& qw, const Tensor& kw, const Tensor& cos, const Tensor& sin, const Tensor& pos) {
+  const int64_t b = x.size(0), s = x.size(1);
+  Tensor q = empty_as(x, {b, s, a.hq, a.d}), k = empty_as(x, {b, s, a.hkv, a.d});
+  check(tpb_qk_norm_fwd(cptr(x), row_pitch(x), cptr(qw), cptr(kw), static_cast<const float*>(cptr(cos)), static_cast<const float*>(cptr(sin)),
+                        (int)cos.size(0), iptr(pos), (int)a.seq, mptr(q), mptr(k), (int)(b * s), (int)a.hq, (int)a.hkv, (int)a.d,
+                        (int)(2 * cos.size(1)), (float)a.eps, a.interleaved, stream()),
+        "qk_norm_fwd");
+  return {q, k, x.as_strided({b, s, a.hkv, a.d}, {x.stride(0), x.stride(1), a.d, 1}, x.storage_offset() + (a.hq + a.hkv) * a.d)};
+}
+
+struct QkNormFn : Function<QkNormFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& qw, const OptTensor& kw, const Tensor& cos,
+                               const Tensor& sin, const OptTensor& pos, int64_t hq, int64_t hkv, int64_t d, int64_t seq, double eps,
+                               bool interleaved) {
+    ctx->save_for_backward({x, get(qw), get(kw), cos, sin, get(pos)});
+    ctx->saved_data["i"] = std::vector<int64_t>{hq, hkv, d, seq, interleaved};
+    ctx->saved_data["e"] = eps;
+    return qk_fwd({hq, hkv, d, seq, interleaved, eps}, x, get(qw), get(kw), cos, sin, get(pos));
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list t = ctx->get_saved_variables();
+    const Tensor &x = t[0], *w = &t[1], &cos = t[3], &sin = t[4], &pos = t[5];
+    const auto i = ctx->saved_data["i"].toIntVector();
+    const QkArgs a{i[0], i[1], i[2], i[3], i[4] != 0, ctx->saved_data["e"].toDouble()};
+    bool need[3] = {ctx->needs_input_grad(0), false, false};
+    for (int j = 0, edge = 1; j < 2; ++j)
+      if (w[j].defined()) need[1 + j] = ctx->needs_input_grad(edge++);
+    variable_list out(12);
+    Tensor dy[3];
+    bool own = !at::GradMode::is_enabled() && qk_tensors(a, x, w[0], w[1], cos, sin, pos);
+    for (int j = 0; own && j < 3; ++j) {
+      dy[j] = dense_grad(grads[j]);
+      own = dy[j].defined();
+    }
+    for (int j = 0; own && j < 2; ++j) own = !need[1 + j] || !any_main_grad(&w[j], 1);
+    if (!own) {
+      py::gil_scoped_acquire gil;
+      const py::object r = py::reinterpret_borrow<py::object>(g_qk_norm_backward)(
+          to_python(grads[0]), to_python(grads[1]), to_python(grads[2]), to_python(x), to_python(w[0]), to_python(w[1]), to_python(cos),
+          to_python(sin), to_python(pos), py::make_tuple(a.hq, a.hkv, a.d, a.seq, a.eps, a.interleaved), py::make_tuple(need[0], need[1], need[2]));
+      for (int j = 0; j < 3; ++j) out[j] = from_python(r[py::int_(j)]);
+      return out;
+    }
+    const int64_t tokens = x.size(0) * x.size(1);
+    Tensor dx = empty_as(x, x.sizes()), sums, dw[2];
+    if (need[1] || need[2]) sums = empty_like_type(x, {tpb_qk_norm_bwd_scratch((int)tokens, (int)a.d)}, at::kFloat);
+    for (int j = 0; j < 2; ++j)
+      if (need[1 + j]) dw[j] = empty_as(w[j], {a.d});
+    check(tpb_qk_norm_bwd(cptr(x), row_pitch(x), cptr(w[0]), cptr(w[1]), static_cast<const float*>(cptr(cos)),
+                          static_cast<const float*>(cptr(sin)), (int)cos.size(0), iptr(pos), (int)a.seq, cptr(dy[0]), cptr(dy[1]), cptr(dy[2]),
+                          mptr(dx), static_cast<float*>(mptr(sums)), mptr(dw[0]), mptr(dw[1]), (int)tokens, (int)a.hq, (int)a.hkv, (int)a.d,
+                          (int)(2 * cos.size(1)), (float)a.eps, a.interleaved, stream()),
+          "qk_norm_bwd");
+    if (need[0]) out[0] = dx;
+    out[1] = dw[0];
+    out[2] = dw[1];
+    return out;
+  }
+};
+
+py::object qk_norm_rope(py::handle x_, py::handle cos_, py::handle sin_, py::handle hq_, py::handle hkv_, py::handle d_, py::handle seq_,
+                        py::handle qw_, py::handle kw_, py::handle eps_, py::handle pos_, bool interleaved) {
+  Tensor x, cos, sin, qw, kw, pos;
+  QkArgs a;
+  a.interleaved = interleaved;
+  if (!whole(hq_, 0, a.hq) || !whole(hkv_, 0, a.hkv) || !whole(d_, 0, a.d) || !whole(seq_, 0, a.seq) || !real(eps_, -1.0, a.eps) ||
+      !unobserved() || !unpack(x_, x) || !unpack(cos_, cos) || !unpack(sin_, sin) || !unpack(qw_, qw) || !unpack(kw_, kw) ||
+      !unpack(pos_, pos))
+    return py::none();
+  if (a.hq < 1 || a.hkv < 1 || !small(a.hq) || !small(a.hkv) || a.d < 16 || a.d > 512 || a.d % 16 || !(a.eps >= 0x1p-126 && a.eps < 0x1p127) ||
+      !small(a.seq) || !qk_tensors(a, x, qw, kw, cos, sin, pos) || x.get_device() != c10::cuda::current_device() ||
+      (pos.defined() && bounds_checked()))
+    return py::none();
+  variable_list y;
+  const bool rec = at::GradMode::is_enabled() && (recording(x) || (qw.defined() && recording(qw)) || (kw.defined() && recording(kw)));
+  if (rec && (has_main_grad(qw_.ptr()) || has_main_grad(kw_.ptr()))) return py::none();
+  {
+    py::gil_scoped_release nogil;
+    y = rec ? QkNormFn::apply(x, some(qw), some(kw), cos, sin, some(pos), a.hq, a.hkv, a.d, a.seq, a.eps, a.interleaved)
+            : qk_fwd(a, x, qw, kw, cos, sin, pos);
+  }
+  return py::make_tuple(y[0], y[1], y[2]);
+}
+
+// ------------------------------------------------------------------------------------------- dropout
+Tensor dropout_now(const Tensor& x, const Tensor& residual, const Tensor& seed, int64_t threshold, int64_t site) {
+  Tensor y = empty_as(x, x.sizes());
+  check(tpb_dropout(cptr(x), cptr(residual), mptr(y), static_cast<const long long*>(cptr(seed)), x.numel(), (int)threshold, (unsigned)site,
+                    stream()),
+        "dropout");
+  return y;
+}
+bool seed_of(const Tensor& seed, const Tensor& x) {
+  return plain_rows(seed, at::kLong) && seed.dim() == 1 && seed.size(0) == 2 && seed.get_device() == x.get_device();
+}
+
+struct DropoutFn : Function<DropoutFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, const Tensor& seed, int64_t threshold, int64_t site) {
+    ctx->save_for_backward({seed});
+    ctx->saved_data["i"] = std::vector<int64_t>{threshold, site, residual.has_value()};
+    ctx->saved_data["z"] = x.sizes().vec();
+    return dropout_now(x, get(residual), seed, threshold, site);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor seed = ctx->get_saved_variables()[0];
+    const auto i = ctx->saved_data["i"].toIntVector();
+    variable_list out(5);
+    if (i[2] && ctx->needs_input_grad(1)) out[1] = grads[0];
+    if (!ctx->needs_input_grad(0)) return out;
+    const Tensor dy = dense_grad(grads[0]);
+    if (dy.defined() && seed_of(seed, dy)) {
+      out[0] = dropout_now(dy, Tensor(), seed, i[0], i[1]);
+    } else {
+      py::gil_scoped_acquire gil;
+      out[0] = from_python(py::reinterpret_borrow<py::object>(g_dropout_backward)(to_python(grads[0]), to_python(seed), i[0], i[1],
+                                                                                 py::tuple(py::cast(ctx->saved_data["z"].toIntVector()))));
+    }
+    return out;
+  }
+};
+
+py::object dropout(py::handle x_, py::handle p_, py::handle seed_, py::handle site_, py::handle res_) {
+  Tensor x, seed, residual, y;
+  double p;
+  int64_t site;
+  if (!real(p_, -1.0, p) || !whole(site_, -1, site) || !unobserved() || !unpack(x_, x) || !unpack(seed_, seed) || !unpack(res_, residual) ||
+      !plain_rows(x) || !aligned(x) || !seed_of(seed, x) || x.get_device() != c10::cuda::current_device())
+    return py::none();
+  if (residual.defined() && (!plain_rows(residual) || !aligned(residual) || residual.sizes() != x.sizes() || residual.get_device() != x.get_device()))
+    return py::none();
+  if (!(p >= 0.0 && p <= 1.0) || site < 0 || site > 0xffffffffLL) return py::none();
+  const int64_t threshold = std::llrint(p * 65536);
+  if (threshold == 0) return py::none();
+  {
+    py::gil_scoped_release nogil;
+    y = at::GradMode::is_enabled() && (recording(x) || (residual.defined() && recording(residual)))
+            ? DropoutFn::apply(x, some(residual), seed, threshold, site)
+            : dropout_now(x, residual, seed, threshold, site);
   }
   return py::cast(y);
 }
@@ -1057,12 +1285,6 @@ py::object grouped_mlp_few_rows(py::handle x_, py::handle rw_, py::handle idx_, 
 // Memory on t's device, for operators that record nothing: straight from the allocator, ahead of every dispatch.
 Tensor fresh(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type) {
   return at::detail::empty_cuda(sizes, type, t.device(), std::nullopt);
-}
-
-// The checks of indices on the host are on: the Python definitions do them.
-bool bounds_checked() {
-  const char* v = std::getenv("TPB_DEBUG_BOUNDS");
-  return v && v[0] == '1' && !v[1];
 }
 
 // The pools of a paged cache and, where they are e4m3, their scales: layouts that the kernels take, on the current device; see
@@ -1232,10 +1454,14 @@ py::object sample_tokens(py::handle x_, py::handle u_, py::handle t_, py::handle
 }  // namespace
 
 PYBIND11_MODULE(_tpb_torch, m) {
-  m.def("configure", [](py::object check_fn, py::object late_wgrads, py::object late_norm) {
+  m.def("configure", [](py::object check_fn, py::object late_wgrads, py::object late_norm, py::object embedding_backward,
+                        py::object qk_norm_backward, py::object dropout_backward) {
     g_check = check_fn.release().ptr();
     g_late_wgrads = late_wgrads.release().ptr();
     g_late_norm = late_norm.release().ptr();
+    g_embedding_backward = embedding_backward.release().ptr();
+    g_qk_norm_backward = qk_norm_backward.release().ptr();
+    g_dropout_backward = dropout_backward.release().ptr();
     g_main_grad = PyUnicode_InternFromString("main_grad");
   });
   m.def("launch_count", []() { return g_launches.load(); });
@@ -1253,6 +1479,8 @@ PYBIND11_MODULE(_tpb_torch, m) {
   m.def("mla_pack", &mla_pack);
   m.def("mla_pack_into", &mla_pack_into);
   m.def("embedding", &embedding);
+  m.def("qk_norm_rope", &qk_norm_rope);
+  m.def("dropout", &dropout);
   m.def("absorb_supported", &absorb_supported);
   m.def("absorb_step", &absorb_step);
   m.def("linear_f32", &linear_f32);

@@ -13,6 +13,29 @@ BF16 = torch.bfloat16
 HALF = 2.0 ** -8              # a rounding to bf16
 
 
+@pytest.fixture(autouse=True, params=["native", "python"])
+def way(request, monkeypatch):
+  """The operators as native torch functions, and their Python definitions over the same kernels."""
+  if request.param == "python":
+    monkeypatch.setattr(ops, "_native", lambda: None)
+  return request.param
+
+
+def test_plain_calls_are_native(cuda_lib, way):
+  g = torch.Generator(device="cuda").manual_seed(0)
+  cos, sin = _tables(9, 32)
+  x, table, seed = _randn(g, 2, 9, 4 * 64), _randn(g, 50, 64), torch.tensor([1, 2], device="cuda")
+  w, ids = _randn(g, 64), torch.randint(0, 50, (2, 9), generator=g, device="cuda")
+  for grad in (False, True):
+    for t in (x, table, w):
+      t.requires_grad_(grad)
+    ws = [None, w]
+    outs = [ops.embedding(ids, table), ops.embedding(ids, table, scale=2.0), ops.dropout(x, 0.1, seed), ops.dropout(x, 0.1, seed, residual=x)]
+    outs += [ops.qk_norm_rope(x, cos, sin, 2, 1, 64, 9, a, b)[0] for a in ws for b in ws]
+    for y in outs:
+      assert y.requires_grad == grad and (not grad or ("CppFunction" in type(y.grad_fn).__name__) == (way == "native"))
+
+
 def _randn(g, *shape, std=1.0):
   return (torch.randn(*shape, generator=g, device="cuda") * std).to(BF16)
 

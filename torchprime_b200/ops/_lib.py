@@ -71,7 +71,8 @@ def _load_native():
   spec = importlib.util.spec_from_file_location("_tpb_torch", path)
   mod = importlib.util.module_from_spec(spec)
   spec.loader.exec_module(mod)
-  mod.configure(check, functional._deliver_wgrads, functional._norm_wgrad)
+  mod.configure(check, functional._deliver_wgrads, functional._norm_wgrad, functional._embedding_backward, functional._qk_norm_backward,
+                functional._dropout_backward)
   _native = mod
 
 

@@ -98,6 +98,12 @@ def in_recomputed_forward() -> bool:
 
 
 # --------------------------------------------------------------------------- helpers
+def _dense(t):
+  """Contiguous and 16-byte aligned."""
+  t = t.contiguous()
+  return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _adjacent(ts) -> bool:
   for a, b in zip(ts[:-1], ts[1:]):
     if not (a.is_contiguous() and b.is_contiguous()):
@@ -723,12 +729,6 @@ def rope_inplace(qkv, cos_half, sin_half, heads, dim, seq_len, pos=None, interle
 
 
 # --------------------------------------------------------------------------- norms of query and key heads
-def _dense(t):
-  """Contiguous and 16-byte aligned."""
-  t = t.contiguous()
-  return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
 def _qk_norm_ok(qkv, q_weight, k_weight, cos, sin, d, eps) -> bool:
   """What the kernels take: see :func:`qk_norm_rope`."""
   rot = 2 * cos.shape[1]
@@ -736,6 +736,22 @@ def _qk_norm_ok(qkv, q_weight, k_weight, cos, sin, d, eps) -> bool:
           and all(t.is_cuda and t.dtype == torch.float32 and t.is_contiguous() and t.data_ptr() % 16 == 0 for t in (cos, sin))
           and all(w is None or (w.is_contiguous() and w.data_ptr() % 16 == 0) for w in (q_weight, k_weight))
           and qkv.shape[0] * qkv.shape[1] * (qkv.shape[2] // d) < 2 ** 31)
+
+
+def _qk_norm_backward(dq, dk, dv, qkv, q_weight, k_weight, cos, sin, pos, args, need):
+  """Gradients of the projection and the two weights; None for what is not needed or was collected in a ``main_grad``."""
+  from . import kernels as k
+  hq, hkv, d, seq_len, eps, interleaved = args
+  # a gradient that is recorded itself, or several at once, and what saved-tensor hooks gave back otherwise take torch's operators
+  if (torch.is_grad_enabled() or batched(dq, dk, dv) or not use_kernels(dq, dk, dv)
+      or not _qk_norm_ok(qkv, q_weight, k_weight, cos, sin, d, eps)
+      or (pos is not None and (pos.device != dq.device or pos.dtype != torch.int32 or not pos.is_contiguous()))):
+    out = ref.qk_norm_rope_grad(dq, dk, dv, qkv, cos, sin, hq, hkv, d, seq_len, q_weight, k_weight, eps, pos, interleaved)
+    return tuple(g if n else None for g, n in zip(out, need))
+  dx, dw = k.qk_norm_bwd(_dense(dq), _dense(dk), _dense(dv), qkv, hq, hkv, d, q_weight, k_weight, cos, sin, seq_len, pos, eps, interleaved,
+                         need[1] or need[2])
+  return (dx if need[0] else None, _norm_wgrad(q_weight, dw[0]) if need[1] else None,
+          _norm_wgrad(k_weight, dw[1]) if need[2] else None)
 
 
 class _QkNormRopeFn(torch.autograd.Function):
@@ -752,19 +768,7 @@ class _QkNormRopeFn(torch.autograd.Function):
 
   @staticmethod
   def backward(ctx, dq, dk, dv):
-    from . import kernels as k
-    qkv, q_weight, k_weight, cos, sin, pos = ctx.saved_tensors
-    hq, hkv, d, seq_len, eps, interleaved = ctx.args
-    need = ctx.needs_input_grad[:3]
-    # a gradient that is recorded itself, or several at once, and what saved-tensor hooks gave back otherwise take torch's operators
-    if (torch.is_grad_enabled() or batched(dq, dk, dv) or not use_kernels(dq, dk, dv)
-        or not _qk_norm_ok(qkv, q_weight, k_weight, cos, sin, d, eps)):
-      out = ref.qk_norm_rope_grad(dq, dk, dv, qkv, cos, sin, hq, hkv, d, seq_len, q_weight, k_weight, eps, pos, interleaved)
-      return (*(g if n else None for g, n in zip(out, need)), None, None, None, None)
-    dx, dw = k.qk_norm_bwd(_dense(dq), _dense(dk), _dense(dv), qkv, hq, hkv, d, q_weight, k_weight, cos, sin, seq_len, pos, eps, interleaved,
-                           need[1] or need[2])
-    return (dx if need[0] else None, _norm_wgrad(q_weight, dw[0]) if need[1] else None,
-            _norm_wgrad(k_weight, dw[1]) if need[2] else None, None, None, None, None)
+    return (*_qk_norm_backward(dq, dk, dv, *ctx.saved_tensors, ctx.args, ctx.needs_input_grad[:3]), None, None, None, None)
 
 
 def qk_norm_rope(qkv, cos_half, sin_half, hq, hkv, d, seq_len, q_weight=None, k_weight=None, eps=1e-6, pos=None, interleaved=False):
@@ -775,6 +779,10 @@ def qk_norm_rope(qkv, cos_half, sin_half, hq, hkv, d, seq_len, q_weight=None, k_
   outside of them counts as the nearest one and is reported (``_lib.raise_on_device_timeout``).
 
   The kernels take bf16, heads and rotated parts of multiples of 16 columns, heads of up to 512, and ``eps`` from 2^-126 on."""
+  if (nat := _native()) is not None:
+    heads = nat.qk_norm_rope(qkv, cos_half, sin_half, hq, hkv, d, seq_len, q_weight, k_weight, eps, pos, interleaved)
+    if heads is not None:
+      return heads
   if qkv.dim() != 3 or hq < 1 or hkv < 1 or d < 1 or qkv.shape[2] != (hq + 2 * hkv) * d:
     raise ValueError(f"qk_norm_rope: {tuple(qkv.shape)} is not [B, S, (hq + 2 hkv) * d] of {hq} and {hkv} heads of {d}")
   if cos_half.dim() != 2 or cos_half.shape != sin_half.shape or not 0 < 2 * cos_half.shape[1] <= d or cos_half.shape[0] == 0:
@@ -803,6 +811,12 @@ def qk_norm_rope(qkv, cos_half, sin_half, hq, hkv, d, seq_len, q_weight=None, k_
 
 
 # --------------------------------------------------------------------------- dropout
+def _dropout_backward(dy, seed, threshold, site, shape):
+  if batched(dy) or not use_kernels(dy) or not _seed_ok(seed):
+    return ref.dropout(dy, ref.dropout_keep(shape, threshold, seed.to(dy.device), site), threshold)
+  return _DropoutFn.apply(dy, None, seed, threshold, site)      # (a gradient that is recorded itself follows)
+
+
 class _DropoutFn(torch.autograd.Function):
   @staticmethod
   def forward(ctx, x, residual, seed, threshold, site):
@@ -814,13 +828,7 @@ class _DropoutFn(torch.autograd.Function):
   @staticmethod
   def backward(ctx, dy):
     (seed,) = ctx.saved_tensors
-    threshold, site, shape = ctx.args
-    dx = None
-    if ctx.needs_input_grad[0]:
-      if batched(dy) or not use_kernels(dy) or not _seed_ok(seed):
-        dx = ref.dropout(dy, ref.dropout_keep(shape, threshold, seed, site), threshold)
-      else:
-        dx = _DropoutFn.apply(dy, None, seed, threshold, site)      # (a gradient that is recorded itself follows)
+    dx = _dropout_backward(dy, seed, *ctx.args) if ctx.needs_input_grad[0] else None
     return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
 
 
@@ -836,6 +844,10 @@ def dropout(x, p, seed, site=0, residual=None, training=True):
   and nothing is stored for it.  Of the step the lower 32 bits count.  ``p`` counts in steps of 2^-16, to the nearest (the
   elements that stay are divided by what that leaves).  A step that is counted up in place between forward and backward is an error of the
   backward pass; give the next step's calls a new tensor, or count up behind the backward pass."""
+  if training and (nat := _native()) is not None:
+    y = nat.dropout(x, p, seed, site, residual)
+    if y is not None:
+      return y
   p = float(p)
   if not 0.0 <= p <= 1.0:
     raise ValueError(f"dropout: p {p}")
@@ -889,13 +901,28 @@ def _embedding_grad(ids, table, dout, scale):
 def _embedding_collect(ids, mg, dout, scale, overwrite):
   """The gradient of a table that collects it in ``mg``."""
   from . import kernels as k
-  dout, ids = dout.contiguous(), ids.contiguous()
-  if mg.data_ptr() % 16 == 0 and dout.data_ptr() % 16 == 0:
+  dout, ids = _dense(dout), ids.contiguous()
+  if mg.data_ptr() % 16 == 0:
     k.embedding_bwd_(dout, ids, mg, scale=scale, overwrite=overwrite)
   else:
-    g = torch.empty(mg.shape, dtype=mg.dtype, device=mg.device)
-    k.embedding_bwd_(dout.clone(), ids, g, scale=scale, overwrite=True)
+    g = k.embedding_bwd_(dout, ids, torch.empty(mg.shape, dtype=mg.dtype, device=mg.device), scale=scale, overwrite=True)
     mg.copy_(g) if overwrite else mg.add_(g)
+
+
+def _embedding_backward(ids, table, dout, scale):
+  """The table's gradient, or None where it collects it in a ``main_grad``."""
+  from . import kernels as k
+  mg = getattr(table, "main_grad", None)
+  if mg is not None:
+    _embedding_collect(ids, mg, dout, scale, bool(getattr(table, "grad_overwrite", False)))
+    table.grad_overwrite = False
+    return None
+  # a gradient that is recorded itself, or several at once, and what saved-tensor hooks gave back otherwise take torch's operators
+  if (batched(dout) or (torch.is_grad_enabled() and dout.requires_grad) or not use_kernels(dout, table)
+      or ids.dtype != torch.int64 or ids.device != dout.device):
+    return _embedding_grad(ids, table, dout, scale)
+  g = torch.empty(table.shape, dtype=table.dtype, device=table.device)
+  return k.embedding_bwd_(_dense(dout), ids.contiguous(), g, scale=scale, overwrite=True)
 
 
 class _EmbeddingFn(torch.autograd.Function):
@@ -908,18 +935,8 @@ class _EmbeddingFn(torch.autograd.Function):
 
   @staticmethod
   def backward(ctx, dout):
-    from . import kernels as k
     ids, table = ctx.saved_tensors
-    mg = getattr(table, "main_grad", None)
-    if mg is not None:
-      _embedding_collect(ids, mg, dout, ctx.scale, bool(getattr(table, "grad_overwrite", False)))
-      table.grad_overwrite = False
-      return None, None, None
-    if batched(dout) or (torch.is_grad_enabled() and dout.requires_grad) or not use_kernels(dout, table):
-      return None, _embedding_grad(ids, table, dout, ctx.scale), None
-    dout = dout.contiguous()
-    g = torch.empty(table.shape, dtype=table.dtype, device=table.device)
-    return None, k.embedding_bwd_(dout if dout.data_ptr() % 16 == 0 else dout.clone(), ids.contiguous(), g, scale=ctx.scale, overwrite=True), None
+    return None, _embedding_backward(ids, table, dout, ctx.scale), None
 
 
 class _EmbeddingPeerFn(torch.autograd.Function):
@@ -958,11 +975,12 @@ def embedding(ids, table, scale=None):
     scale = float(scale)
     if not math.isfinite(scale):
       raise ValueError(f"embedding: scale {scale}")
-  if (nat := _native()) is not None and scale is None:
-    y = nat.embedding(ids, table)
+  if (nat := _native()) is not None:
+    y = nat.embedding(ids, table, 1.0 if scale is None else scale)
     if y is not None:
       return y
-  if use_kernels(table) and table.shape[1] % 8 == 0 and (scale is None or unobserved()):
+  if (use_kernels(table) and table.dim() == 2 and table.shape[1] % 8 == 0 and table.is_contiguous() and table.data_ptr() % 16 == 0
+      and ids.dtype == torch.int64 and ids.device == table.device and (scale is None or unobserved())):
     return _EmbeddingFn.apply(ids, table, 1.0 if scale is None else scale)
   y = F.embedding(ids, table)
   return y if scale is None else (ref.wide(y) * scale).to(table.dtype)
