@@ -4,15 +4,22 @@
 //
 // Both are bound by memory.  The gradient of a training step writes the whole table (most rows as zeros) and reads dout once;
 // what makes it slow otherwise are atomics, which read and write an fp32 table that has to be zeroed before and rounded behind, in an
-// order that differs from run to run.  Here three kernels give every row one writer:
+// order that differs from run to run.  Here every row has one writer:
 //
-// * embedding_plan_kernel puts the tokens in order of their ids.  A CTA has a range of ids and looks at all tokens, so no CTA has to
-//   wait for another: its 32 warps count what each id has in their parts of the tokens, the counts become places (how many
-//   tokens have ids in front of the range is counted on the way), and a second look puts the tokens there, in order.
+// * embedding_plan_kernel puts the tokens in order of their ids.  A CTA has a set of ids (every sets-th one, so that frequent ones, which
+//   have low numbers, are spread) and looks at all tokens, so no CTA has to wait for another: its 32 warps count what each id has in their
+//   parts of the tokens, the counts become places (how many tokens the sets in front have is counted on the way), and a second
+//   look puts the tokens there, in order.  Up to 8192 tokens a warp keeps its part in registers between the looks (9 us); more
+//   are turned into codes by a kernel of their own first, and the second look is at a list of the set's (65536 tokens, 0.3 of them of
+//   one id: 45 us -> 3 + 20).
 // * embedding_sum_kernel cuts that order into chunks of equal size, whatever the ids: a warp adds up 256 columns of a chunk's rows
 //   in fp32.  An id whose tokens lie within a chunk is written at once; one that reaches over a chunk's border leaves its part, at most
-//   two a chunk.  Rows without a token become zeros, between the chunks' loads.
-// * embedding_join_kernel adds up the parts, in the chunks' order; many of them (the padding's row) are shared by a CTA's warps.
+//   two a chunk.  Then the warps write zeros to the rows without a token, handed out by a counter: in equal shares they waited for
+//   the warps whose chunks took long (204 -> 192 us).
+// * embedding_join_kernel adds up the parts in the chunks' order, an id to a warp, or one with many (the padding's row) to a CTA.  (Joined by
+//   whoever leaves the last part, with fences and counters, it all took longer: 65536 tokens 134 -> 148 us.)
+//
+// 8192 tokens of a 128256 x 4096 table: 177 us for 1.12 GB, 171 at a copy's rate; 65536 of 32000 x 2048, 0.3 of them of one id: 127 us for 0.4 GB.
 
 #include <atomic>
 
@@ -25,8 +32,14 @@ int sm_count();
 
 constexpr int EP_WARPS = 32;                 // of the planning kernel
 constexpr int EP_ROWS = 1024;                // most ids to a CTA of it
+constexpr int EP_BATCH = 8;                  // ids of a lane that are asked for at once
+constexpr int EP_SMEM = 220 * 1024;
 constexpr int EJ_WARPS = 32;                 // of the joining kernel
-constexpr int EJ_LONG = 16;                  // parts from which a CTA's warps share an id
+constexpr int EJ_LONG = 8;                   // chunks behind its first from which a CTA's warps share an id (8192 tokens, 65536 with 0.3 of one
+                                             // id: 4 177.0 and 126.7 us, 8 176.8 and 126.6, 16 178.6 and 126.6, 32 180.5 and, with other joins, 143 / 137)
+constexpr int ES_CTAS = 2;                   // of the summing kernel to an SM
+constexpr int ES_AHEAD = 8;                  // rows that a warp of it asks for at once
+constexpr int ES_ZERO = 4;                   // rows that a warp of it looks at for ones without tokens
 
 __device__ __forceinline__ void emb_unpack(const uint4& u, float* f) {
   const float2 a = unpack_bf16(u.x), b = unpack_bf16(u.y), c = unpack_bf16(u.z), d = unpack_bf16(u.w);
@@ -65,55 +78,150 @@ embedding_fwd_kernel(const uint4* __restrict__ table, const long long* __restric
   }
 }
 
-// Scratch of the gradient, in this order: range [rows] (first place, tokens), order [tokens], sorted ids [tokens], number of tokens
-// that have a row [1], parts.
+// Scratch of the gradient, in this order: range [rows] (first place, tokens), order [tokens] (the last one of an id is marked), number of
+// tokens that have a row, a counter, codes [tokens, padded], parts.
 struct EmbGrad {
   const long long* ids;
   const __nv_bfloat16* dout;
   void* dtable;
   int2* range;
-  int *order, *sorted, *valid;
+  unsigned *order, *codes;
+  int *valid, *taken;                        // taken (zeroed by the planning kernel): rows that the sum's warps have looked at
   float* part;                               // [chunks][2][dim]: of the id that began before the chunk, of the one that goes on behind it
   long long row0;
-  int tokens, rows, dim, chunk, chunks, per;  // per: ids to a CTA of the planning kernel
+  int tokens, rows, dim, chunk, chunks;
+  int sets, per, share;                      // CTAs of the planning kernel, most ids to one: id v is the v / sets-th of set v % sets; tokens to a warp
+  int list;                                  // entries of a warp's list there
+  unsigned inv, shift;                       // v / sets = v * inv >> shift
   float scale;
 };
 
+constexpr unsigned EMB_LAST = 1u << 31, EMB_NONE = ~0u;
+
+// An id as its set and its number there; EMB_NONE: it has no row.
+__device__ __forceinline__ unsigned emb_code(const EmbGrad& p, long long id) {
+  const unsigned v = (unsigned)id, q = (unsigned)((unsigned long long)v * p.inv >> p.shift);
+  return id < 0 || id >= p.rows ? EMB_NONE : (v - q * p.sets) * EP_ROWS + q;
+}
+
+// Codes of all tokens: where there are many, the planning kernel's CTAs do not all work them out.
+__global__ void __launch_bounds__(256)
+embedding_code_kernel(const EmbGrad p) {
+  if (!chain_begin()) return;
+  const int t = blockIdx.x * 256 + threadIdx.x, all = EP_WARPS * p.share;
+  if (t < all) p.codes[t] = t < p.tokens ? emb_code(p, p.ids[t] - p.row0) : EMB_NONE;
+}
+
+// CODES: the tokens' codes come from the kernel before, and a warp lists those of its part that are the CTA's (if the list is too short
+// for them it looks at all of them again).  Else a warp has EP_BATCH tokens a lane at most and keeps them.
+template <bool CODES>
 __global__ void __launch_bounds__(EP_WARPS * 32)
 embedding_plan_kernel(const EmbGrad p) {
   if (!chain_begin()) return;
-  extern __shared__ int ep_hist[];           // [warps][per]
+  extern __shared__ __align__(16) int ep_hist[];           // [warps][per], ends [per], lists [warps][list]; per a multiple of 4
   __shared__ int s_warp[EP_WARPS], s_below;
-  const int warp = warp_index(), lane = threadIdx.x & 31;
-  const long long first = p.row0 + (long long)blockIdx.x * p.per;
-  const int mine = min(p.per, p.rows - (int)blockIdx.x * p.per);
-  const int share = ((p.tokens + EP_WARPS * 32 - 1) / (EP_WARPS * 32)) * 32;
-  const int t0 = min(warp * share, p.tokens), t1 = min(t0 + share, p.tokens);
+  const int warp = warp_index(), lane = threadIdx.x & 31, set = blockIdx.x;
+  const unsigned least = set * EP_ROWS, below_me = (1u << lane) - 1;
+  const int t0 = warp * p.share;             // (the codes are padded; a launch without has at most 2^13 tokens)
   int* hist = ep_hist + warp * p.per;
-  for (int i = threadIdx.x; i < EP_WARPS * p.per; i += EP_WARPS * 32) ep_hist[i] = 0;
-  if (threadIdx.x == 0) s_below = 0;
-  __syncthreads();
-  // ---- how many tokens each id has in each warp's part, and how many have ids in front of this CTA's
-  int below = 0;
-#pragma unroll 8
-  for (int t = t0 + lane; t < t1; t += 32) {
-    const long long id = p.ids[t] - first;
-    if (id >= 0 && id < mine) atomicAdd(&hist[id], 1);
-    below += id < 0 && id >= p.row0 - first;
-  }
+  int* ends = ep_hist + EP_WARPS * p.per;
+  unsigned* list = reinterpret_cast<unsigned*>(ends + p.per) + warp * p.list;
+  unsigned code[EP_BATCH];
+  if (!CODES) {
+    long long id[EP_BATCH];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) below += __shfl_xor_sync(0xffffffffu, below, o);
+    for (int i = 0; i < EP_BATCH; ++i) {
+      const int t = t0 + 32 * i + lane;
+      id[i] = 32 * i < p.share && t < p.tokens ? p.ids[t] - p.row0 : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < EP_BATCH; ++i) code[i] = emb_code(p, id[i]);
+  }
+  for (int i = threadIdx.x; i < EP_WARPS * p.per / 4; i += EP_WARPS * 32) reinterpret_cast<int4*>(ep_hist)[i] = make_int4(0, 0, 0, 0);
+  if (threadIdx.x == 0) {
+    s_below = 0;
+    if (set == 0) *p.taken = 0;
+  }
+  __syncthreads();
+  // ---- which tokens of the warp's part have an id of this set, and how many one of a set in front
+  int below = 0, hits = 0;
+  if (CODES) {
+    for (int t = 0; t < p.share; t += 256) {
+      const uint4 c0 = *reinterpret_cast<const uint4*>(p.codes + t0 + t + 4 * lane);
+      const uint4 c1 = *reinterpret_cast<const uint4*>(p.codes + t0 + t + 128 + 4 * lane);
+      const unsigned c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        bool in[4];
+        unsigned who[4], any = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const unsigned v = c[4 * half + i];
+          in[i] = v - least < EP_ROWS;
+          below += v < least;
+          who[i] = __ballot_sync(0xffffffffu, in[i]);
+          any |= who[i];
+        }
+        if (any == 0) continue;
+        int at = hits;                       // tokens of one lane follow one another
+#pragma unroll
+        for (int i = 0; i < 4; ++i) at += __popc(who[i] & below_me);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (in[i] && at < p.list) list[at] = (unsigned)(t + 128 * half + 4 * lane + i) * EP_ROWS | (c[4 * half + i] - least);
+          at += in[i];
+          hits += __popc(who[i]);
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+#pragma unroll
+    for (int i = 0; i < EP_BATCH; ++i) below += code[i] < least;
+  }
+  // f(has, number of the id, token) for the warp's tokens, 32 at a time and in order; those of the set are enough
+  auto each = [&](auto&& f) {
+    if (!CODES) {
+#pragma unroll
+      for (int i = 0; i < EP_BATCH; ++i)
+        if (__any_sync(0xffffffffu, code[i] - least < EP_ROWS)) f(code[i] - least < EP_ROWS, code[i] - least, t0 + 32 * i + lane);
+    } else if (hits <= p.list) {
+      for (int i = 0; i < hits; i += 32) {
+        const unsigned e = i + lane < hits ? list[i + lane] : 0;
+        f(i + lane < hits, e % EP_ROWS, t0 + (int)(e / EP_ROWS));
+      }
+    } else {
+#pragma unroll 4
+      for (int t = 0; t < p.share; t += 32) {
+        const unsigned v = p.codes[t0 + t + lane] - least;
+        f(v < EP_ROWS, v, t0 + t + lane);
+      }
+    }
+  };
+  // ---- how many each id has in each warp's part; many may have one and the same (the padding's)
+  each([&](bool has, unsigned r, int) {
+    const unsigned who = __ballot_sync(0xffffffffu, has);
+    if (who == 0) return;
+    const int leader = __ffs(who) - 1;
+    const unsigned first = __shfl_sync(0xffffffffu, r, leader), same = __ballot_sync(0xffffffffu, has && r == first);
+    if (lane == leader) atomicAdd(&hist[r], __popc(same));
+    else if (has && !(same >> lane & 1)) atomicAdd(&hist[r], 1);
+  });
+  below = __reduce_add_sync(0xffffffffu, below);
   if (lane == 0 && below) atomicAdd(&s_below, below);
   __syncthreads();
   // ---- their places: a thread for each id
-  const int r = threadIdx.x;
-  int count = 0;
-  if (r < mine)
-    for (int w = 0; w < EP_WARPS; ++w) {
-      const int n = ep_hist[w * p.per + r];
-      ep_hist[w * p.per + r] = count;
-      count += n;
-    }
+  const int r = threadIdx.x, row = r * p.sets + set;
+  const bool has_row = r < p.per && row < p.rows;
+  int before[EP_WARPS], count = 0;
+#pragma unroll
+  for (int w = 0; w < EP_WARPS; ++w) before[w] = has_row ? ep_hist[w * p.per + r] : 0;
+#pragma unroll
+  for (int w = 0; w < EP_WARPS; ++w) {
+    const int n = before[w];
+    before[w] = count;
+    count += n;
+  }
   int sum = count;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -122,30 +230,27 @@ embedding_plan_kernel(const EmbGrad p) {
   }
   if (lane == 31) s_warp[warp] = sum;
   __syncthreads();
-  int start = s_below + sum - count;
-  for (int w = 0; w < warp; ++w) start += s_warp[w];
-  if (r < mine) {
-    for (int w = 0; w < EP_WARPS; ++w) ep_hist[w * p.per + r] += start;
-    p.range[blockIdx.x * p.per + r] = make_int2(start, count);
-    if (blockIdx.x * p.per + r == p.rows - 1) *p.valid = start + count;
+  const int start = s_below + sum - count + __reduce_add_sync(0xffffffffu, lane < warp ? s_warp[lane] : 0);
+  if (has_row) {
+#pragma unroll
+    for (int w = 0; w < EP_WARPS; ++w) ep_hist[w * p.per + r] = start + before[w];
+    ends[r] = start + count - 1;
+    p.range[row] = make_int2(start, count);
   }
+  if (set == p.sets - 1 && r == EP_WARPS * 32 - 1) *p.valid = start + count;
   __syncthreads();
   // ---- the tokens, in order: those of one id in a warp's 32 by lane
-  for (int t = t0; t < t1; t += 32) {
-    const long long id = t + lane < t1 ? p.ids[t + lane] - first : -1;
-    const bool in = id >= 0 && id < mine;
-    const unsigned any = __ballot_sync(0xffffffffu, in);
-    if (any == 0) continue;
-    if (in) {
-      const unsigned same = __match_any_sync(any, (int)id);
-      const int at = hist[id] + __popc(same & ((1u << lane) - 1));
-      p.order[at] = t + lane;
-      p.sorted[at] = blockIdx.x * p.per + (int)id;
+  each([&](bool has, unsigned r, int t) {
+    const unsigned any = __ballot_sync(0xffffffffu, has);
+    if (has) {
+      const unsigned same = __match_any_sync(any, r), lower = same & below_me;
+      const int at = hist[r] + __popc(lower);
+      p.order[at] = t | (at == ends[r] ? EMB_LAST : 0);
       __syncwarp(any);
-      if ((same & ((1u << lane) - 1)) == 0) hist[id] = at + __popc(same);
+      if (lower == 0) hist[r] = at + __popc(same);
     }
     __syncwarp();
-  }
+  });
 }
 
 template <bool F32>
@@ -175,56 +280,51 @@ __device__ __forceinline__ void emb_store(void* dtable, long long at, const floa
   }
 }
 
-constexpr int ES_ZERO = 4;       // rows of a warp's look for ones without tokens
-
 template <bool F32, bool ADD>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, ES_CTAS)
 embedding_sum_kernel(const EmbGrad p) {
   if (!chain_begin()) return;
   const int lane = threadIdx.x & 31, blocks = (p.dim + 255) / 256;
-  const long long warp = blockIdx.x * 8LL + warp_index(), stride = gridDim.x * 8LL;
-  const int valid = *p.valid;
-  const long long items = (long long)((valid + p.chunk - 1) / p.chunk) * blocks;
-  for (long long item = warp; item < items; item += stride) {
-    const int c = (int)(item / blocks), col = (int)(item % blocks) * 256 + lane * 8, base = c * p.chunk;
+  const int valid = *p.valid, warps = gridDim.x * 8;
+  const int items = (valid + p.chunk - 1) / p.chunk * blocks;
+  for (int item = blockIdx.x * 8 + warp_index(); item < items; item += warps) {
+    const int c = item / blocks, col = (item - c * blocks) * 256 + lane * 8, base = c * p.chunk;
     const int n = min(p.chunk, valid - base);
     const bool has = col < p.dim;
-    const int before = base > 0 ? p.sorted[base - 1] : -1;
     float acc[8] = {};
-    bool first = true;                       // the id of the chunk's first token
+    bool began = base > 0 && !(p.order[base - 1] & EMB_LAST);        // the first id began before the chunk
     for (int i0 = 0; i0 < n; i0 += 32) {
-      const int m = min(32, n - i0), at = base + i0 + lane;
-      const int tok = lane < m ? p.order[at] : 0, id = lane < m ? p.sorted[at] : -1;
-      const int next = lane < m && at + 1 < valid ? p.sorted[at + 1] : -1;
-      const unsigned ends = __ballot_sync(0xffffffffu, lane < m && (id != next || i0 + lane == n - 1));
-      const unsigned goes = __ballot_sync(0xffffffffu, id == next);
-      for (int j0 = 0; j0 < m; j0 += 8) {
-        uint4 v[8];
+      const int m = min(32, n - i0);
+      const unsigned here = lane < m ? p.order[base + i0 + lane] : EMB_LAST;
+      const int tok = here & ~EMB_LAST;
+      const unsigned last = __ballot_sync(0xffffffffu, here & EMB_LAST), ends = last | (i0 + m == n ? 1u << (m - 1) : 0);
+      const int row = ends >> lane & 1 && lane < m ? (int)(p.ids[tok] - p.row0) : 0;
+      for (int j0 = 0; j0 < m; j0 += ES_AHEAD) {
+        uint4 v[ES_AHEAD];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < ES_AHEAD; ++j) {
           const int t = __shfl_sync(0xffffffffu, tok, j0 + j);
           v[j] = has && j0 + j < m ? *reinterpret_cast<const uint4*>(p.dout + (long long)t * p.dim + col) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < ES_AHEAD; ++j) {
           if (j0 + j >= m) break;
           float x[8];
           emb_unpack(v[j], x);
 #pragma unroll
           for (int e = 0; e < 8; ++e) acc[e] += x[e];
           if (ends >> (j0 + j) & 1) {
-            const int run = __shfl_sync(0xffffffffu, id, j0 + j);
-            const bool began = first && run == before, on = goes >> (j0 + j) & 1;
+            const int id = __shfl_sync(0xffffffffu, row, j0 + j);
             if (has) {
-              if (!began && !on) {
-                emb_store<F32>(p.dtable, (long long)run * p.dim + col, acc, p.scale, ADD);
-              } else {
+              if (began || !(last >> (j0 + j) & 1)) {
                 float4* dst = reinterpret_cast<float4*>(p.part + (2LL * c + (began ? 0 : 1)) * p.dim + col);
                 dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
                 dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+              } else {
+                emb_store<F32>(p.dtable, (long long)id * p.dim + col, acc, p.scale, ADD);
               }
             }
-            first = false;
+            began = false;
 #pragma unroll
             for (int e = 0; e < 8; ++e) acc[e] = 0.f;
           }
@@ -233,13 +333,16 @@ embedding_sum_kernel(const EmbGrad p) {
     }
   }
   if (ADD) return;
-  const long long groups = (p.rows + ES_ZERO - 1) / ES_ZERO;
-  const int vecs = p.dim / (F32 ? 4 : 8);
-  for (long long g = warp; g < groups; g += stride) {
-    const int row = (int)g * ES_ZERO + lane;
+  // rows without a token, to whoever is free (warps end their chunks at times that differ by a fourth of the kernel's)
+  const int groups = (p.rows + ES_ZERO - 1) / ES_ZERO, vecs = p.dim / (F32 ? 4 : 8);
+  auto take = [&]() { return lane == 0 ? atomicAdd(p.taken, 1) : 0; };
+  for (int ahead = take();;) {
+    const int group = __shfl_sync(0xffffffffu, ahead, 0), row = group * ES_ZERO + lane;
+    if (group >= groups) break;
+    ahead = take();
     unsigned none = __ballot_sync(0xffffffffu, lane < ES_ZERO && row < p.rows && p.range[row].y == 0);
     for (; none; none &= none - 1) {
-      uint4* dst = static_cast<uint4*>(p.dtable) + (g * ES_ZERO + __ffs(none) - 1) * vecs;
+      uint4* dst = static_cast<uint4*>(p.dtable) + ((long long)group * ES_ZERO + __ffs(none) - 1) * vecs;
       for (int i = lane; i < vecs; i += 32) dst[i] = make_uint4(0, 0, 0, 0);
     }
   }
@@ -249,13 +352,12 @@ template <bool F32, bool ADD>
 __global__ void __launch_bounds__(EJ_WARPS * 32)
 embedding_join_kernel(const EmbGrad p) {
   if (!chain_begin()) return;
-  __shared__ float s_part[EJ_WARPS][256];
-  __shared__ long long s_long[EJ_WARPS];
+  __shared__ __align__(16) float s_part[EJ_WARPS][256];
+  __shared__ int4 s_long[EJ_WARPS];          // id, first and last chunk, columns
   __shared__ int s_longs;
   const int warp = warp_index(), lane = threadIdx.x & 31, blocks = (p.dim + 255) / 256;
-  const int valid = *p.valid;
-  const long long items = (long long)(valid / p.chunk) * blocks;
-  // the parts from .. to of an id that begins in chunk c (the first one is its second part, the others first parts)
+  const int items = *p.valid / p.chunk * blocks;
+  // the parts from .. to of an id that begins in chunk c (that one's is its second, the others' are first ones)
   auto add_up = [&](int c, int col, int from, int to, float* acc) {
 #pragma unroll 4
     for (int k = from; k <= to; ++k) {
@@ -265,45 +367,54 @@ embedding_join_kernel(const EmbGrad p) {
       acc[4] += b.x; acc[5] += b.y; acc[6] += b.z; acc[7] += b.w;
     }
   };
-  for (long long base = blockIdx.x; base < items; base += (long long)gridDim.x * EJ_WARPS) {
+  for (int base = blockIdx.x; base < items; base += gridDim.x * EJ_WARPS) {
     if (threadIdx.x == 0) s_longs = 0;
     __syncthreads();
-    const long long item = base + (long long)warp * gridDim.x;
+    const int item = base + warp * gridDim.x;
     if (item < items) {
-      const int c = (int)(item / blocks), col = (int)(item % blocks) * 256 + lane * 8, end = (c + 1) * p.chunk;
-      const int row = p.sorted[end - 1];
-      const int2 r = p.range[row];
-      if (r.x >= c * p.chunk && r.x + r.y > end) {       // it begins in the chunk and goes on behind it
+      const int c = item / blocks, col0 = (item - c * blocks) * 256, col = col0 + lane * 8;
+      const unsigned end = p.order[(c + 1) * p.chunk - 1];
+      if (!(end & EMB_LAST)) {               // an id goes on behind the chunk
+        const int row = (int)(p.ids[end] - p.row0);
+        const int2 r = p.range[row];
         const int last = (r.x + r.y - 1) / p.chunk;
-        if (last - c < EJ_LONG) {
+        if (r.x < c * p.chunk) {             // and began before it: whoever has that chunk looks after it
+        } else if (last - c < EJ_LONG) {
           if (col < p.dim) {
             float acc[8] = {};
             add_up(c, col, c, last, acc);
             emb_store<F32>(p.dtable, (long long)row * p.dim + col, acc, p.scale, ADD);
           }
         } else if (lane == 0) {
-          s_long[atomicAdd(&s_longs, 1)] = item;       // (in any order: each is a result of its own)
+          s_long[atomicAdd(&s_longs, 1)] = make_int4(row, c, last, col0);       // (in any order: each is a result of its own)
         }
       }
     }
     __syncthreads();
     const int longs = s_longs;
     for (int i = 0; i < longs; ++i) {
-      const int c = (int)(s_long[i] / blocks), col = (int)(s_long[i] % blocks) * 256 + lane * 8;
-      const int row = p.sorted[(c + 1) * p.chunk - 1];
-      const int2 r = p.range[row];
-      const int n = (r.x + r.y - 1) / p.chunk - c + 1, from = c + (int)((long long)n * warp / EJ_WARPS);
-      const int to = c + (int)((long long)n * (warp + 1) / EJ_WARPS) - 1;
+      const int4 it = s_long[i];
+      const int n = it.z - it.y + 1, from = it.y + (int)((long long)n * warp / EJ_WARPS);
+      const int to = it.y + (int)((long long)n * (warp + 1) / EJ_WARPS) - 1;
       float acc[8] = {};
-      if (col < p.dim) add_up(c, col, from, to, acc);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s_part[warp][lane * 8 + e] = acc[e];
+      if (it.w + lane * 8 < p.dim) add_up(it.y, it.w + lane * 8, from, to, acc);
+      reinterpret_cast<float4*>(s_part[warp])[2 * lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      reinterpret_cast<float4*>(s_part[warp])[2 * lane + 1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
       __syncthreads();
-      if (warp == 0 && col < p.dim) {
-        for (int w = 1; w < EJ_WARPS; ++w)
+      const int col = it.w + threadIdx.x;
+      if (threadIdx.x < 256 && col < p.dim) {
+        float a = s_part[0][threadIdx.x];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) acc[e] += s_part[w][lane * 8 + e];
-        emb_store<F32>(p.dtable, (long long)row * p.dim + col, acc, p.scale, ADD);
+        for (int w = 1; w < EJ_WARPS; ++w) a += s_part[w][threadIdx.x];
+        a = mul_exact(a, p.scale);
+        const long long at = (long long)it.x * p.dim + col;
+        if (F32) {
+          float* dst = static_cast<float*>(p.dtable) + at;
+          *dst = ADD ? *dst + a : a;
+        } else {
+          __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.dtable) + at;
+          *dst = __float2bfloat16(ADD ? __bfloat162float(*dst) + a : a);
+        }
       }
       __syncthreads();
     }
@@ -311,36 +422,47 @@ embedding_join_kernel(const EmbGrad p) {
   }
 }
 
-// Tokens to a chunk: 32, more where the parts would take more than a few thousand rows.
+// Tokens to a chunk: 32; 64 from 2^15 tokens on, where there are warps' work enough and fewer parts to join (65536 tokens, 0.3 of them
+// of one id, 2048 columns: 138 / 129 us; 8192 tokens 178 with 32, 190 with 16); more where the parts would take thousands of rows.
 static int emb_chunk(int tokens) {
-  int c = 32;
+  int c = tokens > 32768 ? 64 : 32;
   while (tokens / c > 4096) c *= 2;
   return c;
 }
 static int emb_per(int rows) {
   const int sms = sm_count(), even = (rows + sms - 1) / sms;
-  return even < 64 ? 64 : even > EP_ROWS ? EP_ROWS : even;
+  return even < 64 ? 64 : even > EP_ROWS ? EP_ROWS : (even + 3) / 4 * 4;
 }
 static long long emb_align(long long n) { return (n + 15) / 16 * 16; }
 
+// Tokens to a warp of the planning kernel: whole rounds of it.
+static int emb_share(int tokens) {
+  const int round = tokens <= EP_WARPS * 32 * EP_BATCH ? 32 : 256;
+  return (int)((tokens + (long long)EP_WARPS * round - 1) / (EP_WARPS * round)) * round;
+}
+
 struct EmbLayout {
-  long long range, order, sorted, valid, part, bytes;
+  long long range, order, valid, codes, part, bytes;
+  int chunk, chunks, share;
+  bool coded;
   EmbLayout(int tokens, int rows, int dim) {
-    const int chunk = emb_chunk(tokens);
-    const long long chunks = (tokens + chunk - 1) / chunk;
+    chunk = emb_chunk(tokens);
+    chunks = (int)((tokens + (long long)chunk - 1) / chunk);
+    share = emb_share(tokens);
+    coded = tokens > EP_WARPS * 32 * EP_BATCH;
     range = 0;
     order = emb_align(range + 8LL * rows);
-    sorted = emb_align(order + 4LL * tokens);
-    valid = emb_align(sorted + 4LL * tokens);
-    part = valid + 16;
-    bytes = part + chunks * 2 * dim * 4;
+    valid = emb_align(order + 4LL * tokens);
+    codes = valid + 16;
+    part = codes + (coded ? 4LL * share * EP_WARPS : 0);
+    bytes = part + 2LL * chunks * dim * 4;
   }
 };
 
 template <bool F32, bool ADD>
 static void launch_embedding_grad(const EmbGrad& p, cudaStream_t stream) {
   const int sms = sm_count();
-  chain(embedding_sum_kernel<F32, ADD>, 6 * sms, 256, 0, stream, p);
+  chain(embedding_sum_kernel<F32, ADD>, ES_CTAS * sms, 256, 0, stream, p);
   if (p.tokens > p.chunk) chain(embedding_join_kernel<F32, ADD>, sms, EJ_WARPS * 32, 0, stream, p);
 }
 
@@ -376,7 +498,7 @@ extern "C" long long tpb_embedding_bwd_scratch(int tokens, int rows_local, int d
 // dtable[v] = (`add`: dtable[v] +) scale * sum of dout[t] over ids[t] = row0 + v; with `add`, rows without a token are left alone.
 extern "C" int tpb_embedding_bwd(const void* dout, const long long* ids, void* dtable, void* scratch, int tokens, int dim, int rows_local,
                                  long long row0, int dtable_is_f32, int add, float scale, void* stream) {
-  if (dim % 8 || dim <= 0 || tokens < 0 || rows_local < 0) return -2;
+  if (dim % 8 || dim <= 0 || tokens < 0 || tokens > 1 << 30 || rows_local < 0) return -2;
   for (const void* a : {dout, (const void*)dtable, (const void*)scratch})
     if (reinterpret_cast<uintptr_t>(a) % 16) return -2;
   if (rows_local == 0 || (tokens == 0 && add)) return 0;
@@ -387,29 +509,43 @@ extern "C" int tpb_embedding_bwd(const void* dout, const long long* ids, void* d
   p.dout = static_cast<const __nv_bfloat16*>(dout);
   p.dtable = dtable;
   p.range = reinterpret_cast<int2*>(s + at.range);
-  p.order = reinterpret_cast<int*>(s + at.order);
-  p.sorted = reinterpret_cast<int*>(s + at.sorted);
+  p.order = reinterpret_cast<unsigned*>(s + at.order);
   p.valid = reinterpret_cast<int*>(s + at.valid);
+  p.taken = p.valid + 1;
+  p.codes = reinterpret_cast<unsigned*>(s + at.codes);
   p.part = reinterpret_cast<float*>(s + at.part);
   p.row0 = row0;
   p.tokens = tokens;
   p.rows = rows_local;
   p.dim = dim;
-  p.chunk = emb_chunk(tokens);
-  p.chunks = (tokens + p.chunk - 1) / p.chunk;
+  p.chunk = at.chunk;
+  p.chunks = at.chunks;
+  p.share = at.share;
   p.per = emb_per(rows_local);
+  p.sets = (rows_local + p.per - 1) / p.per;
+  p.shift = 31;
+  while (1ll << (p.shift - 31) < p.sets) ++p.shift;
+  p.inv = (unsigned)((1ull << p.shift) / p.sets + 1);       // exact for dividends below 2^31
   p.scale = scale;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int smem = EP_WARPS * p.per * 4;
+  const int hists = (EP_WARPS + 1) * p.per * 4, most = (EP_SMEM - hists) / (EP_WARPS * 4);
+  p.list = !at.coded || p.share > 1 << 22 ? 0 : p.share < most ? p.share : most;       // (an entry has 22 bits for the token)
+  const int smem = hists + EP_WARPS * p.list * 4;
   static std::atomic<unsigned> ready{0};              // a bit for each device
   int device = 0;
   cudaError_t set = cudaGetDevice(&device);
   if (set == cudaSuccess && (device > 31 || !(ready.load(std::memory_order_relaxed) >> device & 1))) {
-    set = cudaFuncSetAttribute(embedding_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, EP_WARPS * EP_ROWS * 4);
+    set = cudaFuncSetAttribute(embedding_plan_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, EP_SMEM);
+    if (set == cudaSuccess) set = cudaFuncSetAttribute(embedding_plan_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, EP_SMEM);
     if (set == cudaSuccess && device <= 31) ready.fetch_or(1u << device, std::memory_order_relaxed);
   }
   if (set != cudaSuccess) return 1000 + (int)set;
-  chain(embedding_plan_kernel, (rows_local + p.per - 1) / p.per, EP_WARPS * 32, smem, st, p);
+  if (at.coded) {
+    chain(embedding_code_kernel, (EP_WARPS * p.share + 255) / 256, 256, 0, st, p);
+    chain(embedding_plan_kernel<true>, p.sets, EP_WARPS * 32, smem, st, p);
+  } else {
+    chain(embedding_plan_kernel<false>, p.sets, EP_WARPS * 32, smem, st, p);
+  }
   if (dtable_is_f32) add ? launch_embedding_grad<true, true>(p, st) : launch_embedding_grad<true, false>(p, st);
   else add ? launch_embedding_grad<false, true>(p, st) : launch_embedding_grad<false, false>(p, st);
   const cudaError_t e = cudaGetLastError();
