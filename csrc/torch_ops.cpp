@@ -1080,7 +1080,7 @@ py::object qk_norm_rope(py::handle x_, py::handle cos_, py::handle sin_, py::han
       !unobserved() || !unpack(x_, x) || !unpack(cos_, cos) || !unpack(sin_, sin) || !unpack(qw_, qw) || !unpack(kw_, kw) ||
       !unpack(pos_, pos))
     return py::none();
-  if (a.hq < 1 || a.hkv < 1 || !small(a.hq) || !small(a.hkv) || a.d < 16 || a.d > 512 || a.d % 16 || !(a.eps >= 0x1p-126 && a.eps < 0x1p127) ||
+  if (a.hq < 1 || a.hkv < 1 || a.hq > 1024 || a.hkv > 1024 || a.hq + 2 * a.hkv > 1024 || a.d < 16 || a.d > 512 || a.d % 16 || !(a.eps >= 0x1p-126 && a.eps < 0x1p127) ||
       !small(a.seq) || !qk_tensors(a, x, qw, kw, cos, sin, pos) || x.get_device() != c10::cuda::current_device() ||
       (pos.defined() && bounds_checked()))
     return py::none();

@@ -735,7 +735,7 @@ def _qk_norm_ok(qkv, q_weight, k_weight, cos, sin, d, eps) -> bool:
   return (use_kernels(qkv, q_weight, k_weight) and d % 16 == 0 and d <= 512 and rot % 16 == 0 and eps >= 2.0 ** -126
           and all(t.is_cuda and t.dtype == torch.float32 and t.is_contiguous() and t.data_ptr() % 16 == 0 for t in (cos, sin))
           and all(w is None or (w.is_contiguous() and w.data_ptr() % 16 == 0) for w in (q_weight, k_weight))
-          and qkv.shape[0] * qkv.shape[1] * (qkv.shape[2] // d) < 2 ** 31)
+          and qkv.shape[2] // d <= 1024 and qkv.shape[0] * qkv.shape[1] * (qkv.shape[2] // d) < 2 ** 31)
 
 
 def _qk_norm_backward(dq, dk, dv, qkv, q_weight, k_weight, cos, sin, pos, args, need):
@@ -778,7 +778,8 @@ def qk_norm_rope(qkv, cos_half, sin_half, hq, hkv, d, seq_len, q_weight=None, k_
   token % ``seq_len``; all in fp32, rounded once.  Values are a view of ``qkv``.  cos/sin: fp32 [positions, columns / 2]; a position
   outside of them counts as the nearest one and is reported (``_lib.raise_on_device_timeout``).
 
-  The kernels take bf16, heads and rotated parts of multiples of 16 columns, heads of up to 512, and ``eps`` from 2^-126 on."""
+  The kernels take bf16, heads and rotated parts of multiples of 16 columns, heads of up to 512, up to 1024 heads,
+  and ``eps`` from 2^-126 on."""
   if (nat := _native()) is not None:
     heads = nat.qk_norm_rope(qkv, cos_half, sin_half, hq, hkv, d, seq_len, q_weight, k_weight, eps, pos, interleaved)
     if heads is not None:
