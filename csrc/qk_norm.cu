@@ -234,6 +234,7 @@ struct QkWalk {
 template <int GROUP, bool PAIRS, bool SUMS>
 __global__ void __launch_bounds__(QK_THREADS, QB_CTAS)
 qk_norm_bwd_kernel(const QkNorm p) {
+  if (!chain_begin()) return;
   constexpr int HPW = 32 / GROUP, HEADS = QB_STEPS * HPW;
   extern __shared__ uint4 qk_mem[];          // [stages][steps][4][threads], then the warps' sums
   const int lane = threadIdx.x & 31, warp = warp_index(), group = lane / GROUP;
@@ -246,7 +247,6 @@ qk_norm_bwd_kernel(const QkNorm p) {
   auto blocks_of = [&](int kind) { return kind < 2 ? (p.heads[kind] + HEADS - 1) / HEADS : (v_vecs + VECS * 32 - 1) / (VECS * 32); };
   auto place = [&](int stage, int i, int what) { return qk_mem + ((stage * QB_STEPS + i) * 4 + what) * QK_THREADS + threadIdx.x; };
   float* sums = reinterpret_cast<float*>(qk_mem + QB_STAGES * QB_STEPS * 4 * QK_THREADS);      // of queries, of keys: [warps][d]
-  if (!chain_begin()) return;
   int kind = 0, ask_stage = 0, stage = 0;    // (kind: of the next unit to be asked for)
   QkWalk ahead(blocks_of(0), me, warps);
   auto ask = [&]() {                         // (a group each time, also behind the last unit)
