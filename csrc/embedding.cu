@@ -14,12 +14,12 @@
 //   one id: 45 us -> 3 + 20).
 // * embedding_sum_kernel cuts that order into chunks of equal size, whatever the ids: a warp adds up 256 columns of a chunk's rows
 //   in fp32.  An id whose tokens lie within a chunk is written at once; one that reaches over a chunk's border leaves its part, at most
-//   two a chunk.  Then the warps write zeros to the rows without a token, handed out by a counter: in equal shares they waited for
-//   the warps whose chunks took long (204 -> 192 us).
+//   two a chunk.  Then some warps write zeros to the rows without a token, handed out by a counter: in equal shares they waited for
+//   the warps whose chunks took long (204 -> 192 us); all warps' writes at once are slower than a quarter's.
 // * embedding_join_kernel adds up the parts in the chunks' order, an id to a warp, or one with many (the padding's row) to a CTA.  (Joined by
 //   whoever leaves the last part, with fences and counters, it all took longer: 65536 tokens 134 -> 148 us.)
 //
-// 8192 tokens of a 128256 x 4096 table: 177 us for 1.12 GB, 171 at a copy's rate; 65536 of 32000 x 2048, 0.3 of them of one id: 127 us for 0.4 GB.
+// 8192 tokens of a 128256 x 4096 table: 170 us for 1.12 GB, 171 at a copy's rate; 65536 of 32000 x 2048, 0.3 of them of one id: 103 us for 0.4 GB.
 
 #include <atomic>
 
@@ -37,8 +37,10 @@ constexpr int EP_SMEM = 220 * 1024;
 constexpr int EJ_WARPS = 32;                 // of the joining kernel
 constexpr int EJ_LONG = 8;                   // chunks behind its first from which a CTA's warps share an id (8192 tokens, 65536 with 0.3 of one
                                              // id: 4 177.0 and 126.7 us, 8 176.8 and 126.6, 16 178.6 and 126.6, 32 180.5 and, with other joins, 143 / 137)
-constexpr int ES_CTAS = 2;                   // of the summing kernel to an SM
-constexpr int ES_AHEAD = 8;                  // rows that a warp of it asks for at once
+// Of the summing kernel: CTAs to an SM, rows that a warp asks for ahead, and warps of a CTA that write zeros at the end.  us, 8192 tokens of a 128256 x
+// 4096 table / 65536 of 32000 x 2048, 0.3 of them of one id: 4, 8, 2 170 / 103;  4, 8, 4 175 / 103;  4, 8, 8 184 / 103;  3, 16, 8 180 / 111;  2, 16, 8
+// 198 / 125;  5, 8, 8 - / 129;  two CTAs with eight rows in registers, 8 177 / 127.
+constexpr int ES_CTAS = 4, ES_AHEAD = 8, ES_FILL = 2;
 constexpr int ES_ZERO = 4;                   // rows that a warp of it looks at for ones without tokens
 
 __device__ __forceinline__ void emb_unpack(const uint4& u, float* f) {
@@ -280,10 +282,16 @@ __device__ __forceinline__ void emb_store(void* dtable, long long at, const floa
   }
 }
 
+// Sixteen bytes to this thread's own place in shared memory, or none.
+__device__ __forceinline__ void emb_ask(uint4* dst, const void* src, bool has) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(has ? 16 : 0) : "memory");
+}
+
 template <bool F32, bool ADD>
 __global__ void __launch_bounds__(256, ES_CTAS)
 embedding_sum_kernel(const EmbGrad p) {
   if (!chain_begin()) return;
+  __shared__ uint4 mem[ES_AHEAD][256];       // a thread's own columns of the rows that are under way
   const int lane = threadIdx.x & 31, blocks = (p.dim + 255) / 256;
   const int valid = *p.valid, warps = gridDim.x * 8;
   const int items = (valid + p.chunk - 1) / p.chunk * blocks;
@@ -292,47 +300,50 @@ embedding_sum_kernel(const EmbGrad p) {
     const int n = min(p.chunk, valid - base);
     const bool has = col < p.dim;
     float acc[8] = {};
+    unsigned here = lane < n ? p.order[base + lane] : EMB_LAST;
     bool began = base > 0 && !(p.order[base - 1] & EMB_LAST);        // the first id began before the chunk
+    const __nv_bfloat16* from = p.dout + (has ? col : 0);
+    auto fetch = [&](unsigned tokens, int j, bool there) {             // row j of 32; a group each time
+      const int t = __shfl_sync(0xffffffffu, tokens, j & 31) & ~EMB_LAST;
+      emb_ask(&mem[j % ES_AHEAD][threadIdx.x], from + (there ? (long long)t * p.dim : 0), there && has);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int j = 0; j < ES_AHEAD; ++j) fetch(here, j, j < n);
     for (int i0 = 0; i0 < n; i0 += 32) {
-      const int m = min(32, n - i0);
-      const unsigned here = lane < m ? p.order[base + i0 + lane] : EMB_LAST;
-      const int tok = here & ~EMB_LAST;
+      const int m = min(32, n - i0), left = n - i0 - 32;
+      const unsigned next = lane < left ? p.order[base + i0 + 32 + lane] : EMB_LAST;
       const unsigned last = __ballot_sync(0xffffffffu, here & EMB_LAST), ends = last | (i0 + m == n ? 1u << (m - 1) : 0);
-      const int row = ends >> lane & 1 && lane < m ? (int)(p.ids[tok] - p.row0) : 0;
-      for (int j0 = 0; j0 < m; j0 += ES_AHEAD) {
-        uint4 v[ES_AHEAD];
+      const int row = ends >> lane & 1 && lane < m ? (int)(p.ids[here & ~EMB_LAST] - p.row0) : 0;
+#pragma unroll 4
+      for (int j = 0; j < m; ++j) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(ES_AHEAD - 1) : "memory");
+        float x[8];
+        emb_unpack(mem[j % ES_AHEAD][threadIdx.x], x);
+        const int k = j + ES_AHEAD;
+        fetch(k < 32 ? here : next, k, i0 + k < n);
 #pragma unroll
-        for (int j = 0; j < ES_AHEAD; ++j) {
-          const int t = __shfl_sync(0xffffffffu, tok, j0 + j);
-          v[j] = has && j0 + j < m ? *reinterpret_cast<const uint4*>(p.dout + (long long)t * p.dim + col) : make_uint4(0, 0, 0, 0);
-        }
-#pragma unroll
-        for (int j = 0; j < ES_AHEAD; ++j) {
-          if (j0 + j >= m) break;
-          float x[8];
-          emb_unpack(v[j], x);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) acc[e] += x[e];
-          if (ends >> (j0 + j) & 1) {
-            const int id = __shfl_sync(0xffffffffu, row, j0 + j);
-            if (has) {
-              if (began || !(last >> (j0 + j) & 1)) {
-                float4* dst = reinterpret_cast<float4*>(p.part + (2LL * c + (began ? 0 : 1)) * p.dim + col);
-                dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-              } else {
-                emb_store<F32>(p.dtable, (long long)id * p.dim + col, acc, p.scale, ADD);
-              }
+        for (int e = 0; e < 8; ++e) acc[e] += x[e];
+        if (ends >> j & 1) {
+          const int id = __shfl_sync(0xffffffffu, row, j);
+          if (has) {
+            if (began || !(last >> j & 1)) {
+              float4* dst = reinterpret_cast<float4*>(p.part + (2LL * c + (began ? 0 : 1)) * p.dim + col);
+              dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+              dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+            } else {
+              emb_store<F32>(p.dtable, (long long)id * p.dim + col, acc, p.scale, ADD);
             }
-            began = false;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] = 0.f;
           }
+          began = false;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[e] = 0.f;
         }
       }
+      here = next;
     }
   }
-  if (ADD) return;
+  if (ADD || warp_index() >= ES_FILL) return;
   // rows without a token, to whoever is free (warps end their chunks at times that differ by a fourth of the kernel's)
   const int groups = (p.rows + ES_ZERO - 1) / ES_ZERO, vecs = p.dim / (F32 ? 4 : 8);
   auto take = [&]() { return lane == 0 ? atomicAdd(p.taken, 1) : 0; };
@@ -422,10 +433,12 @@ embedding_join_kernel(const EmbGrad p) {
   }
 }
 
-// Tokens to a chunk: 32; 64 from 2^15 tokens on, where there are warps' work enough and fewer parts to join (65536 tokens, 0.3 of them
-// of one id, 2048 columns: 138 / 129 us; 8192 tokens 178 with 32, 190 with 16); more where the parts would take thousands of rows.
-static int emb_chunk(int tokens) {
-  int c = tokens > 32768 ? 64 : 32;
+// Tokens to a chunk, by the items (a chunk's 256 columns) that chunks of 32 would make: 16 where those are few, so that more warps share the rows,
+// 64 where they are many, for fewer parts to join; more where the parts would take thousands of rows.  us: 333 tokens of 1024 columns 12.1 with
+// 16, 14.1 with 32; 16384 of 512 26.4, 29.0; 4099 of 2048 73.8, 73.7; 8192 of 4096 176, 170; 65536 of 2048 117 with 32, 102 with 64.
+static int emb_chunk(int tokens, int dim) {
+  const long long items = (tokens + 31LL) / 32 * ((dim + 255) / 256);
+  int c = items < 2048 ? 16 : items < 8192 ? 32 : 64;
   while (tokens / c > 4096) c *= 2;
   return c;
 }
@@ -446,7 +459,7 @@ struct EmbLayout {
   int chunk, chunks, share;
   bool coded;
   EmbLayout(int tokens, int rows, int dim) {
-    chunk = emb_chunk(tokens);
+    chunk = emb_chunk(tokens, dim);
     chunks = (int)((tokens + (long long)chunk - 1) / chunk);
     share = emb_share(tokens);
     coded = tokens > EP_WARPS * 32 * EP_BATCH;
