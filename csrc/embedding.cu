@@ -149,31 +149,18 @@ embedding_plan_kernel(const EmbGrad p) {
   int below = 0, hits = 0;
   if (CODES) {
     for (int t = 0; t < p.share; t += 256) {
-      const uint4 c0 = *reinterpret_cast<const uint4*>(p.codes + t0 + t + 4 * lane);
-      const uint4 c1 = *reinterpret_cast<const uint4*>(p.codes + t0 + t + 128 + 4 * lane);
-      const unsigned c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+      unsigned c[8];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        bool in[4];
-        unsigned who[4], any = 0;
+      for (int i = 0; i < 8; ++i) c[i] = p.codes[t0 + t + 32 * i + lane];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const unsigned v = c[4 * half + i];
-          in[i] = v - least < EP_ROWS;
-          below += v < least;
-          who[i] = __ballot_sync(0xffffffffu, in[i]);
-          any |= who[i];
-        }
-        if (any == 0) continue;
-        int at = hits;                       // tokens of one lane follow one another
-#pragma unroll
-        for (int i = 0; i < 4; ++i) at += __popc(who[i] & below_me);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (in[i] && at < p.list) list[at] = (unsigned)(t + 128 * half + 4 * lane + i) * EP_ROWS | (c[4 * half + i] - least);
-          at += in[i];
-          hits += __popc(who[i]);
-        }
+      for (int i = 0; i < 8; ++i) {
+        const bool in = c[i] - least < EP_ROWS;
+        const unsigned who = __ballot_sync(0xffffffffu, in);
+        below += c[i] < least;
+        if (who == 0) continue;
+        const int at = hits + __popc(who & below_me);
+        if (in && at < p.list) list[at] = (unsigned)(t + 32 * i + lane) * EP_ROWS | (c[i] - least);
+        hits += __popc(who);
       }
     }
     __syncwarp();

@@ -108,6 +108,7 @@ bool has_main_grad(PyObject* o) {
 bool any_main_grad(const Tensor* w, int n) {
   py::gil_scoped_acquire gil;
   for (int i = 0; i < n; ++i) {
+    if (!w[i].defined()) continue;
     py::object o = py::reinterpret_steal<py::object>(THPVariable_Wrap(w[i]));
     if (has_main_grad(o.ptr())) return true;
   }
@@ -930,7 +931,7 @@ Tensor dense_grad(const Tensor& g) {
 }
 
 bool ids_of(const Tensor& ids, const Tensor& table) {
-  return plain_rows(ids, at::kLong) && small(ids.numel()) && ids.get_device() == table.get_device();
+  return plain_rows(ids, at::kLong) && ids.numel() <= 1 << 30 && ids.get_device() == table.get_device();
 }
 Tensor embedding_fwd(const Tensor& ids, const Tensor& table, double scale) {
   auto sizes = ids.sizes().vec();
@@ -1045,7 +1046,7 @@ struct QkNormFn : Function<QkNormFn> {
       dy[j] = dense_grad(grads[j]);
       own = dy[j].defined();
     }
-    for (int j = 0; own && j < 2; ++j) own = !need[1 + j] || !any_main_grad(&w[j], 1);
+    own = own && !((need[1] || need[2]) && any_main_grad(w, 2));
     if (!own) {
       py::gil_scoped_acquire gil;
       const py::object r = py::reinterpret_borrow<py::object>(g_qk_norm_backward)(

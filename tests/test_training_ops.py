@@ -176,3 +176,23 @@ def test_scaled_embedding(dtype):
   for bad in (float("nan"), float("inf")):
     with pytest.raises(ValueError):
       ops.embedding(ids, table, scale=bad)
+
+
+def test_llama4_with_the_fused_norms():
+  """The model's option gives its logits and gradients (fp32: another order of two products), and is off unless asked for."""
+  from torchprime_b200.config import compose
+  from torchprime_b200.models.model_utils import initialize_model_class
+  size = ["model=llama-4-text-only-dummy", "model.hidden_size=128", "model.num_attention_heads=4", "model.num_key_value_heads=2", "model.head_dim=32",
+          "model.intermediate_size=48", "model.intermediate_size_mlp=96", "model.num_local_experts=4", "model.vocab_size=256",
+          "model.num_hidden_layers=2", "model.moe_layers=[1]", "model.no_rope_layers=[1,0]"]
+  ids = torch.randint(0, 256, (2, 40), generator=torch.Generator().manual_seed(3))
+  outs = []
+  for extra in ([], ["+model.fused_qk_norm=true"]):
+    torch.manual_seed(0)
+    m = initialize_model_class(compose("default", size + extra).model)
+    assert [layer.self_attn.fused_qk_norm for layer in m.model.layers] == [bool(extra), False]
+    logits, loss = m(ids, labels=ids)
+    loss.backward()
+    outs.append([logits, *(p.grad for p in m.parameters())])
+  for a, b in zip(*outs):
+    assert torch.allclose(a, b, atol=1e-5)

@@ -349,6 +349,157 @@ def test_dropout_notices_a_seed_counted_up(cuda_lib):
     y.sum().backward()
 
 
+# ------------------------------------------------------------------------------------------- all of them
+def _calls(g):
+  """Each operator as a function of its floating inputs, and those inputs."""
+  cos, sin = _tables(9, 32)
+  seed, ids = torch.tensor([5, 6], device="cuda"), torch.randint(0, 50, (2, 9), generator=g, device="cuda")
+  return {"qk": (lambda x, a, b: ops.qk_norm_rope(x, cos, sin, 2, 1, 64, 9, a, b, interleaved=True), [_randn(g, 2, 9, 256), 1 + _randn(g, 64, std=0.3), 1 + _randn(g, 64, std=0.3)]),
+          "embedding": (lambda t: ops.embedding(ids, t, scale=3.0), [_randn(g, 50, 64)]),
+          "dropout": (lambda x, r: ops.dropout(x, 0.3, seed, residual=r), [_randn(g, 2, 9, 64), _randn(g, 2, 9, 64)])}
+
+
+NAMES = ["qk", "embedding", "dropout"]
+listed = lambda t: [t] if torch.is_tensor(t) else list(t)  # noqa: E731
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("give_back", ["elsewhere", "unaligned", "wider", "columns first"])
+def test_saved_tensor_hooks(cuda_lib, name, give_back):
+  """Hooks may give saved tensors back in another layout, alignment or type."""
+  fn, inputs = _calls(torch.Generator(device="cuda").manual_seed(20))[name]
+  inputs = [t.requires_grad_() for t in inputs]
+
+  def back(t):
+    if give_back == "elsewhere":
+      return t.clone()
+    if give_back == "unaligned" and t.element_size() < 8:
+      return torch.cat([t.flatten()[:1], t.flatten()])[1:].view(t.shape)
+    if give_back == "columns first" and t.dim() > 1:
+      return t.transpose(0, 1).contiguous().transpose(0, 1)
+    return t.float() if give_back == "wider" and t.dtype == BF16 else t
+
+  out = listed(fn(*inputs))
+  dy = [torch.randn_like(t) for t in out]
+  want = torch.autograd.grad(out, inputs, dy)
+  with torch.autograd.graph.saved_tensors_hooks(lambda t: t, back):
+    got = torch.autograd.grad(listed(fn(*inputs)), inputs, dy)
+  for a, b in zip(got, want):      # (torch's operators where the kernels cannot go on: a rounding more or less)
+    assert a.shape == b.shape and (a.float() - b.float()).abs().max() <= 4 * HALF * b.float().abs().max()
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_traces_follow_their_input(cuda_lib, name):
+  g = torch.Generator(device="cuda").manual_seed(21)
+  fn, (first, *rest) = _calls(g)[name]
+  second = _randn(g, *first.shape)
+  with torch.no_grad():
+    traced = torch.jit.trace(lambda x: fn(x, *rest), (first,), check_trace=False)
+    for x in (second, first):
+      with ops.backend("torch"):
+        want = listed(fn(x, *rest))
+      for a, b in zip(listed(traced(x)), want):
+        assert (a.float() - b.float()).abs().max() <= 2 * HALF * b.float().abs().max()
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_tangents_and_transforms(cuda_lib, name):
+  """Forward-mode derivatives, torch.func.grad and vmap give what the definitions give."""
+  import torch.autograd.forward_ad as fwd
+  g = torch.Generator(device="cuda").manual_seed(22)
+  fn, (first, *rest) = _calls(g)[name]
+  tangent = _randn(g, *first.shape)
+
+  def every():
+    with fwd.dual_level():
+      duals = [fwd.unpack_dual(t).tangent for t in listed(fn(fwd.make_dual(first, tangent), *rest))]
+    grad = torch.func.grad(lambda x: sum(t.float().square().sum() for t in listed(fn(x, *rest))))(first)
+    many = torch.func.vmap(lambda x: fn(x, *rest))(torch.stack([first, tangent]))
+    return [*duals, grad, *listed(many)]
+
+  got = every()
+  with ops.backend("torch"):
+    want = every()
+  for a, b in zip(got, want):
+    assert a is not None and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_calls_of_other_streams_and_two_at_once(cuda_lib, name):
+  """Two streams' calls do not meet; results and gradients are those of one after the other."""
+  g = torch.Generator(device="cuda").manual_seed(23)
+  fn, inputs = _calls(g)[name]
+  sets = [[t.clone().requires_grad_() for t in inputs], [(2 * t).requires_grad_() for t in inputs]]
+
+  def both(streams):
+    out = []
+    for s, ins in zip(streams, sets):
+      with torch.cuda.stream(s):
+        for _ in range(20):
+          y = listed(fn(*ins))
+          grads = torch.autograd.grad(y, ins, [torch.ones_like(t) for t in y])
+        out += [*(t.detach() for t in y), *grads]
+    torch.cuda.synchronize()
+    return out
+
+  now = torch.cuda.current_stream()
+  torch.cuda.synchronize()
+  for a, b in zip(both([torch.cuda.Stream(), torch.cuda.Stream()]), both([now, now])):
+    assert torch.equal(a, b)
+
+
+def test_empty_calls(cuda_lib):
+  cos, sin = _tables(9, 32)
+  w = torch.ones(64, device="cuda", dtype=BF16, requires_grad=True)
+  for shape in ((0, 9, 256), (2, 0, 256)):
+    x = torch.empty(shape, device="cuda", dtype=BF16, requires_grad=True)
+    out = ops.qk_norm_rope(x, cos, sin, 2, 1, 64, 9, w, w)
+    dx, dw = torch.autograd.grad(out, (x, w), [torch.ones_like(t) for t in out])
+    assert [t.shape[2] for t in out] == [2, 1, 1] and dx.shape == shape and not dw.any()
+    y = ops.dropout(x, 0.5, torch.tensor([1, 2], device="cuda"))
+    assert y.shape == shape and torch.autograd.grad(y, x, torch.ones_like(y))[0].shape == shape
+
+
+def test_numbers_of_numpy(cuda_lib):
+  import numpy as np
+  g = torch.Generator(device="cuda").manual_seed(24)
+  cos, sin = _tables(9, 32)
+  x, seed = _randn(g, 2, 9, 256), torch.tensor([1, 2], device="cuda")
+  i = np.int64
+  for a, b in zip(ops.qk_norm_rope(x, cos, sin, i(2), i(1), i(64), i(9), eps=np.float32(1e-5)), ops.qk_norm_rope(x, cos, sin, 2, 1, 64, 9, eps=float(np.float32(1e-5)))):
+    assert torch.equal(a, b)
+  assert torch.equal(ops.dropout(x, np.float64(0.3), seed, site=i(4)), ops.dropout(x, 0.3, seed, site=4))
+  assert torch.equal(ops.embedding(torch.arange(2, device="cuda"), x[0], scale=np.float64(0.5)), x[0, :2] * 0.5)
+
+
+def test_llama4_attention_with_the_fused_norms(cuda_lib):
+  """The model's option: the same up to the roundings of the separate passes (three more of heads' values, which attention hands on), in
+  results and gradients, with positions of packed rows."""
+  from torchprime_b200.config import compose
+  from torchprime_b200.models.llama4 import Llama4TextAttention
+  g = torch.Generator(device="cuda").manual_seed(25)
+  size = ["model=llama-4-text-only-dummy", "model.hidden_size=512", "model.num_attention_heads=4", "model.num_key_value_heads=2", "model.head_dim=128",
+          "model.no_rope_layers=[1,0]"]
+  cos, sin = _tables(300, 64)
+  x, dy = _randn(g, 2, 150, 512).requires_grad_(), _randn(g, 2, 150, 512)
+  pos = (torch.arange(300, device="cuda") % 100).to(torch.int32)
+  got = []
+  state = None
+  for fused in (False, True):
+    cfg = compose("default", size + ([f"+model.fused_qk_norm={str(fused).lower()}"] if fused else [])).model
+    m = Llama4TextAttention(cfg, 0).cuda().to(BF16)
+    assert m.fused_qk_norm == fused and not Llama4TextAttention(cfg, 1).fused_qk_norm
+    if state is None:
+      for p in m.parameters():
+        torch.nn.init.normal_(p, std=0.05)
+      state = m.state_dict()
+    m.load_state_dict(state)
+    y = m(x, cos, sin, position_ids=pos)
+    got.append([y, *torch.autograd.grad(y, [x, *m.parameters()], dy)])
+  for a, b in zip(*got):
+    assert (a.float() - b.float()).abs().max() <= 8 * HALF * a.float().abs().max()
+
+
 # ------------------------------------------------------------------------------------------- together
 def _block(p, ids, cos, sin, seed, drop, o):
   """Embedding, dropout, norm, projection, normalised heads, attention, projection, dropout with the residual."""

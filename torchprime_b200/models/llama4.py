@@ -201,6 +201,8 @@ class Llama4TextAttention(nn.Module):
     self.o_proj = nn.Linear(config.hidden_size, config.hidden_size, bias=bias)
     if config.get("use_qk_norm", False) and self.use_rope:
       self.qk_norm = Llama4TextL2Norm(config.rms_norm_eps)
+    # one pass instead of the rotation's and the norms' (in front of the rotation, which does not change them; rounded once, not twice)
+    self.fused_qk_norm = hasattr(self, "qk_norm") and bool(config.get("fused_qk_norm", False))
     self.attention_kernel = config.get("attention_kernel", None)
     self.tp_group = None   # set by the engine: q/k/v column-parallel (heads split), o row-parallel
 
@@ -215,13 +217,16 @@ class Llama4TextAttention(nn.Module):
       if self.q_proj.bias is not None:
         bias = torch.cat([self.q_proj.bias, self.k_proj.bias, self.v_proj.bias])
       qkv = ops.linear(x, [self.q_proj.weight, self.k_proj.weight, self.v_proj.weight], bias=bias)
-      if self.use_rope:
-        qkv = ops.rope_inplace(qkv, rope_cos, rope_sin, hq + hkv, d, s, pos=position_ids, interleaved=True)
-      q = qkv[..., : hq * d].view(b, s, hq, d)
-      k = qkv[..., hq * d: (hq + hkv) * d].view(b, s, hkv, d)
-      v = qkv[..., (hq + hkv) * d:].view(b, s, hkv, d)
-      if hasattr(self, "qk_norm"):
-        q, k = self.qk_norm(q), self.qk_norm(k)
+      if self.fused_qk_norm:
+        q, k, v = ops.qk_norm_rope(qkv, rope_cos, rope_sin, hq, hkv, d, s, eps=self.qk_norm.eps, pos=position_ids, interleaved=True)
+      else:
+        if self.use_rope:
+          qkv = ops.rope_inplace(qkv, rope_cos, rope_sin, hq + hkv, d, s, pos=position_ids, interleaved=True)
+        q = qkv[..., : hq * d].view(b, s, hq, d)
+        k = qkv[..., hq * d: (hq + hkv) * d].view(b, s, hkv, d)
+        v = qkv[..., (hq + hkv) * d:].view(b, s, hkv, d)
+        if hasattr(self, "qk_norm"):
+          q, k = self.qk_norm(q), self.qk_norm(k)
       if self.attn_temperature_tuning and not self.use_rope:
         pos = torch.arange(s, device=x.device).float() if position_ids is None else position_ids.view(b, s).float()
         scales = torch.log(torch.floor((pos + 1.0) / self.floor_scale) + 1.0) * self.attn_scale + 1.0

@@ -802,12 +802,13 @@ def qk_norm_rope(qkv, cos_half, sin_half, hq, hkv, d, seq_len, q_weight=None, k_
   if not 0.0 <= eps < float("inf"):
     raise ValueError(f"qk_norm_rope: eps {eps}")
   _debug.check_index("qk_norm_rope", "pos", pos, 0, cos_half.shape[0])
+  _settle(qkv, q_weight, k_weight)
   if (unobserved() and _qk_norm_ok(qkv, q_weight, k_weight, cos_half, sin_half, d, eps)
       and not (torch.is_grad_enabled() and (cos_half.requires_grad or sin_half.requires_grad))):
     if pos is not None:
       pos = pos.clamp(-1, 2 ** 31 - 1).to(torch.int32) if pos.dtype == torch.int64 else pos
       pos = pos.contiguous()
-    return _QkNormRopeFn.apply(qkv, q_weight, k_weight, cos_half, sin_half, pos, (hq, hkv, d, seq_len, eps, bool(interleaved)))
+    return _QkNormRopeFn.apply(qkv, q_weight, k_weight, cos_half, sin_half, pos, (int(hq), int(hkv), int(d), int(seq_len), eps, bool(interleaved)))
   return ref.qk_norm_rope(qkv, cos_half, sin_half, hq, hkv, d, seq_len, q_weight, k_weight, eps, pos, interleaved)
 
 
@@ -864,7 +865,7 @@ def dropout(x, p, seed, site=0, residual=None, training=True):
   if not 0 <= site < 2 ** 32:
     raise ValueError(f"dropout: site {site}")
   if use_kernels(x, residual) and unobserved():
-    return _DropoutFn.apply(x, residual, seed.contiguous(), threshold, site)
+    return _DropoutFn.apply(x, residual, seed.contiguous(), threshold, int(site))
   return ref.dropout(x, ref.dropout_keep(x.shape, threshold, seed, site), threshold, residual)
 
 
@@ -980,8 +981,8 @@ def embedding(ids, table, scale=None):
     y = nat.embedding(ids, table, 1.0 if scale is None else scale)
     if y is not None:
       return y
-  if (use_kernels(table) and table.dim() == 2 and table.shape[1] % 8 == 0 and table.is_contiguous() and table.data_ptr() % 16 == 0
-      and ids.dtype == torch.int64 and ids.device == table.device and (scale is None or unobserved())):
+  if (use_kernels(table) and unobserved() and table.dim() == 2 and table.shape[1] % 8 == 0 and table.is_contiguous()
+      and table.data_ptr() % 16 == 0 and ids.dtype == torch.int64 and ids.device == table.device and ids.numel() <= 1 << 30):
     return _EmbeddingFn.apply(ids, table, 1.0 if scale is None else scale)
   y = F.embedding(ids, table)
   return y if scale is None else (ref.wide(y) * scale).to(table.dtype)
