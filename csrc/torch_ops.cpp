@@ -918,6 +918,11 @@ bool mla_pack_into(py::handle kv_, py::handle rot_, int64_t heads, int64_t dn, i
 }
 
 // ------------------------------------------------------------------------------------------- without gradients only
+// Memory on t's device, where nothing is recorded (a node's forward and backward, too): straight from the allocator, ahead of every dispatch.
+Tensor fresh(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::detail::empty_cuda(sizes, type, t.device(), std::nullopt);
+}
+
 // A tensor as an argument of a Python function.
 py::object to_python(const Tensor& t) {
   return t.defined() ? py::reinterpret_steal<py::object>(THPVariable_Wrap(t)) : py::object(py::none());
@@ -936,7 +941,7 @@ bool ids_of(const Tensor& ids, const Tensor& table) {
 Tensor embedding_fwd(const Tensor& ids, const Tensor& table, double scale) {
   auto sizes = ids.sizes().vec();
   sizes.push_back(table.size(1));
-  Tensor y = empty_as(table, sizes);
+  Tensor y = fresh(table, sizes, at::kBFloat16);
   check(tpb_embedding_fwd(cptr(table), static_cast<const long long*>(cptr(ids)), mptr(y), (int)ids.numel(), (int)table.size(1),
                           table.size(0), 0, (float)scale, stream()),
         "embedding_fwd");
@@ -960,8 +965,8 @@ struct EmbeddingFn : Function<EmbeddingFn> {
               Tensor(), Tensor()};
     }
     const int tokens = (int)ids.numel(), rows = (int)table.size(0), dim = (int)table.size(1);
-    Tensor dtable = empty_as(table, table.sizes());
-    Tensor scratch = empty_like_type(table, {tpb_embedding_bwd_scratch(tokens, rows, dim)}, at::kByte);
+    Tensor dtable = fresh(table, table.sizes(), at::kBFloat16);
+    Tensor scratch = fresh(table, {tpb_embedding_bwd_scratch(tokens, rows, dim)}, at::kByte);
     check(tpb_embedding_bwd(cptr(dout), static_cast<const long long*>(cptr(ids)), mptr(dtable), mptr(scratch), tokens, dim, rows, 0, 0, 0,
                             (float)scale, stream()),
           "embedding_bwd");
@@ -1014,7 +1019,7 @@ bool qk_tensors(const QkArgs& a, const Tensor& x, const Tensor& qw, const Tensor
 
 variable_list qk_fwd(const QkArgs& a, const Tensor& x, const Tensor& qw, const Tensor& kw, const Tensor& cos, const Tensor& sin, const Tensor& pos) {
   const int64_t b = x.size(0), s = x.size(1);
-  Tensor q = empty_as(x, {b, s, a.hq, a.d}), k = empty_as(x, {b, s, a.hkv, a.d});
+  Tensor q = fresh(x, {b, s, a.hq, a.d}, at::kBFloat16), k = fresh(x, {b, s, a.hkv, a.d}, at::kBFloat16);
   check(tpb_qk_norm_fwd(cptr(x), row_pitch(x), cptr(qw), cptr(kw), static_cast<const float*>(cptr(cos)), static_cast<const float*>(cptr(sin)),
                         (int)cos.size(0), iptr(pos), (int)a.seq, mptr(q), mptr(k), (int)(b * s), (int)a.hq, (int)a.hkv, (int)a.d,
                         (int)(2 * cos.size(1)), (float)a.eps, a.interleaved, stream()),
@@ -1056,10 +1061,10 @@ struct QkNormFn : Function<QkNormFn> {
       return out;
     }
     const int64_t tokens = x.size(0) * x.size(1);
-    Tensor dx = empty_as(x, x.sizes()), sums, dw[2];
-    if (need[1] || need[2]) sums = empty_like_type(x, {tpb_qk_norm_bwd_scratch((int)tokens, (int)a.d)}, at::kFloat);
+    Tensor dx = fresh(x, x.sizes(), at::kBFloat16), sums, dw[2];
+    if (need[1] || need[2]) sums = fresh(x, {tpb_qk_norm_bwd_scratch((int)tokens, (int)a.d)}, at::kFloat);
     for (int j = 0; j < 2; ++j)
-      if (need[1 + j]) dw[j] = empty_as(w[j], {a.d});
+      if (need[1 + j]) dw[j] = fresh(x, {a.d}, at::kBFloat16);
     check(tpb_qk_norm_bwd(cptr(x), row_pitch(x), cptr(w[0]), cptr(w[1]), static_cast<const float*>(cptr(cos)),
                           static_cast<const float*>(cptr(sin)), (int)cos.size(0), iptr(pos), (int)a.seq, cptr(dy[0]), cptr(dy[1]), cptr(dy[2]),
                           mptr(dx), static_cast<float*>(mptr(sums)), mptr(dw[0]), mptr(dw[1]), (int)tokens, (int)a.hq, (int)a.hkv, (int)a.d,
@@ -1098,7 +1103,7 @@ py::object qk_norm_rope(py::handle x_, py::handle cos_, py::handle sin_, py::han
 
 // ------------------------------------------------------------------------------------------- dropout
 Tensor dropout_now(const Tensor& x, const Tensor& residual, const Tensor& seed, int64_t threshold, int64_t site) {
-  Tensor y = empty_as(x, x.sizes());
+  Tensor y = fresh(x, x.sizes(), at::kBFloat16);
   check(tpb_dropout(cptr(x), cptr(residual), mptr(y), static_cast<const long long*>(cptr(seed)), x.numel(), (int)threshold, (unsigned)site,
                     stream()),
         "dropout");
@@ -1281,11 +1286,6 @@ py::object grouped_mlp_few_rows(py::handle x_, py::handle rw_, py::handle idx_, 
           "moe_combine");
   }
   return py::cast(y);
-}
-
-// Memory on t's device, for operators that record nothing: straight from the allocator, ahead of every dispatch.
-Tensor fresh(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type) {
-  return at::detail::empty_cuda(sizes, type, t.device(), std::nullopt);
 }
 
 // The pools of a paged cache and, where they are e4m3, their scales: layouts that the kernels take, on the current device; see
