@@ -498,7 +498,7 @@ extern "C" long long tpb_embedding_bwd_scratch(int tokens, int rows_local, int d
 // dtable[v] = (`add`: dtable[v] +) scale * sum of dout[t] over ids[t] = row0 + v; with `add`, rows without a token are left alone.
 extern "C" int tpb_embedding_bwd(const void* dout, const long long* ids, void* dtable, void* scratch, int tokens, int dim, int rows_local,
                                  long long row0, int dtable_is_f32, int add, float scale, void* stream) {
-  if (dim % 8 || dim <= 0 || tokens < 0 || tokens > 1 << 30 || rows_local < 0) return -2;
+  if (dim % 8 || dim <= 0 || tokens < 0 || tokens > 1 << 30 || rows_local < 0 || rows_local > 1 << 30) return -2;
   for (const void* a : {dout, (const void*)dtable, (const void*)scratch})
     if (reinterpret_cast<uintptr_t>(a) % 16) return -2;
   if (rows_local == 0 || (tokens == 0 && add)) return 0;

@@ -313,7 +313,7 @@ qk_norm_bwd_kernel(const QkNorm p) {
           g = qk_times(g, w);
           dot = qk_dot(g, x);
         }
-        const float r = rsqrtf(qk_sum<GROUP>(qk_dot(x, x)) * inv_d + p.eps), k = -r * r * r * (qk_sum<GROUP>(dot) * inv_d);
+        const float r = rsqrtf(qk_sum<GROUP>(qk_dot(x, x)) * inv_d + p.eps), k = -r * (r * (r * (qk_sum<GROUP>(dot) * inv_d)));      // (r^3 may overflow)
         const f32x2 rr = f2_pack(r, r), kk = f2_pack(k, k);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {

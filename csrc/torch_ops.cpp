@@ -977,7 +977,7 @@ struct EmbeddingFn : Function<EmbeddingFn> {
 py::object embedding(py::handle ids_, py::handle table_, double scale) {
   Tensor ids, table, y;
   if (!unobserved() || !unpack(ids_, ids) || !unpack(table_, table) || !plain_rows(table) || table.dim() != 2 || table.size(1) % 8 ||
-      !aligned(table) || !small(table.size(0)) || !small(table.size(1)) || !ids_of(ids, table) ||
+      !aligned(table) || table.size(0) > 1 << 30 || !small(table.size(1)) || !ids_of(ids, table) ||
       table.get_device() != c10::cuda::current_device())
     return py::none();
   const bool rec = at::GradMode::is_enabled() && recording(table);
@@ -1034,7 +1034,9 @@ struct QkNormFn : Function<QkNormFn> {
     ctx->save_for_backward({x, get(qw), get(kw), cos, sin, get(pos)});
     ctx->saved_data["i"] = std::vector<int64_t>{hq, hkv, d, seq, interleaved};
     ctx->saved_data["e"] = eps;
-    return qk_fwd({hq, hkv, d, seq, interleaved, eps}, x, get(qw), get(kw), cos, sin, get(pos));
+    variable_list y = qk_fwd({hq, hkv, d, seq, interleaved, eps}, x, get(qw), get(kw), cos, sin, get(pos));
+    if (!ctx->needs_input_grad(0)) ctx->mark_non_differentiable({y[2]});
+    return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list t = ctx->get_saved_variables();

@@ -199,6 +199,29 @@ def test_qk_norm_rope_gradients_recorded_or_several_at_once(cuda_lib):
   assert not only[..., : 2 * 64].any() and not only[..., 3 * 64:].any() and torch.equal(only[..., 128: 192], plain[0][..., 128: 192])
 
 
+def test_qk_norm_rope_over_a_frozen_projection(cuda_lib):
+  """Only the weights learn: the values have no gradient, and what uses them does not ask for one."""
+  g = torch.Generator(device="cuda").manual_seed(26)
+  cos, sin = _tables(9, 32)
+  x, w = _randn(g, 2, 9, 4 * 64), (1 + _randn(g, 64, std=0.3)).requires_grad_()
+  q, k_, v = ops.qk_norm_rope(x, cos, sin, 2, 1, 64, 9, q_weight=w)
+  assert q.requires_grad and not v.requires_grad
+  dq = _randn(g, *q.shape)
+  (dw,) = torch.autograd.grad(q, w, dq)
+  want, size = _qk_exact(x, cos, sin, 2, 1, 64, 9, w, None, 1e-6, None, False, [dq, torch.zeros_like(k_), torch.zeros_like(v)])
+  assert bool(((dw.double() - want[1]).abs() <= HALF * want[1].abs() + 2.0 ** -16 * size[1]).all())
+
+
+def test_qk_norm_rope_of_small_eps(cuda_lib):
+  """The third power of the factor leaves fp32, the gradient does not."""
+  g = torch.Generator(device="cuda").manual_seed(27)
+  cos, sin = _tables(8, 64)
+  x = _randn(g, 1, 8, 6 * 128)
+  x[0, 1, :128] = 0
+  x[0, 2] *= 2.0 ** -48
+  _check_qk(x, cos, sin, 4, 1, 128, None, 1 + _randn(g, 128, std=0.3), eps=2.0 ** -100, g=g)
+
+
 def test_weights_collect_their_gradients(cuda_lib):
   """Norm weights and tables with a main_grad: overwritten first, then added to."""
   g = torch.Generator(device="cuda").manual_seed(11)

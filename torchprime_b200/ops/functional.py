@@ -764,7 +764,10 @@ class _QkNormRopeFn(torch.autograd.Function):
     ctx.save_for_backward(qkv, q_weight, k_weight, cos, sin, pos)
     ctx.args = args
     q, kk = k.qk_norm_fwd(qkv, hq, hkv, d, q_weight, k_weight, cos, sin, seq_len, pos, eps, interleaved)
-    return q, kk, qkv[..., (hq + hkv) * d:].unflatten(-1, (hkv, d))
+    v = qkv[..., (hq + hkv) * d:].unflatten(-1, (hkv, d))
+    if not ctx.needs_input_grad[0]:
+      ctx.mark_non_differentiable(v)
+    return q, kk, v
 
   @staticmethod
   def backward(ctx, dq, dk, dv):
@@ -982,7 +985,8 @@ def embedding(ids, table, scale=None):
     if y is not None:
       return y
   if (use_kernels(table) and unobserved() and table.dim() == 2 and table.shape[1] % 8 == 0 and table.is_contiguous()
-      and table.data_ptr() % 16 == 0 and ids.dtype == torch.int64 and ids.device == table.device and ids.numel() <= 1 << 30):
+      and table.data_ptr() % 16 == 0 and ids.dtype == torch.int64 and ids.device == table.device and ids.numel() <= 1 << 30
+      and table.shape[0] <= 1 << 30):
     return _EmbeddingFn.apply(ids, table, 1.0 if scale is None else scale)
   y = F.embedding(ids, table)
   return y if scale is None else (ref.wide(y) * scale).to(table.dtype)

@@ -116,7 +116,7 @@ def qk_norm_rope_grad(dq, dk, dv, qkv, cos_half, sin_half, hq, hkv, d, seq_len, 
     g = _turn(wide(dy), cos, -sin, interleaved)
     dw = None if w is None else (g * (t * r)).sum((0, 1, 2)).to(w.dtype)
     g = g if w is None else g * wide(w)
-    return (r * g - t * (r * r * r * (g * t).mean(-1, keepdim=True))).to(qkv.dtype), dw
+    return (r * g - t * (r * (r * (r * (g * t).mean(-1, keepdim=True))))).to(qkv.dtype), dw
 
   gq, dwq = head(dq, x[:, :, :hq], q_weight)
   gk, dwk = head(dk, x[:, :, hq: hq + hkv], k_weight)
