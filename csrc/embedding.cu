@@ -35,8 +35,9 @@ constexpr int EP_ROWS = 1024;                // most ids to a CTA of it
 constexpr int EP_BATCH = 8;                  // ids of a lane that are asked for at once
 constexpr int EP_SMEM = 220 * 1024;
 constexpr int EJ_WARPS = 32;                 // of the joining kernel
-constexpr int EJ_LONG = 8;                   // chunks behind its first from which a CTA's warps share an id (8192 tokens, 65536 with 0.3 of one
-                                             // id: 4 177.0 and 126.7 us, 8 176.8 and 126.6, 16 178.6 and 126.6, 32 180.5 and, with other joins, 143 / 137)
+// Chunks behind its first from which a CTA's warps share an id.  8192 tokens, and 65536 with 0.3 of one id (when all took 177 and 127 us): 4 177.0
+// and 126.7, 8 176.8 and 126.6, 16 178.6 and 126.8.
+constexpr int EJ_LONG = 8;
 // Of the summing kernel: CTAs to an SM, rows that a warp asks for ahead, and warps of a CTA that write zeros at the end.  us, 8192 tokens of a 128256 x
 // 4096 table / 65536 of 32000 x 2048, 0.3 of them of one id: 4, 8, 2 170 / 103;  4, 8, 4 175 / 103;  4, 8, 8 184 / 103;  3, 16, 8 180 / 111;  2, 16, 8
 // 198 / 125;  5, 8, 8 - / 129;  two CTAs with eight rows in registers, 8 177 / 127.
@@ -51,7 +52,8 @@ __device__ __forceinline__ uint4 emb_pack(const float* f) {
   return make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
 }
 
-// A warp takes up to 4 x 32 vectors of a token's row.
+// A warp takes up to 4 x 32 vectors of a token's row, all asked for before the first is used.  4099 rows of 5120 11.6 us, 12.8 at a copy's rate (some
+// rows come from L2 a second time).
 template <bool SCALED>
 __global__ void __launch_bounds__(256)
 embedding_fwd_kernel(const uint4* __restrict__ table, const long long* __restrict__ ids, uint4* __restrict__ out, unsigned units,
@@ -91,7 +93,7 @@ struct EmbGrad {
   int *valid, *taken;                        // taken (zeroed by the planning kernel): rows that the sum's warps have looked at
   float* part;                               // [chunks][2][dim]: of the id that began before the chunk, of the one that goes on behind it
   long long row0;
-  int tokens, rows, dim, chunk, chunks;
+  int tokens, rows, dim, chunk;
   int sets, per, share;                      // CTAs of the planning kernel, most ids to one: id v is the v / sets-th of set v % sets; tokens to a warp
   int list;                                  // entries of a warp's list there
   unsigned inv, shift;                       // v / sets = v * inv >> shift
@@ -519,7 +521,6 @@ extern "C" int tpb_embedding_bwd(const void* dout, const long long* ids, void* d
   p.rows = rows_local;
   p.dim = dim;
   p.chunk = at.chunk;
-  p.chunks = at.chunks;
   p.share = at.share;
   p.per = emb_per(rows_local);
   p.sets = (rows_local + p.per - 1) / p.per;
