@@ -271,9 +271,9 @@ __device__ __forceinline__ void emb_store(void* dtable, long long at, const floa
   }
 }
 
-// Sixteen bytes to this thread's own place in shared memory, or none.
-__device__ __forceinline__ void emb_ask(uint4* dst, const void* src, bool has) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(has ? 16 : 0) : "memory");
+// Sixteen bytes to this thread's own place in shared memory.
+__device__ __forceinline__ void emb_ask(uint4* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 
 template <bool F32, bool ADD>
@@ -294,7 +294,7 @@ embedding_sum_kernel(const EmbGrad p) {
     const __nv_bfloat16* from = p.dout + (has ? col : 0);
     auto fetch = [&](unsigned tokens, int j, bool there) {             // row j of 32; a group each time
       const int t = __shfl_sync(0xffffffffu, tokens, j & 31) & ~EMB_LAST;
-      emb_ask(&mem[j % ES_AHEAD][threadIdx.x], from + (there ? (long long)t * p.dim : 0), there && has);
+      if (there && has) emb_ask(&mem[j % ES_AHEAD][threadIdx.x], from + (long long)t * p.dim);        // (what is asked for is also waited for)
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
