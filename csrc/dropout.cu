@@ -99,6 +99,7 @@ dropout_kernel(const Dropout p) {
     y[i] = make_uint4(drop_pair(v.x, bits.x, most, p.up, RES ? &r.x : nullptr), drop_pair(v.y, bits.y, most, p.up, RES ? &r.y : nullptr),
                       drop_pair(v.z, bits.z, most, p.up, RES ? &r.z : nullptr), drop_pair(v.w, bits.w, most, p.up, RES ? &r.w : nullptr));
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");      // (of a thread without a vector: zeros on their way to its places)
   if (blockIdx.x == gridDim.x - 1 && threadIdx.x < p.n % 8) {      // what does not fill a vector
     const unsigned long long i = vecs * 8 + threadIdx.x;
     const uint4 bits = philox(make_uint4((uint32_t)vecs, (uint32_t)(vecs >> 32), step, p.site), keys);
