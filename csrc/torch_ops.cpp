@@ -1035,7 +1035,8 @@ struct QkNormFn : Function<QkNormFn> {
     ctx->saved_data["i"] = std::vector<int64_t>{hq, hkv, d, seq, interleaved};
     ctx->saved_data["e"] = eps;
     variable_list y = qk_fwd({hq, hkv, d, seq, interleaved, eps}, x, get(qw), get(kw), cos, sin, get(pos));
-    if (!ctx->needs_input_grad(0)) ctx->mark_non_differentiable({y[2]});
+    // (needs_input_grad is the backward pass's: in a forward that one reruns it looks the edge up in that pass's graph)
+    if (!recording(x)) ctx->mark_non_differentiable({y[2]});
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {

@@ -1,0 +1,64 @@
+"""Norms of query and key heads, the embedding and dropout inside autograd: recomputed layers under partial backward passes."""
+
+import pytest
+import torch
+
+from torchprime_b200.ops import functional as ops
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+@pytest.fixture(autouse=True, params=["native", "python"])
+def way(request, monkeypatch):
+  """The operators as native torch functions, and their Python definitions over the same kernels."""
+  if request.param == "python":
+    monkeypatch.setattr(ops, "_native", lambda: None)
+  return request.param
+
+
+def _randn(g, *shape, std=1.0):
+  return (torch.randn(*shape, generator=g, device="cuda") * std).to(BF16)
+
+
+def _tables(n, half):
+  angle = torch.arange(n, device="cuda")[:, None].double() * 10000.0 ** (-torch.arange(half, device="cuda").double() / half)
+  return angle.cos().float().contiguous(), angle.sin().float().contiguous()
+
+
+class _Rerun(torch.autograd.Function):
+  """A layer that runs without a graph, and once more with one when its gradients are asked for."""
+
+  @staticmethod
+  def forward(ctx, fn, x, *weights):
+    ctx.fn = fn
+    ctx.save_for_backward(x, *weights)
+    return fn(x, *weights)
+
+  @staticmethod
+  def backward(ctx, *dy):
+    again = [t.detach().requires_grad_(need) for t, need in zip(ctx.saved_tensors, ctx.needs_input_grad[1:])]
+    with torch.enable_grad():
+      y = ctx.fn(*again)
+    pairs = [(a, b) for a, b in zip(y, dy) if a.requires_grad]
+    torch.autograd.backward([a for a, _ in pairs], [b for _, b in pairs])
+    return (None, *(t.grad for t in again))
+
+
+@pytest.mark.parametrize("how", ["grad", "inputs", "all"])
+def test_a_layer_rerun_in_a_backward_pass_has_its_values_gradient(cuda_lib, how):
+  g = torch.Generator(device="cuda").manual_seed(1)
+  cos, sin = _tables(9, 32)
+  x, w = _randn(g, 2, 9, 4 * 64).requires_grad_(), (1 + _randn(g, 64, std=0.3)).requires_grad_()
+  dy = [_randn(g, 2, 9, n, 64) for n in (2, 1, 1)]
+  layer = lambda x, w: ops.qk_norm_rope(x, cos, sin, 2, 1, 64, 9, w, w)  # noqa: E731
+  want = torch.autograd.grad(layer(x, w), (x, w), dy)
+  y = _Rerun.apply(layer, x, w)
+  if how == "grad":
+    got = torch.autograd.grad(y, (x, w), dy)
+  else:
+    torch.autograd.backward(y, dy, **(dict(inputs=[x, w]) if how == "inputs" else {}))
+    got = (x.grad, w.grad)
+  assert torch.equal(got[0][..., 3 * 64:], dy[2].view(2, 9, 64))
+  for a, b in zip(got, want):
+    assert torch.equal(a, b)
