@@ -49,6 +49,12 @@ extern "C" void tpb_status_clear(void) {
     for (int i = 0; i < 4; ++i) tpb::g_status_host[i] = 0;
 }
 extern "C" int tpb_sm_count(void) { return tpb::sm_count(); }
+extern "C" unsigned long long tpb_capture_id(void* stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id) != cudaSuccess) return 0;
+  return status == cudaStreamCaptureStatusActive ? id : 0;
+}
 
 // A wait that is meant to run out: spins (bounded by `budget_cycles`) until *flag == expected and
 // reports kTimeoutPeerFlag into the status block when the budget is exhausted.  Used by the

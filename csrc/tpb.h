@@ -26,6 +26,8 @@ enum {
 int tpb_status(int* out4);
 void tpb_status_clear(void);
 int tpb_sm_count(void);
+// Number of the capture that the stream is part of, each of a process its own; 0: none.
+unsigned long long tpb_capture_id(void* stream);
 // Bounded device-side wait on a flag (failure-detection building block): *result = 1 when the flag
 // reached `expected`, -1 (and status code 5) when `budget_cycles` ran out first.
 int tpb_bounded_wait(const unsigned* flag, unsigned expected, long long budget_cycles, int* result, void* stream);

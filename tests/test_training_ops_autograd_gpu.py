@@ -1,4 +1,5 @@
-"""Norms of query and key heads, the embedding and dropout inside autograd: recomputed layers under partial backward passes."""
+"""Norms of query and key heads, the embedding and dropout inside autograd: recomputed layers under partial backward passes, gradients
+that are collected in a ``main_grad``."""
 
 import pytest
 import torch
@@ -62,3 +63,46 @@ def test_a_layer_rerun_in_a_backward_pass_has_its_values_gradient(cuda_lib, how)
   assert torch.equal(got[0][..., 3 * 64:], dy[2].view(2, 9, 64))
   for a, b in zip(got, want):
     assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------------- main_grad
+def _collect(t, dtype=torch.float32):
+  """The same numbers as a parameter that collects its gradient."""
+  p = t.detach().clone().requires_grad_()
+  p.main_grad, p.grad_overwrite = torch.full(t.shape, 7.0, device="cuda", dtype=dtype), True
+  return p
+
+
+def _captured(step):
+  side = torch.cuda.Stream()
+  side.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(side):
+    step()
+  torch.cuda.current_stream().wait_stream(side)
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    step()
+  return graph
+
+
+def test_a_captured_pass_adds_up_the_gradients_of_a_shared_weight(cuda_lib):
+  """One weight for queries and keys; a table that is the output projection too; two microbatches in one graph."""
+  g = torch.Generator(device="cuda").manual_seed(3)
+  cos, sin = _tables(9, 32)
+  table, w, x = _randn(g, 64, 64, std=0.1), 1 + _randn(g, 64, std=0.3), _randn(g, 2, 9, 4 * 64)
+  ids, dout = torch.randint(0, 64, (40,), generator=g, device="cuda"), _randn(g, 40, 64)
+  dq, dk = _randn(g, 2, 9, 2, 64), _randn(g, 2, 9, 1, 64)
+
+  def step(table, w):
+    for _ in range(2):
+      q, kk, _ = ops.qk_norm_rope(x, cos, sin, 2, 1, 64, 9, w, w)
+      torch.autograd.grad((q, kk), w, (dq, dk), allow_unused=True)
+      torch.autograd.grad(ops.linear(ops.embedding(ids, table), [table]), table, dout, allow_unused=True)
+
+  mine, want = ([_collect(t) for t in (table, w)] for _ in range(2))
+  graph = _captured(lambda: step(*mine))
+  for _ in range(2):
+    graph.replay()
+  step(*want)
+  for a, b in zip(mine, want):
+    assert torch.equal(a.main_grad, b.main_grad)

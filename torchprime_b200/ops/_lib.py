@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_float, c_int, c_longlong, c_uint, c_void_p
+from ctypes import c_float, c_int, c_longlong, c_uint, c_ulonglong, c_void_p
 
 import torch
 
@@ -122,6 +122,7 @@ def _declare(L):
     fn.restype = c_int
   for name, args in {"tpb_embedding_bwd_scratch": [I, I, I], "tpb_qk_norm_bwd_scratch": [I, I]}.items():
     getattr(L, name).argtypes, getattr(L, name).restype = args, LL
+  L.tpb_capture_id.argtypes, L.tpb_capture_id.restype = [P], c_ulonglong
   L.tpb_status_clear.argtypes = []
   L.tpb_status_clear.restype = None
   _declare_optional(L)

@@ -134,13 +134,27 @@ def _grad_sink(weights):
   return _fused_view(mgs)
 
 
+def _capture() -> int:
+  """Number of the CUDA graph capture that the current stream is part of, or 0."""
+  return _lib.lib().tpb_capture_id(_lib.stream_ptr()) if torch.cuda.is_current_stream_capturing() else 0
+
+
 def overwrites_grad(w) -> bool:
   """Whether the gradient about to be delivered replaces the content of ``w.main_grad`` (first
   gradient of the step) or adds to it.  A backward pass that is being captured into a CUDA graph is
-  replayed once per step, so what it records is always the overwriting form."""
-  if w.is_cuda and torch.cuda.is_current_stream_capturing():
-    return True
+  replayed once per step, so what it records first for a weight is always the overwriting form; a weight
+  that gets several gradients in a step (one for queries and keys, a table that is the output projection
+  too, microbatches) has them added up if they are captured into one graph."""
+  if w.is_cuda and (capture := _capture()):
+    return getattr(w, "grad_capture", 0) != capture
   return bool(getattr(w, "grad_overwrite", False))
+
+
+def grad_delivered(w):
+  """``w.main_grad`` holds a gradient of this step (or of the pass that is being captured): the next one adds to it."""
+  w.grad_overwrite = False
+  if w.is_cuda and (capture := _capture()):
+    w.grad_capture = capture
 
 
 def _wgrad_into(sink, weights, dy2, x2):
@@ -154,7 +168,7 @@ def _wgrad_into(sink, weights, dy2, x2):
   if push is not None:
     if overwrite and all(getattr(w, "rs_push", None) is not None for w in weights) and push(sink, dy2, x2):
       for w in weights:
-        w.grad_overwrite = False
+        grad_delivered(w)
       return
     if not overwrite:
       push.func.__self__.check_not_pushed(push.args[0], sink)
@@ -163,7 +177,7 @@ def _wgrad_into(sink, weights, dy2, x2):
   else:
     k.gemm(dy2, x2, a_mn=True, b_mn=True, out=sink, epi=k.EPI_BF16 if overwrite else k.EPI_BF16_ACC)
   for w in weights:
-    w.grad_overwrite = False
+    grad_delivered(w)
 
 
 # --------------------------------------------------------------------------- gathers in flight
@@ -565,7 +579,7 @@ def _norm_wgrad(w, dw_f32):
     k.cast_f32_to_bf16_(dw_f32, mg, 1.0, accumulate=not overwrite)
   else:
     mg.copy_(dw_f32 if overwrite else mg.float() + dw_f32)
-  w.grad_overwrite = False
+  grad_delivered(w)
   return None
 
 
@@ -964,8 +978,7 @@ class _EmbeddingPeerFn(torch.autograd.Function):
     table = ctx.table
     overwrite = overwrites_grad(table)
     _embedding_collect(ids, table.main_grad, dout, 1.0, overwrite)
-    if overwrite:
-      table.grad_overwrite = False
+    grad_delivered(table)
     return None, None, None
 
 

@@ -373,9 +373,9 @@ def _deliver_wgrad(w, compute):
   """Run ``compute(out, accumulate)`` into ``w.main_grad`` when present, else return a fresh gradient."""
   mg = getattr(w, "main_grad", None)
   if mg is not None:
-    from .functional import overwrites_grad
+    from .functional import grad_delivered, overwrites_grad
     compute(mg, not overwrites_grad(w))
-    w.grad_overwrite = False
+    grad_delivered(w)
     return None
   g = torch.empty(w.shape, dtype=torch.bfloat16, device=w.device)
   compute(g, False)
