@@ -50,3 +50,12 @@ def test_a_cpu_weight_has_no_capture(monkeypatch):
   assert ops.overwrites_grad(w)
   ops.grad_delivered(w)
   assert not ops.overwrites_grad(w)
+
+
+def test_a_captured_table_replaces(capture, monkeypatch):
+  """A table whose warm-up pass has cleared the flag: overwritten by the first gradient of a capture, added to by the next."""
+  table, how = SimpleNamespace(is_cuda=True, main_grad="sink", grad_overwrite=False), []
+  monkeypatch.setattr(ops, "_embedding_collect", lambda ids, mg, dout, scale, overwrite: how.append(overwrite))
+  for capture.id in (0, 7, 7, 8):
+    assert ops._embedding_backward(None, table, None, 1.0) is None
+  assert how == [False, True, False, True]

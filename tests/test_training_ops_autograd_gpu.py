@@ -106,3 +106,29 @@ def test_a_captured_pass_adds_up_the_gradients_of_a_shared_weight(cuda_lib):
   step(*want)
   for a, b in zip(mine, want):
     assert torch.equal(a.main_grad, b.main_grad)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+def test_a_captured_pass_replaces_what_its_last_replay_collected(cuda_lib, dtype):
+  """A table's and a norm's gradient, each replay with other incoming gradients."""
+  g = torch.Generator(device="cuda").manual_seed(2)
+  cos, sin = _tables(9, 32)
+  table, w, x = _randn(g, 50, 64), 1 + _randn(g, 64, std=0.3), _randn(g, 2, 9, 4 * 64)
+  ids, dout = torch.randint(0, 50, (40,), generator=g, device="cuda"), _randn(g, 40, 64)
+  dq, dk = _randn(g, 2, 9, 2, 64), _randn(g, 2, 9, 1, 64)
+
+  def step(table, w):
+    assert torch.autograd.grad(ops.embedding(ids, table, scale=3.0), table, dout, allow_unused=True) == (None,)
+    q, kk, _ = ops.qk_norm_rope(x, cos, sin, 2, 1, 64, 9, w)
+    assert torch.autograd.grad((q, kk), w, (dq, dk), allow_unused=True) == (None,)
+
+  mine = [_collect(t, dtype) for t in (table, w)]
+  graph = _captured(lambda: step(*mine))
+  for _ in range(2):
+    for t in (dout, dq, dk):
+      t.copy_(_randn(g, *t.shape))
+    graph.replay()
+    want = [_collect(t, dtype) for t in (table, w)]
+    step(*want)
+    for a, b in zip(mine, want):
+      assert torch.equal(a.main_grad, b.main_grad)

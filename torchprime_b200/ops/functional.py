@@ -933,8 +933,8 @@ def _embedding_backward(ids, table, dout, scale):
   from . import kernels as k
   mg = getattr(table, "main_grad", None)
   if mg is not None:
-    _embedding_collect(ids, mg, dout, scale, bool(getattr(table, "grad_overwrite", False)))
-    table.grad_overwrite = False
+    _embedding_collect(ids, mg, dout, scale, overwrites_grad(table))
+    grad_delivered(table)
     return None
   # a gradient that is recorded itself, or several at once, and what saved-tensor hooks gave back otherwise take torch's operators
   if (batched(dout) or (torch.is_grad_enabled() and dout.requires_grad) or not use_kernels(dout, table)
