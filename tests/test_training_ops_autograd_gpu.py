@@ -3,11 +3,13 @@ that are collected in a ``main_grad``."""
 
 import pytest
 import torch
+from torch.utils._python_dispatch import TorchDispatchMode
 
 from torchprime_b200.ops import functional as ops
 
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
+HALF = 2.0 ** -8              # a rounding to bf16
 
 
 @pytest.fixture(autouse=True, params=["native", "python"])
@@ -132,3 +134,27 @@ def test_a_captured_pass_replaces_what_its_last_replay_collected(cuda_lib, dtype
     step(*want)
     for a, b in zip(mine, want):
       assert torch.equal(a.main_grad, b.main_grad)
+
+
+# ------------------------------------------------------------------------------------------- definitions in place of kernels
+class _Mode(TorchDispatchMode):
+  def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+    return func(*args, **(kwargs or {}))
+
+
+def test_ids_without_a_row_where_something_follows_the_operators(cuda_lib):
+  """Under a dispatch mode, in a trace and as int32: what the kernels give."""
+  g = torch.Generator(device="cuda").manual_seed(8)
+  table = _randn(g, 50, 64).requires_grad_()
+  ids, dout = torch.randint(-20, 70, (6, 40), generator=g, device="cuda"), _randn(g, 6, 40, 64)
+  want = ops.embedding(ids, table, scale=0.5)
+  (dt,) = torch.autograd.grad(want, table, dout)
+  with _Mode():
+    ys = [ops.embedding(ids, table, scale=0.5)]
+  ys.append(ops.embedding(ids.int(), table, scale=0.5))
+  traced = torch.jit.trace(lambda i, t: ops.embedding(i, t, scale=0.5), (ids % 50, table))
+  ys.append(traced(ids, table))
+  for y in ys:
+    (got,) = torch.autograd.grad(y, table, dout)
+    # (sums of up to 15 rows in another order and, in torch's operator, other roundings)
+    assert torch.equal(y, want) and (got.double() - dt.double()).abs().max() <= 15 * HALF * dt.double().abs().max()

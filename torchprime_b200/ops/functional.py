@@ -986,9 +986,17 @@ def embedding_peer(ids, table, peer):
   return _EmbeddingPeerFn.apply(ids, table, peer)
 
 
+def _embedding_rows(ids, table):
+  """Rows of the table in torch operations; zeros and no gradient for ids without one (torch's own lookup ends the process there)."""
+  if table.shape[0] == 0:
+    return table.new_zeros(*ids.shape, table.shape[1])
+  ok = (ids >= 0) & (ids < table.shape[0])
+  return torch.where(ok[..., None], F.embedding(torch.where(ok, ids, 0), table), 0.0)
+
+
 def embedding(ids, table, scale=None):
-  """Rows ``ids`` of the table, times the number ``scale`` (rounded once; None: as they are).  On the kernels an id without a row gives
-  zeros and no gradient, and the table's gradient adds up each id's tokens in their order: it is the same in every run."""
+  """Rows ``ids`` of the table, times the number ``scale`` (rounded once; None: as they are).  Of a table that the kernels take an id
+  without a row gives zeros and no gradient, and the table's gradient adds up each id's tokens in their order: it is the same in every run."""
   if scale is not None:
     scale = float(scale)
     if not math.isfinite(scale):
@@ -997,11 +1005,13 @@ def embedding(ids, table, scale=None):
     y = nat.embedding(ids, table, 1.0 if scale is None else scale)
     if y is not None:
       return y
-  if (use_kernels(table) and unobserved() and table.dim() == 2 and table.shape[1] % 8 == 0 and table.is_contiguous()
-      and table.data_ptr() % 16 == 0 and ids.dtype == torch.int64 and ids.device == table.device and ids.numel() <= 1 << 30
-      and table.shape[0] <= 1 << 30):
-    return _EmbeddingFn.apply(ids, table, 1.0 if scale is None else scale)
-  y = F.embedding(ids, table)
+  if use_kernels(table) and table.dim() == 2 and table.shape[1] % 8 == 0:
+    if (unobserved() and table.is_contiguous() and table.data_ptr() % 16 == 0 and ids.dtype == torch.int64 and ids.device == table.device
+        and ids.numel() <= 1 << 30 and table.shape[0] <= 1 << 30):
+      return _EmbeddingFn.apply(ids, table, 1.0 if scale is None else scale)
+    y = _embedding_rows(ids, table)
+  else:
+    y = F.embedding(ids, table)
   return y if scale is None else (ref.wide(y) * scale).to(table.dtype)
 
 
