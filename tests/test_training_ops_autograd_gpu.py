@@ -1,6 +1,8 @@
 """Norms of query and key heads, the embedding and dropout inside autograd: recomputed layers under partial backward passes, gradients
 that are collected in a ``main_grad``."""
 
+import contextlib
+
 import pytest
 import torch
 from torch.utils._python_dispatch import TorchDispatchMode
@@ -158,3 +160,21 @@ def test_ids_without_a_row_where_something_follows_the_operators(cuda_lib):
     (got,) = torch.autograd.grad(y, table, dout)
     # (sums of up to 15 rows in another order and, in torch's operator, other roundings)
     assert torch.equal(y, want) and (got.double() - dt.double()).abs().max() <= 15 * HALF * dt.double().abs().max()
+
+
+def test_weights_collect_their_gradients_where_something_follows_the_operators(cuda_lib):
+  g = torch.Generator(device="cuda").manual_seed(9)
+  cos, sin = _tables(9, 32)
+  table, w, x = _randn(g, 50, 64), 1 + _randn(g, 64, std=0.3), _randn(g, 2, 9, 4 * 64).requires_grad_()
+  ids, dout = torch.randint(0, 50, (40,), generator=g, device="cuda"), _randn(g, 40, 64)
+  dy = [_randn(g, 2, 9, n, 64) for n in (2, 1, 1)]
+  for dtype in (torch.float32, BF16):
+    mine, want = ([_collect(t, dtype) for t in (table, w)] for _ in range(2))
+    for ps, mode in ((mine, _Mode()), (want, contextlib.nullcontext())):
+      with mode:
+        for _ in range(2):
+          ops.embedding(ids, ps[0], scale=3.0).backward(dout)
+          torch.autograd.backward(ops.qk_norm_rope(x, cos, sin, 2, 1, 64, 9, q_weight=ps[1]), dy)
+    for a, b in zip(mine, want):
+      # (torch's operators round each row of the table's gradient, up to eight to an id, and the weights' sums)
+      assert a.grad is None and (a.main_grad - b.main_grad).abs().max() <= 12 * HALF * b.main_grad.abs().max()

@@ -157,6 +157,36 @@ def grad_delivered(w):
     w.grad_capture = capture
 
 
+class _CollectFn(torch.autograd.Function):
+  """A weight as it is, whose gradient goes to its ``main_grad``: what definitions in torch operations read in its place."""
+
+  @staticmethod
+  def forward(ctx, w):
+    ctx.w = w
+    return w.view_as(w)
+
+  @staticmethod
+  def backward(ctx, dw):
+    w, mg = ctx.w, getattr(ctx.w, "main_grad", None)
+    if mg is None or batched(dw) or (torch.is_grad_enabled() and dw.requires_grad):
+      return dw
+    mg.copy_(dw) if overwrites_grad(w) else mg.add_(dw)
+    grad_delivered(w)
+    return None
+
+  @staticmethod
+  def jvp(ctx, dw):
+    return dw.view_as(dw)
+
+
+def _collecting(w):
+  """``w``, or what stands for it where its gradient is to go to a ``main_grad``."""
+  if (w is None or getattr(w, "main_grad", None) is None or not w.requires_grad or not torch.is_grad_enabled()
+      or torch._C._functorch.peek_interpreter_stack() is not None):
+    return w
+  return _CollectFn.apply(w)
+
+
 def _wgrad_into(sink, weights, dy2, x2):
   """dW = dy2^T @ x2 written into the main_grad sink (overwrite or accumulate).  Under the FSDP
   engine's peer-memory collectives the parameters carry ``rs_push``: the GEMM epilogue then stores
@@ -826,6 +856,8 @@ def qk_norm_rope(qkv, cos_half, sin_half, hq, hkv, d, seq_len, q_weight=None, k_
       pos = pos.clamp(-1, 2 ** 31 - 1).to(torch.int32) if pos.dtype == torch.int64 else pos
       pos = pos.contiguous()
     return _QkNormRopeFn.apply(qkv, q_weight, k_weight, cos_half, sin_half, pos, (int(hq), int(hkv), int(d), int(seq_len), eps, bool(interleaved)))
+  if use_kernels(qkv, q_weight, k_weight):
+    q_weight, k_weight = _collecting(q_weight), _collecting(k_weight)
   return ref.qk_norm_rope(qkv, cos_half, sin_half, hq, hkv, d, seq_len, q_weight, k_weight, eps, pos, interleaved)
 
 
@@ -1009,7 +1041,7 @@ def embedding(ids, table, scale=None):
     if (unobserved() and table.is_contiguous() and table.data_ptr() % 16 == 0 and ids.dtype == torch.int64 and ids.device == table.device
         and ids.numel() <= 1 << 30 and table.shape[0] <= 1 << 30):
       return _EmbeddingFn.apply(ids, table, 1.0 if scale is None else scale)
-    y = _embedding_rows(ids, table)
+    y = _embedding_rows(ids, _collecting(table))
   else:
     y = F.embedding(ids, table)
   return y if scale is None else (ref.wide(y) * scale).to(table.dtype)
