@@ -19,6 +19,8 @@
 // * embedding_join_kernel adds up the parts in the chunks' order, an id to a warp, or one with many (the padding's row) to a CTA.  (Joined by
 //   whoever leaves the last part, with fences and counters, it all took longer: 65536 tokens 134 -> 148 us.)
 //
+// Few tokens take two other kernels, which have no more to do than the tokens ask for (see below).
+//
 // 8192 tokens of a 128256 x 4096 table: 170 us for 1.12 GB, 171 at a copy's rate; 65536 of 32000 x 2048, 0.3 of them of one id: 103 us for 0.4 GB.
 
 #include <atomic>
@@ -271,6 +273,19 @@ __device__ __forceinline__ void emb_store(void* dtable, long long at, const floa
   }
 }
 
+// One column of a row.
+template <bool F32>
+__device__ __forceinline__ void emb_store1(void* dtable, long long at, float a, float scale, bool add) {
+  a = mul_exact(a, scale);
+  if (F32) {
+    float* dst = static_cast<float*>(dtable) + at;
+    *dst = add ? *dst + a : a;
+  } else {
+    __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(dtable) + at;
+    *dst = __float2bfloat16(add ? __bfloat162float(*dst) + a : a);
+  }
+}
+
 // Sixteen bytes to this thread's own place in shared memory.
 __device__ __forceinline__ void emb_ask(uint4* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
@@ -406,19 +421,241 @@ embedding_join_kernel(const EmbGrad p) {
         float a = s_part[0][threadIdx.x];
 #pragma unroll
         for (int w = 1; w < EJ_WARPS; ++w) a += s_part[w][threadIdx.x];
-        a = mul_exact(a, p.scale);
-        const long long at = (long long)it.x * p.dim + col;
-        if (F32) {
-          float* dst = static_cast<float*>(p.dtable) + at;
-          *dst = ADD ? *dst + a : a;
-        } else {
-          __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.dtable) + at;
-          *dst = __float2bfloat16(ADD ? __bfloat162float(*dst) + a : a);
-        }
+        emb_store1<F32>(p.dtable, (long long)it.x * p.dim + col, a, p.scale, ADD);
       }
       __syncthreads();
     }
     __syncthreads();
+  }
+}
+
+// ---- few tokens: each is compared with all the others, once, and then every id's run of the order has a warp to itself.  Nothing is counted
+// for ids without a token, and no parts are joined.  Gradients that are added, up to EF_MOST tokens; us, this / the three kernels above, ids evenly
+// spread and half of them one, fp32: 64 tokens of 128256 x 4096 4.9 / 25.5 and 4.9 / 19.5, 1024 11 / 28 and 10.5 / 28, 4096 37 / 50 and 36 / 49; 4096 of
+// 2000 x 1024 14 / 16 and 21 / 19 (8192, when a long run still took longer: 28 / 18).  Gradients that are written, for which the ranking
+// kernel zeroes the table as well, up to EF_WRITTEN, bf16: 64 of 128256 x 4096 145 / 153, 2048 of 32000 x 2048 27 / 31 and 29 / 32, of 2000 x 1024
+// 10.6 / 13.3 and 12.6 / 14.6; 4096 of them 14.2 / 14.2 and 21 / 17.
+constexpr int EF_MOST = 4096, EF_WRITTEN = 2048;
+constexpr int EF_WARPS = 16;                 // of the ranking kernel
+constexpr int EF_ZEROS = 16;                 // vectors of a thread of it that writes zeros
+
+struct EmbFew {
+  const long long* ids;
+  const __nv_bfloat16* dout;
+  void* dtable;
+  int2* order;                               // [tokens]: a token and its row, or -1 (those are last); by row, then by token
+  long long row0;
+  int tokens, rows, dim;
+  int rankers;                               // CTAs that rank
+  int longs, blocks;                         // CTAs to a team for long runs; blocks of ER_VECS x 256 columns
+  long long zeros;                           // vectors of the table, if it is written
+  float scale;
+};
+
+// The place of a token is how many stand in front: those of lower rows, and of its own row those with lower numbers.  A warp compares its token with
+// all of them, which the CTA has as rows in shared memory: two instructions each.  The CTAs behind write zeros to the table.
+__global__ void __launch_bounds__(EF_WARPS * 32)
+embedding_rank_kernel(const EmbFew p) {
+  if (!chain_begin()) return;
+  if ((int)blockIdx.x >= p.rankers) {
+    uint4* dst = static_cast<uint4*>(p.dtable);
+    const long long i0 = (blockIdx.x - p.rankers) * (EF_WARPS * 32LL * EF_ZEROS) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < EF_ZEROS; ++i)
+      if (i0 + EF_WARPS * 32 * i < p.zeros) dst[i0 + EF_WARPS * 32 * i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  __shared__ __align__(16) unsigned s_row[EF_MOST];
+  const int lane = threadIdx.x & 31, t = blockIdx.x * EF_WARPS + warp_index(), all = (p.tokens + 3) / 4 * 4;      // (up to EF_MOST)
+#pragma unroll 4
+  for (int i = threadIdx.x; i < all; i += EF_WARPS * 32) {
+    const long long id = i < p.tokens ? p.ids[i] - p.row0 : -1;
+    s_row[i] = id < 0 || id >= p.rows ? EMB_NONE : (unsigned)id;
+  }
+  __syncthreads();
+  if (t >= p.tokens) return;
+  const unsigned me = s_row[t];
+  int less = 0, i = lane * 4;
+#pragma unroll 4
+  for (; i + 4 <= t; i += 128) {
+    const uint4 c = *reinterpret_cast<const uint4*>(s_row + i);
+    less += (c.x <= me) + (c.y <= me) + (c.z <= me) + (c.w <= me);
+  }
+  if (i <= t) {                              // the vector that it is in
+    for (int k = i; k < i + 4; ++k) less += k < t ? s_row[k] <= me : s_row[k] < me;
+    i += 128;
+  }
+#pragma unroll 4
+  for (; i < all; i += 128) {
+    const uint4 c = *reinterpret_cast<const uint4*>(s_row + i);
+    less += (c.x < me) + (c.y < me) + (c.z < me) + (c.w < me);
+  }
+  less = __reduce_add_sync(0xffffffffu, less);
+  if (lane == 0) p.order[less] = make_int2(t, (int)me);      // (EMB_NONE: -1)
+}
+
+// Old numbers of eight columns, loaded ahead of their sum.
+template <bool F32>
+struct EmbOld {
+  uint4 a, b;
+  __device__ __forceinline__ void load(const void* dtable, long long at) {
+    if (F32) {
+      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(dtable) + at);
+      a = src[0];
+      b = src[1];
+    } else {
+      a = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(dtable) + at);
+    }
+  }
+  __device__ __forceinline__ void add_to(float* f) const {
+    float o[8];
+    if (F32) {
+      o[0] = __uint_as_float(a.x); o[1] = __uint_as_float(a.y); o[2] = __uint_as_float(a.z); o[3] = __uint_as_float(a.w);
+      o[4] = __uint_as_float(b.x); o[5] = __uint_as_float(b.y); o[6] = __uint_as_float(b.z); o[7] = __uint_as_float(b.w);
+    } else {
+      emb_unpack(a, o);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] += o[e];
+  }
+};
+template <bool F32>
+__device__ __forceinline__ void emb_write(void* dtable, long long at, const float* f) {
+  if (F32) {
+    float4* dst = reinterpret_cast<float4*>(static_cast<float*>(dtable) + at);
+    dst[0] = make_float4(f[0], f[1], f[2], f[3]);
+    dst[1] = make_float4(f[4], f[5], f[6], f[7]);
+  } else {
+    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(dtable) + at) = emb_pack(f);
+  }
+}
+
+// Runs of the order, a warp to each of less than ER_LONG tokens and ER_VECS x 256 columns: the old numbers and the first rows are asked for at once.
+// Longer ones: the first p.longs x ER_TEAMS CTAs, 64 columns each.  A team looks through the order for the runs that are its own (by their place, at
+// most one in ER_LONG); a warp takes one, an eighth of it every fourth row, or, from ER_ALL tokens on, the whole CTA.
+constexpr int ER_WARPS = 8, ER_VECS = 2, ER_TEAMS = 4, ER_LONG = 32, ER_ALL = 128;
+
+// Rows j0, j0 + step, ... by 32, of the run of `row` that begins at `from`, added up for a lane's eight columns, then over the warp's eighths.
+__device__ __forceinline__ void emb_run(const EmbFew& p, int from, int row, int j0, int step, int col, float* acc) {
+  const int lane = threadIdx.x & 31;
+  const __nv_bfloat16* src = p.dout + (col < p.dim ? col : 0);
+  auto tokens = [&](int j) {                 // of places j + lane of the run; -1 behind it
+    const int at = from + j + lane;
+    const int2 e = at < p.tokens ? p.order[at] : make_int2(0, -1);
+    return e.y == row ? e.x : -1;
+  };
+#pragma unroll
+  for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+  int here = tokens(j0);
+  while (__shfl_sync(0xffffffffu, here, 0) >= 0) {
+    uint4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int t = __shfl_sync(0xffffffffu, here, 4 * i + lane / 8);
+      v[i] = t >= 0 && col < p.dim ? *reinterpret_cast<const uint4*>(src + (long long)t * p.dim) : make_uint4(0, 0, 0, 0);
+    }
+    j0 += step;
+    here = tokens(j0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float x[8];
+      emb_unpack(v[i], x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += x[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], 8);
+    acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], 16);
+  }
+}
+
+template <bool F32, bool ADD>
+__global__ void __launch_bounds__(ER_WARPS * 32, 4)
+embedding_run_kernel(const EmbFew p) {
+  if (!chain_begin()) return;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  auto row_at = [&](int i) { return i >= 0 && i < p.tokens ? p.order[i].y : -1; };
+  if (blockIdx.x < (unsigned)p.longs * ER_TEAMS) {
+    __shared__ int s_run[EF_MOST / ER_LONG], s_all[EF_MOST / ER_ALL], s_runs, s_alls;
+    __shared__ __align__(16) float s_part[ER_WARPS][64];
+    const int team = blockIdx.x % ER_TEAMS, col0 = blockIdx.x / ER_TEAMS * 64, col = col0 + lane % 8 * 8;
+    if (threadIdx.x == 0) s_runs = s_alls = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int i = threadIdx.x; i < p.tokens; i += ER_WARPS * 32) {
+      const int row = row_at(i);
+      if (row < 0 || row_at(i + ER_LONG - 1) != row || row_at(i - 1) == row || i / ER_LONG % ER_TEAMS != team) continue;
+      if (row_at(i + ER_ALL - 1) == row) s_all[atomicAdd(&s_alls, 1)] = i;        // (in any order: each is a result of its own)
+      else s_run[atomicAdd(&s_runs, 1)] = i;
+    }
+    __syncthreads();
+    const int runs = s_runs, alls = s_alls;
+    float acc[8];
+    for (int k = 0; k < alls; ++k) {
+      const int row = row_at(s_all[k]);
+      emb_run(p, s_all[k], row, warp * 32, ER_WARPS * 32, col, acc);
+      if (lane < 8) {
+        reinterpret_cast<float4*>(s_part[warp])[2 * lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        reinterpret_cast<float4*>(s_part[warp])[2 * lane + 1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+      }
+      __syncthreads();
+      if (threadIdx.x < 64 && col0 + (int)threadIdx.x < p.dim) {
+        float a = s_part[0][threadIdx.x];
+#pragma unroll
+        for (int w = 1; w < ER_WARPS; ++w) a += s_part[w][threadIdx.x];
+        emb_store1<F32>(p.dtable, (long long)row * p.dim + col0 + threadIdx.x, a, p.scale, ADD);
+      }
+      __syncthreads();
+    }
+    for (int k = warp; k < runs; k += ER_WARPS) {
+      const int row = row_at(s_run[k]);
+      emb_run(p, s_run[k], row, 0, 32, col, acc);
+      if (lane < 8 && col < p.dim) emb_store<F32>(p.dtable, (long long)row * p.dim + col, acc, p.scale, ADD);
+    }
+    return;
+  }
+  const unsigned unit = (blockIdx.x - p.longs * ER_TEAMS) * ER_WARPS + warp;
+  const int at = unit / p.blocks, col = (unit - at * p.blocks) * (ER_VECS * 256) + lane * 8;
+  if (at >= p.tokens) return;
+  const int2 here = at + lane < p.tokens ? p.order[at + lane] : make_int2(0, -1);
+  const int row = __shfl_sync(0xffffffffu, here.y, 0), n = __ffs(__ballot_sync(0xffffffffu, here.y != row)) - 1;
+  if (row < 0 || n < 0 || row_at(at - 1) == row) return;       // (no difference: ER_LONG or more)
+  const long long to = (long long)row * p.dim + col;
+  auto load = [&](int j, int i) {
+    const int t = __shfl_sync(0xffffffffu, here.x, j & 31);
+    return j < n && col + 256 * i < p.dim ? *reinterpret_cast<const uint4*>(p.dout + (long long)t * p.dim + col + 256 * i) : make_uint4(0, 0, 0, 0);
+  };
+  EmbOld<F32> old[ER_VECS];
+  uint4 first[ER_VECS];
+#pragma unroll
+  for (int i = 0; i < ER_VECS; ++i) {
+    first[i] = load(0, i);
+    if (ADD && col + 256 * i < p.dim) old[i].load(p.dtable, to + 256 * i);
+  }
+#pragma unroll
+  for (int i = 0; i < ER_VECS; ++i) {
+    float acc[8];
+    emb_unpack(first[i], acc);
+    for (int j = 1; j < n; j += 8) {
+      uint4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = load(j + k, i);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        float x[8];
+        emb_unpack(v[k], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] += x[e];
+      }
+    }
+    if (col + 256 * i < p.dim) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] = mul_exact(acc[e], p.scale);
+      if (ADD) old[i].add_to(acc);
+      emb_write<F32>(p.dtable, to + 256 * i, acc);
+    }
   }
 }
 
@@ -461,6 +698,21 @@ struct EmbLayout {
   }
 };
 
+static bool emb_few(int tokens, int dim, bool add) { return tokens <= (add ? EF_MOST : EF_WRITTEN) && dim <= 1 << 20; }
+
+template <bool F32, bool ADD>
+static void launch_embedding_few(EmbFew& p, cudaStream_t stream) {
+  constexpr long long PER = EF_WARPS * 32LL * EF_ZEROS;
+  p.rankers = (p.tokens + EF_WARPS - 1) / EF_WARPS;
+  p.zeros = ADD ? 0 : (long long)p.rows * p.dim / (F32 ? 4 : 8);
+  chain(embedding_rank_kernel, (unsigned)(p.rankers + (p.zeros + PER - 1) / PER), EF_WARPS * 32, 0, stream, p);
+  p.longs = p.tokens >= ER_LONG ? (p.dim + 63) / 64 : 0;
+  p.blocks = (p.dim + ER_VECS * 256 - 1) / (ER_VECS * 256);
+  if (p.tokens > 0)
+    chain(embedding_run_kernel<F32, ADD>, p.longs * ER_TEAMS + (unsigned)(((long long)p.tokens * p.blocks + ER_WARPS - 1) / ER_WARPS), ER_WARPS * 32, 0,
+          stream, p);
+}
+
 template <bool F32, bool ADD>
 static void launch_embedding_grad(const EmbGrad& p, cudaStream_t stream) {
   const int sms = sm_count();
@@ -494,7 +746,9 @@ extern "C" int tpb_embedding_fwd(const void* table, const long long* ids, void* 
 
 // Bytes of scratch for tpb_embedding_bwd.
 extern "C" long long tpb_embedding_bwd_scratch(int tokens, int rows_local, int dim) {
-  return EmbLayout(tokens, rows_local, dim).bytes;
+  const long long order = 8LL * tokens;      // of few tokens
+  const long long all = emb_few(tokens, dim, false) ? 0 : EmbLayout(tokens, rows_local, dim).bytes;
+  return all > order ? all : order;
 }
 
 // dtable[v] = (`add`: dtable[v] +) scale * sum of dout[t] over ids[t] = row0 + v; with `add`, rows without a token are left alone.
@@ -504,6 +758,23 @@ extern "C" int tpb_embedding_bwd(const void* dout, const long long* ids, void* d
   for (const void* a : {dout, (const void*)dtable, (const void*)scratch})
     if (reinterpret_cast<uintptr_t>(a) % 16) return -2;
   if (rows_local == 0 || (tokens == 0 && add)) return 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (emb_few(tokens, dim, add != 0)) {
+    EmbFew p = {};
+    p.ids = ids;
+    p.dout = static_cast<const __nv_bfloat16*>(dout);
+    p.dtable = dtable;
+    p.order = static_cast<int2*>(scratch);
+    p.row0 = row0;
+    p.tokens = tokens;
+    p.rows = rows_local;
+    p.dim = dim;
+    p.scale = scale;
+    if (dtable_is_f32) add ? launch_embedding_few<true, true>(p, st) : launch_embedding_few<true, false>(p, st);
+    else add ? launch_embedding_few<false, true>(p, st) : launch_embedding_few<false, false>(p, st);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? 0 : 1000 + (int)e;
+  }
   const EmbLayout at(tokens, rows_local, dim);
   char* s = static_cast<char*>(scratch);
   EmbGrad p = {};
@@ -528,7 +799,6 @@ extern "C" int tpb_embedding_bwd(const void* dout, const long long* ids, void* d
   while (1ll << (p.shift - 31) < p.sets) ++p.shift;
   p.inv = (unsigned)((1ull << p.shift) / p.sets + 1);       // exact for dividends below 2^31
   p.scale = scale;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int hists = (EP_WARPS + 1) * p.per * 4, most = (EP_SMEM - hists) / (EP_WARPS * 4);
   p.list = !at.coded || p.share > 1 << 22 ? 0 : p.share < most ? p.share : most;       // (an entry has 22 bits for the token)
   const int smem = hists + EP_WARPS * p.list * 4;
