@@ -1,5 +1,5 @@
 """Norms of query and key heads, the embedding and dropout inside autograd: recomputed layers under partial backward passes, gradients
-that are collected in a ``main_grad``."""
+that are collected in a ``main_grad``, numbers that are not finite."""
 
 import contextlib
 
@@ -8,6 +8,8 @@ import torch
 from torch.utils._python_dispatch import TorchDispatchMode
 
 from torchprime_b200.ops import functional as ops
+from torchprime_b200.ops import kernels as k
+from torchprime_b200.ops import reference as ref
 
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
@@ -178,3 +180,83 @@ def test_weights_collect_their_gradients_where_something_follows_the_operators(c
     for a, b in zip(mine, want):
       # (torch's operators round each row of the table's gradient, up to eight to an id, and the weights' sums)
       assert a.grad is None and (a.main_grad - b.main_grad).abs().max() <= 12 * HALF * b.main_grad.abs().max()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+def test_weights_that_collect_their_gradients_from_after_the_forward_pass_on(cuda_lib, dtype):
+  g = torch.Generator(device="cuda").manual_seed(4)
+  cos, sin = _tables(9, 32)
+  x, dy = _randn(g, 2, 9, 4 * 64).requires_grad_(), [_randn(g, 2, 9, n, 64) for n in (2, 1, 1)]
+  table, wq, wk = _randn(g, 50, 64), 1 + _randn(g, 64, std=0.3), 1 + _randn(g, 64, std=0.3)
+  ids, dout = torch.randint(0, 50, (40,), generator=g, device="cuda"), _randn(g, 40, 64)
+  results = []
+  for late in (False, True):
+    ps = [_collect(t, dtype) if not late else t.detach().clone().requires_grad_() for t in (table, wq, wk)]
+    y, heads = ops.embedding(ids, ps[0], scale=3.0), ops.qk_norm_rope(x, cos, sin, 2, 1, 64, 9, *ps[1:])
+    if late:
+      for p in ps:
+        p.main_grad, p.grad_overwrite = torch.full(p.shape, 7.0, device="cuda", dtype=dtype), True
+    torch.autograd.backward([y, *heads], [dout, *dy])
+    assert all(p.grad is None and not p.grad_overwrite for p in ps)
+    results.append([x.grad, *(p.main_grad for p in ps)])
+    x.grad = None
+  for a, b in zip(*results):
+    assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------------- not finite
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_qk_norm_rope_gradient_of_numbers_that_are_not_finite(cuda_lib, bad, interleaved):
+  """They reach what the formula says and nothing else: the head of theirs, and their columns (or all, of a head that is not
+  finite itself) of the weights' sums."""
+  g = torch.Generator(device="cuda").manual_seed(5)
+  b, s, hq, hkv, d = 2, 33, 6, 2, 64
+  cos, sin = _tables(s, d // 2)
+  for where in ("dq", "dk", "dv", "q", "k"):
+    x = _randn(g, b, s, (hq + 2 * hkv) * d)
+    dy = [_randn(g, b, s, n, d) for n in (hq, hkv, hkv)]
+    if where[0] == "d":
+      dy[("dq", "dk", "dv").index(where)][1, 7, 1, 5] = bad
+    else:
+      x[1, 7, (0 if where == "q" else hq) * d + 5] = bad
+    x.requires_grad_()
+    wq, wk = ((1 + _randn(g, d, std=0.3)).requires_grad_() for _ in range(2))
+    got = torch.autograd.grad(ops.qk_norm_rope(x, cos, sin, hq, hkv, d, s, wq, wk, interleaved=interleaved), (x, wq, wk), dy)
+    up = [t.detach().double() for t in (*dy, x, cos, sin, wq, wk)]
+    want = ref.qk_norm_rope_grad(*up[:6], hq, hkv, d, s, *up[6:], 1e-6, None, interleaved)
+    for a, w in zip(got, want):
+      assert torch.equal(a.isfinite(), w.isfinite()), where
+      # against the largest: a rounding of the result, and fp32 sums of up to 400 terms
+      ok = w.isfinite()
+      assert not ok.any() or (a[ok].double() - w[ok]).abs().max() <= (HALF + 400 * 2.0 ** -23) * w[ok].abs().max()
+
+
+@pytest.mark.parametrize("tokens", [40, 3000, 9000])
+def test_embedding_gradient_of_numbers_that_are_not_finite(cuda_lib, tokens):
+  g = torch.Generator(device="cuda").manual_seed(6)
+  table, ids = _randn(g, 300, 72).requires_grad_(), torch.randint(0, 300, (tokens,), generator=g, device="cuda")
+  ids[:3], ids[3:20] = 7, 9
+  dout = _randn(g, tokens, 72)
+  dout[0, 3], dout[1, 4], dout[2, 5], dout[3, 5], dout[4, 5] = float("nan"), float("inf"), float("-inf"), float("inf"), float("-inf")
+  (got,) = torch.autograd.grad(ops.embedding(ids, table, scale=0.5), table, dout)
+  want = torch.zeros(300, 72, device="cuda", dtype=torch.float64).index_add_(0, ids, dout.double() * 0.5)
+  for test in (torch.isnan, torch.isposinf, torch.isneginf):
+    assert torch.equal(test(got), test(want))
+  ok = want.isfinite()
+  assert (got[ok].double() - want[ok]).abs().max() <= (HALF + tokens * 2.0 ** -23) * want[ok].abs().max()
+  added = torch.ones(300, 72, device="cuda")
+  k.embedding_bwd_(dout, ids, added, scale=0.5)
+  for test in (torch.isnan, torch.isposinf, torch.isneginf):
+    assert torch.equal(test(added), test(want))
+
+
+def test_dropout_gradient_of_numbers_that_are_not_finite(cuda_lib):
+  g = torch.Generator(device="cuda").manual_seed(7)
+  x, seed = _randn(g, 5, 1001).requires_grad_(), torch.tensor([3, 9], device="cuda")
+  dy = _randn(g, 5, 1001)
+  dy[0], dy[1], dy[2] = float("nan"), float("inf"), float("-inf")
+  (dx,) = torch.autograd.grad(ops.dropout(x, 0.25, seed, site=4), x, dy)
+  keep = ref.dropout_keep(dy.shape, 16384, seed, 4)
+  assert bool(keep[:3].any()) and not bool(keep[:3].all()) and not bool(dx[~keep].any())
+  assert torch.equal(dx.nan_to_num(1.0, 2.0, 3.0), ref.dropout(dy, keep, 16384).nan_to_num(1.0, 2.0, 3.0))
