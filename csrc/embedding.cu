@@ -1,10 +1,11 @@
 // Embedding: rows of a table, scaled, and the table's gradient by sorted tokens.
 //
-//   out[t] = scale * E[id[t]],   dE[v] (+)= scale * sum of dout[t] over the tokens t with id[t] = v, in ascending order of t.
+//   out[t] = scale * E[id[t]],   dE[v] (+)= scale * sum of dout[t] over the tokens t with id[t] = v.
 //
 // Both are bound by memory.  The gradient of a training step writes the whole table (most rows as zeros) and reads dout once;
 // what makes it slow otherwise are atomics, which read and write an fp32 table that has to be zeroed before and rounded behind, in an
-// order that differs from run to run.  Here every row has one writer:
+// order that differs from run to run.  Here every row has one writer, and the order of its sum follows from the ids alone: a chunk's tokens
+// ascending, then the chunks' parts ascending or, of an id with many, in 32 shares of them:
 //
 // * embedding_plan_kernel puts the tokens in order of their ids.  A CTA has a set of ids (every sets-th one, so that frequent ones, which
 //   have low numbers, are spread) and looks at all tokens, so no CTA has to wait for another: its 32 warps count what each id has in their
@@ -19,7 +20,8 @@
 // * embedding_join_kernel adds up the parts in the chunks' order, an id to a warp, or one with many (the padding's row) to a CTA.  (Joined by
 //   whoever leaves the last part, with fences and counters, it all took longer: 65536 tokens 134 -> 148 us.)
 //
-// Few tokens take two other kernels, which have no more to do than the tokens ask for (see below).
+// Few tokens take two other kernels, embedding_rank_kernel and embedding_run_kernel, which have no more to do than the tokens ask for.  (Added up by
+// atomics in L2, red.v4.f32, the rows of the many tokens' form took longer, too: 8192 of 128256 x 4096 67 -> 86 us.)
 //
 // 8192 tokens of a 128256 x 4096 table: 170 us for 1.12 GB, 171 at a copy's rate; 65536 of 32000 x 2048, 0.3 of them of one id: 103 us for 0.4 GB.
 
@@ -530,12 +532,15 @@ __device__ __forceinline__ void emb_write(void* dtable, long long at, const floa
   }
 }
 
-// Runs of the order, a warp to each of less than ER_LONG tokens and ER_VECS x 256 columns: the old numbers and the first rows are asked for at once.
+// Runs of the order, a warp to each of less than ER_LONG tokens and ER_VECS x 256 columns, in ascending order: the old numbers and the first row are
+// asked for at once, then eight rows at a time.
 // Longer ones: the first p.longs x ER_TEAMS CTAs, 64 columns each.  A team looks through the order for the runs that are its own (by their place, at
-// most one in ER_LONG); a warp takes one, an eighth of it every fourth row, or, from ER_ALL tokens on, the whole CTA.
+// most one in ER_LONG); a warp takes one, a fourth of its lanes every fourth row, or, from ER_ALL tokens on, the whole CTA.  2048 tokens of 128256 x 4096,
+// fp32, 16 us (13 at a copy's rate for what is read and written), behind 6 of ranking: it ends soon after it has got going.  us: a CTA of 16 warps for
+// 16 places and 256 columns, with barriers for the long runs, 38 for both kernels, now 21; two rows at a time instead of eight 20 to 24 with frequent ids.
 constexpr int ER_WARPS = 8, ER_VECS = 2, ER_TEAMS = 4, ER_LONG = 32, ER_ALL = 128;
 
-// Rows j0, j0 + step, ... by 32, of the run of `row` that begins at `from`, added up for a lane's eight columns, then over the warp's eighths.
+// Rows j0, j0 + step, ... by 32, of the run of `row` that begins at `from`, added up for a lane's eight columns, then over the warp's fourths.
 __device__ __forceinline__ void emb_run(const EmbFew& p, int from, int row, int j0, int step, int col, float* acc) {
   const int lane = threadIdx.x & 31;
   const __nv_bfloat16* src = p.dout + (col < p.dim ? col : 0);

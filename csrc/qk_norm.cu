@@ -162,7 +162,8 @@ __device__ __forceinline__ void qk_wait() {
 
 constexpr int QF_CTAS = 4;                   // of the forward kernel to an SM (64 registers)
 // Of the gradient's: heads of a warp at a time (in steps of 32 / GROUP), CTAs to an SM, stages of a thread's.  8192 tokens of 32 / 8 heads, 32768
-// of 64 / 8, us: 2, 2, 2 54 and 311;  2, 2, 3 55 and 313;  3, 2, 2 56 and 318;  4, 1, 3 66 and 358;  1, 2, 6 70 and 382 (with the values behind).
+// of 64 / 8, us: 2, 2, 2 54 and 311;  2, 2, 3 55 and 313;  3, 2, 2 56 and 318;  4, 1, 3 66 and 358;  1, 2, 6 70 and 382 (with the values behind).  There a unit is
+// exactly the eight keys of a token; where it is not, most of it is empty: 8192 tokens of 7 / 1 heads 24.4 (8.3 at a copy's rate), of 10 / 2 of 256 40.1 (25.6).
 constexpr int QB_STEPS = 2, QB_CTAS = 2, QB_STAGES = 2;
 
 // A warp takes up to STEPS x 32 / GROUP heads of a token, queries and keys, and leaves.  What it reads is all asked for first, into shared

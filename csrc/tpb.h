@@ -98,7 +98,7 @@ int tpb_clip_coef(const float* sumsq, float max_norm, float* coef, float* norm_o
 // out[t,:] = scale * table[ids[t] - row0,:]; zeros for ids without a row here (embedding.cu)
 int tpb_embedding_fwd(const void* table, const long long* ids, void* out, int tokens, int dim,
                       long long vocab, long long row0, float scale, void* stream);
-// dtable[v,:] = (`add`: dtable[v,:] +) scale * sum of dout[t,:] over ids[t] - row0 = v, in the order of t
+// dtable[v,:] = (`add`: dtable[v,:] +) scale * sum of dout[t,:] over ids[t] - row0 = v, in an order that the ids decide
 long long tpb_embedding_bwd_scratch(int tokens, int rows_local, int dim);     // bytes
 int tpb_embedding_bwd(const void* dout, const long long* ids, void* dtable, void* scratch, int tokens, int dim,
                       int rows_local, long long row0, int dtable_is_f32, int add, float scale, void* stream);

@@ -1028,7 +1028,8 @@ def _embedding_rows(ids, table):
 
 def embedding(ids, table, scale=None):
   """Rows ``ids`` of the table, times the number ``scale`` (rounded once; None: as they are).  Of a table that the kernels take an id
-  without a row gives zeros and no gradient, and the table's gradient adds up each id's tokens in their order: it is the same in every run."""
+  without a row gives zeros and no gradient, and the table's gradient adds up each id's tokens in an order that the ids alone decide: it is
+  the same in every run."""
   if scale is not None:
     scale = float(scale)
     if not math.isfinite(scale):

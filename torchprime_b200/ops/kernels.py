@@ -193,8 +193,8 @@ def embedding_fwd(table, ids, row0=0, scale=1.0):
 
 
 def embedding_bwd_(dout, ids, dtable, row0=0, scale=1.0, overwrite=False):
-  """Adds ``scale`` times the sum of every id's rows of ``dout``, in the tokens' order, to ``dtable`` (fp32 or bf16, row 0 of which
-  is id ``row0``); with ``overwrite`` it becomes that sum, rows without a token zeros."""
+  """Adds ``scale`` times the sum of every id's rows of ``dout``, in an order that the ids decide, to ``dtable`` (fp32 or bf16, row 0 of
+  which is id ``row0``); with ``overwrite`` it becomes that sum, rows without a token zeros."""
   flat = ids.reshape(-1)
   d2 = dout.reshape(flat.numel(), dtable.shape[1])
   assert flat.is_contiguous() and flat.dtype == torch.int64
